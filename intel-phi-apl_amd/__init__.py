@@ -95,7 +95,53 @@ _SIGS = {
     "rt_gguf_tensor_type_name": (_c.c_char_p, [_c.c_uint32]),
     "rt_gguf_upload": (_int, [_vp, _vp, _c.c_char_p, _c.c_char_p, _c.c_size_t]),
     "rt_gguf_release": (None, [_vp, _vp]),
+    "rt_conv_silu_dev": (None, [_vp, _vp, _vp, _long, _long, _vp, _long, _vp, _vp, _vp, _long]),
+    "rt_delta_rule_dev": (None, [_vp, _vp, _vp]),
+    "rt_rope_kv_dev": (None, [_vp, _vp, _vp, _vp]),
+    "rt_attn_kv_dev": (None, [_vp, _vp, _vp, _vp]),
 }
+
+
+class Seqs(_c.Structure):
+    """struct rt_seqs (include/q8_mix.h): the new tokens of a call, sequence by sequence."""
+
+    _fields_ = [("n", _long), ("t", _long), ("longest", _long), ("start", _vp), ("past", _vp)]
+
+
+class Delta(_c.Structure):
+    """struct rt_delta (include/q8_mix.h): the gated delta rule."""
+
+    _fields_ = [("k_heads", _long), ("v_heads", _long), ("k_dim", _long), ("v_dim", _long), ("tiled", _long), ("q", _vp), ("k", _vp), ("v", _vp),
+                ("q_ld", _long), ("k_ld", _long), ("v_ld", _long), ("a", _vp), ("b", _vp), ("a_ld", _long), ("b_ld", _long), ("decay", _vp), ("dt", _vp),
+                ("eps", _c.c_float), ("scale", _c.c_float), ("s_in", _vp), ("s_out", _vp), ("z", _vp), ("z_ld", _long), ("nw", _vp),
+                ("nw_eps", _c.c_float), ("o", _vp), ("o_ld", _long)]
+
+
+# the cache's types (RT_F32, RT_F16, RT_BF16)
+TYPES = {"f32": 0, "f16": 1, "bf16": 2}
+
+
+class Kv(_c.Structure):
+    """struct rt_kv (include/q8_mix.h): a paged key-value cache."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("type", _long), ("dim", _long), ("heads", _long), ("page", _long), ("pages", _long), ("table", _vp),
+                ("table_ld", _long)]
+
+
+class Rope(_c.Structure):
+    """struct rt_rope (include/q8_mix.h): head norms, rotation, and the way into the cache."""
+
+    _fields_ = [("q", _vp), ("q_ld", _long), ("q_hd", _long), ("q_heads", _long), ("k", _vp), ("v", _vp), ("k_ld", _long), ("k_hd", _long),
+                ("v_ld", _long), ("v_hd", _long), ("q_norm", _vp), ("k_norm", _vp), ("eps", _c.c_float), ("rot", _long), ("pairs", _long),
+                ("freq", _vp), ("out", _vp), ("out_ld", _long), ("out_hd", _long)]
+
+
+class Attn(_c.Structure):
+    """struct rt_attn (include/q8_mix.h): attention over the cache."""
+
+    _fields_ = [("q", _vp), ("q_ld", _long), ("q_hd", _long), ("q_heads", _long), ("scale", _c.c_float), ("gate", _vp), ("gate_ld", _long),
+                ("gate_hd", _long), ("o", _vp), ("o_ld", _long)]
+
 
 
 class GgufKey(_c.Structure):

@@ -15,11 +15,13 @@
 #include <unistd.h>
 
 #include <chrono>
+#include <initializer_list>
 #include <unordered_map>
 #include <vector>
 
 #include "../../include/q8_rt.h"
 #include "q8_device.h"
+#include "q8_mix.h"
 #include "q8_wait.h"
 
 #define HIPCHECK(call)                                                                                                 \
@@ -1647,6 +1649,256 @@ void rt_device_info(struct rt *R, char *name, long name_len, int *cus)
     }
     if (cus)
         *cus = p.multiProcessorCount;
+}
+
+} /* extern "C" */
+
+/* ---- the operators between the products (include/q8_mix.h) */
+
+namespace {
+
+/* The calling thread on the runtime's GPU for the call, whichever it was on */
+struct on_gpu {
+    int was = 0;
+    const int gpu;
+    explicit on_gpu(const ctx *c) : gpu(c->device)
+    {
+        HIPCHECK(hipGetDevice(&was));
+        if (was != gpu)
+            HIPCHECK(hipSetDevice(gpu));
+    }
+    ~on_gpu()
+    {
+        if (was != gpu)
+            (void)hipSetDevice(was);
+    }
+};
+
+/* The bytes of an array from its first element to its last */
+struct span {
+    const char *p;
+    size_t n;
+};
+span rows_span(const void *p, long t, long ld, long width) { return {(const char *)p, p ? sizeof(float) * (size_t)((t - 1) * ld + width) : 0}; }
+bool meet(span a, span b) { return a.n && b.n && a.p < b.p + b.n && b.p < a.p + a.n; }
+
+/* No array that the call writes shares memory with one that it reads or writes besides */
+void check_apart(const char *fn, const char *what, span w, std::initializer_list<span> others)
+{
+    for (const span &o : others)
+        if (meet(w, o))
+            failf(fn, "%s overlaps another array of the call", what);
+}
+
+void check_words(const char *fn, const void *p, unsigned align, const char *what)
+{
+    if (!p || ((uintptr_t)p & (align - 1)))
+        failf(fn, "%s must be a %u-byte aligned device address", what, align);
+}
+
+/* a stride of token rows `width` wide */
+void check_ld(const char *fn, long ld, long width, const char *what)
+{
+    if (ld < width || ld % 4 || ld > 1L << 40)
+        failf(fn, "%s must be a multiple of 4 of at least %ld", what, width);
+}
+
+void check_seqs(const char *fn, const struct rt_seqs *s, bool past)
+{
+    if (!s)
+        fail(fn, "needs its sequences (struct rt_seqs)");
+    if (s->n < 1 || s->n > 65535 || s->t < 1 || s->t > RT_TOKENS_MAX || s->longest < 1 || s->longest > s->t)
+        failf(fn, "needs 1 to 65535 sequences, 1 to %ld tokens and longest from 1 to t", RT_TOKENS_MAX);
+    check_words(fn, s->start, 4, "start");
+    if (past)
+        check_words(fn, s->past, 4, "past");
+}
+
+void check_kv(const char *fn, const struct rt_kv *kv)
+{
+    if (!kv)
+        fail(fn, "needs its cache (struct rt_kv)");
+    if (kv->type != RT_F32 && kv->type != RT_F16 && kv->type != RT_BF16)
+        fail(fn, "the cache's type must be RT_F32, RT_F16 or RT_BF16");
+    if (kv->dim < 32 || kv->dim > 256 || kv->dim % 32)
+        fail(fn, "a head's size must be a multiple of 32, 32 to 256");
+    if (kv->heads < 1 || kv->heads > RT_HEADS_MAX)
+        failf(fn, "needs 1 to %ld key-value heads", RT_HEADS_MAX);
+    if (kv->page < 1 || kv->page > 1L << 30 || kv->pages < 1 || kv->pages >= 1L << 31 || kv->table_ld < 1 || kv->table_ld >= 1L << 31)
+        fail(fn, "needs pages of 1 to 2^30 positions, 1 to 2^31 - 1 of them, and as many a sequence");
+    if ((double)kv->pages * (double)kv->page * (double)(kv->heads * kv->dim) > 1e15)
+        fail(fn, "the cache is larger than any memory");
+    check_dev_ptr(fn, kv->k, "the cache's k");
+    check_dev_ptr(fn, kv->v, "the cache's v");
+    check_words(fn, kv->table, 4, "the page table");
+}
+
+span kv_span(const struct rt_kv *kv, const void *p)
+{
+    return {(const char *)p, (size_t)(kv->pages * kv->page * kv->heads * kv->dim) * (kv->type == RT_F32 ? 4 : 2)};
+}
+
+/* heads that lie hd floats apart in rows ld apart: any order of the two, for an output each element
+ * once. x is read where `in` */
+void check_heads(const char *fn, const void *p, long t, long ld, long hd, long heads, long dim, bool in, const char *what)
+{
+    check_dev_ptr(fn, p, what);
+    if (ld < 0 || hd < 0 || ld % 4 || hd % 4 || ld > 1L << 40 || hd > 1L << 40)
+        failf(fn, "%s: strides are multiples of 4, 0 or more", what);
+    if (!in && !((t == 1 || ld >= (heads - 1) * hd + dim) && (heads == 1 || hd >= dim)) && !((heads == 1 || hd >= (t - 1) * ld + dim) && (t == 1 || ld >= dim)))
+        failf(fn, "%s: its heads must not overlap", what);
+}
+span heads_span(const void *p, long t, long ld, long hd, long heads, long dim)
+{
+    return {(const char *)p, p ? sizeof(float) * (size_t)((t - 1) * ld + (heads - 1) * hd + dim) : 0};
+}
+span words_span(const void *p, size_t bytes) { return {(const char *)p, p ? bytes : 0}; }
+
+/* a state that the call replaces: s_out is s_in, or apart from it */
+void check_state(const char *fn, const float *in, const float *out, size_t floats)
+{
+    check_dev_ptr(fn, in, "s_in");
+    check_dev_ptr(fn, out, "s_out");
+    if (in != out && meet({(const char *)in, 4 * floats}, {(const char *)out, 4 * floats}))
+        fail(fn, "s_out must be s_in or apart from it");
+}
+
+} /* namespace */
+
+extern "C" {
+
+void rt_conv_silu_dev(struct rt *R, const struct rt_seqs *s, const float *x, long x_ld, long ch, const float *w, long taps, const float *s_in,
+                      float *s_out, float *y, long y_ld)
+{
+    const char *fn = "rt_conv_silu_dev";
+    ctx *c = get(R, fn);
+    check_seqs(fn, s, false);
+    if (ch < 4 || ch % 4 || ch > 1L << 24 || taps < 2 || taps > 8)
+        fail(fn, "needs a multiple of 4 channels, at most 2^24, and 2 to 8 taps");
+    check_dev_ptr(fn, x, "x");
+    check_dev_ptr(fn, w, "w");
+    check_dev_ptr(fn, y, "y");
+    check_ld(fn, x_ld, ch, "x_ld");
+    check_ld(fn, y_ld, ch, "y_ld");
+    const size_t state = (size_t)(s->n * (taps - 1) * ch);
+    check_state(fn, s_in, s_out, state);
+    const span in[] = {rows_span(x, s->t, x_ld, ch), words_span(w, 4 * (size_t)(ch * taps)), words_span(s->start, 4 * (size_t)(s->n + 1))};
+    check_apart(fn, "y", rows_span(y, s->t, y_ld, ch), {in[0], in[1], in[2], words_span(s_in, 4 * state), words_span(s_out, 4 * state)});
+    check_apart(fn, "s_out", words_span(s_out, 4 * state), {in[0], in[1], in[2]});
+    const on_gpu g(c);
+    q8_launch_conv((q8_stream_t)c->stream, *s, x, x_ld, ch, w, taps, s_in, s_out, y, y_ld);
+    launched("the short convolution");
+}
+
+void rt_delta_rule_dev(struct rt *R, const struct rt_seqs *s, const struct rt_delta *a)
+{
+    const char *fn = "rt_delta_rule_dev";
+    ctx *c = get(R, fn);
+    check_seqs(fn, s, false);
+    if (!a)
+        fail(fn, "needs its arguments (struct rt_delta)");
+    if (a->k_heads < 1 || a->v_heads < 1 || a->v_heads > RT_HEADS_MAX || a->v_heads % a->k_heads)
+        failf(fn, "needs 1 to %ld value heads, a multiple of the key heads", RT_HEADS_MAX);
+    if (a->k_dim != 32 && a->k_dim != 64 && a->k_dim != 96 && a->k_dim != 128 && a->k_dim != 192 && a->k_dim != 256)
+        fail(fn, "k_dim must be 32, 64, 96, 128, 192 or 256");
+    if (a->v_dim < 16 || a->v_dim > 512 || a->v_dim % 16)
+        fail(fn, "v_dim must be a multiple of 16, 16 to 512");
+    const long kw = a->k_heads * a->k_dim, vw = a->v_heads * a->v_dim;
+    check_dev_ptr(fn, a->q, "q");
+    check_dev_ptr(fn, a->k, "k");
+    check_dev_ptr(fn, a->v, "v");
+    check_dev_ptr(fn, a->o, "o");
+    check_ld(fn, a->q_ld, kw, "q_ld");
+    check_ld(fn, a->k_ld, kw, "k_ld");
+    check_ld(fn, a->v_ld, vw, "v_ld");
+    check_ld(fn, a->o_ld, vw, "o_ld");
+    check_words(fn, a->a, 4, "a");
+    check_words(fn, a->b, 4, "b");
+    check_words(fn, a->decay, 4, "decay");
+    check_words(fn, a->dt, 4, "dt");
+    if (a->a_ld < a->v_heads || a->b_ld < a->v_heads || a->a_ld > 1L << 40 || a->b_ld > 1L << 40)
+        fail(fn, "a_ld and b_ld must be at least v_heads");
+    if (a->z) {
+        check_dev_ptr(fn, a->z, "z");
+        check_dev_ptr(fn, a->nw, "nw");
+        check_ld(fn, a->z_ld, vw, "z_ld");
+    }
+    const size_t state = (size_t)(s->n * a->v_heads * a->k_dim * a->v_dim);
+    check_state(fn, a->s_in, a->s_out, state);
+    const long t = s->t;
+    const span in[] = {rows_span(a->q, t, a->q_ld, kw),           rows_span(a->k, t, a->k_ld, kw),           rows_span(a->v, t, a->v_ld, vw),
+                       rows_span(a->a, t, a->a_ld, a->v_heads),   rows_span(a->b, t, a->b_ld, a->v_heads),   rows_span(a->decay, 1, 0, a->v_heads),
+                       rows_span(a->dt, 1, 0, a->v_heads),        rows_span(a->z, t, a->z_ld, vw),           words_span(a->z ? a->nw : nullptr, 4 * (size_t)a->v_dim),
+                       words_span(s->start, 4 * (size_t)(s->n + 1))};
+    const span o = rows_span(a->o, t, a->o_ld, vw), out = words_span(a->s_out, 4 * state);
+    check_apart(fn, "o", o, {in[0], in[1], in[2], in[3], in[4], in[5], in[6], in[7], in[8], in[9], out, words_span(a->s_in, 4 * state)});
+    check_apart(fn, "s_out", out, {in[0], in[1], in[2], in[3], in[4], in[5], in[6], in[7], in[8], in[9]});
+    const on_gpu g(c);
+    q8_launch_delta((q8_stream_t)c->stream, *s, *a);
+    launched("the delta rule");
+}
+
+void rt_rope_kv_dev(struct rt *R, const struct rt_seqs *s, const struct rt_kv *kv, const struct rt_rope *a)
+{
+    const char *fn = "rt_rope_kv_dev";
+    ctx *c = get(R, fn);
+    check_seqs(fn, s, true);
+    check_kv(fn, kv);
+    if (!a)
+        fail(fn, "needs its arguments (struct rt_rope)");
+    if (a->q_heads < 1 || a->q_heads > RT_HEADS_MAX)
+        failf(fn, "needs 1 to %ld query heads", RT_HEADS_MAX);
+    if (a->rot < 0 || a->rot > kv->dim || a->rot % 2)
+        fail(fn, "rot must be even, 0 to a head's size");
+    const long t = s->t, d = kv->dim;
+    check_heads(fn, a->q, t, a->q_ld, a->q_hd, a->q_heads, d, true, "q");
+    check_heads(fn, a->k, t, a->k_ld, a->k_hd, kv->heads, d, true, "k");
+    check_heads(fn, a->v, t, a->v_ld, a->v_hd, kv->heads, d, true, "v");
+    check_heads(fn, a->out, t, a->out_ld, a->out_hd, a->q_heads, d, false, "out");
+    if (a->q_norm)
+        check_dev_ptr(fn, a->q_norm, "q_norm");
+    if (a->k_norm)
+        check_dev_ptr(fn, a->k_norm, "k_norm");
+    if (a->rot)
+        check_words(fn, a->freq, 8, "freq");
+    const span q = heads_span(a->q, t, a->q_ld, a->q_hd, a->q_heads, d), k = heads_span(a->k, t, a->k_ld, a->k_hd, kv->heads, d),
+               v = heads_span(a->v, t, a->v_ld, a->v_hd, kv->heads, d), out = heads_span(a->out, t, a->out_ld, a->out_hd, a->q_heads, d),
+               ck = kv_span(kv, kv->k), cv = kv_span(kv, kv->v);
+    const span in[] = {words_span(a->q_norm, 4 * (size_t)d), words_span(a->k_norm, 4 * (size_t)d), words_span(a->rot ? a->freq : nullptr, 4 * (size_t)a->rot),
+                       words_span(s->start, 4 * (size_t)(s->n + 1)), words_span(s->past, 4 * (size_t)s->n),
+                       words_span(kv->table, 4 * (size_t)(s->n * kv->table_ld))};
+    const bool in_place = a->out == a->q && a->out_ld == a->q_ld && a->out_hd == a->q_hd;
+    check_apart(fn, "out", out, {in_place ? span{nullptr, 0} : q, k, v, ck, cv, in[0], in[1], in[2], in[3], in[4], in[5]});
+    check_apart(fn, "the cache's k", ck, {q, k, v, cv, in[0], in[1], in[2], in[3], in[4], in[5]});
+    check_apart(fn, "the cache's v", cv, {q, k, v, in[0], in[1], in[2], in[3], in[4], in[5]});
+    const on_gpu g(c);
+    q8_launch_rope((q8_stream_t)c->stream, *s, *kv, *a);
+    launched("the rotation");
+}
+
+void rt_attn_kv_dev(struct rt *R, const struct rt_seqs *s, const struct rt_kv *kv, const struct rt_attn *a)
+{
+    const char *fn = "rt_attn_kv_dev";
+    ctx *c = get(R, fn);
+    check_seqs(fn, s, true);
+    check_kv(fn, kv);
+    if (!a)
+        fail(fn, "needs its arguments (struct rt_attn)");
+    if (a->q_heads < 1 || a->q_heads > RT_HEADS_MAX || a->q_heads % kv->heads)
+        failf(fn, "needs 1 to %ld query heads, a multiple of the key-value heads", RT_HEADS_MAX);
+    const long t = s->t, d = kv->dim;
+    check_heads(fn, a->q, t, a->q_ld, a->q_hd, a->q_heads, d, true, "q");
+    if (a->gate)
+        check_heads(fn, a->gate, t, a->gate_ld, a->gate_hd, a->q_heads, d, true, "gate");
+    check_dev_ptr(fn, a->o, "o");
+    check_ld(fn, a->o_ld, a->q_heads * d, "o_ld");
+    check_apart(fn, "o", rows_span(a->o, t, a->o_ld, a->q_heads * d),
+                {heads_span(a->q, t, a->q_ld, a->q_hd, a->q_heads, d), heads_span(a->gate, t, a->gate_ld, a->gate_hd, a->q_heads, d), kv_span(kv, kv->k),
+                 kv_span(kv, kv->v), words_span(s->start, 4 * (size_t)(s->n + 1)), words_span(s->past, 4 * (size_t)s->n),
+                 words_span(kv->table, 4 * (size_t)(s->n * kv->table_ld))});
+    const on_gpu g(c);
+    q8_launch_attn((q8_stream_t)c->stream, *s, *kv, *a);
+    launched("the attention");
 }
 
 } /* extern "C" */
