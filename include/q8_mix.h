@@ -86,7 +86,7 @@ struct rt_kv {
     long type;        /* RT_F32, RT_F16 or RT_BF16 */
     long dim;         /* a head's size: a multiple of 32, 32 to 256 */
     long heads;       /* key-value heads */
-    long page, pages; /* positions a page (1 or more), pages in the cache */
+    long page, pages; /* positions a page (1 or more), pages in the cache: pages * heads * page < 2^31 */
     const int *table; /* device [n][table_ld]: entries that no position uses may be anything */
     long table_ld;    /* pages a sequence may have */
 };

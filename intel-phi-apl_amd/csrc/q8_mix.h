@@ -9,7 +9,9 @@ void q8_launch_conv(q8_stream_t s, const rt_seqs &b, const float *x, long x_ld, 
                     float *y, long y_ld);
 void q8_launch_rope(q8_stream_t s, const rt_seqs &b, const rt_kv &kv, const rt_rope &a);
 void q8_launch_delta(q8_stream_t s, const rt_seqs &b, const rt_delta &a);
-void q8_launch_attn(q8_stream_t s, const rt_seqs &b, const rt_kv &kv, const rt_attn &a);
+/* part: q8_attn_part_floats floats of workspace (none: may be NULL) */
+long q8_attn_part_floats(const rt_seqs &b, const rt_kv &kv, const rt_attn &a);
+void q8_launch_attn(q8_stream_t s, const rt_seqs &b, const rt_kv &kv, const rt_attn &a, float *part);
 
 #if defined(__HIPCC__)
 

@@ -125,6 +125,9 @@ struct ctx {
     void *ximg = nullptr;
     /* the device address of `scratch` on this runtime's GPU (rt_gemm_dev_noalloc's partials) */
     float *noalloc_part = nullptr;
+    /* the operators between the products: the attention's partial results */
+    float *mix = nullptr;
+    size_t mix_cap = 0;
     /* the greedy next token's candidates */
     void *amax = nullptr;
     size_t amax_cap = 0;
@@ -311,6 +314,19 @@ float *reserve_rpart(ctx *c, size_t need)
         c->rpart_cap = need;
     }
     return c->rpart;
+}
+
+/* the workspace of the operators between the products, at least n floats */
+float *reserve_mix(ctx *c, size_t n)
+{
+    if (n > c->mix_cap) {
+        no_capture(c, "the workspace of the operators between the products");
+        if (c->mix)
+            c->retired.push_back(c->mix);
+        HIPCHECK(hipMalloc((void **)&c->mix, n * sizeof(float)));
+        c->mix_cap = n;
+    }
+    return c->mix;
 }
 
 void reserve_gemm(ctx *c, long rows, long cols, long t)
@@ -890,6 +906,8 @@ void rt_fini(struct rt *R)
         HIPCHECK(hipFree(c->epi));
     if (c->rpart)
         HIPCHECK(hipFree(c->rpart));
+    if (c->mix)
+        HIPCHECK(hipFree(c->mix));
     if (c->ximg)
         HIPCHECK(hipFree(c->ximg));
     for (void *p : c->retired)
@@ -1726,8 +1744,8 @@ void check_kv(const char *fn, const struct rt_kv *kv)
         failf(fn, "needs 1 to %ld key-value heads", RT_HEADS_MAX);
     if (kv->page < 1 || kv->page > 1L << 30 || kv->pages < 1 || kv->pages >= 1L << 31 || kv->table_ld < 1 || kv->table_ld >= 1L << 31)
         fail(fn, "needs pages of 1 to 2^30 positions, 1 to 2^31 - 1 of them, and as many a sequence");
-    if ((double)kv->pages * (double)kv->page * (double)(kv->heads * kv->dim) > 1e15)
-        fail(fn, "the cache is larger than any memory");
+    if ((double)kv->pages * (double)kv->page * (double)kv->heads >= 2147483648.0)
+        fail(fn, "needs fewer than 2^31 rows (pages x heads x page) in the cache");
     check_dev_ptr(fn, kv->k, "the cache's k");
     check_dev_ptr(fn, kv->v, "the cache's v");
     check_words(fn, kv->table, 4, "the page table");
@@ -1897,7 +1915,7 @@ void rt_attn_kv_dev(struct rt *R, const struct rt_seqs *s, const struct rt_kv *k
                  kv_span(kv, kv->v), words_span(s->start, 4 * (size_t)(s->n + 1)), words_span(s->past, 4 * (size_t)s->n),
                  words_span(kv->table, 4 * (size_t)(s->n * kv->table_ld))});
     const on_gpu g(c);
-    q8_launch_attn((q8_stream_t)c->stream, *s, *kv, *a);
+    q8_launch_attn((q8_stream_t)c->stream, *s, *kv, *a, reserve_mix(c, (size_t)q8_attn_part_floats(*s, *kv, *a)));
     launched("the attention");
 }
 

@@ -88,7 +88,7 @@ DRIVER = textwrap.dedent(
         *[("head's size", lambda f=f, k=k: f(cache=kv(dim=k))) for f in (rope, attn) for k in (16, 48, 288)],
         *[("key-value heads", lambda f=f: f(cache=kv(heads=0))) for f in (rope, attn)],
         *[("needs pages", lambda f=f, k=k: f(cache=kv(**k))) for f in (rope, attn) for k in (dict(page=0), dict(pages=0), dict(table_ld=0), dict(pages=1 << 31))],
-        *[("larger than any memory", lambda f=f: f(cache=kv(pages=(1 << 31) - 1, page=1 << 30))) for f in (rope, attn)],
+        *[("fewer than 2^31 rows", lambda f=f: f(cache=kv(pages=(1 << 31) - 1, page=1 << 30))) for f in (rope, attn)],
         *[("the page table", lambda f=f: f(cache=kv(table=None))) for f in (rope, attn)],
         *[("cache's v must", lambda f=f: f(cache=kv(v=at(70) + 2))) for f in (rope, attn)],
         ("query heads", lambda: rope(q_heads=0)),
