@@ -4,9 +4,11 @@
 namespace {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 
 constexpr int WAVES = 4;
-constexpr int LEAST = WAVES; /* tiles a chunk at least: one a wave */
+constexpr int LEAST = 2 * WAVES; /* position tiles a chunk at least: two of 16 a wave; every chunk is an even number of them */
 
 /* p / page for p < 2^31: (p * mul) >> shift with shift = 31 + ceil(log2 page), mul = ceil(2^shift / page): exact, as
  * the excess mul * page - 2^shift is below page <= 2^(shift - 31) */
@@ -19,105 +21,90 @@ struct paging {
  * sequence; a sequence's positions, in tiles of 16, are cut into chunks of one size for the whole batch. */
 struct plan {
     paging pg;
-    int group;     /* query heads a key-value head */
-    long cap;      /* positions that the table reaches */
-    long target;   /* chunks (a key-value head) to spread all tiles over; 0: one a row tile */
-    long slots;    /* partial results a key-value head */
-    float *part;   /* [heads][slots][16][dim], then [heads][slots][16][2]: maximum and sum */
-    float qscale;  /* scale * log2 e: scores are in powers of two */
+    int group;   /* query heads a key-value head */
+    int cap;     /* positions that the table reaches */
+    int target;  /* chunks (a key-value head) to spread all tiles over; 0: one a row tile */
+    int slots;   /* partial results a key-value head */
+    float qscale; /* scale * log2 e: scores are in powers of two */
+    float *part; /* [heads][slots][16][dim], then [heads][slots][16][2]: maximum and sum */
 };
 
 struct seq_plan {
-    long first, n;      /* its rows of the token-major arrays */
-    long past, tiles;   /* position tiles of all it sees, within the table */
-    long rows, chunks;  /* row tiles, and chunks of each */
+    int first, n;     /* its rows of the token-major arrays */
+    int past, tiles;  /* position tiles of all it sees, within the table */
+    int rows, chunks; /* row tiles, and chunks of each */
 };
 
-__device__ __forceinline__ seq_plan plan_of(const rt_seqs &b, const plan &p, long s, long chunk)
+__device__ __forceinline__ seq_plan plan_of(const rt_seqs &b, const plan &p, int s, int chunk)
 {
     seq_plan q;
-    long last;
-    q8_rows_of(b, s, q.first, last);
-    q.n = last - q.first;
+    long first, last;
+    q8_rows_of(b, s, first, last);
+    q.first = (int)first;
+    q.n = (int)(last - first);
     q.past = b.past[s];
-    const long len = q.past + q.n;
-    q.tiles = len <= 0 ? 0 : ((len < p.cap ? len : p.cap) + 15) / 16;
-    q.rows = (q.n * p.group + 15) / 16;
-    q.chunks = chunk > 0 && q.tiles > chunk ? (q.tiles + chunk - 1) / chunk : 1;
+    const long len = (long)q.past + q.n;
+    q.tiles = len <= 0 ? 0 : (int)((len < p.cap ? len : p.cap) + 15) / 16;
+    q.rows = (int)(((uint32_t)q.n * (uint32_t)p.group + 15) / 16);
+    q.chunks = chunk > 0 && q.tiles > chunk ? (int)((uint32_t)(q.tiles + chunk - 1) / (uint32_t)chunk) : 1;
     return q;
 }
 
-__device__ __forceinline__ long wave_sum(long v)
-{
-    for (int o = 32; o >= 1; o >>= 1)
-        v += __shfl_xor(v, o, 64);
-    return v;
-}
+__device__ __forceinline__ int first_lane(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 /* tiles a chunk: every sequence's tiles over the target, the same for each of them, so that workgroups
  * read the same amounts whatever the lengths (a share of each sequence's own length left the short ones'
  * workgroups waiting for the longest) */
-__device__ __forceinline__ long chunk_of(const rt_seqs &b, const plan &p)
+__device__ __forceinline__ int chunk_of(const rt_seqs &b, const plan &p)
 {
     if (p.target <= 0)
         return 0;
-    long all = 0;
-    for (long s = threadIdx.x & 63; s < b.n; s += 64) {
-        const seq_plan q = plan_of(b, p, s, 0);
-        all += q.rows * q.tiles;
+    double all = 0.0; /* whole numbers */
+    if (b.n == 1) {
+        const seq_plan q = plan_of(b, p, 0, 0);
+        all = (double)q.rows * q.tiles;
+    } else {
+        for (int s = threadIdx.x & 63; s < (int)b.n; s += 64) {
+            const seq_plan q = plan_of(b, p, s, 0);
+            all += (double)q.rows * q.tiles;
+        }
+        for (int o = 32; o >= 1; o >>= 1)
+            all += __shfl_xor(all, o, 64);
     }
-    if (b.n > 1)
-        all = wave_sum(all);
-    else
-        all = __shfl(all, 0, 64);
-    const long c = (all + p.target - 1) / p.target;
-    return c < LEAST ? LEAST : c;
+    const double c = all / p.target + 1.0; /* as far as 2^27 tiles: one a row tile there */
+    return c < LEAST ? LEAST : c < 1e8 ? first_lane((int)c + 1) & ~1 : 0;
 }
 
 /* The sequence whose row tiles' chunks hold number i of all, -1 behind the last; before = the chunks of
  * those before it */
-__device__ __forceinline__ long sequence_of_chunk(const rt_seqs &b, const plan &p, long chunk, long i, long &before)
+__device__ __forceinline__ int sequence_of_chunk(const rt_seqs &b, const plan &p, int chunk, int i, int &before)
 {
-    const int lane = threadIdx.x & 63;
     before = 0;
-    for (long s0 = 0; s0 < b.n; s0 += 64) {
-        long c = 0;
-        if (s0 + lane < b.n) {
+    if (b.n == 1) {
+        const seq_plan q = plan_of(b, p, 0, chunk);
+        return i < q.rows * q.chunks ? 0 : -1;
+    }
+    const int lane = threadIdx.x & 63;
+    for (int s0 = 0; s0 < (int)b.n; s0 += 64) {
+        int c = 0;
+        if (s0 + lane < (int)b.n) {
             const seq_plan q = plan_of(b, p, s0 + lane, chunk);
             c = q.rows * q.chunks;
         }
-        long upto = c;
-        if (b.n > 1)
-            for (int o = 1; o < 64; o <<= 1) {
-                const long u = __shfl_up(upto, o, 64);
-                upto += lane >= o ? u : 0;
-            }
+        int upto = c;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(upto, o, 64);
+            upto += lane >= o ? u : 0;
+        }
         const unsigned long long m = __ballot(i < before + upto);
         if (m) {
             const int at = __ffsll((long long)m) - 1;
-            before += __shfl(upto - c, at, 64);
+            before += __builtin_amdgcn_readlane(upto - c, at);
             return s0 + at;
         }
-        before += __shfl(upto, 63, 64);
+        before += __builtin_amdgcn_readlane(upto, 63);
     }
     return -1;
-}
-
-template <int TYPE>
-struct elem {
-    static constexpr int bytes = TYPE == RT_F32 ? 4 : 2;
-};
-
-/* element e of 32-bit words w, in F32 (exact) */
-template <int TYPE>
-__device__ __forceinline__ float element(const uint32_t *w, int e)
-{
-    if constexpr (TYPE == RT_F32)
-        return __builtin_bit_cast(float, w[e]);
-    else if constexpr (TYPE == RT_F16)
-        return (float)__builtin_bit_cast(_Float16, (uint16_t)(w[e / 2] >> (16 * (e & 1))));
-    else
-        return __builtin_bit_cast(float, e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
 }
 
 template <int WORDS>
@@ -154,131 +141,233 @@ __device__ __forceinline__ void store_row(const rt_attn &a, long dim, long token
     *(float4 *)(a.o + token * a.o_ld + head * dim + at) = v;
 }
 
-/* A workgroup takes a chunk of positions for a row tile; its waves take the chunk's position tiles in
- * turn, and join at the end through LDS.
+/* A workgroup takes a chunk of positions for a row tile (16 query rows); its waves take the chunk's position tiles
+ * in turn, and join at the end through LDS.
  *
- * Per tile of 16 positions a wave computes S^T = K Q^T (v_mfma_f32_16x16x4_f32: K's rows are the
- * positions), so that lane 16 g + c has the scores of query row c at positions 4 g .. 4 g + 3, which is how the
- * next product wants its second operand: O^T += V^T P^T takes them as they are, position 4 g + r in its step
- * r. So nothing passes through LDS, and the cache's rows go from memory to the matrix cores in the registers that
- * they were loaded into: lane 16 g + c loads K's row c, 16 bytes of each 64 from byte 16 g on, and V's rows 4 g ..
- * 4 g + 3, elements c * VEC .. of each 16 * VEC. The products are F32 whatever the cache's type.
+ * A wave computes S^T = K Q^T, K's rows being the positions, so that lane 16 g + c has the scores of query
+ * row c at positions 4 g .. 4 g + 3 of 16. The next product, O^T += V^T P^T, takes them as its second operand as
+ * they lie, if its first has V's rows in the same order. So the cache's rows go from memory to the matrix cores in
+ * the registers that they were loaded into: lane 16 g + c loads K's row c, 16 bytes of each 64 from byte 16 g on,
+ * and V's rows 4 g .. 4 g + 3, VEC elements of each 16 * VEC from c * VEC on. The output's element (i * 16 + 4 g + r)
+ * * VEC + e of query row c is acc[i * VEC + e][r].
  *
  * The softmax's maximum is a running one that is raised only when a score passes it by more than SLACK (a
  * power of two: the exponentials stay below 2^SLACK): then the sums and outputs are scaled, which a tile
  * rarely needs after the first. Each lane sums its own positions; the four lanes of a row add up at the end. */
 constexpr float SLACK = 8.0f;
 
-template <int D, int TYPE>
-__global__ __launch_bounds__(64 * WAVES, D *elem<TYPE>::bytes > 512 ? 1 : 2) void attn_tile_k(rt_seqs b, rt_kv kv, rt_attn a, plan p)
-{
-    constexpr int SIZE = elem<TYPE>::bytes, E = 16 / SIZE, NK = D / (4 * E);
-    constexpr int VE = D / 16, VEC = VE % E == 0 ? E : VE % (E / 2) == 0 ? E / 2 : 2, NV = VE / VEC, VW = VEC * SIZE / 4;
-    constexpr int LD = D + 4; /* rows of the waves' outputs in LDS, off each other's banks */
-    __shared__ __align__(16) float so[WAVES][16][LD];
-    __shared__ float sm[WAVES][16], sl[WAVES][16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
-    const long kh = blockIdx.y, chunk = chunk_of(b, p);
-    const long head_rows = kh * kv.page, page_rows = kv.heads * kv.page;
-    /* with starts that overlap there may be more chunks than slots: those are left out */
-    for (long number = blockIdx.x; p.target == 0 || number < p.slots; number += gridDim.x) {
-        long before;
-        const long s = sequence_of_chunk(b, p, chunk, number, before);
-        if (s < 0)
-            return;
-        const seq_plan q = plan_of(b, p, s, chunk);
-        const long z = (number - before) / q.chunks, part = (number - before) % q.chunks;
-        const int32_t *table = kv.table + s * kv.table_ld;
-        /* this lane's query row: token j of the sequence, head h; it sees positions up to lim */
-        const long row = z * 16 + c, j = row / p.group, h = kh * p.group + row % p.group;
-        const bool live = j < q.n;
-        const long seen = q.past + j;
-        const int lim = !live || seen < 0 ? -1 : (int)(seen < p.cap ? seen : p.cap - 1);
-        const long j0 = z * 16 / p.group, j1 = (z * 16 + 15) / p.group < q.n ? (z * 16 + 15) / p.group : q.n - 1; /* the row tile's tokens */
-        const long end = q.past + j1 < p.cap ? q.past + j1 : p.cap - 1;
-        const int last = (int)(end < -1 ? -1 : end); /* the last position that any row sees */
-        const int least = (int)(q.past + j0 < -1 ? -1 : q.past + j0 > last ? last : q.past + j0); /* every row sees up to here */
-        const long t0 = part * chunk, t1 = last < 0 ? 0 : last / 16 + 1;
-        const int stop = (int)(q.chunks > 1 && t0 + chunk < t1 ? t0 + chunk : t1);
+/* A workgroup's share: chunk `part` of sequence s's row tile z, and what its lane has of it */
+struct share {
+    seq_plan q;
+    const int32_t *table;
+    int z, j0, j1;   /* the row tile, and its tokens */
+    int j, h;        /* the lane's query row: token and head */
+    bool live;       /* there is one */
+    int lim;         /* the last position that the lane's row sees, -1 none */
+    int last, least; /* the last that any row of the tile sees, and the last that all do */
+    int t0, t1;      /* the chunk's position tiles, 16 each */
+};
 
-        float qv[NK * E];
+__device__ __forceinline__ bool share_of(const rt_seqs &b, const rt_kv &kv, const plan &p, int chunk, int number, share &u)
+{
+    int before;
+    const int s = first_lane(sequence_of_chunk(b, p, chunk, number, before));
+    if (s < 0)
+        return false;
+    u.q = plan_of(b, p, s, chunk);
+    const seq_plan &q = u.q;
+    number -= before;
+    u.z = first_lane((int)((uint32_t)number / (uint32_t)q.chunks));
+    const int part = number - u.z * q.chunks, row = u.z * 16 + (int)(threadIdx.x & 15);
+    u.table = kv.table + s * kv.table_ld;
+    u.j = (int)((uint32_t)row / (uint32_t)p.group);
+    u.h = (int)blockIdx.y * p.group + (row - u.j * p.group);
+    u.live = u.j < q.n;
+    const auto sees = [&](int j) { /* the last position that token j sees, within the table */
+        const long pos = (long)q.past + j;
+        return pos < 0 ? -1 : pos < p.cap ? (int)pos : p.cap - 1;
+    };
+    u.lim = u.live ? sees(u.j) : -1;
+    u.j0 = first_lane((int)((uint32_t)(u.z * 16) / (uint32_t)p.group));
+    u.j1 = first_lane((int)((uint32_t)(u.z * 16 + 15) / (uint32_t)p.group));
+    u.j1 = u.j1 < q.n ? u.j1 : q.n - 1;
+    u.last = sees(u.j1);
+    u.least = sees(u.j0);
+    u.t0 = part * chunk;
+    u.t1 = u.last < 0 ? 0 : u.last / 16 + 1;
+    if (q.chunks > 1 && u.t0 + chunk < u.t1)
+        u.t1 = u.t0 + chunk;
+    return true;
+}
+
+/* A position's page from the table, and its row in the cache's k and v counted from the head's first page
+ * (-1: it has none) */
+__device__ __forceinline__ int entry_of(const rt_kv &kv, const plan &p, const int32_t *table, int pos)
+{
+    const uint32_t pg = (uint32_t)(((uint64_t)(uint32_t)pos * p.pg.mul) >> p.pg.shift);
+    return (long)pg < kv.table_ld ? table[pg] : -1;
+}
+__device__ __forceinline__ int row_of(const rt_kv &kv, const plan &p, int pos, int entry)
+{
+    const uint32_t pg = (uint32_t)(((uint64_t)(uint32_t)pos * p.pg.mul) >> p.pg.shift);
+    return entry >= 0 && entry < kv.pages ? entry * (int)(kv.heads * kv.page) + (pos - (int)(pg * (uint32_t)kv.page)) : -1;
+}
+__device__ __forceinline__ const char *address(const void *cache, int row, uint32_t head_rows, int bytes)
+{
+    return (const char *)cache + (uint64_t)((uint32_t)(row < 0 ? 0 : row) + head_rows) * (uint32_t)bytes;
+}
+
+/* The running maximum raised where a lane's largest score passes it by SLACK, and the reference that
+ * the exponents are taken from */
+template <int VE>
+__device__ __forceinline__ float reference(float top, float &m, float &l, v4f (&acc)[VE])
+{
+    if (__ballot(top > m + SLACK)) {
+        const float raised = fmaxf(m, group_max(top)), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - raised);
+        m = raised;
+        l *= f;
 #pragma unroll
-        for (int i = 0; i < NK; i++)
+        for (int i = 0; i < VE; i++)
+            acc[i] *= f;
+    }
+    return m == -INFINITY ? 0.0f : m;
+}
+
+/* The waves' results, scaled to the largest of their maxima and added in the waves' order: the output, or
+ * the chunk's part of it */
+template <int D>
+constexpr int joint_bytes() { return WAVES * 16 * (D + 4 + 2) * 4; }
+
+template <int D, int VEC>
+__device__ __forceinline__ void finish(char *lds, const rt_kv &kv, const rt_attn &a, const plan &p, const share &u, int number, float m, float l, const v4f (&acc)[D / 16])
+{
+    constexpr int LD = D + 4; /* rows off each other's banks */
+    float(*so)[16][LD] = (float(*)[16][LD])lds;
+    float(*sm)[16] = (float(*)[16])(lds + WAVES * 16 * LD * 4), (*sl)[16] = sm + WAVES;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    const int kh = (int)blockIdx.y;
+    l = group_sum(l);
+    __syncthreads();
+    if (g == 0)
+        sm[wave][c] = m, sl[wave][c] = l;
+    __syncthreads();
+    float top = sm[0][c];
 #pragma unroll
-            for (int e = 0; e < E; e += 4) {
-                float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-                if (live)
-                    v = *(const float4 *)(a.q + (q.first + j) * a.q_ld + h * a.q_hd + (i * 4 + g) * E + e);
-                qv[i * E + e] = v.x * p.qscale, qv[i * E + e + 1] = v.y * p.qscale, qv[i * E + e + 2] = v.z * p.qscale, qv[i * E + e + 3] = v.w * p.qscale;
-            }
+    for (int w = 1; w < WAVES; w++)
+        top = fmaxf(top, sm[w][c]);
+    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+    const int left = u.q.n * p.group - u.z * 16, rows = left < 16 ? left : 16;
+    if (c < rows)
+#pragma unroll
+        for (int i = 0; i < D / 16 / VEC; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int e = 0; e < VEC; e += 2)
+                    *(float2 *)&so[wave][c][(i * 16 + 4 * g + r) * VEC + e] = float2{acc[i * VEC + e][r] * f, acc[i * VEC + e + 1][r] * f};
+    __syncthreads();
+    for (int i = tid; i < rows * (D / 4); i += 64 * WAVES) {
+        const int r = i / (D / 4), d = 4 * (i % (D / 4));
+        float t = sm[0][r], sum = 0.0f;
+        for (int w = 1; w < WAVES; w++)
+            t = fmaxf(t, sm[w][r]);
+        float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int w = 0; w < WAVES; w++) {
+            const float4 x = *(const float4 *)&so[w][r][d];
+            v = float4{v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w};
+            sum += sl[w][r] * (sm[w][r] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(sm[w][r] - t));
+        }
+        const int jr = (int)((uint32_t)(u.z * 16 + r) / (uint32_t)p.group), hr = kh * p.group + (u.z * 16 + r - jr * p.group);
+        const long pos = (long)u.q.past + jr;
+        if (pos >= p.cap)
+            sum = NAN; /* a position that the table does not reach */
+        if (u.q.chunks == 1) {
+            store_row(a, D, u.q.first + jr, hr, d, v, sum, pos < 0);
+        } else {
+            const long slot = (long)kh * p.slots + number;
+            *(float4 *)(p.part + (slot * 16 + r) * D + d) = v;
+            if (d == 0)
+                *(float2 *)(p.part + kv.heads * p.slots * 16 * D + (slot * 16 + r) * 2) = float2{t, sum};
+        }
+    }
+    __syncthreads();
+}
+
+/* The most elements (at most full) that a lane's VE elements of a V row divide into */
+constexpr int pieces(int ve, int full) { return ve % full == 0 ? full : ve % (full / 2) == 0 ? full / 2 : 2; }
+
+/* An F32 cache, 16 positions a tile, on v_mfma_f32_16x16x4_f32: position 4 g + r in the second product's step r. */
+template <int D>
+__global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seqs b, rt_kv kv, rt_attn a, plan p)
+{
+    constexpr int NK = D / 16, VE = D / 16, VEC = pieces(VE, 4), NV = VE / VEC;
+    __shared__ __align__(16) char lds[joint_bytes<D>()];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    const int chunk = chunk_of(b, p);
+    const uint32_t head_rows = (uint32_t)(blockIdx.y * kv.page);
+    /* with starts that overlap there may be more chunks than slots: those are left out */
+    for (int number = (int)blockIdx.x; p.target == 0 || number < p.slots; number += (int)gridDim.x) {
+        share u;
+        if (!share_of(b, kv, p, chunk, number, u))
+            return;
+        float qv[NK][4];
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+            float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (u.live)
+                v = *(const float4 *)(a.q + (long)(u.q.first + u.j) * a.q_ld + u.h * a.q_hd + (i * 4 + g) * 4);
+            qv[i][0] = v.x * p.qscale, qv[i][1] = v.y * p.qscale, qv[i][2] = v.z * p.qscale, qv[i][3] = v.w * p.qscale;
+        }
         v4f acc[VE];
 #pragma unroll
         for (int i = 0; i < VE; i++)
             acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         float m = -INFINITY, l = 0.0f;
-
-        /* a position's row in the cache's k and v, counted from the head's first page, or -1 where there is
-         * none; entry: its page from the table, loaded a tile ahead */
-        const auto entry_of = [&](int pos) {
-            const uint32_t pg = (uint32_t)(((uint64_t)(uint32_t)pos * p.pg.mul) >> p.pg.shift);
-            return (long)pg < kv.table_ld ? table[pg] : -1;
-        };
-        const auto row_of = [&](int pos, int entry) {
-            const uint32_t pg = (uint32_t)(((uint64_t)(uint32_t)pos * p.pg.mul) >> p.pg.shift);
-            return entry >= 0 && entry < kv.pages ? (int)(entry * page_rows + (pos - (long)pg * kv.page)) : -1;
-        };
-        const auto at = [&](const void *cache, int r) { return (const char *)cache + (size_t)((r < 0 ? 0 : r) + head_rows) * (D * SIZE); };
-        const auto here = [&](int tile) { return tile * 16 + c < last ? tile * 16 + c : last; };
-
-        uint32_t kw[NK][4], vw[4][NV][VW];
-        int tile = (int)t0 + wave, row_now = -1, entry = -1;
-        if (tile < stop) {
-            row_now = row_of(here(tile), entry_of(here(tile)));
-            entry = entry_of(here(tile + WAVES));
+        const auto here = [&](int tile) { return tile * 16 + c < u.last ? tile * 16 + c : u.last; };
+        const auto load_k = [&](uint32_t (*kw)[4], int row) {
+            const char *at = address(kv.k, row, head_rows, D * 4) + g * 16;
 #pragma unroll
             for (int i = 0; i < NK; i++)
-                load_words<4>(kw[i], at(kv.k, row_now) + (i * 4 + g) * 16);
+                load_words<4>(kw[i], at + i * 64);
+        };
+        uint32_t kw[NK][4], vw[4][NV][VEC];
+        int tile = (int)u.t0 + wave, row_now = -1, entry = -1;
+        const int stop = (int)u.t1;
+        if (tile < stop) {
+            row_now = row_of(kv, p, here(tile), entry_of(kv, p, u.table, here(tile)));
+            entry = entry_of(kv, p, u.table, here(tile + WAVES));
+            load_k(kw, row_now);
         }
         for (; tile < stop; tile += WAVES) {
             int rows[4];
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 rows[r] = __shfl(row_now, 4 * g + r, 64);
+                const char *at = address(kv.v, rows[r], head_rows, D * 4) + c * VEC * 4;
 #pragma unroll
                 for (int i = 0; i < NV; i++)
-                    load_words<VW>(vw[r][i], at(kv.v, rows[r]) + (i * 16 + c) * VEC * SIZE);
+                    load_words<VEC>(vw[r][i], at + i * 16 * VEC * 4);
             }
-            v4f s2[2] = {v4f{0.0f, 0.0f, 0.0f, 0.0f}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
+            v4f s[2] = {v4f{0.0f, 0.0f, 0.0f, 0.0f}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
             for (int i = 0; i < NK; i++)
 #pragma unroll
-                for (int e = 0; e < E; e++)
-                    s2[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(element<TYPE>(kw[i], e), qv[i * E + e], s2[e & 1], 0, 0, 0);
+                for (int e = 0; e < 4; e++)
+                    s[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kw[i][e]), qv[i][e], s[e & 1], 0, 0, 0);
             if (tile + WAVES < stop) {
-                row_now = row_of(here(tile + WAVES), entry);
-                entry = entry_of(here(tile + 2 * WAVES));
-#pragma unroll
-                for (int i = 0; i < NK; i++)
-                    load_words<4>(kw[i], at(kv.k, row_now) + (i * 4 + g) * 16);
+                row_now = row_of(kv, p, here(tile + WAVES), entry);
+                entry = entry_of(kv, p, u.table, here(tile + 2 * WAVES));
+                load_k(kw, row_now);
             }
             float x[4];
-            const bool whole = tile * 16 + 15 <= least; /* every row sees every position of the tile */
+            const bool whole = tile * 16 + 15 <= u.least; /* every row sees every position of the tile */
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                x[r] = rows[r] < 0 ? NAN : s2[0][r] + s2[1][r];
-                if (!whole && tile * 16 + 4 * g + r > lim)
+                x[r] = rows[r] < 0 ? NAN : s[0][r] + s[1][r];
+                if (!whole && tile * 16 + 4 * g + r > u.lim)
                     x[r] = -INFINITY;
             }
-            const float top = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-            if (__ballot(top > m + SLACK)) {
-                const float raised = fmaxf(m, group_max(top)), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - raised);
-                m = raised;
-                l *= f;
-#pragma unroll
-                for (int i = 0; i < VE; i++)
-                    acc[i] *= f;
-            }
-            const float ref = m == -INFINITY ? 0.0f : m;
+            const float ref = reference(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), m, l, acc);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 x[r] = __builtin_amdgcn_exp2f(x[r] - ref);
@@ -291,99 +380,339 @@ __global__ __launch_bounds__(64 * WAVES, D *elem<TYPE>::bytes > 512 ? 1 : 2) voi
                     for (int i = 0; i < NV; i++)
 #pragma unroll
                         for (int e = 0; e < VEC; e++)
-                            acc[i * VEC + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(element<TYPE>(vw[r][i], e), x[r], acc[i * VEC + e], 0, 0, 0);
+                            acc[i * VEC + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vw[r][i][e]), x[r], acc[i * VEC + e], 0, 0, 0);
             } else {
                 /* positions that some of the rows do not see: 0 times an infinite or NaN value would be NaN,
                  * so each token's rows are computed apart, without the values behind it */
-                for (long jj = j0; jj <= j1; jj++) {
-                    const long upto = q.past + jj;
+                for (int jj = u.j0; jj <= u.j1; jj++) {
+                    const long upto = (long)u.q.past + jj < u.last ? (long)u.q.past + jj : u.last;
 #pragma unroll
                     for (int i = 0; i < NV; i++)
 #pragma unroll
                         for (int e = 0; e < VEC; e++) {
                             v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                            for (int r = 0; r < 4; r++) {
-                                const bool sees = tile * 16 + 4 * g + r <= upto && tile * 16 + 4 * g + r <= last;
-                                o = __builtin_amdgcn_mfma_f32_16x16x4f32(sees ? element<TYPE>(vw[r][i], e) : 0.0f, x[r], o, 0, 0, 0);
-                            }
-                            if (j == jj)
+                            for (int r = 0; r < 4; r++)
+                                o = __builtin_amdgcn_mfma_f32_16x16x4f32(tile * 16 + 4 * g + r <= upto ? __builtin_bit_cast(float, vw[r][i][e]) : 0.0f, x[r], o, 0, 0, 0);
+                            if (u.j == jj)
                                 acc[i * VEC + e] += o;
                         }
                 }
             }
         }
-
-        /* the waves' results, scaled to the largest of their maxima, added in the waves' order */
-        l = group_sum(l);
-        if (g == 0)
-            sm[wave][c] = m, sl[wave][c] = l;
-        __syncthreads();
-        float top = sm[0][c];
-#pragma unroll
-        for (int w = 1; w < WAVES; w++)
-            top = fmaxf(top, sm[w][c]);
-        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-#pragma unroll
-        for (int i = 0; i < NV; i++)
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-#pragma unroll
-                for (int e = 0; e < VEC; e += 2)
-                    *(float2 *)&so[wave][c][(i * 16 + 4 * g + r) * VEC + e] = float2{acc[i * VEC + e][r] * f, acc[i * VEC + e + 1][r] * f};
-        __syncthreads();
-        const long left = q.n * p.group - z * 16;
-        const int rows_here = (int)(left < 16 ? left : 16);
-        for (int i = tid; i < rows_here * (D / 4); i += 64 * WAVES) {
-            const int r = i / (D / 4), d = 4 * (i % (D / 4));
-            float t = sm[0][r], sum = 0.0f;
-            for (int w = 1; w < WAVES; w++)
-                t = fmaxf(t, sm[w][r]);
-            float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-            for (int w = 0; w < WAVES; w++) {
-                const float4 u = *(const float4 *)&so[w][r][d];
-                v = float4{v.x + u.x, v.y + u.y, v.z + u.z, v.w + u.w};
-                sum += sl[w][r] * (sm[w][r] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(sm[w][r] - t));
-            }
-            const long jr = (z * 16 + r) / p.group, hr = kh * p.group + (z * 16 + r) % p.group, pos = q.past + jr;
-            if (pos >= p.cap)
-                sum = NAN; /* a position that the table does not reach */
-            if (q.chunks == 1) {
-                store_row(a, D, q.first + jr, hr, d, v, sum, pos < 0);
-            } else {
-                const long slot = kh * p.slots + number;
-                *(float4 *)(p.part + (slot * 16 + r) * D + d) = v;
-                if (d == 0)
-                    *(float2 *)(p.part + kv.heads * p.slots * 16 * D + (slot * 16 + r) * 2) = float2{t, sum};
-            }
-        }
-        __syncthreads();
+        finish<D, VEC>(lds, kv, a, p, u, number, m, l, acc);
     }
 }
 
-/* A query row's chunks joined: each scaled to the largest maximum, added wave by wave and then over the
- * waves, in one order. */
-__global__ __launch_bounds__(64 * WAVES) void attn_join_k(rt_seqs b, rt_kv kv, rt_attn a, plan p)
+/* A 16-bit cache, 32 positions a tile (two of 16, a and b), on v_mfma_f32_16x16x32: the cache's values are its
+ * operands as they are, and the F32 queries and weights are cut into LIMBS 16-bit values each, every one the
+ * rest of those before rounded to nearest: in F16 two of them are off by 2^-24 of the value, in BF16 three by 2^-27,
+ * so the products are as exact as F32 ones, at 2/16 and 3/16 of their time. F16 has few exponents: a row of queries
+ * is scaled by the power of two that brings its largest to 2^14 (and its scores back), and the weights are
+ * taken 2^(14 - SLACK) times as large, which the sum that divides them is, too: what then falls below F16's smallest
+ * steps is 2^-31 of the largest weight.
+ * The queries' limbs stay in LDS for the four waves. The second product's first operand is V transposed: of a
+ * lane's 8 rows, the same element of two at a time by v_perm_b32. */
+template <int TYPE>
+struct half_of;
+template <>
+struct half_of<RT_F16> {
+    static constexpr int LIMBS = 2;
+    static constexpr float LIFT = 14.0f - SLACK;
+    static constexpr uint32_t INF = 0x7c00;
+    static __device__ __forceinline__ uint16_t round(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
+    static __device__ __forceinline__ float back(uint16_t x) { return (float)__builtin_bit_cast(_Float16, x); }
+    static __device__ __forceinline__ v4f mfma(uint4 x, uint4 y, v4f z) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, y), z, 0, 0, 0); }
+};
+template <>
+struct half_of<RT_BF16> {
+    static constexpr int LIMBS = 3;
+    static constexpr float LIFT = 0.0f;
+    static constexpr uint32_t INF = 0x7f80;
+    static __device__ __forceinline__ uint16_t round(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
+    static __device__ __forceinline__ float back(uint16_t x) { return __builtin_bit_cast(float, (uint32_t)x << 16); }
+    static __device__ __forceinline__ v4f mfma(uint4 x, uint4 y, v4f z) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, x), __builtin_bit_cast(b8, y), z, 0, 0, 0); }
+};
+
+/* 8 F32 values as LIMBS operands */
+template <int TYPE>
+__device__ __forceinline__ void limbs_of(const float *x, uint4 *out)
 {
-    __shared__ __align__(16) float4 so[WAVES][64];
+    typedef half_of<TYPE> H;
+    float rest[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        rest[e] = x[e];
+#pragma unroll
+    for (int n = 0; n < H::LIMBS; n++) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            const uint16_t lo = H::round(rest[e]), hi = H::round(rest[e + 1]);
+            w[e / 2] = lo | (uint32_t)hi << 16;
+            rest[e] -= H::back(lo);
+            rest[e + 1] -= H::back(hi);
+        }
+        out[n] = uint4{w[0], w[1], w[2], w[3]};
+    }
+}
+
+/* An infinite key or value is one in its product with the first limb; the others would make NaN of it (they
+ * may be 0, or of the other sign), so where there may be one they get it as 0, and NaN, too */
+template <int TYPE>
+__device__ __forceinline__ uint4 finite_only(uint4 x)
+{
+    constexpr uint32_t TOP = half_of<TYPE>::INF;
+    const auto one = [](uint32_t w) { return ((w & TOP) == TOP ? 0u : w & 0xffffu) | ((w >> 16 & TOP) == TOP ? 0u : w & 0xffff0000u); };
+    return uint4{one(x.x), one(x.y), one(x.z), one(x.w)};
+}
+
+typedef unsigned short u2 __attribute__((ext_vector_type(2)));
+/* the larger magnitudes of two pairs of 16-bit values, as their bits: an infinity or NaN stays the largest */
+__device__ __forceinline__ uint32_t larger(uint32_t x, uint32_t y)
+{
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u2, x), __builtin_bit_cast(u2, y & 0x7fff7fffu)));
+}
+
+template <int D, int TYPE>
+__global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_half_k(rt_seqs b, rt_kv kv, rt_attn a, plan p)
+{
+    typedef half_of<TYPE> H;
+    constexpr int LIMBS = H::LIMBS, NK = D / 32, VE = D / 16, VEC = pieces(VE, 8), NV = VE / VEC, VW = VEC / 2;
+    __shared__ __align__(16) char lds[joint_bytes<D>() > NK * LIMBS * 1024 ? joint_bytes<D>() : NK * LIMBS * 1024];
+    uint4(*sq)[LIMBS][64] = (uint4(*)[LIMBS][64])lds; /* until the waves join */
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    const int chunk = chunk_of(b, p);
+    const uint32_t head_rows = (uint32_t)(blockIdx.y * kv.page);
+    for (int number = (int)blockIdx.x; p.target == 0 || number < p.slots; number += (int)gridDim.x) {
+        share u;
+        if (!share_of(b, kv, p, chunk, number, u))
+            return;
+        const int stop = (int)(u.t1 + 1) / 2; /* tiles of 32: a chunk is a whole number of them, but for the last */
+        int tile = (int)(u.t0 / 2) + wave, row_a = -1, row_b = -1, entry_a = -1, entry_b = -1;
+        const auto here = [&](int i) { return i < u.last ? i : u.last; };
+        uint4 ka[NK], kb[NK];
+        const auto load_k = [&](uint4 *kw, int row) {
+            const char *at = address(kv.k, row, head_rows, D * 2) + g * 16;
+#pragma unroll
+            for (int i = 0; i < NK; i++)
+                kw[i] = *(const uint4 *)(at + i * 64);
+        };
+        const auto rows_next = [&](int t) {
+            row_a = row_of(kv, p, here(t * 32 + c), entry_a);
+            row_b = row_of(kv, p, here(t * 32 + 16 + c), entry_b);
+            entry_a = entry_of(kv, p, u.table, here((t + WAVES) * 32 + c));
+            entry_b = entry_of(kv, p, u.table, here((t + WAVES) * 32 + 16 + c));
+        };
+        if (tile < stop) {
+            entry_a = entry_of(kv, p, u.table, here(tile * 32 + c));
+            entry_b = entry_of(kv, p, u.table, here(tile * 32 + 16 + c));
+            rows_next(tile);
+            load_k(ka, row_a);
+            load_k(kb, row_b);
+        }
+        /* the queries' limbs, the same for every wave: wave w makes those of columns 32 i, i = w, w + WAVES, ... */
+        const float *query = a.q + (u.live ? (long)(u.q.first + u.j) * a.q_ld + u.h * a.q_hd : 0) + g * 8;
+        float back = 1.0f;
+        int up = 0;
+        if (TYPE == RT_F16) {
+            float most = 0.0f;
+            for (int i = 0; i < NK; i++)
+#pragma unroll
+                for (int e = 0; e < 8; e += 4) {
+                    const float4 v = *(const float4 *)(query + i * 32 + e);
+                    most = fmaxf(fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
+                }
+            most = group_max(most * fabsf(p.qscale));
+            up = most > 0.0f && most < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(most) : 0;
+            up = up > 120 ? 120 : up < -120 ? -120 : up;
+            back = ldexpf(1.0f, -up);
+        }
+        for (int i = wave; i < NK; i += WAVES) {
+            float qv[8];
+            uint4 w[LIMBS];
+#pragma unroll
+            for (int e = 0; e < 8; e += 4) {
+                const float4 v = *(const float4 *)(query + i * 32 + e);
+                qv[e] = v.x, qv[e + 1] = v.y, qv[e + 2] = v.z, qv[e + 3] = v.w;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                qv[e] = u.live ? ldexpf(qv[e] * p.qscale, up) : 0.0f;
+            limbs_of<TYPE>(qv, w);
+#pragma unroll
+            for (int n = 0; n < LIMBS; n++)
+                sq[i][n][lane] = w[n];
+        }
+        __syncthreads();
+        v4f acc[VE];
+#pragma unroll
+        for (int i = 0; i < VE; i++)
+            acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        float m = -INFINITY, l = 0.0f;
+        for (; tile < stop; tile += WAVES) {
+            int rows[8]; /* rows 4 g + r of a, then of b */
+            uint32_t vw[NV][8][VW];
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                rows[r] = __shfl(r < 4 ? row_a : row_b, 4 * g + (r & 3), 64);
+                const char *at = address(kv.v, rows[r], head_rows, D * 2) + c * VEC * 2;
+#pragma unroll
+                for (int i = 0; i < NV; i++)
+                    load_words<VW>(vw[i][r], at + i * 16 * VEC * 2);
+            }
+            v4f sa = {0.0f, 0.0f, 0.0f, 0.0f}, sb = sa;
+            /* the scheduler is held to one step's limbs ahead: left free it reads them all before the first
+             * product, and spills */
+            __builtin_amdgcn_sched_barrier(0);
+            uint4 qw[2][LIMBS];
+#pragma unroll
+            for (int n = 0; n < LIMBS; n++)
+                qw[0][n] = sq[0][n][lane];
+#pragma unroll
+            for (int i = 0; i < NK; i++) {
+#pragma unroll
+                for (int n = 0; n < LIMBS && i + 1 < NK; n++)
+                    qw[(i + 1) & 1][n] = sq[i + 1][n][lane];
+#pragma unroll
+                for (int n = 0; n < LIMBS; n++) {
+                    sa = H::mfma(ka[i], qw[i & 1][n], sa);
+                    sb = H::mfma(kb[i], qw[i & 1][n], sb);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            const v4f odd = (sa + sb) * 0.0f; /* NaN: a score is infinite or NaN */
+            if (__ballot(odd[0] + odd[1] + odd[2] + odd[3] != 0.0f)) {
+                sa = v4f{0.0f, 0.0f, 0.0f, 0.0f}, sb = sa;
+#pragma unroll
+                for (int i = 0; i < NK; i++) {
+#pragma unroll
+                    for (int n = 0; n < LIMBS; n++) {
+                        const uint4 w = sq[i][n][lane];
+                        sa = H::mfma(n ? finite_only<TYPE>(ka[i]) : ka[i], w, sa);
+                        sb = H::mfma(n ? finite_only<TYPE>(kb[i]) : kb[i], w, sb);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if (tile + WAVES < stop) {
+                rows_next(tile + WAVES);
+                load_k(ka, row_a);
+                load_k(kb, row_b);
+            }
+            float x[8];
+            const bool whole = tile * 32 + 31 <= u.least; /* every row sees every position of the tile */
+            float top = -INFINITY;
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                x[r] = rows[r] < 0 ? NAN : back * (r < 4 ? sa[r & 3] : sb[r & 3]);
+                if (!whole && tile * 32 + (r & 4) * 4 + 4 * g + (r & 3) > u.lim)
+                    x[r] = -INFINITY;
+                top = fmaxf(top, x[r]);
+            }
+            const float ref = reference(top, m, l, acc) - H::LIFT;
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                x[r] = __builtin_amdgcn_exp2f(x[r] - ref);
+                l += x[r];
+            }
+            uint4 w[LIMBS];
+            limbs_of<TYPE>(x, w);
+            const auto turned = [](const uint32_t(&v)[8][VW], int e) {
+                const uint32_t pick = e & 1 ? 0x07060302u : 0x05040100u;
+                return uint4{__builtin_amdgcn_perm(v[1][e / 2], v[0][e / 2], pick), __builtin_amdgcn_perm(v[3][e / 2], v[2][e / 2], pick),
+                             __builtin_amdgcn_perm(v[5][e / 2], v[4][e / 2], pick), __builtin_amdgcn_perm(v[7][e / 2], v[6][e / 2], pick)};
+            };
+            /* values that the row tile's one token does not see are 0: 0 times an infinite or NaN one would be NaN */
+            const bool one = u.j0 == u.j1;
+            uint32_t size = 0;
+#pragma unroll
+            for (int r = 0; r < 8; r++) {
+                const bool hide = !whole && one && tile * 32 + (r & 4) * 4 + 4 * g + (r & 3) > u.last;
+#pragma unroll
+                for (int i = 0; i < NV; i++)
+#pragma unroll
+                    for (int e = 0; e < VW; e++) {
+                        vw[i][r][e] = hide ? 0 : vw[i][r][e];
+                        size = larger(size, vw[i][r][e]);
+                    }
+            }
+            const bool finite = (size & 0xffffu) < H::INF && size >> 16 < H::INF;
+            if ((whole || one) && !__ballot(!finite)) {
+#pragma unroll
+                for (int i = 0; i < NV; i++)
+#pragma unroll
+                    for (int e = 0; e < VEC; e++) {
+                        const uint4 v = turned(vw[i], e);
+#pragma unroll
+                        for (int n = 0; n < LIMBS; n++)
+                            acc[i * VEC + e] = H::mfma(v, w[n], acc[i * VEC + e]);
+                        if (e & 1)
+                            __builtin_amdgcn_sched_barrier(0);
+                    }
+            } else {
+                /* several tokens that see different positions of the tile, or values that are not finite: each token's
+                 * rows computed apart, without the values behind it. The values are loaded again, so that the
+                 * fast path keeps its registers */
+                for (int jj = u.j0; jj <= u.j1; jj++) {
+                    const long upto = (long)u.q.past + jj < u.last ? (long)u.q.past + jj : u.last;
+#pragma unroll
+                    for (int i = 0; i < NV; i++) {
+                        uint32_t again[8][VW];
+#pragma unroll
+                        for (int r = 0; r < 8; r++) {
+                            load_words<VW>(again[r], address(kv.v, rows[r], head_rows, D * 2) + (i * 16 + c) * VEC * 2);
+                            const bool hide = tile * 32 + (r & 4) * 4 + 4 * g + (r & 3) > upto;
+#pragma unroll
+                            for (int e = 0; e < VW; e++)
+                                again[r][e] = hide ? 0 : again[r][e];
+                        }
+#pragma unroll
+                        for (int e = 0; e < VEC; e++) {
+                            const uint4 v = turned(again, e);
+                            v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                            for (int n = 0; n < LIMBS; n++)
+                                o = H::mfma(n ? finite_only<TYPE>(v) : v, w[n], o);
+                            if (u.j == jj)
+                                acc[i * VEC + e] += o;
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+                    asm volatile("" ::: "memory"); /* the loads stay in the loop, and out of registers */
+                }
+            }
+        }
+        finish<D, VEC>(lds, kv, a, p, u, number, m, l, acc);
+    }
+}
+
+/* A query row's chunks joined, 64 elements of it a workgroup: each scaled to the largest maximum, added by 16
+ * threads an element in turn and then over the 16, in one order. */
+__global__ __launch_bounds__(256) void attn_join_k(rt_seqs b, rt_kv kv, rt_attn a, plan p)
+{
+    __shared__ __align__(16) float4 so[16][16];
     const long i = blockIdx.x, h = blockIdx.y, s = q8_sequence_of(b, i);
     if (s < 0)
         return;
-    const long chunk = chunk_of(b, p);
-    const seq_plan q = plan_of(b, p, s, chunk);
+    const int chunk = chunk_of(b, p);
+    const seq_plan q = plan_of(b, p, (int)s, chunk);
     if (q.chunks == 1)
         return;
-    long before = 0;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (long k = lane; k < s; k += 64) {
-        const seq_plan o = plan_of(b, p, k, chunk);
-        before += o.rows * o.chunks;
+    int before = 0;
+    const int lane = threadIdx.x & 63;
+    if (s > 0) {
+        for (int k = lane; k < (int)s; k += 64) {
+            const seq_plan o = plan_of(b, p, k, chunk);
+            before += o.rows * o.chunks;
+        }
+        for (int o = 32; o >= 1; o >>= 1)
+            before += __shfl_xor(before, o, 64);
     }
-    before = wave_sum(before);
-    const long kh = h / p.group, row = (i - q.first) * p.group + h % p.group, z = row / 16, r = row % 16;
-    if (before + (z + 1) * q.chunks > p.slots)
+    const int kh = (int)h / p.group, row = (int)(i - q.first) * p.group + (int)h % p.group, z = row / 16, r = row % 16;
+    if ((long)before + (long)(z + 1) * q.chunks > p.slots)
         return;
-    const long slot = kh * p.slots + before + z * q.chunks, D = kv.dim;
+    const long slot = (long)kh * p.slots + before + z * q.chunks, D = kv.dim;
     const float *ml = p.part + kv.heads * p.slots * 16 * D;
     float top = -INFINITY;
     for (long k = lane; k < q.chunks; k += 64)
@@ -396,22 +725,24 @@ __global__ __launch_bounds__(64 * WAVES) void attn_join_k(rt_seqs b, rt_kv kv, r
         sum += v.y * (v.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(v.x - top));
     }
     sum = q8_wave_sum(sum);
+    const int at = threadIdx.x & 15, turn = threadIdx.x >> 4;
+    const long d = 64 * (long)blockIdx.z + 4 * at;
     float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (4 * lane < D)
+    if (d < D)
 #pragma unroll 4
-        for (long k = wave; k < q.chunks; k += WAVES) {
+        for (long k = turn; k < q.chunks; k += 16) {
             const float x = ml[((slot + k) * 16 + r) * 2], f = x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(x - top);
-            const float4 u = *(const float4 *)(p.part + ((slot + k) * 16 + r) * D + 4 * lane);
-            v = float4{fmaf(u.x, f, v.x), fmaf(u.y, f, v.y), fmaf(u.z, f, v.z), fmaf(u.w, f, v.w)};
+            const float4 w = *(const float4 *)(p.part + ((slot + k) * 16 + r) * D + d);
+            v = float4{fmaf(w.x, f, v.x), fmaf(w.y, f, v.y), fmaf(w.z, f, v.z), fmaf(w.w, f, v.w)};
         }
-    so[wave][lane] = v;
+    so[turn][at] = v;
     __syncthreads();
-    if (wave == 0 && 4 * lane < D) {
-        for (int w = 1; w < WAVES; w++) {
-            const float4 u = so[w][lane];
-            v = float4{v.x + u.x, v.y + u.y, v.z + u.z, v.w + u.w};
+    if (turn == 0 && d < D) {
+        for (int w = 1; w < 16; w++) {
+            const float4 x = so[w][at];
+            v = float4{v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w};
         }
-        store_row(a, D, i, h, 4 * lane, v, sum, false);
+        store_row(a, D, i, h, d, v, sum, false);
     }
 }
 
@@ -421,7 +752,10 @@ void launch(hipStream_t s, dim3 grid, const rt_seqs &b, const rt_kv &kv, const r
     switch (kv.dim) {
 #define DIM(D)                                                                                                                                             \
     case D:                                                                                                                                                \
-        attn_tile_k<D, TYPE><<<grid, 64 * WAVES, 0, s>>>(b, kv, a, p);                                                                                     \
+        if constexpr (TYPE == RT_F32)                                                                                                                      \
+            attn_f32_k<D><<<grid, 64 * WAVES, 0, s>>>(b, kv, a, p);                                                                                        \
+        else                                                                                                                                               \
+            attn_half_k<D, TYPE><<<grid, 64 * WAVES, 0, s>>>(b, kv, a, p);                                                                                 \
         break;
         DIM(32)
         DIM(64)
@@ -435,16 +769,16 @@ void launch(hipStream_t s, dim3 grid, const rt_seqs &b, const rt_kv &kv, const r
     }
 }
 
-/* Enough chunks for two workgroups a compute unit twice over, so that the last ones to end leave few idle */
-constexpr long CHUNKS = 1024, SLOTS = 4096;
+/* Row tiles of a call at most, and the chunks (a key-value head) to spread them over: so many that with each
+ * row tile's last one, which is smaller, they fill the workgroups that run at once (two a compute unit) a
+ * whole number of times, at least half of them whole; none (0) when the row tiles alone are more than SLOTS */
+constexpr long SLOTS = 4096;
 
-/* Row tiles of a call at most, and the chunks to spread them over: none when there are as many row tiles as chunks
- * would fill SLOTS with, else at least as many as row tiles */
 void plan_chunks(const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long &tiles, long &target)
 {
     tiles = b.t * (a.q_heads / kv.heads) / 16 + b.n;
-    const long want = (CHUNKS + kv.heads - 1) / kv.heads;
-    target = tiles * kv.heads > SLOTS || kv.table_ld * kv.page <= 16 * LEAST ? 0 : tiles > want ? tiles : want;
+    const long once = ((kv.dim > 128 ? 256 : 512) + kv.heads - 1) / kv.heads;
+    target = tiles * kv.heads > SLOTS || kv.table_ld * kv.page <= 16 * LEAST ? 0 : (2 * tiles + once - 1) / once * once - tiles;
 }
 
 } /* namespace */
@@ -459,8 +793,9 @@ long q8_attn_part_floats(const rt_seqs &b, const rt_kv &kv, const rt_attn &a)
 void q8_launch_attn(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const rt_attn &a, float *part)
 {
     plan p;
-    long tiles;
-    plan_chunks(b, kv, a, tiles, p.target);
+    long tiles, target;
+    plan_chunks(b, kv, a, tiles, target);
+    p.target = (int)target;
     int up = 0;
     while ((1L << up) < kv.page)
         up++;
@@ -468,8 +803,8 @@ void q8_launch_attn(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const
     p.pg.mul = (uint32_t)((((__uint128_t)1 << p.pg.shift) + kv.page - 1) / kv.page);
     p.group = (int)(a.q_heads / kv.heads);
     const long reach = (1L << 31) - 4096;
-    p.cap = kv.table_ld > reach / kv.page ? reach : kv.table_ld * kv.page;
-    p.slots = p.target + tiles;
+    p.cap = (int)(kv.table_ld > reach / kv.page ? reach : kv.table_ld * kv.page);
+    p.slots = (int)(target + (target ? tiles : 0));
     p.part = part;
     p.qscale = (float)((double)a.scale * 1.4426950408889634074);
     const hipStream_t s = (hipStream_t)stream;
@@ -482,5 +817,5 @@ void q8_launch_attn(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const
     else
         launch<RT_BF16>(s, grid, b, kv, a, p);
     if (p.target)
-        attn_join_k<<<dim3((unsigned)b.t, (unsigned)a.q_heads), 64 * WAVES, 0, s>>>(b, kv, a, p);
+        attn_join_k<<<dim3((unsigned)b.t, (unsigned)a.q_heads, (unsigned)((kv.dim + 63) / 64)), 256, 0, s>>>(b, kv, a, p);
 }

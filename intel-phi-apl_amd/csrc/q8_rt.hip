@@ -1905,6 +1905,8 @@ void rt_attn_kv_dev(struct rt *R, const struct rt_seqs *s, const struct rt_kv *k
     if (a->q_heads < 1 || a->q_heads > RT_HEADS_MAX || a->q_heads % kv->heads)
         failf(fn, "needs 1 to %ld query heads, a multiple of the key-value heads", RT_HEADS_MAX);
     const long t = s->t, d = kv->dim;
+    if (t * (a->q_heads / kv->heads) >= 1L << 31)
+        fail(fn, "needs fewer than 2^31 query rows (tokens x query heads a key-value head)");
     check_heads(fn, a->q, t, a->q_ld, a->q_hd, a->q_heads, d, true, "q");
     if (a->gate)
         check_heads(fn, a->gate, t, a->gate_ld, a->gate_hd, a->q_heads, d, true, "gate");
