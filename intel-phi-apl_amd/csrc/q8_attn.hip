@@ -8,7 +8,6 @@ typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 
 constexpr int WAVES = 4;
-constexpr int LEAST = 2 * WAVES; /* position tiles a chunk at least: two of 16 a wave; every chunk is an even number of them */
 
 /* p / page for p < 2^31: (p * mul) >> shift with shift = 31 + ceil(log2 page), mul = ceil(2^shift / page): exact, as
  * the excess mul * page - 2^shift is below page <= 2^(shift - 31) */
@@ -23,6 +22,7 @@ struct plan {
     paging pg;
     int group;   /* query heads a key-value head */
     int cap;     /* positions that the table reaches */
+    int least;   /* tiles a chunk at least: one load of each wave, 16 positions of F32, 32 of 16 bits */
     int target;  /* chunks (a key-value head) to spread all tiles over; 0: one a row tile */
     int slots;   /* partial results a key-value head */
     float qscale; /* scale * log2 e: scores are in powers of two */
@@ -72,7 +72,7 @@ __device__ __forceinline__ int chunk_of(const rt_seqs &b, const plan &p)
             all += __shfl_xor(all, o, 64);
     }
     const double c = all / p.target + 1.0; /* as far as 2^27 tiles: one a row tile there */
-    return c < LEAST ? LEAST : c < 1e8 ? first_lane((int)c + 1) & ~1 : 0;
+    return c < p.least ? p.least : c < 1e8 ? first_lane((int)c + 1) & ~1 : 0;
 }
 
 /* The sequence whose row tiles' chunks hold number i of all, -1 behind the last; before = the chunks of
@@ -687,12 +687,14 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_half_k(rt_se
     }
 }
 
-/* A query row's chunks joined, 64 elements of it a workgroup: each scaled to the largest maximum, added by 16
- * threads an element in turn and then over the 16, in one order. */
+/* A query row's chunks joined, 64 elements of it a workgroup, 16 threads an element: each takes every 16th chunk,
+ * loading its elements and its maximum and sum at once, with a running maximum of its own; then the 16 are scaled
+ * to the largest and added in one order. Bound by the latency of its few dependent loads. */
 __global__ __launch_bounds__(256) void attn_join_k(rt_seqs b, rt_kv kv, rt_attn a, plan p)
 {
     __shared__ __align__(16) float4 so[16][16];
-    const long i = blockIdx.x, h = blockIdx.y, s = q8_sequence_of(b, i);
+    __shared__ float sm[16], sl[16];
+    const long i = blockIdx.x, h = blockIdx.y, s = b.n == 1 ? (b.start[0] <= i && i < b.start[1] ? 0 : -1) : q8_sequence_of(b, i);
     if (s < 0)
         return;
     const int chunk = chunk_of(b, p);
@@ -713,34 +715,45 @@ __global__ __launch_bounds__(256) void attn_join_k(rt_seqs b, rt_kv kv, rt_attn 
     if ((long)before + (long)(z + 1) * q.chunks > p.slots)
         return;
     const long slot = (long)kh * p.slots + before + z * q.chunks, D = kv.dim;
-    const float *ml = p.part + kv.heads * p.slots * 16 * D;
-    float top = -INFINITY;
-    for (long k = lane; k < q.chunks; k += 64)
-        top = fmaxf(top, ml[((slot + k) * 16 + r) * 2]);
-    for (int o = 32; o >= 1; o >>= 1)
-        top = fmaxf(top, __shfl_xor(top, o, 64));
-    float sum = 0.0f;
-    for (long k = lane; k < q.chunks; k += 64) {
-        const float2 v = *(const float2 *)(ml + ((slot + k) * 16 + r) * 2);
-        sum += v.y * (v.x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(v.x - top));
-    }
-    sum = q8_wave_sum(sum);
     const int at = threadIdx.x & 15, turn = threadIdx.x >> 4;
-    const long d = 64 * (long)blockIdx.z + 4 * at;
+    const long d = 64 * (long)blockIdx.z + 4 * at, dd = d < D ? d : 0;
+    const float *ml = p.part + kv.heads * p.slots * 16 * D + (slot * 16 + r) * 2, *part = p.part + (slot * 16 + r) * D + dd;
     float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-    if (d < D)
-#pragma unroll 4
-        for (long k = turn; k < q.chunks; k += 16) {
-            const float x = ml[((slot + k) * 16 + r) * 2], f = x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(x - top);
-            const float4 w = *(const float4 *)(p.part + ((slot + k) * 16 + r) * D + d);
-            v = float4{fmaf(w.x, f, v.x), fmaf(w.y, f, v.y), fmaf(w.z, f, v.z), fmaf(w.w, f, v.w)};
+    float m = -INFINITY, l = 0.0f;
+    for (int k0 = turn; k0 < q.chunks; k0 += 64) {
+        float2 x[4];
+        float4 w[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int at_chunk = k0 + 16 * k < q.chunks ? k0 + 16 * k : k0;
+            x[k] = *(const float2 *)(ml + (long)at_chunk * 32);
+            w[k] = *(const float4 *)(part + (long)at_chunk * 16 * D);
         }
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (k0 + 16 * k < q.chunks) {
+                /* a chunk whose maximum is -infinity holds zeros, or NaN: taken as it is */
+                const float top = fmaxf(m, x[k].x), f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top),
+                            e = x[k].x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(x[k].x - top);
+                v = float4{fmaf(w[k].x, e, v.x * f), fmaf(w[k].y, e, v.y * f), fmaf(w[k].z, e, v.z * f), fmaf(w[k].w, e, v.w * f)};
+                l = fmaf(x[k].y, e, l * f);
+                m = top;
+            }
+    }
     so[turn][at] = v;
+    if (at == 0)
+        sm[turn] = m, sl[turn] = l;
     __syncthreads();
     if (turn == 0 && d < D) {
-        for (int w = 1; w < 16; w++) {
-            const float4 x = so[w][at];
-            v = float4{v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w};
+        float top = sm[0], sum = 0.0f;
+        for (int k = 1; k < 16; k++)
+            top = fmaxf(top, sm[k]);
+        v = float4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = 0; k < 16; k++) {
+            const float f = sm[k] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(sm[k] - top);
+            const float4 x = so[k][at];
+            v = float4{fmaf(x.x, f, v.x), fmaf(x.y, f, v.y), fmaf(x.z, f, v.z), fmaf(x.w, f, v.w)};
+            sum = fmaf(sl[k], f, sum);
         }
         store_row(a, D, i, h, d, v, sum, false);
     }
@@ -774,11 +787,13 @@ void launch(hipStream_t s, dim3 grid, const rt_seqs &b, const rt_kv &kv, const r
  * whole number of times, at least half of them whole; none (0) when the row tiles alone are more than SLOTS */
 constexpr long SLOTS = 4096;
 
+int least_tiles(const rt_kv &kv) { return kv.type == RT_F32 ? WAVES : 2 * WAVES; }
+
 void plan_chunks(const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long &tiles, long &target)
 {
     tiles = b.t * (a.q_heads / kv.heads) / 16 + b.n;
     const long once = ((kv.dim > 128 ? 256 : 512) + kv.heads - 1) / kv.heads;
-    target = tiles * kv.heads > SLOTS || kv.table_ld * kv.page <= 16 * LEAST ? 0 : (2 * tiles + once - 1) / once * once - tiles;
+    target = tiles * kv.heads > SLOTS || kv.table_ld * kv.page <= 16 * least_tiles(kv) ? 0 : (2 * tiles + once - 1) / once * once - tiles;
 }
 
 } /* namespace */
@@ -796,6 +811,7 @@ void q8_launch_attn(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const
     long tiles, target;
     plan_chunks(b, kv, a, tiles, target);
     p.target = (int)target;
+    p.least = least_tiles(kv);
     int up = 0;
     while ((1L << up) < kv.page)
         up++;
