@@ -8,7 +8,9 @@
 void q8_launch_conv(q8_stream_t s, const rt_seqs &b, const float *x, long x_ld, long ch, const float *w, long taps, const float *s_in, float *s_out,
                     float *y, long y_ld);
 void q8_launch_rope(q8_stream_t s, const rt_seqs &b, const rt_kv &kv, const rt_rope &a);
-void q8_launch_delta(q8_stream_t s, const rt_seqs &b, const rt_delta &a);
+/* prep: q8_delta_prep_floats floats of workspace (none: may be NULL) */
+long q8_delta_prep_floats(const rt_seqs &b, const rt_delta &a);
+void q8_launch_delta(q8_stream_t s, const rt_seqs &b, const rt_delta &a, float *prep);
 /* part: q8_attn_part_floats floats of workspace (none: may be NULL) */
 long q8_attn_part_floats(const rt_seqs &b, const rt_kv &kv, const rt_attn &a);
 void q8_launch_attn(q8_stream_t s, const rt_seqs &b, const rt_kv &kv, const rt_attn &a, float *part);

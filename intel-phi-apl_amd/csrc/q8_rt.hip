@@ -125,7 +125,7 @@ struct ctx {
     void *ximg = nullptr;
     /* the device address of `scratch` on this runtime's GPU (rt_gemm_dev_noalloc's partials) */
     float *noalloc_part = nullptr;
-    /* the operators between the products: the attention's partial results */
+    /* the operators between the products: the attention's partial results, the delta rule's chunks */
     float *mix = nullptr;
     size_t mix_cap = 0;
     /* the greedy next token's candidates */
@@ -1821,6 +1821,8 @@ void rt_delta_rule_dev(struct rt *R, const struct rt_seqs *s, const struct rt_de
         fail(fn, "k_dim must be 32, 64, 96, 128, 192 or 256");
     if (a->v_dim < 16 || a->v_dim > 512 || a->v_dim % 16)
         fail(fn, "v_dim must be a multiple of 16, 16 to 512");
+    if (s->n * a->v_heads * (a->v_dim / 16) >= 1L << 24)
+        fail(fn, "needs fewer than 2^24 sequences x value heads x 16 columns of v_dim");
     const long kw = a->k_heads * a->k_dim, vw = a->v_heads * a->v_dim;
     check_dev_ptr(fn, a->q, "q");
     check_dev_ptr(fn, a->k, "k");
@@ -1852,7 +1854,7 @@ void rt_delta_rule_dev(struct rt *R, const struct rt_seqs *s, const struct rt_de
     check_apart(fn, "o", o, {in[0], in[1], in[2], in[3], in[4], in[5], in[6], in[7], in[8], in[9], out, words_span(a->s_in, 4 * state)});
     check_apart(fn, "s_out", out, {in[0], in[1], in[2], in[3], in[4], in[5], in[6], in[7], in[8], in[9]});
     const on_gpu g(c);
-    q8_launch_delta((q8_stream_t)c->stream, *s, *a);
+    q8_launch_delta((q8_stream_t)c->stream, *s, *a, reserve_mix(c, (size_t)q8_delta_prep_floats(*s, *a)));
     launched("the delta rule");
 }
 
