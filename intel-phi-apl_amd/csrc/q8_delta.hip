@@ -149,8 +149,11 @@ template <int DK>
 __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int most, long from, float *out)
 {
     constexpr int NT = DK / 16, LK = DK + 4, LT = CHUNK + 4;
-    __shared__ __align__(16) float sk[CHUNK][LK], sd[CHUNK][LT], sa[CHUNK][LT], st[CHUNK][LT];
-    __shared__ __align__(16) float salpha[CHUNK], sbeta[CHUNK], srk[CHUNK], srq[CHUNK];
+    constexpr int KEYS = CHUNK * LK, MATRIX = CHUNK * LT;
+    __shared__ __align__(16) float lds[KEYS > 3 * MATRIX ? KEYS : 3 * MATRIX];
+    float(*sk)[LK] = (float(*)[LK])lds;
+    float(*sd)[LT] = (float(*)[LT])lds, (*sa)[LT] = sd + CHUNK, (*st)[LT] = sa + CHUNK;
+    __shared__ __align__(16) float sbeta[CHUNK], srk[CHUNK], srq[CHUNK];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
     const long slot = from + blockIdx.x, kh = blockIdx.y, s = sequence_of_slot(b, slot);
     if (s < 0)
@@ -199,71 +202,83 @@ __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int m
                 qt[j] = mfma4(qv[t], *(const float4 *)&sk[16 * j + c][16 * t + 4 * g], qt[j]);
     }
 
+    __syncthreads(); /* the keys' place is the matrices' now */
+
     const int heads = (int)(a.v_heads / a.k_heads);
     for (int hn = 0; hn < heads; hn++) {
         const long h = a.tiled ? kh + hn * a.k_heads : kh * heads + hn;
-        float *mine = out + ((long)blockIdx.x * a.v_heads + h) * PREP;
-        if (tid < CHUNK) {
-            salpha[tid] = tid < n ? decay_of(a.a[(at + tid) * a.a_ld + h], a.dt[h], a.decay[h]) : 1.0f;
-            sbeta[tid] = tid < n ? q8_sigmoid(a.b[(at + tid) * a.b_ld + h]) : 0.0f;
-        }
-        __syncthreads();
+        float *mine = out + ((long)blockIdx.x * a.v_heads + h) * PREP, *factor = mine + 2 * PAIRS * 256;
+        /* lane i of every wave: token i's gates */
+        const float alpha = lane < n ? decay_of(a.a[(at + lane) * a.a_ld + h], a.dt[h], a.decay[h]) : 1.0f;
+        if (wave == 0)
+            sbeta[lane] = lane < n ? q8_sigmoid(a.b[(at + lane) * a.b_ld + h]) : 0.0f;
         {
-            /* the decays between tokens: lane j has column j, and goes down the rows; gamma along with it */
-            const float alpha = salpha[lane];
-            float d = 1.0f, gamma = 1.0f;
-            for (int i = 0; i < 16 * wave + 16; i++) {
+            /* the decays between tokens: lane j has column j and goes down to the wave's rows */
+            float d = 1.0f;
+            for (int i = 0; i < 16 * wave; i++) {
                 const float x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, alpha), i));
                 d = i <= lane ? 1.0f : d * x;
-                gamma *= x;
-                if (i >= 16 * wave) {
-                    sd[i][lane] = i >= lane ? d : 0.0f;
-                    if (lane == 0) {
-                        mine[2 * PAIRS * 256 + i] = gamma * srk[i];
-                        mine[2 * PAIRS * 256 + CHUNK + i] = gamma * srq[i];
-                    }
-                }
             }
-            if (wave == 3) {
-                mine[2 * PAIRS * 256 + 2 * CHUNK + lane] = d * srk[lane];
-                if (lane == 0)
-                    mine[2 * PAIRS * 256 + 3 * CHUNK] = gamma;
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int i = 16 * wave + r;
+                const float x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, alpha), i));
+                d = i <= lane ? 1.0f : d * x;
+                sd[i][lane] = i >= lane ? d : 0.0f;
             }
         }
         __syncthreads();
-        /* A, and P in the decays' place */
+        const float first_alpha = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, alpha), 0));
+        const float gamma = sd[lane][0] * first_alpha; /* of token `lane` */
+        if (wave == 0)
+            factor[lane] = gamma * srk[lane];
+        else if (wave == 1)
+            factor[CHUNK + lane] = gamma * srq[lane];
+        else if (wave == 2)
+            factor[2 * CHUNK + lane] = sd[CHUNK - 1][lane] * srk[lane];
+        else if (lane == CHUNK - 1)
+            factor[3 * CHUNK] = gamma;
+        /* A, and P, which takes the decays' place */
+        const float4 bk = *(const float4 *)&sbeta[16 * wave + 4 * g] * *(const float4 *)&srk[16 * wave + 4 * g], qf = *(const float4 *)&srq[16 * (3 - wave) + 4 * g];
+        const float *bf = &bk.x, *qs = &qf.x;
+        float pr[TILES][4];
 #pragma unroll
         for (int j = 0; j < TILES; j++) {
-            if (j <= wave) {
-                const float rk = srk[16 * j + c];
+            const float rk = srk[16 * j + c];
+            if (j <= wave)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const int i = 16 * wave + 4 * g + r;
-                    sa[i][16 * j + c] = i > 16 * j + c ? sbeta[i] * srk[i] * rk * kt[j][r] * sd[i][16 * j + c] : 0.0f;
+                    sa[i][16 * j + c] = i > 16 * j + c ? bf[r] * rk * kt[j][r] * sd[i][16 * j + c] : 0.0f;
                 }
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int j = 0; j < TILES; j++) {
-            if (j <= 3 - wave) {
-                const float rk = srk[16 * j + c];
+            if (j <= 3 - wave)
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const int i = 16 * (3 - wave) + 4 * g + r;
-                    sd[i][16 * j + c] = i >= 16 * j + c ? srq[i] * rk * qt[j][r] * sd[i][16 * j + c] : 0.0f;
+                    pr[j][r] = i >= 16 * j + c ? qs[r] * rk * qt[j][r] * sd[i][16 * j + c] : 0.0f;
                 }
-            }
         }
+        __syncthreads();
+#pragma unroll
+        for (int j = 0; j < TILES; j++)
+            if (j <= 3 - wave)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    sd[16 * (3 - wave) + 4 * g + r][16 * j + c] = pr[j][r];
         {
             /* the diagonal's inverses: column c of block `wave` */
             float x[16];
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                x[i] = i == c ? 1.0f : 0.0f;
+                float4 row[4];
+#pragma unroll
+                for (int k = 0; k < i; k += 4)
+                    row[k / 4] = *(const float4 *)&sa[16 * wave + i][16 * wave + k];
+                float u[2] = {i == c ? 1.0f : 0.0f, 0.0f};
 #pragma unroll
                 for (int k = 0; k < i; k++)
-                    x[i] = k < c ? x[i] : fmaf(-sa[16 * wave + i][16 * wave + k], x[k], x[i]);
+                    u[k & 1] = fmaf(-(&row[k / 4].x)[k & 3], x[k], u[k & 1]);
+                x[i] = u[0] + u[1];
                 if (g == 0)
                     st[16 * wave + i][16 * wave + c] = x[i];
             }
@@ -274,10 +289,11 @@ __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int m
             if (wave < TILES - d) {
                 const int i = wave + d, j = wave;
                 v4f m = {0.0f, 0.0f, 0.0f, 0.0f};
-                for (int k = j; k < i; k++)
-                    m = mfma4(*(const float4 *)&sa[16 * i + c][16 * k + 4 * g],
-                              float4{st[16 * k + 4 * g][16 * j + c], st[16 * k + 4 * g + 1][16 * j + c], st[16 * k + 4 * g + 2][16 * j + c],
-                                     st[16 * k + 4 * g + 3][16 * j + c]},
+#pragma unroll
+                for (int k = 0; k < d; k++)
+                    m = mfma4(*(const float4 *)&sa[16 * i + c][16 * (j + k) + 4 * g],
+                              float4{st[16 * (j + k) + 4 * g][16 * j + c], st[16 * (j + k) + 4 * g + 1][16 * j + c], st[16 * (j + k) + 4 * g + 2][16 * j + c],
+                                     st[16 * (j + k) + 4 * g + 3][16 * j + c]},
                               m);
                 m = mfma4(*(const float4 *)&st[16 * i + c][16 * i + 4 * g], as4(m), v4f{0.0f, 0.0f, 0.0f, 0.0f});
 #pragma unroll
@@ -301,32 +317,39 @@ __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int m
                 }
         const bool odd = __ballot(!finite) != 0;
         if (lane == 0)
-            mine[2 * PAIRS * 256 + 3 * CHUNK + 4 + wave] = odd ? 1.0f : 0.0f;
+            factor[3 * CHUNK + 4 + wave] = odd ? 1.0f : 0.0f;
         __syncthreads();
     }
 }
 
-/* A workgroup 16 columns of a sequence's head; wave w has tokens 16 w .. 16 w + 15 of the chunk and every fourth 16
- * rows of the state from 16 w on. The state stays in LDS from chunk to chunk. A chunk:
+/* A workgroup 16 columns of a sequence's head. Its waves' halves share a SIMD each: wave w < 4 has the keys of
+ * tokens 16 w .. 16 w + 15 of a chunk and T's rows for them, wave 4 + w the queries of tokens 16 (3 - w) .. and P's
+ * rows, so that each SIMD has the same number of matrix instructions (116 a chunk at k_dim 128), and wave v the state's
+ * rows 16 v .., 16 (v + 8) ... The state stays in LDS from chunk to chunk. A chunk, with a barrier behind each
+ * line (the second half's work stands in brackets):
  *
- *   K S0 and Q S0 of the wave's tokens;  R = V - gamma K S0            -> LDS
- *   d = T R;                             d, and D_C d                  -> LDS
- *   S = gamma_C S0 + K^T (D_C d);  O = gamma Q S0 + P d                -> LDS, HBM
+ *   R = V - gamma K S0
+ *   d = T R, D_C d                                 [gamma Q S0]
+ *   S = gamma_C S0 + K^T (D_C d)                   [the same, and O = gamma Q S0 + P d]
  *
- * 104 to 128 matrix instructions a wave at k_dim 128, which bound it; what a chunk needs is loaded a chunk ahead. The
- * workgroups of a head are on one XCD, whose L2 then has K, Q, T and P for all of them.
+ * What a wave needs of the next chunk is loaded as soon as this one's has been used. The workgroups of a head are
+ * on one XCD, whose L2 then has K, Q, T and P for all of them.
  *
  * A chunk with anything that is not finite goes token by token: in the products 0 times a later token's NaN
  * would reach earlier ones. */
+constexpr int CHUNK_THREADS = 512;
+
 template <int DK>
-__global__ __launch_bounds__(256) void delta_chunk_k(rt_seqs b, rt_delta a, int most, long from, long count, const float *prep)
+__global__ __launch_bounds__(CHUNK_THREADS) void delta_chunk_k(rt_seqs b, rt_delta a, int most, long from, long count, const float *prep)
 {
     constexpr int NT = DK / 16, LK = DK + 4;
     __shared__ __align__(16) float sk[CHUNK][LK];
     __shared__ __align__(16) float4 ss[NT][64], sr[TILES][64], sv[TILES][64], sw[TILES][64];
-    __shared__ float red[5][4][16];
+    __shared__ float red[5][8][16];
     __shared__ int sodd;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+    const bool keys = wave < 4;
+    const int tile = keys ? wave : 7 - wave;
     const int slices = (int)(a.v_dim / 16), x = (int)(blockIdx.x % 8), y = (int)(blockIdx.x / 8), slice = y % slices;
     const long unit = (long)(y / slices) * 8 + x, s = unit / a.v_heads, h = unit % a.v_heads;
     if (s >= b.n)
@@ -340,88 +363,104 @@ __global__ __launch_bounds__(256) void delta_chunk_k(rt_seqs b, rt_delta a, int 
         return;
     const long col = 16 * slice + c, state = (s * a.v_heads + h) * DK * a.v_dim + col;
     const float *s_in = c0 == 0 ? a.s_in : a.s_out;
-#pragma unroll
-    for (int t = wave; t < NT; t += 4) {
+    for (int t = wave; t < NT; t += 8) {
         const float *p = s_in + state + (16 * t + 4 * g) * a.v_dim;
         ss[t][lane] = float4{p[0], p[a.v_dim], p[2 * a.v_dim], p[3 * a.v_dim]};
     }
     if (tid == 0)
         sodd = 0;
 
-    float4 kv[NT], qv[NT], tv[TILES], pv[TILES], gk, gq, gd;
+    /* the wave's rows of K or Q, of T or P, and their factors: of chunk n, whose rows behind the sequence are 0 */
+    const float *rows = (keys ? a.k : a.q) + kh * DK + 4 * g, *values = a.v + h * a.v_dim + col;
+    const long ld = keys ? a.k_ld : a.q_ld;
+    float4 xv[NT], mv[TILES], factor, decay;
     float v[4], gamma, odd_in;
-    const auto load = [&](long n) {
-        const long row = first + n * CHUNK + 16 * wave;
-        const bool here = row + c < last;
-        const float *kp = a.k + (row + c) * a.k_ld + kh * DK + 4 * g, *qp = a.q + (row + c) * a.q_ld + kh * DK + 4 * g;
-        const float *mine = prep + ((slot + n - from) * a.v_heads + h) * PREP, *factor = mine + 2 * PAIRS * 256;
+    const auto load_rows = [&](long n) {
+        const long row = first + n * CHUNK + 16 * tile + c;
+        const float *p = rows + (row < last ? row : first) * ld;
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            kv[t] = here ? *(const float4 *)(kp + 16 * t) : float4{0.0f, 0.0f, 0.0f, 0.0f};
-            qv[t] = here ? *(const float4 *)(qp + 16 * t) : float4{0.0f, 0.0f, 0.0f, 0.0f};
+            xv[t] = *(const float4 *)(p + 16 * t);
+            if (row >= last)
+                xv[t] = float4{0.0f, 0.0f, 0.0f, 0.0f};
         }
+    };
+    const auto part = [&](long n) { return prep + ((slot + n - from) * a.v_heads + h) * PREP; };
+    const auto load_matrix = [&](long n) {
+        const float *p = part(n) + ((keys ? 0 : PAIRS) + tile * (tile + 1) / 2) * 256 + lane * 4;
 #pragma unroll
         for (int j = 0; j < TILES; j++)
-            if (j <= wave) {
-                tv[j] = *(const float4 *)(mine + (wave * (wave + 1) / 2 + j) * 256 + lane * 4);
-                pv[j] = *(const float4 *)(mine + (PAIRS + wave * (wave + 1) / 2 + j) * 256 + lane * 4);
-            }
-        gk = *(const float4 *)(factor + 16 * wave + 4 * g);
-        gq = *(const float4 *)(factor + CHUNK + 16 * wave + 4 * g);
-        gd = *(const float4 *)(factor + 2 * CHUNK + 16 * wave + 4 * g);
-        gamma = factor[3 * CHUNK];
-        odd_in = factor[3 * CHUNK + 4 + wave];
-#pragma unroll
-        for (int r = 0; r < 4; r++)
-            v[r] = row + 4 * g + r < last ? a.v[(row + 4 * g + r) * a.v_ld + h * a.v_dim + col] : 0.0f;
+            if (j <= tile)
+                mv[j] = *(const float4 *)(p + j * 256);
     };
-    load(c0);
+    const auto load_factors = [&](long n) {
+        const float *p = part(n) + 2 * PAIRS * 256;
+        factor = *(const float4 *)(p + (keys ? 0 : CHUNK) + 16 * tile + 4 * g);
+        decay = *(const float4 *)(p + 2 * CHUNK + 16 * tile + 4 * g);
+        gamma = p[3 * CHUNK];
+        odd_in = p[3 * CHUNK + 4 + (wave & 3)];
+        const long row = first + n * CHUNK + 16 * tile + 4 * g;
+        if (keys)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                v[r] = row + r < last ? values[(row + r) * a.v_ld] : 0.0f;
+    };
+    load_rows(c0);
+    load_factors(c0);
+    load_matrix(c0);
     __syncthreads();
     for (long n = c0; n < c1; n++) {
-        const long row = first + n * CHUNK + 16 * wave;
-        /* the wave's rows of K for the state's product, and whether the chunk is odd */
+        const long row = first + n * CHUNK + 16 * tile, next = n + 1 < c1 ? n + 1 : n;
+        const auto with_state = [&]() {
+            v4f z[2] = {v4f{0.0f, 0.0f, 0.0f, 0.0f}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-        for (int t = 0; t < NT; t++)
-            *(float4 *)&sk[16 * wave + c][16 * t + 4 * g] = kv[t];
-        if (__ballot(odd_in != 0.0f || !finite4(float4{v[0], v[1], v[2], v[3]})) && lane == 0)
-            sodd = 1;
-        v4f ks[2] = {v4f{0.0f, 0.0f, 0.0f, 0.0f}, v4f{0.0f, 0.0f, 0.0f, 0.0f}}, qs[2] = {ks[0], ks[0]};
+            for (int t = 0; t < NT; t++)
+                z[t & 1] = mfma4(xv[t], ss[t][lane], z[t & 1]);
+            return z[0] + z[1];
+        };
+        const float end = gamma;
+        float4 scaled = factor, left = decay;
+        v4f mine = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (keys) {
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
-            const float4 st = ss[t][lane];
-            ks[t & 1] = mfma4(kv[t], st, ks[t & 1]);
-            qs[t & 1] = mfma4(qv[t], st, qs[t & 1]);
+            for (int t = 0; t < NT; t++)
+                *(float4 *)&sk[16 * tile + c][16 * t + 4 * g] = xv[t];
+            if (__ballot(odd_in != 0.0f || !finite4(float4{v[0], v[1], v[2], v[3]})) && lane == 0)
+                sodd = 1;
+            const v4f z = with_state();
+            sr[tile][lane] = float4{fmaf(-scaled.x, z[0], v[0]), fmaf(-scaled.y, z[1], v[1]), fmaf(-scaled.z, z[2], v[2]), fmaf(-scaled.w, z[3], v[3])};
+            load_rows(next);
         }
-        const v4f k0 = ks[0] + ks[1], q0 = qs[0] + qs[1];
-        sr[wave][lane] = float4{fmaf(-gk.x, k0[0], v[0]), fmaf(-gk.y, k0[1], v[1]), fmaf(-gk.z, k0[2], v[2]), fmaf(-gk.w, k0[3], v[3])};
+        load_factors(next);
         __syncthreads();
         if (sodd) {
-            /* token by token: the thread has rows 16 t + 4 g .. + 3, t = wave, wave + 4, ..., of column c */
+            /* token by token: the thread has rows 16 t + 4 g .. + 3, t = wave, wave + 8, ..., of column c */
             const int tokens = (int)(last - (first + n * CHUNK) < CHUNK ? last - (first + n * CHUNK) : CHUNK);
             for (int j = 0; j < tokens; j++) {
                 const long i = first + n * CHUNK + j;
                 float sum[5] = {};
-                for (int t = wave; t < NT; t += 4) {
+                for (int t = wave; t < NT; t += 8) {
                     const float4 kj = *(const float4 *)(a.k + i * a.k_ld + kh * DK + 16 * t + 4 * g), qj = *(const float4 *)(a.q + i * a.q_ld + kh * DK + 16 * t + 4 * g);
                     sum[0] += dot4(kj, ss[t][lane]), sum[1] += dot4(qj, ss[t][lane]);
                     sum[2] += dot4(kj, kj), sum[3] += dot4(qj, qj), sum[4] += dot4(qj, kj);
                 }
-#pragma unroll
                 for (int k = 0; k < 5; k++) {
                     sum[k] = group_sum(sum[k]);
                     if (g == 0)
                         red[k][wave][c] = sum[k];
                 }
                 __syncthreads();
-#pragma unroll
-                for (int k = 0; k < 5; k++)
-                    sum[k] = (red[k][0][c] + red[k][1][c]) + (red[k][2][c] + red[k][3][c]);
+                for (int k = 0; k < 5; k++) {
+                    sum[k] = 0.0f;
+                    for (int w = 0; w < 8; w++)
+                        sum[k] += red[k][w][c];
+                }
                 const float alpha = decay_of(a.a[i * a.a_ld + h], a.dt[h], a.decay[h]), beta = q8_sigmoid(a.b[i * a.b_ld + h]);
                 const float rk = a.eps >= 0.0f ? 1.0f / sqrtf(sum[2] + a.eps) : 1.0f, rq = a.scale * (a.eps >= 0.0f ? 1.0f / sqrtf(sum[3] + a.eps) : 1.0f);
                 const float d = beta * (a.v[i * a.v_ld + h * a.v_dim + col] - alpha * rk * sum[0]);
                 if (tid < 16)
                     a.o[i * a.o_ld + h * a.v_dim + col] = fmaf(rq * alpha, sum[1], rq * (rk * sum[4]) * d);
-                for (int t = wave; t < NT; t += 4) {
+                for (int t = wave; t < NT; t += 8) {
                     const float4 kj = *(const float4 *)(a.k + i * a.k_ld + kh * DK + 16 * t + 4 * g), o = ss[t][lane];
                     ss[t][lane] = float4{fmaf(rk * kj.x, d, alpha * o.x), fmaf(rk * kj.y, d, alpha * o.y), fmaf(rk * kj.z, d, alpha * o.z), fmaf(rk * kj.w, d, alpha * o.w)};
                 }
@@ -429,50 +468,54 @@ __global__ __launch_bounds__(256) void delta_chunk_k(rt_seqs b, rt_delta a, int 
             }
             if (tid == 0)
                 sodd = 0;
-            if (n + 1 < c1)
-                load(n + 1);
+            if (!keys)
+                load_rows(next);
+            load_matrix(next);
             __syncthreads();
             continue;
         }
-        v4f d = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int j = 0; j < TILES; j++)
-            if (j <= wave)
-                d = mfma4(tv[j], sr[j][lane], d);
-        sv[wave][lane] = as4(d);
-        sw[wave][lane] = as4(d) * gd;
-        const float4 go = gq;
-        const float end = gamma;
-        float4 po[TILES];
-#pragma unroll
-        for (int j = 0; j < TILES; j++)
-            po[j] = pv[j];
-        if (n + 1 < c1)
-            load(n + 1);
-        __syncthreads();
-#pragma unroll
-        for (int t = wave; t < NT; t += 4) {
-            const float4 o = ss[t][lane];
-            v4f z = {end * o.x, end * o.y, end * o.z, end * o.w};
+        if (keys) {
 #pragma unroll
             for (int j = 0; j < TILES; j++)
-                z = mfma4(float4{sk[16 * j + 4 * g][16 * t + c], sk[16 * j + 4 * g + 1][16 * t + c], sk[16 * j + 4 * g + 2][16 * t + c], sk[16 * j + 4 * g + 3][16 * t + c]},
-                          sw[j][lane], z);
-            ss[t][lane] = as4(z);
+                if (j <= tile)
+                    mine = mfma4(mv[j], sr[j][lane], mine);
+            sv[tile][lane] = as4(mine);
+            sw[tile][lane] = as4(mine) * left;
+            load_matrix(next);
+        } else {
+            mine = with_state();
+            mine = v4f{scaled.x * mine[0], scaled.y * mine[1], scaled.z * mine[2], scaled.w * mine[3]};
+            load_rows(next);
         }
-        v4f o = {go.x * q0[0], go.y * q0[1], go.z * q0[2], go.w * q0[3]};
+        __syncthreads();
 #pragma unroll
-        for (int j = 0; j < TILES; j++)
-            if (j <= wave)
-                o = mfma4(po[j], sv[j][lane], o);
+        for (int t0 = 0; t0 < NT; t0 += 8) {
+            const int t = t0 + wave;
+            if (t < NT) {
+                const float4 o = ss[t][lane];
+                v4f z[2] = {v4f{end * o.x, end * o.y, end * o.z, end * o.w}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-        for (int r = 0; r < 4; r++)
-            if (row + 4 * g + r < last)
-                a.o[(row + 4 * g + r) * a.o_ld + h * a.v_dim + col] = o[r];
+                for (int j = 0; j < TILES; j++)
+                    z[j & 1] = mfma4(float4{sk[16 * j + 4 * g][16 * t + c], sk[16 * j + 4 * g + 1][16 * t + c], sk[16 * j + 4 * g + 2][16 * t + c],
+                                            sk[16 * j + 4 * g + 3][16 * t + c]},
+                                     sw[j][lane], z[j & 1]);
+                ss[t][lane] = as4(z[0] + z[1]);
+            }
+        }
+        if (!keys) {
+#pragma unroll
+            for (int j = 0; j < TILES; j++)
+                if (j <= tile)
+                    mine = mfma4(mv[j], sv[j][lane], mine);
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                if (row + 4 * g + r < last)
+                    a.o[(row + 4 * g + r) * a.o_ld + h * a.v_dim + col] = mine[r];
+            load_matrix(next);
+        }
         __syncthreads();
     }
-#pragma unroll
-    for (int t = wave; t < NT; t += 4) {
+    for (int t = wave; t < NT; t += 8) {
         float *p = a.s_out + state + (16 * t + 4 * g) * a.v_dim;
         const float4 z = ss[t][lane];
         p[0] = z.x, p[a.v_dim] = z.y, p[2 * a.v_dim] = z.z, p[3 * a.v_dim] = z.w;
@@ -528,7 +571,7 @@ static void launch_delta(hipStream_t s, const rt_seqs &b, const rt_delta &a, flo
     for (long from = 0; from < all; from += most) {
         const long count = all - from < most ? all - from : most;
         delta_prep_k<DK><<<dim3((unsigned)count, (unsigned)a.k_heads), 256, 0, s>>>(b, a, SHORT, from, prep);
-        delta_chunk_k<DK><<<dim3((unsigned)(units * (a.v_dim / 16))), 256, 0, s>>>(b, a, SHORT, from, count, prep);
+        delta_chunk_k<DK><<<dim3((unsigned)(units * (a.v_dim / 16))), CHUNK_THREADS, 0, s>>>(b, a, SHORT, from, count, prep);
     }
 }
 
