@@ -10,6 +10,13 @@ __device__ __forceinline__ float decay_of(float a, float dt, float rate)
     return expf(rate * (fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x)))));
 }
 
+/* nw * (o * r) * SiLU(z) */
+__device__ __forceinline__ float4 gated(float4 o, float r, float4 w, float4 z)
+{
+    return float4{w.x * (o.x * r) * (z.x * q8_sigmoid(z.x)), w.y * (o.y * r) * (z.y * q8_sigmoid(z.y)), w.z * (o.z * r) * (z.z * q8_sigmoid(z.z)),
+                  w.w * (o.w * r) * (z.w * q8_sigmoid(z.w))};
+}
+
 /* Token by token. A wave owns 16 columns of a head's state: lane 16 c + g holds rows g*KR .. g*KR + KR - 1
  * of columns 4 c .. 4 c + 3, so a column's dot products go over a row of 16 lanes. Both products with
  * the state are taken before it changes, in one reduction:
@@ -328,8 +335,8 @@ __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int m
  * rows 16 v .., 16 (v + 8) ... The state stays in LDS from chunk to chunk. A chunk, with a barrier behind each
  * line (the second half's work stands in brackets):
  *
- *   R = V - gamma K S0
- *   d = T R, D_C d                                 [gamma Q S0]
+ *   R = V - gamma K S0                             [Q S0, half of it]
+ *   d = T R, D_C d                                 [the other half]
  *   S = gamma_C S0 + K^T (D_C d)                   [the same, and O = gamma Q S0 + P d]
  *
  * What a wave needs of the next chunk is loaded as soon as this one's has been used. The workgroups of a head are
@@ -340,203 +347,297 @@ __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int m
 constexpr int CHUNK_THREADS = 512;
 
 template <int DK>
-__global__ __launch_bounds__(CHUNK_THREADS) void delta_chunk_k(rt_seqs b, rt_delta a, int most, long from, long count, const float *prep)
+struct chunk_lds {
+    float sk[DK][CHUNK + 4];                                          /* the chunk's keys, transposed */
+    float4 ss[DK / 16][64], sr[TILES][64], sv[TILES][64], sw[TILES][64]; /* S0, R, d, D_C d as results lie */
+    float red[5][8][16];
+    int odd;
+};
+
+/* A workgroup's unit: columns col - c .. + 15 of head h of sequence s, chunks [c0, c1) of it */
+struct chunk_unit {
+    long first, last, slot, h, kh, col, c0, c1;
+    int slice, slices;
+};
+
+/* A chunk token by token, on the state in LDS: the thread has rows 16 t + 4 g .. + 3, t = wave, wave + 8, ..., of
+ * column c */
+template <int DK>
+__device__ __forceinline__ void odd_chunk(const rt_delta &a, const chunk_unit &u, chunk_lds<DK> &m, long n)
 {
-    constexpr int NT = DK / 16, LK = DK + 4;
-    __shared__ __align__(16) float sk[CHUNK][LK];
-    __shared__ __align__(16) float4 ss[NT][64], sr[TILES][64], sv[TILES][64], sw[TILES][64];
-    __shared__ float red[5][8][16];
-    __shared__ int sodd;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
-    const bool keys = wave < 4;
-    const int tile = keys ? wave : 7 - wave;
-    const int slices = (int)(a.v_dim / 16), x = (int)(blockIdx.x % 8), y = (int)(blockIdx.x / 8), slice = y % slices;
-    const long unit = (long)(y / slices) * 8 + x, s = unit / a.v_heads, h = unit % a.v_heads;
-    if (s >= b.n)
-        return;
-    const long kh = a.tiled ? h % a.k_heads : h / (a.v_heads / a.k_heads);
-    long first, last;
-    q8_rows_of(b, s, first, last);
-    const long slot = slot_of(first, s), chunks = (last - first + CHUNK - 1) / CHUNK;
-    const long c0 = from > slot ? from - slot : 0, c1 = from + count - slot < chunks ? from + count - slot : chunks;
-    if (last - first <= most || c0 >= c1)
-        return;
-    const long col = 16 * slice + c, state = (s * a.v_heads + h) * DK * a.v_dim + col;
-    const float *s_in = c0 == 0 ? a.s_in : a.s_out;
-    for (int t = wave; t < NT; t += 8) {
-        const float *p = s_in + state + (16 * t + 4 * g) * a.v_dim;
-        ss[t][lane] = float4{p[0], p[a.v_dim], p[2 * a.v_dim], p[3 * a.v_dim]};
+    const long from = u.first + n * CHUNK, to = from + CHUNK < u.last ? from + CHUNK : u.last;
+    for (long i = from; i < to; i++) {
+        const float *kp = a.k + i * a.k_ld + u.kh * DK + 4 * g, *qp = a.q + i * a.q_ld + u.kh * DK + 4 * g;
+        float sum[5] = {};
+        for (int t = wave; t < DK / 16; t += 8) {
+            const float4 kj = *(const float4 *)(kp + 16 * t), qj = *(const float4 *)(qp + 16 * t);
+            sum[0] += dot4(kj, m.ss[t][lane]), sum[1] += dot4(qj, m.ss[t][lane]);
+            sum[2] += dot4(kj, kj), sum[3] += dot4(qj, qj), sum[4] += dot4(qj, kj);
+        }
+#pragma unroll
+        for (int k = 0; k < 5; k++) {
+            sum[k] = group_sum(sum[k]);
+            if (g == 0)
+                m.red[k][wave][c] = sum[k];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 5; k++) {
+            sum[k] = 0.0f;
+            for (int w = 0; w < 8; w++)
+                sum[k] += m.red[k][w][c];
+        }
+        const float alpha = decay_of(a.a[i * a.a_ld + u.h], a.dt[u.h], a.decay[u.h]), beta = q8_sigmoid(a.b[i * a.b_ld + u.h]);
+        const float rk = a.eps >= 0.0f ? 1.0f / sqrtf(sum[2] + a.eps) : 1.0f, rq = a.scale * (a.eps >= 0.0f ? 1.0f / sqrtf(sum[3] + a.eps) : 1.0f);
+        const float d = beta * (a.v[i * a.v_ld + u.h * a.v_dim + u.col] - alpha * rk * sum[0]);
+        if (tid < 16)
+            a.o[i * a.o_ld + u.h * a.v_dim + u.col] = fmaf(rq * alpha, sum[1], rq * (rk * sum[4]) * d);
+        for (int t = wave; t < DK / 16; t += 8) {
+            const float4 kj = *(const float4 *)(kp + 16 * t), o = m.ss[t][lane];
+            m.ss[t][lane] = float4{fmaf(rk * kj.x, d, alpha * o.x), fmaf(rk * kj.y, d, alpha * o.y), fmaf(rk * kj.z, d, alpha * o.z), fmaf(rk * kj.w, d, alpha * o.w)};
+        }
+        __syncthreads();
     }
     if (tid == 0)
-        sodd = 0;
+        m.odd = 0;
+    __syncthreads();
+}
 
-    /* the wave's rows of K or Q, of T or P, and their factors: of chunk n, whose rows behind the sequence are 0 */
-    const float *rows = (keys ? a.k : a.q) + kh * DK + 4 * g, *values = a.v + h * a.v_dim + col;
-    const long ld = keys ? a.k_ld : a.q_ld;
-    float4 xv[NT], mv[TILES], factor, decay;
-    float v[4], gamma, odd_in;
+/* The chunks, as one half of the waves sees them. Every load is unconditional (rows behind the sequence's end are
+ * the chunk's first one again, whose products go nowhere), and the halves have loops of their own: under a branch the
+ * compiler no longer knows how many loads are in flight, and waits for those of the next chunk with this one's. */
+template <int DK, bool KEYS>
+__device__ __forceinline__ void chunk_loop(const rt_delta &a, const chunk_unit &u, chunk_lds<DK> &m, const float *prep)
+{
+    constexpr int NT = DK / 16;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+    const int tile = KEYS ? wave : 7 - wave;
+    const long ld = KEYS ? a.k_ld : a.q_ld, part = a.v_heads * (long)PREP;
+    const float *rows = (KEYS ? a.k : a.q) + u.first * ld + u.kh * DK + 4 * g, *values = a.v + u.first * a.v_ld + u.h * a.v_dim + u.col;
+    const float *matrix = prep + u.slot * part + u.h * PREP + ((KEYS ? 0 : PAIRS) + tile * (tile + 1) / 2) * 256 + lane * 4;
+    const float *factors = prep + u.slot * part + u.h * PREP + 2 * PAIRS * 256;
+    const long count = u.last - u.first;
+    float4 xv[NT], mv[TILES], scale, left;
+    float v[4], gamma, odd;
     const auto load_rows = [&](long n) {
-        const long row = first + n * CHUNK + 16 * tile + c;
-        const float *p = rows + (row < last ? row : first) * ld;
+        const long i = n * CHUNK + 16 * tile + c;
+        const float *p = rows + (i < count ? i : n * CHUNK) * ld;
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
+        for (int t = 0; t < NT; t++)
             xv[t] = *(const float4 *)(p + 16 * t);
-            if (row >= last)
-                xv[t] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+        scale = *(const float4 *)(factors + n * part + (KEYS ? 0 : CHUNK) + 16 * tile + 4 * g);
+        if constexpr (KEYS) {
+            odd = factors[n * part + 3 * CHUNK + 4 + wave];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const long k = n * CHUNK + 16 * tile + 4 * g + r;
+                v[r] = values[(k < count ? k : n * CHUNK) * a.v_ld];
+            }
         }
     };
-    const auto part = [&](long n) { return prep + ((slot + n - from) * a.v_heads + h) * PREP; };
     const auto load_matrix = [&](long n) {
-        const float *p = part(n) + ((keys ? 0 : PAIRS) + tile * (tile + 1) / 2) * 256 + lane * 4;
 #pragma unroll
         for (int j = 0; j < TILES; j++)
-            if (j <= tile)
-                mv[j] = *(const float4 *)(p + j * 256);
+            mv[j] = *(const float4 *)(matrix + n * part + (j < tile ? j : tile) * 256);
+        if constexpr (KEYS)
+            left = *(const float4 *)(factors + n * part + 2 * CHUNK + 16 * tile + 4 * g);
     };
-    const auto load_factors = [&](long n) {
-        const float *p = part(n) + 2 * PAIRS * 256;
-        factor = *(const float4 *)(p + (keys ? 0 : CHUNK) + 16 * tile + 4 * g);
-        decay = *(const float4 *)(p + 2 * CHUNK + 16 * tile + 4 * g);
-        gamma = p[3 * CHUNK];
-        odd_in = p[3 * CHUNK + 4 + (wave & 3)];
-        const long row = first + n * CHUNK + 16 * tile + 4 * g;
-        if (keys)
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-                v[r] = row + r < last ? values[(row + r) * a.v_ld] : 0.0f;
+    /* Into the XCD's L2, two chunks ahead: the head's workgroups there take a share of the chunk's lines each (128
+     * bytes: its keys, its queries, its part of prep), and the last wave the rows of V that are its own. Loads that
+     * find their lines there come back within a line of the chunk; from HBM they did not. */
+    float ahead = 0.0f;
+    const auto fetch = [&](long n) {
+        constexpr int ROW = DK / 32, SHARED = 2 * CHUNK * ROW + PREP_BYTES / 128;
+        const long i0 = n * CHUNK, rest = count - i0;
+        int l = u.slice + u.slices * ((wave - 4) * 64 + lane);
+        const float *p = nullptr;
+        if (wave == 7) {
+            p = values + (i0 + (lane < rest ? lane : 0)) * a.v_ld - c;
+        } else if (l < 2 * CHUNK * ROW) {
+            const bool q = l >= CHUNK * ROW;
+            l -= q ? CHUNK * ROW : 0;
+            const long i = i0 + (l / ROW < rest ? l / ROW : 0);
+            p = (q ? a.q + (u.first + i) * a.q_ld : a.k + (u.first + i) * a.k_ld) + u.kh * DK + l % ROW * 32;
+        } else if (l < SHARED) {
+            p = prep + (u.slot + n) * part + u.h * PREP + (l - 2 * CHUNK * ROW) * 32;
+        }
+        if (p)
+            ahead = *p;
     };
-    load_rows(c0);
-    load_factors(c0);
-    load_matrix(c0);
+    if constexpr (KEYS)
+        __builtin_amdgcn_s_setprio(1); /* the chain from state to state is theirs */
+    load_rows(u.c0);
+    load_matrix(u.c0);
+    gamma = factors[u.c0 * part + 3 * CHUNK];
     __syncthreads();
-    for (long n = c0; n < c1; n++) {
-        const long row = first + n * CHUNK + 16 * tile, next = n + 1 < c1 ? n + 1 : n;
-        const auto with_state = [&]() {
-            v4f z[2] = {v4f{0.0f, 0.0f, 0.0f, 0.0f}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
+    for (long n = u.c0; n < u.c1; n++) {
+        const long next = n + 1 < u.c1 ? n + 1 : n;
+        v4f z = {0.0f, 0.0f, 0.0f, 0.0f};
+        const int here = (int)(count - n * CHUNK < CHUNK ? count - n * CHUNK : CHUNK) - 16 * tile - 4 * g; /* rows from 4 g on that there are */
+        if constexpr (KEYS) {
 #pragma unroll
             for (int t = 0; t < NT; t++)
-                z[t & 1] = mfma4(xv[t], ss[t][lane], z[t & 1]);
-            return z[0] + z[1];
-        };
-        const float end = gamma;
-        float4 scaled = factor, left = decay;
-        v4f mine = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (keys) {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    m.sk[16 * t + 4 * g + e][16 * tile + c] = (&xv[t].x)[e];
+            v4f y[2] = {z, z};
 #pragma unroll
             for (int t = 0; t < NT; t++)
-                *(float4 *)&sk[16 * tile + c][16 * t + 4 * g] = xv[t];
-            if (__ballot(odd_in != 0.0f || !finite4(float4{v[0], v[1], v[2], v[3]})) && lane == 0)
-                sodd = 1;
-            const v4f z = with_state();
-            sr[tile][lane] = float4{fmaf(-scaled.x, z[0], v[0]), fmaf(-scaled.y, z[1], v[1]), fmaf(-scaled.z, z[2], v[2]), fmaf(-scaled.w, z[3], v[3])};
+                y[t & 1] = mfma4(xv[t], m.ss[t][lane], y[t & 1]);
+            y[0] += y[1];
+            if (__ballot(odd != 0.0f || !finite4(float4{v[0], v[1], v[2], v[3]})) && lane == 0)
+                m.odd = 1;
+            m.sr[tile][lane] = float4{here > 0 ? fmaf(-scale.x, y[0][0], v[0]) : 0.0f, here > 1 ? fmaf(-scale.y, y[0][1], v[1]) : 0.0f,
+                                      here > 2 ? fmaf(-scale.z, y[0][2], v[2]) : 0.0f, here > 3 ? fmaf(-scale.w, y[0][3], v[3]) : 0.0f};
             load_rows(next);
-        }
-        load_factors(next);
-        __syncthreads();
-        if (sodd) {
-            /* token by token: the thread has rows 16 t + 4 g .. + 3, t = wave, wave + 8, ..., of column c */
-            const int tokens = (int)(last - (first + n * CHUNK) < CHUNK ? last - (first + n * CHUNK) : CHUNK);
-            for (int j = 0; j < tokens; j++) {
-                const long i = first + n * CHUNK + j;
-                float sum[5] = {};
-                for (int t = wave; t < NT; t += 8) {
-                    const float4 kj = *(const float4 *)(a.k + i * a.k_ld + kh * DK + 16 * t + 4 * g), qj = *(const float4 *)(a.q + i * a.q_ld + kh * DK + 16 * t + 4 * g);
-                    sum[0] += dot4(kj, ss[t][lane]), sum[1] += dot4(qj, ss[t][lane]);
-                    sum[2] += dot4(kj, kj), sum[3] += dot4(qj, qj), sum[4] += dot4(qj, kj);
-                }
-                for (int k = 0; k < 5; k++) {
-                    sum[k] = group_sum(sum[k]);
-                    if (g == 0)
-                        red[k][wave][c] = sum[k];
-                }
-                __syncthreads();
-                for (int k = 0; k < 5; k++) {
-                    sum[k] = 0.0f;
-                    for (int w = 0; w < 8; w++)
-                        sum[k] += red[k][w][c];
-                }
-                const float alpha = decay_of(a.a[i * a.a_ld + h], a.dt[h], a.decay[h]), beta = q8_sigmoid(a.b[i * a.b_ld + h]);
-                const float rk = a.eps >= 0.0f ? 1.0f / sqrtf(sum[2] + a.eps) : 1.0f, rq = a.scale * (a.eps >= 0.0f ? 1.0f / sqrtf(sum[3] + a.eps) : 1.0f);
-                const float d = beta * (a.v[i * a.v_ld + h * a.v_dim + col] - alpha * rk * sum[0]);
-                if (tid < 16)
-                    a.o[i * a.o_ld + h * a.v_dim + col] = fmaf(rq * alpha, sum[1], rq * (rk * sum[4]) * d);
-                for (int t = wave; t < NT; t += 8) {
-                    const float4 kj = *(const float4 *)(a.k + i * a.k_ld + kh * DK + 16 * t + 4 * g), o = ss[t][lane];
-                    ss[t][lane] = float4{fmaf(rk * kj.x, d, alpha * o.x), fmaf(rk * kj.y, d, alpha * o.y), fmaf(rk * kj.z, d, alpha * o.z), fmaf(rk * kj.w, d, alpha * o.w)};
-                }
-                __syncthreads();
-            }
-            if (tid == 0)
-                sodd = 0;
-            if (!keys)
-                load_rows(next);
-            load_matrix(next);
-            __syncthreads();
-            continue;
-        }
-        if (keys) {
-#pragma unroll
-            for (int j = 0; j < TILES; j++)
-                if (j <= tile)
-                    mine = mfma4(mv[j], sr[j][lane], mine);
-            sv[tile][lane] = as4(mine);
-            sw[tile][lane] = as4(mine) * left;
-            load_matrix(next);
         } else {
-            mine = with_state();
-            mine = v4f{scaled.x * mine[0], scaled.y * mine[1], scaled.z * mine[2], scaled.w * mine[3]};
-            load_rows(next);
+            asm volatile("" : : "v"(ahead));
+            fetch(n + 2 < u.c1 ? n + 2 : n);
+#pragma unroll
+            for (int t = 0; t < NT / 2; t++)
+                z = mfma4(xv[t], m.ss[t][lane], z);
         }
         __syncthreads();
-#pragma unroll
-        for (int t0 = 0; t0 < NT; t0 += 8) {
-            const int t = t0 + wave;
-            if (t < NT) {
-                const float4 o = ss[t][lane];
-                v4f z[2] = {v4f{end * o.x, end * o.y, end * o.z, end * o.w}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
+        const bool whole = __builtin_amdgcn_readfirstlane(m.odd) == 0;
+        if (!whole)
+            odd_chunk(a, u, m, n);
+        if constexpr (KEYS) {
+            if (whole) {
 #pragma unroll
                 for (int j = 0; j < TILES; j++)
-                    z[j & 1] = mfma4(float4{sk[16 * j + 4 * g][16 * t + c], sk[16 * j + 4 * g + 1][16 * t + c], sk[16 * j + 4 * g + 2][16 * t + c],
-                                            sk[16 * j + 4 * g + 3][16 * t + c]},
-                                     sw[j][lane], z[j & 1]);
-                ss[t][lane] = as4(z[0] + z[1]);
+                    if (j <= tile)
+                        z = mfma4(mv[j], m.sr[j][lane], z);
+                m.sv[tile][lane] = as4(z);
+                m.sw[tile][lane] = as4(z) * left;
             }
-        }
-        if (!keys) {
-#pragma unroll
-            for (int j = 0; j < TILES; j++)
-                if (j <= tile)
-                    mine = mfma4(mv[j], sv[j][lane], mine);
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-                if (row + 4 * g + r < last)
-                    a.o[(row + 4 * g + r) * a.o_ld + h * a.v_dim + col] = mine[r];
             load_matrix(next);
+        } else {
+            if (whole) {
+#pragma unroll
+                for (int t = NT / 2; t < NT; t++)
+                    z = mfma4(xv[t], m.ss[t][lane], z);
+                z = v4f{scale.x * z[0], scale.y * z[1], scale.z * z[2], scale.w * z[3]};
+            }
+            load_rows(next);
+        }
+        __syncthreads();
+        if (whole) {
+#pragma unroll
+            for (int t0 = 0; t0 < NT; t0 += 8) {
+                const int t = t0 + wave;
+                if (t < NT) {
+                    const float4 o = m.ss[t][lane];
+                    v4f s[2] = {v4f{gamma * o.x, gamma * o.y, gamma * o.z, gamma * o.w}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+                    for (int j = 0; j < TILES; j++)
+                        s[j & 1] = mfma4(*(const float4 *)&m.sk[16 * t + c][16 * j + 4 * g], m.sw[j][lane], s[j & 1]);
+                    m.ss[t][lane] = as4(s[0] + s[1]);
+                }
+            }
+            if constexpr (!KEYS)
+#pragma unroll
+                for (int j = 0; j < TILES; j++)
+                    if (j <= tile)
+                        z = mfma4(mv[j], m.sv[j][lane], z);
+        }
+        gamma = factors[next * part + 3 * CHUNK];
+        if constexpr (!KEYS) {
+            load_matrix(next);
+            float *o = a.o + (u.first + n * CHUNK + 16 * tile + 4 * g) * a.o_ld + u.h * a.v_dim + u.col;
+            if (whole)
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    if (r < here)
+                        o[r * a.o_ld] = z[r];
         }
         __syncthreads();
     }
-    for (int t = wave; t < NT; t += 8) {
+}
+
+template <int DK>
+__global__ __launch_bounds__(CHUNK_THREADS) void delta_chunk_k(rt_seqs b, rt_delta a, int most, long from, long count, const float *prep)
+{
+    __shared__ __align__(16) chunk_lds<DK> m;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
+    const int slices = (int)(a.v_dim / 16), x = (int)(blockIdx.x % 8), y = (int)(blockIdx.x / 8), slice = y % slices;
+    const long unit = (long)(y / slices) * 8 + x, s = unit / a.v_heads;
+    if (s >= b.n)
+        return;
+    chunk_unit u;
+    u.h = unit % a.v_heads;
+    u.kh = a.tiled ? u.h % a.k_heads : u.h / (a.v_heads / a.k_heads);
+    q8_rows_of(b, s, u.first, u.last);
+    const long slot = slot_of(u.first, s), chunks = (u.last - u.first + CHUNK - 1) / CHUNK;
+    u.slot = slot - from; /* of chunk 0, in this launch's parts */
+    u.c0 = from > slot ? from - slot : 0;
+    u.c1 = from + count - slot < chunks ? from + count - slot : chunks;
+    if (u.last - u.first <= most || u.c0 >= u.c1)
+        return;
+    u.col = 16 * slice + c;
+    u.slice = slice, u.slices = slices;
+    const long state = (s * a.v_heads + u.h) * DK * a.v_dim + u.col;
+    const float *s_in = u.c0 == 0 ? a.s_in : a.s_out;
+    for (int t = wave; t < DK / 16; t += 8) {
+        const float *p = s_in + state + (16 * t + 4 * g) * a.v_dim;
+        m.ss[t][lane] = float4{p[0], p[a.v_dim], p[2 * a.v_dim], p[3 * a.v_dim]};
+    }
+    if (tid == 0)
+        m.odd = 0;
+    if (wave < 4)
+        chunk_loop<DK, true>(a, u, m, prep);
+    else
+        chunk_loop<DK, false>(a, u, m, prep);
+    for (int t = wave; t < DK / 16; t += 8) {
         float *p = a.s_out + state + (16 * t + 4 * g) * a.v_dim;
-        const float4 z = ss[t][lane];
+        const float4 z = m.ss[t][lane];
         p[0] = z.x, p[a.v_dim] = z.y, p[2 * a.v_dim] = z.z, p[3 * a.v_dim] = z.w;
     }
 }
 
-/* o <- nw * o / sqrt(eps + mean(o^2)) * SiLU(z), a wave a head of a token */
-__global__ __launch_bounds__(256) void gated_norm_k(rt_seqs b, rt_delta a)
+/* o <- nw * o / sqrt(eps + mean(o^2)) * SiLU(z), the rows from the first sequence's first to the last one's last. LANES
+ * lanes (a power of two) hold a head, 4 elements each, NV times; NORM_RUN heads a lane one after the other, all loaded
+ * first. Bound by HBM: o and z once, o once. */
+constexpr int NORM_RUN = 4;
+
+template <int NV>
+__global__ __launch_bounds__(256) void gated_norm_k(rt_seqs b, rt_delta a, int lanes)
 {
-    const long i = blockIdx.x, h = 4 * (long)blockIdx.y + (threadIdx.x >> 6);
-    if (q8_sequence_of(b, i) < 0 || h >= a.v_heads)
-        return;
-    const int lane = threadIdx.x & 63;
-    float *o = a.o + i * a.o_ld + h * a.v_dim;
-    const float *z = a.z + i * a.z_ld + h * a.v_dim;
-    float sum = 0.0f;
-    for (long c = lane; c < a.v_dim; c += 64)
-        sum = fmaf(o[c], o[c], sum);
-    const float r = 1.0f / sqrtf(a.nw_eps + q8_wave_sum(sum) / (float)a.v_dim);
-    for (long c = lane; c < a.v_dim; c += 64)
-        o[c] = a.nw[c] * (o[c] * r) * (z[c] * q8_sigmoid(z[c]));
+    const long first = b.start[0] > 0 ? b.start[0] : 0, last = (long)b.start[b.n] < b.t ? b.start[b.n] : b.t, items = (last - first) * a.v_heads;
+    const int per = 256 / lanes, at = 4 * ((int)threadIdx.x & (lanes - 1));
+    const long i0 = (long)blockIdx.x * NORM_RUN * per + (int)threadIdx.x / lanes;
+    float4 o[NORM_RUN][NV], z[NORM_RUN][NV], w[NV];
+    float *to[NORM_RUN];
+#pragma unroll
+    for (int n = 0; n < NV; n++)
+        w[n] = at + 256 * n < a.v_dim ? *(const float4 *)(a.nw + at + 256 * n) : float4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < NORM_RUN; k++) {
+        const long item = i0 + k * per, row = first + (item < items ? item : 0) / a.v_heads, h = (item < items ? item : 0) % a.v_heads;
+        to[k] = item < items ? a.o + row * a.o_ld + h * a.v_dim + at : nullptr;
+#pragma unroll
+        for (int n = 0; n < NV; n++) {
+            o[k][n] = z[k][n] = float4{0.0f, 0.0f, 0.0f, 0.0f};
+            if (to[k] && at + 256 * n < a.v_dim) {
+                o[k][n] = *(const float4 *)(to[k] + 256 * n);
+                z[k][n] = *(const float4 *)(a.z + row * a.z_ld + h * a.v_dim + at + 256 * n);
+            }
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < NORM_RUN; k++) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NV; n++)
+            sum += dot4(o[k][n], o[k][n]);
+        for (int m = lanes >> 1; m >= 1; m >>= 1)
+            sum += __shfl_xor(sum, m, 64);
+        const float r = 1.0f / sqrtf(a.nw_eps + sum / (float)a.v_dim);
+#pragma unroll
+        for (int n = 0; n < NV; n++)
+            if (to[k] && at + 256 * n < a.v_dim)
+                *(float4 *)(to[k] + 256 * n) = gated(o[k][n], r, w[n], z[k][n]);
+    }
 }
 
 } /* namespace */
@@ -591,6 +692,15 @@ void q8_launch_delta(q8_stream_t stream, const rt_seqs &b, const rt_delta &a, fl
         KDIM(256)
 #undef KDIM
     }
-    if (a.z)
-        gated_norm_k<<<dim3((unsigned)b.t, (unsigned)((a.v_heads + 3) / 4)), 256, 0, s>>>(b, a);
+    if (a.z) {
+        int lanes = 4;
+        while (lanes < 64 && 4 * lanes < a.v_dim)
+            lanes *= 2;
+        const long a_block = NORM_RUN * (256 / lanes);
+        const dim3 grid((unsigned)((b.t * a.v_heads + a_block - 1) / a_block));
+        if (a.v_dim > 256)
+            gated_norm_k<2><<<grid, 256, 0, s>>>(b, a, lanes);
+        else
+            gated_norm_k<1><<<grid, 256, 0, s>>>(b, a, lanes);
+    }
 }
