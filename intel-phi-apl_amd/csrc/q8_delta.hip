@@ -10,6 +10,7 @@ __device__ __forceinline__ float decay_of(float a, float dt, float rate)
     return expf(rate * (fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x)))));
 }
 
+__device__ __forceinline__ float dot4(float4 x, float4 y) { return fmaf(x.w, y.w, fmaf(x.z, y.z, fmaf(x.y, y.y, x.x * y.x))); }
 /* nw * (o * r) * SiLU(z) */
 __device__ __forceinline__ float4 gated(float4 o, float r, float4 w, float4 z)
 {
@@ -17,72 +18,148 @@ __device__ __forceinline__ float4 gated(float4 o, float r, float4 w, float4 z)
                   w.w * (o.w * r) * (z.w * q8_sigmoid(z.w))};
 }
 
-/* Token by token. A wave owns 16 columns of a head's state: lane 16 c + g holds rows g*KR .. g*KR + KR - 1
- * of columns 4 c .. 4 c + 3, so a column's dot products go over a row of 16 lanes. Both products with
- * the state are taken before it changes, in one reduction:
+/* the sum over each group of G lanes (4, 8 or 16, aligned), in every lane of it */
+template <int G>
+__device__ __forceinline__ float lanes_sum(float v)
+{
+    v += Q8_DPP(v, 0xb1);
+    v += Q8_DPP(v, 0x4e);
+    if (G >= 8)
+        v += Q8_DPP(v, 0x141);
+    if (G >= 16)
+        v += Q8_DPP(v, 0x140);
+    return v;
+}
+
+/* Token by token. A wave owns COLS columns of a head's state, 4 a lane: lane RG c + g has rows g*KR .. g*KR + KR - 1 of
+ * columns 4 c .. 4 c + 3, so a column's dot products go over RG neighbouring lanes. Both products with the state
+ * are taken before it changes, in one reduction:
  *
  *   S' = alpha S + k d^T,  d = beta (v - alpha S^T k),  S'^T q = alpha S^T q + (q.k) d
  *
- * and so are |q|^2, |k|^2 and q.k, whose scales are applied to the results. Bound by HBM (the state, read
- * and written once) on many sequences, by latency on one. */
-template <int KR>
-__global__ __launch_bounds__(64) void delta_step_k(rt_seqs b, rt_delta a, int most)
+ * and so are |q|^2, |k|^2 and q.k, whose scales are applied to the results. The gates of 64 tokens are computed at
+ * once, a lane a token. The next token's rows are loaded while this one's are used, and the first one's before the
+ * state, as loads come back in order. With the output's norm the head's waves are one workgroup (NORM), whose sums of
+ * squares meet in LDS, and each lane gates one column; else each wave is a workgroup.
+ * Bound by HBM (the state, read and written once) on many sequences, by latency on one. 32 columns a wave read whole
+ * 128-byte lines (64 sequences of 32 heads of 128 x 128: 52 us, 5.3 TB/s; with 16 columns 76) and their stores
+ * pass the caches, which would only lose other data to them (57 us otherwise); 16 columns have half the arithmetic a
+ * token and lane, and twice the waves, where there are few. */
+constexpr int STEP_WAVES = 8; /* of a workgroup, at most */
+typedef float v4f __attribute__((ext_vector_type(4)));
+
+template <int DK, int COLS, bool NORM>
+__global__ __launch_bounds__(NORM ? 64 * STEP_WAVES : 64) void delta_step_k(rt_seqs b, rt_delta a, int most)
 {
-    const int lane = threadIdx.x, g = lane & 15, c = 4 * (lane >> 4);
-    const long s = blockIdx.z, h = blockIdx.y, col = 16 * (long)blockIdx.x + c;
+    constexpr int RG = 256 / COLS, KR = DK / RG, W = KR % 4 == 0 ? 4 : 2;
+    __shared__ float squares[2][STEP_WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6, g = lane % RG;
+    const long s = blockIdx.z, h = blockIdx.y, own = COLS * ((long)blockIdx.x * waves + wave) + 4 * (lane / RG), col = own < a.v_dim ? own : 0;
+    const bool live = own < a.v_dim;
     const long kh = a.tiled ? h % a.k_heads : h / (a.v_heads / a.k_heads);
     long first, last;
     q8_rows_of(b, s, first, last);
     if (last - first > most)
         return; /* in chunks */
-    const long base = ((s * a.v_heads + h) * a.k_dim + g * KR) * a.v_dim + col;
+    float q[KR], k[KR], qn[KR], kn[KR], z = 0.0f, zn = 0.0f;
+    float4 v, vn;
+    const auto load = [&](long i) {
+        const float *qp = a.q + i * a.q_ld + kh * DK + g * KR, *kp = a.k + i * a.k_ld + kh * DK + g * KR;
+#pragma unroll
+        for (int r = 0; r < KR; r += W)
+            if constexpr (W == 4)
+                *(float4 *)(qn + r) = *(const float4 *)(qp + r), *(float4 *)(kn + r) = *(const float4 *)(kp + r);
+            else
+                *(float2 *)(qn + r) = *(const float2 *)(qp + r), *(float2 *)(kn + r) = *(const float2 *)(kp + r);
+        vn = *(const float4 *)(a.v + i * a.v_ld + h * a.v_dim + col);
+        if (NORM)
+            zn = a.z[i * a.z_ld + h * a.v_dim + col + (g & 3)];
+    };
+    const float rate = a.decay[h], dt = a.dt[h];
+    float ga = 0.0f, gb = 0.0f;
+    if (first < last) {
+        const long i = first + lane < last ? first + lane : first;
+        ga = a.a[i * a.a_ld + h], gb = a.b[i * a.b_ld + h];
+        load(first);
+    }
+    const float w = NORM ? a.nw[col + (g & 3)] : 0.0f;
+    const long base = ((s * a.v_heads + h) * DK + g * KR) * a.v_dim + col;
     float4 st[KR];
 #pragma unroll
     for (int r = 0; r < KR; r++)
         st[r] = *(const float4 *)(a.s_in + base + r * a.v_dim);
-    const float rate = a.decay[h], dt = a.dt[h];
-    for (long i = first; i < last; i++) {
-        float q[KR], k[KR];
-#pragma unroll
-        for (int r = 0; r < KR; r += 2) {
-            *(float2 *)(q + r) = *(const float2 *)(a.q + i * a.q_ld + kh * a.k_dim + g * KR + r);
-            *(float2 *)(k + r) = *(const float2 *)(a.k + i * a.k_ld + kh * a.k_dim + g * KR + r);
+    for (long i0 = first; i0 < last; i0 += 64) {
+        if (i0 > first) {
+            const long i = i0 + lane < last ? i0 + lane : i0;
+            ga = a.a[i * a.a_ld + h], gb = a.b[i * a.b_ld + h];
         }
-        const float4 v = *(const float4 *)(a.v + i * a.v_ld + h * a.v_dim + col);
-        const float alpha = decay_of(a.a[i * a.a_ld + h], dt, rate), beta = q8_sigmoid(a.b[i * a.b_ld + h]);
-        float qq = 0.0f, kk = 0.0f, qk = 0.0f;
-        float4 sq = {0.0f, 0.0f, 0.0f, 0.0f}, sk = sq;
+        const int alphas = __builtin_bit_cast(int, decay_of(ga, dt, rate)), betas = __builtin_bit_cast(int, q8_sigmoid(gb));
+        const int count = (int)(last - i0 < 64 ? last - i0 : 64);
+        for (int j = 0; j < count; j++) {
+            const long i = i0 + j;
 #pragma unroll
-        for (int r = 0; r < KR; r++) {
-            qq = fmaf(q[r], q[r], qq);
-            kk = fmaf(k[r], k[r], kk);
-            qk = fmaf(q[r], k[r], qk);
-            sq = float4{fmaf(st[r].x, q[r], sq.x), fmaf(st[r].y, q[r], sq.y), fmaf(st[r].z, q[r], sq.z), fmaf(st[r].w, q[r], sq.w)};
-            sk = float4{fmaf(st[r].x, k[r], sk.x), fmaf(st[r].y, k[r], sk.y), fmaf(st[r].z, k[r], sk.z), fmaf(st[r].w, k[r], sk.w)};
-        }
-        qk = q8_row_sum(qk);
-        sq = float4{q8_row_sum(sq.x), q8_row_sum(sq.y), q8_row_sum(sq.z), q8_row_sum(sq.w)};
-        sk = float4{q8_row_sum(sk.x), q8_row_sum(sk.y), q8_row_sum(sk.z), q8_row_sum(sk.w)};
-        float rq = 1.0f, rk = 1.0f;
-        if (a.eps >= 0.0f) {
-            rq = 1.0f / sqrtf(q8_row_sum(qq) + a.eps);
-            rk = 1.0f / sqrtf(q8_row_sum(kk) + a.eps);
-        }
-        const float ak = alpha * rk;
-        const float4 d = {beta * (v.x - ak * sk.x), beta * (v.y - ak * sk.y), beta * (v.z - ak * sk.z), beta * (v.w - ak * sk.w)};
-        const float oq = a.scale * rq, od = oq * (rk * qk), oa = oq * alpha;
-        if (g == 0)
-            *(float4 *)(a.o + i * a.o_ld + h * a.v_dim + col) =
-                float4{fmaf(oa, sq.x, od * d.x), fmaf(oa, sq.y, od * d.y), fmaf(oa, sq.z, od * d.z), fmaf(oa, sq.w, od * d.w)};
+            for (int r = 0; r < KR; r++)
+                q[r] = qn[r], k[r] = kn[r];
+            v = vn, z = zn;
+            load(i + 1 < last ? i + 1 : i);
+            const float alpha = __builtin_bit_cast(float, __builtin_amdgcn_readlane(alphas, j)), beta = __builtin_bit_cast(float, __builtin_amdgcn_readlane(betas, j));
+            float qq = 0.0f, kk = 0.0f, qk = 0.0f;
+            float4 sq = {0.0f, 0.0f, 0.0f, 0.0f}, sk = sq;
 #pragma unroll
-        for (int r = 0; r < KR; r++) {
-            const float kr = rk * k[r];
-            st[r] = float4{fmaf(kr, d.x, alpha * st[r].x), fmaf(kr, d.y, alpha * st[r].y), fmaf(kr, d.z, alpha * st[r].z), fmaf(kr, d.w, alpha * st[r].w)};
+            for (int r = 0; r < KR; r++) {
+                qq = fmaf(q[r], q[r], qq);
+                kk = fmaf(k[r], k[r], kk);
+                qk = fmaf(q[r], k[r], qk);
+                sq = float4{fmaf(st[r].x, q[r], sq.x), fmaf(st[r].y, q[r], sq.y), fmaf(st[r].z, q[r], sq.z), fmaf(st[r].w, q[r], sq.w)};
+                sk = float4{fmaf(st[r].x, k[r], sk.x), fmaf(st[r].y, k[r], sk.y), fmaf(st[r].z, k[r], sk.z), fmaf(st[r].w, k[r], sk.w)};
+            }
+            float rq = 1.0f, rk = 1.0f;
+            if (a.eps >= 0.0f) {
+                rq = 1.0f / sqrtf(lanes_sum<RG>(qq) + a.eps);
+                rk = 1.0f / sqrtf(lanes_sum<RG>(kk) + a.eps);
+            }
+            qk = lanes_sum<RG>(qk);
+            sk = float4{lanes_sum<RG>(sk.x), lanes_sum<RG>(sk.y), lanes_sum<RG>(sk.z), lanes_sum<RG>(sk.w)};
+            sq = float4{lanes_sum<RG>(sq.x), lanes_sum<RG>(sq.y), lanes_sum<RG>(sq.z), lanes_sum<RG>(sq.w)};
+            const float ak = alpha * rk;
+            const float4 d = {beta * (v.x - ak * sk.x), beta * (v.y - ak * sk.y), beta * (v.z - ak * sk.z), beta * (v.w - ak * sk.w)};
+            const float oq = a.scale * rq, od = oq * (rk * qk), oa = oq * alpha;
+            const float4 o = {fmaf(oa, sq.x, od * d.x), fmaf(oa, sq.y, od * d.y), fmaf(oa, sq.z, od * d.z), fmaf(oa, sq.w, od * d.w)};
+            if (NORM) {
+                float sum = live ? dot4(o, o) : 0.0f;
+#pragma unroll
+                for (int m = RG; m < 64; m *= 2)
+                    sum += __shfl_xor(sum, m, 64);
+                if (lane == 0)
+                    squares[j & 1][wave] = sum;
+            }
+#pragma unroll
+            for (int r = 0; r < KR; r++) {
+                const float kr = rk * k[r];
+                st[r] = float4{fmaf(kr, d.x, alpha * st[r].x), fmaf(kr, d.y, alpha * st[r].y), fmaf(kr, d.z, alpha * st[r].z), fmaf(kr, d.w, alpha * st[r].w)};
+            }
+            float *to = a.o + i * a.o_ld + h * a.v_dim + col;
+            if (NORM) {
+                __syncthreads();
+                float sum = 0.0f;
+                for (int n = 0; n < waves; n++)
+                    sum += squares[j & 1][n];
+                const float mine = (g & 2) ? (g & 1 ? o.w : o.z) : (g & 1 ? o.y : o.x);
+                if (g < 4 && live)
+                    to[g] = w * (mine * (1.0f / sqrtf(a.nw_eps + sum / (float)a.v_dim))) * (z * q8_sigmoid(z));
+            } else if (g == 0 && live) {
+                *(float4 *)to = o;
+            }
         }
     }
+    if (live)
 #pragma unroll
-    for (int r = 0; r < KR; r++)
-        *(float4 *)(a.s_out + base + r * a.v_dim) = st[r];
+        for (int r = 0; r < KR; r++) {
+            if (COLS == 32)
+                __builtin_nontemporal_store(v4f{st[r].x, st[r].y, st[r].z, st[r].w}, (v4f *)(a.s_out + base + r * a.v_dim));
+            else
+                *(float4 *)(a.s_out + base + r * a.v_dim) = st[r];
+        }
 }
 
 /* ---- longer sequences, CHUNK tokens at a time
@@ -108,8 +185,6 @@ constexpr int CHUNK = 64, TILES = CHUNK / 16, PAIRS = TILES * (TILES + 1) / 2;
 constexpr int PREP = 2 * PAIRS * 256 + 4 * CHUNK;
 constexpr int PREP_BYTES = 4 * PREP;
 
-typedef float v4f __attribute__((ext_vector_type(4)));
-
 __device__ __forceinline__ v4f mfma4(float4 x, float4 y, v4f z)
 {
     z = __builtin_amdgcn_mfma_f32_16x16x4f32(x.x, y.x, z, 0, 0, 0);
@@ -118,7 +193,6 @@ __device__ __forceinline__ v4f mfma4(float4 x, float4 y, v4f z)
     return __builtin_amdgcn_mfma_f32_16x16x4f32(x.w, y.w, z, 0, 0, 0);
 }
 __device__ __forceinline__ float4 as4(v4f x) { return float4{x[0], x[1], x[2], x[3]}; }
-__device__ __forceinline__ float dot4(float4 x, float4 y) { return fmaf(x.w, y.w, fmaf(x.z, y.z, fmaf(x.y, y.y, x.x * y.x))); }
 __device__ __forceinline__ float group_sum(float v)
 {
     v += __shfl_xor(v, 16, 64);
@@ -596,47 +670,45 @@ __global__ __launch_bounds__(CHUNK_THREADS) void delta_chunk_k(rt_seqs b, rt_del
 }
 
 /* o <- nw * o / sqrt(eps + mean(o^2)) * SiLU(z), the rows from the first sequence's first to the last one's last. LANES
- * lanes (a power of two) hold a head, 4 elements each, NV times; NORM_RUN heads a lane one after the other, all loaded
- * first. Bound by HBM: o and z once, o once. */
+ * lanes (a power of two) hold a head, 4 elements each, NV times, of NORM_RUN rows one after the other, all loaded
+ * first. Bound by HBM: o and z once, o once (8192 rows of 32 heads of 128: 70 us, 5.7 TB/s). */
 constexpr int NORM_RUN = 4;
 
 template <int NV>
 __global__ __launch_bounds__(256) void gated_norm_k(rt_seqs b, rt_delta a, int lanes)
 {
-    const long first = b.start[0] > 0 ? b.start[0] : 0, last = (long)b.start[b.n] < b.t ? b.start[b.n] : b.t, items = (last - first) * a.v_heads;
     const int per = 256 / lanes, at = 4 * ((int)threadIdx.x & (lanes - 1));
-    const long i0 = (long)blockIdx.x * NORM_RUN * per + (int)threadIdx.x / lanes;
+    const long i0 = (long)blockIdx.x * NORM_RUN, own = (long)blockIdx.y * per + (int)threadIdx.x / lanes, h = own < a.v_heads ? own : 0;
     float4 o[NORM_RUN][NV], z[NORM_RUN][NV], w[NV];
-    float *to[NORM_RUN];
-#pragma unroll
-    for (int n = 0; n < NV; n++)
-        w[n] = at + 256 * n < a.v_dim ? *(const float4 *)(a.nw + at + 256 * n) : float4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int k = 0; k < NORM_RUN; k++) {
-        const long item = i0 + k * per, row = first + (item < items ? item : 0) / a.v_heads, h = (item < items ? item : 0) % a.v_heads;
-        to[k] = item < items ? a.o + row * a.o_ld + h * a.v_dim + at : nullptr;
+        const long row = i0 + k < b.t ? i0 + k : i0;
 #pragma unroll
         for (int n = 0; n < NV; n++) {
-            o[k][n] = z[k][n] = float4{0.0f, 0.0f, 0.0f, 0.0f};
-            if (to[k] && at + 256 * n < a.v_dim) {
-                o[k][n] = *(const float4 *)(to[k] + 256 * n);
-                z[k][n] = *(const float4 *)(a.z + row * a.z_ld + h * a.v_dim + at + 256 * n);
-            }
+            const long c = h * a.v_dim + (at + 256 * n < a.v_dim ? at + 256 * n : 0);
+            o[k][n] = *(const float4 *)(a.o + row * a.o_ld + c);
+            z[k][n] = *(const float4 *)(a.z + row * a.z_ld + c);
         }
     }
+#pragma unroll
+    for (int n = 0; n < NV; n++)
+        w[n] = *(const float4 *)(a.nw + (at + 256 * n < a.v_dim ? at + 256 * n : 0));
+    const long first = b.start[0], last = b.start[b.n];
 #pragma unroll
     for (int k = 0; k < NORM_RUN; k++) {
         float sum = 0.0f;
 #pragma unroll
         for (int n = 0; n < NV; n++)
-            sum += dot4(o[k][n], o[k][n]);
+            sum += at + 256 * n < a.v_dim ? dot4(o[k][n], o[k][n]) : 0.0f;
         for (int m = lanes >> 1; m >= 1; m >>= 1)
             sum += __shfl_xor(sum, m, 64);
         const float r = 1.0f / sqrtf(a.nw_eps + sum / (float)a.v_dim);
+        const long row = i0 + k;
+        if (row < b.t && row >= first && row < last && own < a.v_heads)
 #pragma unroll
-        for (int n = 0; n < NV; n++)
-            if (to[k] && at + 256 * n < a.v_dim)
-                *(float4 *)(to[k] + 256 * n) = gated(o[k][n], r, w[n], z[k][n]);
+            for (int n = 0; n < NV; n++)
+                if (at + 256 * n < a.v_dim)
+                    *(float4 *)(a.o + row * a.o_ld + h * a.v_dim + at + 256 * n) = gated(o[k][n], r, w[n], z[k][n]);
     }
 }
 
@@ -660,29 +732,46 @@ long q8_delta_prep_floats(const rt_seqs &b, const rt_delta &a)
     return b.longest > SHORT ? (all < most ? all : most) * a.v_heads * PREP : 0;
 }
 
+/* true where the output's norm and gate were done with it */
 template <int DK>
-static void launch_delta(hipStream_t s, const rt_seqs &b, const rt_delta &a, float *prep)
+static bool launch_delta(hipStream_t s, const rt_seqs &b, const rt_delta &a, float *prep)
 {
     const bool chunked = b.longest > SHORT;
-    const dim3 grid((unsigned)(a.v_dim / 16), (unsigned)a.v_heads, (unsigned)b.n);
-    delta_step_k<DK / 16><<<grid, 64, 0, s>>>(b, a, chunked ? SHORT : 0x7fffffff);
+    const int limit = chunked ? SHORT : 0x7fffffff;
+    const auto waves = [&](int cols) { return (unsigned)((a.v_dim + cols - 1) / cols); };
+    /* 16 columns a wave for several tokens, or as long as that gives no more waves than the GPU has places for two of
+     * each SIMD */
+    const bool few = b.longest > 1 || b.n * a.v_heads * waves(16) <= 2048;
+    /* the norm with it where that leaves no compute unit without a head: on fewer, a head's waves share one, and a launch
+     * more costs less (one sequence of 32 heads, 8 tokens: 21 us with it, 14 apart) */
+    const bool normed = a.z && !chunked && waves(32) <= STEP_WAVES && b.n * a.v_heads >= 256;
+    if (normed && few && waves(16) <= STEP_WAVES)
+        delta_step_k<DK, 16, true><<<dim3(1, (unsigned)a.v_heads, (unsigned)b.n), 64 * waves(16), 0, s>>>(b, a, limit);
+    else if (normed)
+        delta_step_k<DK, 32, true><<<dim3(1, (unsigned)a.v_heads, (unsigned)b.n), 64 * waves(32), 0, s>>>(b, a, limit);
+    else if (few)
+        delta_step_k<DK, 16, false><<<dim3(waves(16), (unsigned)a.v_heads, (unsigned)b.n), 64, 0, s>>>(b, a, limit);
+    else
+        delta_step_k<DK, 32, false><<<dim3(waves(32), (unsigned)a.v_heads, (unsigned)b.n), 64, 0, s>>>(b, a, limit);
     if (!chunked)
-        return;
+        return normed;
     const long all = slots_of(b), most = slots_a_launch(a), units = (b.n * a.v_heads + 7) / 8 * 8;
     for (long from = 0; from < all; from += most) {
         const long count = all - from < most ? all - from : most;
         delta_prep_k<DK><<<dim3((unsigned)count, (unsigned)a.k_heads), 256, 0, s>>>(b, a, SHORT, from, prep);
         delta_chunk_k<DK><<<dim3((unsigned)(units * (a.v_dim / 16))), CHUNK_THREADS, 0, s>>>(b, a, SHORT, from, count, prep);
     }
+    return false;
 }
 
 void q8_launch_delta(q8_stream_t stream, const rt_seqs &b, const rt_delta &a, float *prep)
 {
     const hipStream_t s = (hipStream_t)stream;
+    bool normed = false;
     switch (a.k_dim) {
 #define KDIM(K)                                                                                                                                            \
     case K:                                                                                                                                                \
-        launch_delta<K>(s, b, a, prep);                                                                                                                    \
+        normed = launch_delta<K>(s, b, a, prep);                                                                                                                  \
         break;
         KDIM(32)
         KDIM(64)
@@ -692,12 +781,11 @@ void q8_launch_delta(q8_stream_t stream, const rt_seqs &b, const rt_delta &a, fl
         KDIM(256)
 #undef KDIM
     }
-    if (a.z) {
+    if (a.z && !normed) {
         int lanes = 4;
         while (lanes < 64 && 4 * lanes < a.v_dim)
             lanes *= 2;
-        const long a_block = NORM_RUN * (256 / lanes);
-        const dim3 grid((unsigned)((b.t * a.v_heads + a_block - 1) / a_block));
+        const dim3 grid((unsigned)((b.t + NORM_RUN - 1) / NORM_RUN), (unsigned)((a.v_heads * lanes + 255) / 256));
         if (a.v_dim > 256)
             gated_norm_k<2><<<grid, 256, 0, s>>>(b, a, lanes);
         else
