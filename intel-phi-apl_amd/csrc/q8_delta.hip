@@ -247,18 +247,26 @@ __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int m
     const int n = (int)(last - at < CHUNK ? last - at : CHUNK);
     const int kr = 16 * wave + c, qr = 16 * (3 - wave) + c;
 
+    const int heads = (int)(a.v_heads / a.k_heads);
+    const auto head = [&](int hn) { return a.tiled ? kh + hn * a.k_heads : kh * heads + hn; };
+    float ga, gb, rate, dt; /* the next value head's gates of token `lane` */
+    const auto load_gates = [&](int hn) {
+        const long h = head(hn), i = at + (lane < n ? lane : 0);
+        ga = a.a[i * a.a_ld + h], gb = a.b[i * a.b_ld + h], rate = a.decay[h], dt = a.dt[h];
+    };
     float4 qv[NT], kv[NT];
     float kk = 0.0f, qq = 0.0f;
+    const float *kp = a.k + (at + (kr < n ? kr : 0)) * a.k_ld + kh * DK + 4 * g, *qp = a.q + (at + (qr < n ? qr : 0)) * a.q_ld + kh * DK + 4 * g;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-        kv[t] = qv[t] = float4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (kr < n)
-            kv[t] = *(const float4 *)(a.k + (at + kr) * a.k_ld + kh * DK + 16 * t + 4 * g);
-        if (qr < n)
-            qv[t] = *(const float4 *)(a.q + (at + qr) * a.q_ld + kh * DK + 16 * t + 4 * g);
+        kv[t] = *(const float4 *)(kp + 16 * t);
+        qv[t] = *(const float4 *)(qp + 16 * t);
     }
+    load_gates(0);
 #pragma unroll
     for (int t = 0; t < NT; t++) {
+        kv[t] = kr < n ? kv[t] : float4{0.0f, 0.0f, 0.0f, 0.0f};
+        qv[t] = qr < n ? qv[t] : float4{0.0f, 0.0f, 0.0f, 0.0f};
         *(float4 *)&sk[kr][16 * t + 4 * g] = kv[t];
         kk += dot4(kv[t], kv[t]);
         qq += dot4(qv[t], qv[t]);
@@ -285,26 +293,33 @@ __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int m
 
     __syncthreads(); /* the keys' place is the matrices' now */
 
-    const int heads = (int)(a.v_heads / a.k_heads);
     for (int hn = 0; hn < heads; hn++) {
-        const long h = a.tiled ? kh + hn * a.k_heads : kh * heads + hn;
+        const long h = head(hn);
         float *mine = out + ((long)blockIdx.x * a.v_heads + h) * PREP, *factor = mine + 2 * PAIRS * 256;
         /* lane i of every wave: token i's gates */
-        const float alpha = lane < n ? decay_of(a.a[(at + lane) * a.a_ld + h], a.dt[h], a.decay[h]) : 1.0f;
+        const float alpha = lane < n ? decay_of(ga, dt, rate) : 1.0f;
         if (wave == 0)
-            sbeta[lane] = lane < n ? q8_sigmoid(a.b[(at + lane) * a.b_ld + h]) : 0.0f;
+            sbeta[lane] = lane < n ? q8_sigmoid(gb) : 0.0f;
+        load_gates(hn + 1 < heads ? hn + 1 : hn);
         {
-            /* the decays between tokens: lane j has column j and goes down to the wave's rows */
-            float d = 1.0f;
-            for (int i = 0; i < 16 * wave; i++) {
-                const float x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, alpha), i));
-                d = i <= lane ? 1.0f : d * x;
-            }
+            /* the decays between tokens, lane j with column j: up to the end of its own 16 rows by a scan from the
+             * back, then by whole 16s, then down the wave's rows */
+            const auto from = [](float v, int i) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), i)); };
+            float rest = alpha; /* alpha_j .. of its 16, to the last */
+#define BACK(ctrl) rest *= __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0x3f800000, __builtin_bit_cast(int, rest), ctrl, 0xf, 0xf, false))
+            BACK(0x101); /* row_shl:1: from the lane behind, 1 beyond the row */
+            BACK(0x102);
+            BACK(0x104);
+            BACK(0x108);
+#undef BACK
+            const float own = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0x3f800000, __builtin_bit_cast(int, rest), 0x101, 0xf, 0xf, false));
+            float d = lane < 16 * wave ? own : 1.0f;
+            for (int k = 1; k < wave; k++)
+                d *= (lane >> 4) < k ? from(rest, 16 * k) : 1.0f;
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 const int i = 16 * wave + r;
-                const float x = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, alpha), i));
-                d = i <= lane ? 1.0f : d * x;
+                d = i <= lane ? 1.0f : d * from(alpha, i);
                 sd[i][lane] = i >= lane ? d : 0.0f;
             }
         }
@@ -550,15 +565,14 @@ __device__ __forceinline__ void chunk_loop(const rt_delta &a, const chunk_unit &
         v4f z = {0.0f, 0.0f, 0.0f, 0.0f};
         const int here = (int)(count - n * CHUNK < CHUNK ? count - n * CHUNK : CHUNK) - 16 * tile - 4 * g; /* rows from 4 g on that there are */
         if constexpr (KEYS) {
+            v4f y[2] = {z, z};
 #pragma unroll
-            for (int t = 0; t < NT; t++)
+            for (int t = 0; t < NT; t++) {
+                y[t & 1] = mfma4(xv[t], m.ss[t][lane], y[t & 1]);
 #pragma unroll
                 for (int e = 0; e < 4; e++)
                     m.sk[16 * t + 4 * g + e][16 * tile + c] = (&xv[t].x)[e];
-            v4f y[2] = {z, z};
-#pragma unroll
-            for (int t = 0; t < NT; t++)
-                y[t & 1] = mfma4(xv[t], m.ss[t][lane], y[t & 1]);
+            }
             y[0] += y[1];
             if (__ballot(odd != 0.0f || !finite4(float4{v[0], v[1], v[2], v[3]})) && lane == 0)
                 m.odd = 1;
