@@ -22,7 +22,8 @@ struct plan {
     paging pg;
     int group;   /* query heads a key-value head */
     int cap;     /* positions that the table reaches */
-    int least;   /* tiles a chunk at least: one load of each wave, 16 positions of F32, 32 of 16 bits */
+    int tile;    /* 16s of positions that a wave takes at once (a power of two): chunks are whole numbers of them */
+    int least;   /* 16s a chunk at least: one tile of each wave */
     int target;  /* chunks (a key-value head) to spread all tiles over; 0: one a row tile */
     int slots;   /* partial results a key-value head */
     float qscale; /* scale * log2 e: scores are in powers of two */
@@ -72,7 +73,7 @@ __device__ __forceinline__ int chunk_of(const rt_seqs &b, const plan &p)
             all += __shfl_xor(all, o, 64);
     }
     const double c = all / p.target + 1.0; /* as far as 2^27 tiles: one a row tile there */
-    return c < p.least ? p.least : c < 1e8 ? first_lane((int)c + 1) & ~1 : 0;
+    return c < p.least ? p.least : c < 1e8 ? (first_lane((int)c) + p.tile - 1) & ~(p.tile - 1) : 0;
 }
 
 /* The sequence whose row tiles' chunks hold number i of all, -1 behind the last; before = the chunks of
@@ -118,6 +119,18 @@ __device__ __forceinline__ void load_words(uint32_t *w, const char *p)
         *w = *(const uint32_t *)p;
 }
 
+/* The same for values, which are read once, in whole lines an instruction: not kept in the caches (32 sequences of 100 to
+ * 16384 positions 220 us, 234 without). A key row's line is read by two instructions, and has to be. */
+template <int WORDS>
+__device__ __forceinline__ void stream_words(uint32_t *w, const char *p)
+{
+    typedef uint32_t words __attribute__((ext_vector_type(WORDS)));
+    const words x = __builtin_nontemporal_load((const words *)p);
+#pragma unroll
+    for (int i = 0; i < WORDS; i++)
+        w[i] = x[i];
+}
+
 /* the largest of a value's copies in lanes l, l ^ 16, l ^ 32, l ^ 48, and their sum */
 __device__ __forceinline__ float group_max(float v)
 {
@@ -131,11 +144,14 @@ __device__ __forceinline__ float group_sum(float v)
 }
 
 /* o's final form: the gate, and what a row that sees nothing gives */
-__device__ __forceinline__ void store_row(const rt_attn &a, long dim, long token, long head, long at, float4 v, float l, bool empty)
+__device__ __forceinline__ float4 gate_of(const rt_attn &a, long token, long head, long at)
+{
+    return a.gate ? *(const float4 *)(a.gate + token * a.gate_ld + head * a.gate_hd + at) : float4{0.0f, 0.0f, 0.0f, 0.0f};
+}
+__device__ __forceinline__ void store_row(const rt_attn &a, long dim, long token, long head, long at, float4 v, float l, bool empty, float4 g)
 {
     v = empty ? float4{0.0f, 0.0f, 0.0f, 0.0f} : float4{v.x / l, v.y / l, v.z / l, v.w / l};
     if (a.gate) {
-        const float4 g = *(const float4 *)(a.gate + token * a.gate_ld + head * a.gate_hd + at);
         v = float4{v.x * q8_sigmoid(g.x), v.y * q8_sigmoid(g.y), v.z * q8_sigmoid(g.z), v.w * q8_sigmoid(g.w)};
     }
     *(float4 *)(a.o + token * a.o_ld + head * dim + at) = v;
@@ -282,7 +298,7 @@ __device__ __forceinline__ void finish(char *lds, const rt_kv &kv, const rt_attn
         if (pos >= p.cap)
             sum = NAN; /* a position that the table does not reach */
         if (u.q.chunks == 1) {
-            store_row(a, D, u.q.first + jr, hr, d, v, sum, pos < 0);
+            store_row(a, D, u.q.first + jr, hr, d, v, sum, pos < 0, gate_of(a, u.q.first + jr, hr, d));
         } else {
             const long slot = (long)kh * p.slots + number;
             *(float4 *)(p.part + (slot * 16 + r) * D + d) = v;
@@ -310,14 +326,6 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
         share u;
         if (!share_of(b, kv, p, chunk, number, u))
             return;
-        float qv[NK][4];
-#pragma unroll
-        for (int i = 0; i < NK; i++) {
-            float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (u.live)
-                v = *(const float4 *)(a.q + (long)(u.q.first + u.j) * a.q_ld + u.h * a.q_hd + (i * 4 + g) * 4);
-            qv[i][0] = v.x * p.qscale, qv[i][1] = v.y * p.qscale, qv[i][2] = v.z * p.qscale, qv[i][3] = v.w * p.qscale;
-        }
         v4f acc[VE];
 #pragma unroll
         for (int i = 0; i < VE; i++)
@@ -338,6 +346,14 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
             entry = entry_of(kv, p, u.table, here(tile + WAVES));
             load_k(kw, row_now);
         }
+        float qv[NK][4];
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+            float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (u.live)
+                v = *(const float4 *)(a.q + (long)(u.q.first + u.j) * a.q_ld + u.h * a.q_hd + (i * 4 + g) * 4);
+            qv[i][0] = v.x * p.qscale, qv[i][1] = v.y * p.qscale, qv[i][2] = v.z * p.qscale, qv[i][3] = v.w * p.qscale;
+        }
         for (; tile < stop; tile += WAVES) {
             int rows[4];
 #pragma unroll
@@ -346,7 +362,7 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
                 const char *at = address(kv.v, rows[r], head_rows, D * 4) + c * VEC * 4;
 #pragma unroll
                 for (int i = 0; i < NV; i++)
-                    load_words<VEC>(vw[r][i], at + i * 16 * VEC * 4);
+                    stream_words<VEC>(vw[r][i], at + i * 16 * VEC * 4);
             }
             v4f s[2] = {v4f{0.0f, 0.0f, 0.0f, 0.0f}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
@@ -404,7 +420,7 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
     }
 }
 
-/* A 16-bit cache, 32 positions a tile (two of 16, a and b), on v_mfma_f32_16x16x32: the cache's values are its
+/* A 16-bit cache, 32 or 64 positions a tile, on v_mfma_f32_16x16x32: the cache's values are its
  * operands as they are, and the F32 queries and weights are cut into LIMBS 16-bit values each, every one the
  * rest of those before rounded to nearest: in F16 two of them are off by 2^-24 of the value, in BF16 three by 2^-27,
  * so the products are as exact as F32 ones, at 2/16 and 3/16 of their time. F16 has few exponents: a row of queries
@@ -474,11 +490,17 @@ __device__ __forceinline__ uint32_t larger(uint32_t x, uint32_t y)
     return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u2, x), __builtin_bit_cast(u2, y & 0x7fff7fffu)));
 }
 
+/* 16s of positions a tile: a tile's keys (and values) are 64 registers a lane from heads of 128 up, which then are one wave
+ * a SIMD; smaller heads have two waves, which hold more in flight between them (64 elements, F16, 16 sequences of 500
+ * to 9000: 43 us; with 64 positions a tile, which spills there, 62) */
+constexpr int sixteens(long d) { return d == 128 ? 4 : 2; }
+constexpr bool alone(long d) { return d >= 128; }
+
 template <int D, int TYPE>
-__global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_half_k(rt_seqs b, rt_kv kv, rt_attn a, plan p)
+__global__ __launch_bounds__(64 * WAVES, alone(D) ? 1 : 2) void attn_half_k(rt_seqs b, rt_kv kv, rt_attn a, plan p)
 {
     typedef half_of<TYPE> H;
-    constexpr int LIMBS = H::LIMBS, NK = D / 32, VE = D / 16, VEC = pieces(VE, 8), NV = VE / VEC, VW = VEC / 2;
+    constexpr int LIMBS = H::LIMBS, NK = D / 32, VE = D / 16, VEC = pieces(VE, 8), NV = VE / VEC, VW = VEC / 2, SUB = sixteens(D), POS = 16 * SUB;
     __shared__ __align__(16) char lds[joint_bytes<D>() > NK * LIMBS * 1024 ? joint_bytes<D>() : NK * LIMBS * 1024];
     uint4(*sq)[LIMBS][64] = (uint4(*)[LIMBS][64])lds; /* until the waves join */
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
@@ -488,28 +510,34 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_half_k(rt_se
         share u;
         if (!share_of(b, kv, p, chunk, number, u))
             return;
-        const int stop = (int)(u.t1 + 1) / 2; /* tiles of 32: a chunk is a whole number of them, but for the last */
-        int tile = (int)(u.t0 / 2) + wave, row_a = -1, row_b = -1, entry_a = -1, entry_b = -1;
+        const int stop = (u.t1 + SUB - 1) / SUB; /* tiles: a chunk is a whole number of them, but for the last */
+        int tile = u.t0 / SUB + wave, row[SUB], entry[SUB];
         const auto here = [&](int i) { return i < u.last ? i : u.last; };
-        uint4 ka[NK], kb[NK];
-        const auto load_k = [&](uint4 *kw, int row) {
-            const char *at = address(kv.k, row, head_rows, D * 2) + g * 16;
+        uint4 kx[SUB][NK];
+        const auto load_k = [&]() {
 #pragma unroll
-            for (int i = 0; i < NK; i++)
-                kw[i] = *(const uint4 *)(at + i * 64);
+            for (int n = 0; n < SUB; n++) {
+                const char *at = address(kv.k, row[n], head_rows, D * 2) + g * 16;
+#pragma unroll
+                for (int i = 0; i < NK; i++)
+                    kx[n][i] = *(const uint4 *)(at + i * 64);
+            }
+        };
+        const auto load_entries = [&](int t) {
+#pragma unroll
+            for (int n = 0; n < SUB; n++)
+                entry[n] = entry_of(kv, p, u.table, here(t * POS + 16 * n + c));
         };
         const auto rows_next = [&](int t) {
-            row_a = row_of(kv, p, here(t * 32 + c), entry_a);
-            row_b = row_of(kv, p, here(t * 32 + 16 + c), entry_b);
-            entry_a = entry_of(kv, p, u.table, here((t + WAVES) * 32 + c));
-            entry_b = entry_of(kv, p, u.table, here((t + WAVES) * 32 + 16 + c));
+#pragma unroll
+            for (int n = 0; n < SUB; n++)
+                row[n] = row_of(kv, p, here(t * POS + 16 * n + c), entry[n]);
+            load_entries(t + WAVES);
         };
         if (tile < stop) {
-            entry_a = entry_of(kv, p, u.table, here(tile * 32 + c));
-            entry_b = entry_of(kv, p, u.table, here(tile * 32 + 16 + c));
+            load_entries(tile);
             rows_next(tile);
-            load_k(ka, row_a);
-            load_k(kb, row_b);
+            load_k();
         }
         /* the queries' limbs, the same for every wave: wave w makes those of columns 32 i, i = w, w + WAVES, ... */
         const float *query = a.q + (u.live ? (long)(u.q.first + u.j) * a.q_ld + u.h * a.q_hd : 0) + g * 8;
@@ -551,17 +579,20 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_half_k(rt_se
             acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         float m = -INFINITY, l = 0.0f;
         for (; tile < stop; tile += WAVES) {
-            int rows[8]; /* rows 4 g + r of a, then of b */
-            uint32_t vw[NV][8][VW];
+            int rows[4 * SUB]; /* rows 4 g + r of each 16 */
+            uint32_t vw[NV][4 * SUB][VW];
 #pragma unroll
-            for (int r = 0; r < 8; r++) {
-                rows[r] = __shfl(r < 4 ? row_a : row_b, 4 * g + (r & 3), 64);
+            for (int r = 0; r < 4 * SUB; r++) {
+                rows[r] = __shfl(row[r / 4], 4 * g + r % 4, 64);
                 const char *at = address(kv.v, rows[r], head_rows, D * 2) + c * VEC * 2;
 #pragma unroll
                 for (int i = 0; i < NV; i++)
-                    load_words<VW>(vw[i][r], at + i * 16 * VEC * 2);
+                    stream_words<VW>(vw[i][r], at + i * 16 * VEC * 2);
             }
-            v4f sa = {0.0f, 0.0f, 0.0f, 0.0f}, sb = sa;
+            v4f s[SUB];
+#pragma unroll
+            for (int n = 0; n < SUB; n++)
+                s[n] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
             /* the scheduler is held to one step's limbs ahead: left free it reads them all before the first
              * product, and spills */
             __builtin_amdgcn_sched_barrier(0);
@@ -575,50 +606,58 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_half_k(rt_se
                 for (int n = 0; n < LIMBS && i + 1 < NK; n++)
                     qw[(i + 1) & 1][n] = sq[i + 1][n][lane];
 #pragma unroll
-                for (int n = 0; n < LIMBS; n++) {
-                    sa = H::mfma(ka[i], qw[i & 1][n], sa);
-                    sb = H::mfma(kb[i], qw[i & 1][n], sb);
-                }
+                for (int n = 0; n < LIMBS; n++)
+#pragma unroll
+                    for (int k = 0; k < SUB; k++)
+                        s[k] = H::mfma(kx[k][i], qw[i & 1][n], s[k]);
                 __builtin_amdgcn_sched_barrier(0);
             }
-            const v4f odd = (sa + sb) * 0.0f; /* NaN: a score is infinite or NaN */
+            v4f odd = s[0] * 0.0f; /* NaN: a score is infinite or NaN */
+#pragma unroll
+            for (int n = 1; n < SUB; n++)
+                odd += s[n] * 0.0f;
             if (__ballot(odd[0] + odd[1] + odd[2] + odd[3] != 0.0f)) {
-                sa = v4f{0.0f, 0.0f, 0.0f, 0.0f}, sb = sa;
+#pragma unroll
+                for (int n = 0; n < SUB; n++)
+                    s[n] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int i = 0; i < NK; i++) {
 #pragma unroll
                     for (int n = 0; n < LIMBS; n++) {
                         const uint4 w = sq[i][n][lane];
-                        sa = H::mfma(n ? finite_only<TYPE>(ka[i]) : ka[i], w, sa);
-                        sb = H::mfma(n ? finite_only<TYPE>(kb[i]) : kb[i], w, sb);
+#pragma unroll
+                        for (int k = 0; k < SUB; k++)
+                            s[k] = H::mfma(n ? finite_only<TYPE>(kx[k][i]) : kx[k][i], w, s[k]);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
             if (tile + WAVES < stop) {
                 rows_next(tile + WAVES);
-                load_k(ka, row_a);
-                load_k(kb, row_b);
+                load_k();
             }
-            float x[8];
-            const bool whole = tile * 32 + 31 <= u.least; /* every row sees every position of the tile */
+            const auto place = [&](int r) { return tile * POS + r / 4 * 16 + 4 * g + r % 4; }; /* the lane's positions */
+            float x[4 * SUB];
+            const bool whole = tile * POS + POS - 1 <= u.least; /* every row sees every position of the tile */
             float top = -INFINITY;
 #pragma unroll
-            for (int r = 0; r < 8; r++) {
-                x[r] = rows[r] < 0 ? NAN : back * (r < 4 ? sa[r & 3] : sb[r & 3]);
-                if (!whole && tile * 32 + (r & 4) * 4 + 4 * g + (r & 3) > u.lim)
+            for (int r = 0; r < 4 * SUB; r++) {
+                x[r] = rows[r] < 0 ? NAN : back * s[r / 4][r % 4];
+                if (!whole && place(r) > u.lim)
                     x[r] = -INFINITY;
                 top = fmaxf(top, x[r]);
             }
             const float ref = reference(top, m, l, acc) - H::LIFT;
 #pragma unroll
-            for (int r = 0; r < 8; r++) {
+            for (int r = 0; r < 4 * SUB; r++) {
                 x[r] = __builtin_amdgcn_exp2f(x[r] - ref);
                 l += x[r];
             }
-            uint4 w[LIMBS];
-            limbs_of<TYPE>(x, w);
-            const auto turned = [](const uint32_t(&v)[8][VW], int e) {
+            uint4 w[SUB / 2][LIMBS];
+#pragma unroll
+            for (int k = 0; k < SUB / 2; k++)
+                limbs_of<TYPE>(x + 8 * k, w[k]);
+            const auto turned = [](const uint32_t(*v)[VW], int e) {
                 const uint32_t pick = e & 1 ? 0x07060302u : 0x05040100u;
                 return uint4{__builtin_amdgcn_perm(v[1][e / 2], v[0][e / 2], pick), __builtin_amdgcn_perm(v[3][e / 2], v[2][e / 2], pick),
                              __builtin_amdgcn_perm(v[5][e / 2], v[4][e / 2], pick), __builtin_amdgcn_perm(v[7][e / 2], v[6][e / 2], pick)};
@@ -627,8 +666,8 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_half_k(rt_se
             const bool one = u.j0 == u.j1;
             uint32_t size = 0;
 #pragma unroll
-            for (int r = 0; r < 8; r++) {
-                const bool hide = !whole && one && tile * 32 + (r & 4) * 4 + 4 * g + (r & 3) > u.last;
+            for (int r = 0; r < 4 * SUB; r++) {
+                const bool hide = !whole && one && place(r) > u.last;
 #pragma unroll
                 for (int i = 0; i < NV; i++)
 #pragma unroll
@@ -643,10 +682,13 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_half_k(rt_se
                 for (int i = 0; i < NV; i++)
 #pragma unroll
                     for (int e = 0; e < VEC; e++) {
-                        const uint4 v = turned(vw[i], e);
 #pragma unroll
-                        for (int n = 0; n < LIMBS; n++)
-                            acc[i * VEC + e] = H::mfma(v, w[n], acc[i * VEC + e]);
+                        for (int k = 0; k < SUB / 2; k++) {
+                            const uint4 v = turned(vw[i] + 8 * k, e);
+#pragma unroll
+                            for (int n = 0; n < LIMBS; n++)
+                                acc[i * VEC + e] = H::mfma(v, w[k][n], acc[i * VEC + e]);
+                        }
                         if (e & 1)
                             __builtin_amdgcn_sched_barrier(0);
                     }
@@ -657,29 +699,31 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_half_k(rt_se
                 for (int jj = u.j0; jj <= u.j1; jj++) {
                     const long upto = (long)u.q.past + jj < u.last ? (long)u.q.past + jj : u.last;
 #pragma unroll
-                    for (int i = 0; i < NV; i++) {
-                        uint32_t again[8][VW];
+                    for (int k = 0; k < SUB / 2; k++)
 #pragma unroll
-                        for (int r = 0; r < 8; r++) {
-                            load_words<VW>(again[r], address(kv.v, rows[r], head_rows, D * 2) + (i * 16 + c) * VEC * 2);
-                            const bool hide = tile * 32 + (r & 4) * 4 + 4 * g + (r & 3) > upto;
+                        for (int i = 0; i < NV; i++) {
+                            uint32_t again[8][VW];
 #pragma unroll
-                            for (int e = 0; e < VW; e++)
-                                again[r][e] = hide ? 0 : again[r][e];
+                            for (int r = 0; r < 8; r++) {
+                                load_words<VW>(again[r], address(kv.v, rows[8 * k + r], head_rows, D * 2) + (i * 16 + c) * VEC * 2);
+                                const bool hide = place(8 * k + r) > upto;
+#pragma unroll
+                                for (int e = 0; e < VW; e++)
+                                    again[r][e] = hide ? 0 : again[r][e];
+                            }
+#pragma unroll
+                            for (int e = 0; e < VEC; e++) {
+                                const uint4 v = turned(again, e);
+                                v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                                for (int n = 0; n < LIMBS; n++)
+                                    o = H::mfma(n ? finite_only<TYPE>(v) : v, w[k][n], o);
+                                if (u.j == jj)
+                                    acc[i * VEC + e] += o;
+                                __builtin_amdgcn_sched_barrier(0);
+                            }
+                            asm volatile("" ::: "memory"); /* the loads stay in the loop, and out of registers */
                         }
-#pragma unroll
-                        for (int e = 0; e < VEC; e++) {
-                            const uint4 v = turned(again, e);
-                            v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                            for (int n = 0; n < LIMBS; n++)
-                                o = H::mfma(n ? finite_only<TYPE>(v) : v, w[n], o);
-                            if (u.j == jj)
-                                acc[i * VEC + e] += o;
-                            __builtin_amdgcn_sched_barrier(0);
-                        }
-                    }
-                    asm volatile("" ::: "memory"); /* the loads stay in the loop, and out of registers */
                 }
             }
         }
@@ -694,6 +738,9 @@ __global__ __launch_bounds__(256) void attn_join_k(rt_seqs b, rt_kv kv, rt_attn 
 {
     __shared__ __align__(16) float4 so[16][16];
     __shared__ float sm[16], sl[16];
+    const int at = threadIdx.x & 15, turn = threadIdx.x >> 4;
+    const long D = kv.dim, d = 64 * (long)blockIdx.z + 4 * at, dd = d < D ? d : 0;
+    const float4 gate = gate_of(a, blockIdx.x, blockIdx.y, dd);
     const long i = blockIdx.x, h = blockIdx.y, s = b.n == 1 ? (b.start[0] <= i && i < b.start[1] ? 0 : -1) : q8_sequence_of(b, i);
     if (s < 0)
         return;
@@ -714,9 +761,7 @@ __global__ __launch_bounds__(256) void attn_join_k(rt_seqs b, rt_kv kv, rt_attn 
     const int kh = (int)h / p.group, row = (int)(i - q.first) * p.group + (int)h % p.group, z = row / 16, r = row % 16;
     if ((long)before + (long)(z + 1) * q.chunks > p.slots)
         return;
-    const long slot = (long)kh * p.slots + before + z * q.chunks, D = kv.dim;
-    const int at = threadIdx.x & 15, turn = threadIdx.x >> 4;
-    const long d = 64 * (long)blockIdx.z + 4 * at, dd = d < D ? d : 0;
+    const long slot = (long)kh * p.slots + before + z * q.chunks;
     const float *ml = p.part + kv.heads * p.slots * 16 * D + (slot * 16 + r) * 2, *part = p.part + (slot * 16 + r) * D + dd;
     float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
@@ -755,7 +800,7 @@ __global__ __launch_bounds__(256) void attn_join_k(rt_seqs b, rt_kv kv, rt_attn 
             v = float4{fmaf(x.x, f, v.x), fmaf(x.y, f, v.y), fmaf(x.z, f, v.z), fmaf(x.w, f, v.w)};
             sum = fmaf(sl[k], f, sum);
         }
-        store_row(a, D, i, h, d, v, sum, false);
+        store_row(a, D, i, h, d, v, sum, false, gate);
     }
 }
 
@@ -783,17 +828,18 @@ void launch(hipStream_t s, dim3 grid, const rt_seqs &b, const rt_kv &kv, const r
 }
 
 /* Row tiles of a call at most, and the chunks (a key-value head) to spread them over: so many that with each
- * row tile's last one, which is smaller, they fill the workgroups that run at once (two a compute unit) a
+ * row tile's last one, which is smaller, they fill the workgroups that run at once (one or two a compute unit) a
  * whole number of times, at least half of them whole; none (0) when the row tiles alone are more than SLOTS */
 constexpr long SLOTS = 4096;
 
-int least_tiles(const rt_kv &kv) { return kv.type == RT_F32 ? WAVES : 2 * WAVES; }
+int tile_of(const rt_kv &kv) { return kv.type == RT_F32 ? 1 : sixteens(kv.dim); }
 
 void plan_chunks(const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long &tiles, long &target)
 {
     tiles = b.t * (a.q_heads / kv.heads) / 16 + b.n;
-    const long once = ((kv.dim > 128 ? 256 : 512) + kv.heads - 1) / kv.heads;
-    target = tiles * kv.heads > SLOTS || kv.table_ld * kv.page <= 16 * least_tiles(kv) ? 0 : (2 * tiles + once - 1) / once * once - tiles;
+    const bool single = kv.type == RT_F32 ? kv.dim > 128 : alone(kv.dim);
+    const long once = ((single ? 256 : 512) + kv.heads - 1) / kv.heads;
+    target = tiles * kv.heads > SLOTS || kv.table_ld * kv.page <= 16 * WAVES * tile_of(kv) ? 0 : (2 * tiles + once - 1) / once * once - tiles;
 }
 
 } /* namespace */
@@ -811,7 +857,8 @@ void q8_launch_attn(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const
     long tiles, target;
     plan_chunks(b, kv, a, tiles, target);
     p.target = (int)target;
-    p.least = least_tiles(kv);
+    p.tile = tile_of(kv);
+    p.least = WAVES * p.tile;
     int up = 0;
     while ((1L << up) < kv.page)
         up++;

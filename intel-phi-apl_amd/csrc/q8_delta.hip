@@ -341,18 +341,26 @@ __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int m
 #pragma unroll
         for (int j = 0; j < TILES; j++) {
             const float rk = srk[16 * j + c];
-            if (j <= wave)
+            if (j <= wave) {
+                float d[4];
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    d[r] = sd[16 * wave + 4 * g + r][16 * j + c];
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const int i = 16 * wave + 4 * g + r;
-                    sa[i][16 * j + c] = i > 16 * j + c ? bf[r] * rk * kt[j][r] * sd[i][16 * j + c] : 0.0f;
+                    const float x = bf[r] * rk * kt[j][r] * d[r];
+                    sa[16 * wave + 4 * g + r][16 * j + c] = 16 * wave + 4 * g + r > 16 * j + c ? x : 0.0f;
                 }
-            if (j <= 3 - wave)
+            }
+            if (j <= 3 - wave) {
+                float d[4]; /* 0 behind the diagonal */
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const int i = 16 * (3 - wave) + 4 * g + r;
-                    pr[j][r] = i >= 16 * j + c ? qs[r] * rk * qt[j][r] * sd[i][16 * j + c] : 0.0f;
-                }
+                for (int r = 0; r < 4; r++)
+                    d[r] = sd[16 * (3 - wave) + 4 * g + r][16 * j + c];
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    pr[j][r] = qs[r] * rk * qt[j][r] * d[r];
+            }
         }
         __syncthreads();
 #pragma unroll
@@ -398,20 +406,20 @@ __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int m
             }
             __syncthreads();
         }
-        bool finite = true;
-        int pair = 0;
+        float4 check = {0.0f, 0.0f, 0.0f, 0.0f}; /* 0, or NaN */
 #pragma unroll
-        for (int i = 0; i < TILES; i++)
-#pragma unroll
-            for (int j = 0; j <= i; j++, pair++)
-                if (pair % 4 == wave) {
-                    const float4 t = *(const float4 *)&st[16 * i + c][16 * j + 4 * g] * *(const float4 *)&sbeta[16 * j + 4 * g];
-                    const float4 p = *(const float4 *)&sd[16 * i + c][16 * j + 4 * g];
-                    finite = finite && finite4(t) && finite4(p);
-                    *(float4 *)(mine + pair * 256 + lane * 4) = t;
-                    *(float4 *)(mine + (PAIRS + pair) * 256 + lane * 4) = p;
-                }
-        const bool odd = __ballot(!finite) != 0;
+        for (int k = 0; k < 3; k++) {
+            const int pair = wave + 4 * k, i = pair < 1 ? 0 : pair < 3 ? 1 : pair < 6 ? 2 : 3, j = pair - i * (i + 1) / 2;
+            if (pair < PAIRS) {
+                const float4 t = *(const float4 *)&st[16 * i + c][16 * j + 4 * g] * *(const float4 *)&sbeta[16 * j + 4 * g];
+                const float4 p = *(const float4 *)&sd[16 * i + c][16 * j + 4 * g];
+                check = float4{fmaf(t.x, 0.0f, check.x), fmaf(t.y, 0.0f, check.y), fmaf(t.z, 0.0f, check.z), fmaf(t.w, 0.0f, check.w)};
+                check = float4{fmaf(p.x, 0.0f, check.x), fmaf(p.y, 0.0f, check.y), fmaf(p.z, 0.0f, check.z), fmaf(p.w, 0.0f, check.w)};
+                *(float4 *)(mine + pair * 256 + lane * 4) = t;
+                *(float4 *)(mine + (PAIRS + pair) * 256 + lane * 4) = p;
+            }
+        }
+        const bool odd = __ballot(!finite4(check)) != 0;
         if (lane == 0)
             factor[3 * CHUNK + 4 + wave] = odd ? 1.0f : 0.0f;
         __syncthreads();
