@@ -389,7 +389,17 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
                 x[r] = __builtin_amdgcn_exp2f(x[r] - ref);
                 l += x[r];
             }
-            if (whole) {
+            const bool one = u.j0 == u.j1;
+            if (whole || one) {
+                /* values that the row tile's one token does not see are 0: 0 times an infinite or NaN one would be NaN */
+                if (!whole)
+#pragma unroll
+                    for (int r = 0; r < 4; r++)
+#pragma unroll
+                        for (int i = 0; i < NV; i++)
+#pragma unroll
+                            for (int e = 0; e < VEC; e++)
+                                vw[r][i][e] = tile * 16 + 4 * g + r > u.last ? 0 : vw[r][i][e];
 #pragma unroll
                 for (int r = 0; r < 4; r++)
 #pragma unroll

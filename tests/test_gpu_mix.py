@@ -465,3 +465,167 @@ def test_calls_repeat_bit_for_bit(rt, q8rt):
     again = run_delta(rt, q8rt, x, start, True), run_attn(rt, q8rt, cache, q, starts([1, 1]), [2999, 69], 0.1)
     for a, b in zip((*first[0], first[1]), (*again[0], again[1])):
         assert np.array_equal(a.view(np.uint32), b.view(np.uint32))
+
+
+# ---- recorded steps
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16"])
+def test_recorded_decode_steps_go_on(rt, q8rt, kind):
+    """A decode step of all four operators, recorded once and replayed as positions, pages and states move on in
+    device memory: every replay's outputs and states bit for bit an eager run's, with eager work and waits
+    between the replays."""
+    rng = np.random.default_rng(21)
+    n, ch, hk, hv, dk, dv, hq, kvh, dim, page, steps = 3, 384, 1, 2, 128, 64, 4, 2, 64, 8, 4
+    lens = [5, 40, 300]
+    start = starts([1] * n)
+    cache = Paged(rng, kind, [v + steps for v in lens], kvh, dim, page)
+    xs = rng.standard_normal((steps, n, ch)).astype(np.float32)
+    w, conv_in = rng.standard_normal((ch, 4)).astype(np.float32), rng.standard_normal((n, 3, ch)).astype(np.float32)
+    a, b = (rng.standard_normal((n, hv)).astype(np.float32) for _ in range(2))
+    decay, dt = -np.ones(hv, np.float32), np.zeros(hv, np.float32)
+    state = (0.1 * rng.standard_normal((n, hv, dk, dv))).astype(np.float32)
+    qkv = rng.standard_normal((steps, n, (hq + 2 * kvh) * dim)).astype(np.float32)
+    freq = 1e4 ** (-np.arange(0, dim, 2) / dim)
+
+    def run(recorded):
+        with Call(rt, q8rt) as d:
+            lib, R = rt.lib, rt.R
+            past = d.put(np.array(lens, np.int32))
+            s = q8rt.Seqs(n=n, t=n, longest=1, start=d.put(start.astype(np.int32)), past=past)
+            x, y = d.put(xs[0]), d.out("y", (n, ch), np.float32)
+            cs, ss = d.out("cs", conv_in.shape, np.float32, conv_in), d.out("ss", state.shape, np.float32, state)
+            kv = cache.struct(d, written=True)
+            src, q, o, da = d.put(qkv[0]), d.out("q", (n, hq, dim), np.float32), d.out("o", (n, hq * dim), np.float32), d.out("do", (n, hv * dv), np.float32)
+            width = (hq + 2 * kvh) * dim
+            delta = q8rt.Delta(k_heads=hk, v_heads=hv, k_dim=dk, v_dim=dv, q=y, q_ld=ch, k=y + 4 * dk, k_ld=ch, v=y + 8 * dk, v_ld=ch, a=d.put(a), a_ld=hv, b=d.put(b),
+                               b_ld=hv, decay=d.put(decay), dt=d.put(dt), eps=EPS, scale=dk ** -0.5, s_in=ss, s_out=ss, o=da, o_ld=hv * dv)
+            rope = q8rt.Rope(q=src, q_ld=width, q_hd=dim, q_heads=hq, k=src + 4 * hq * dim, k_ld=width, k_hd=dim, v=src + 4 * (hq + kvh) * dim, v_ld=width, v_hd=dim,
+                             eps=EPS, rot=dim, freq=d.put(freq), out=q, out_ld=hq * dim, out_hd=dim)
+            attn = q8rt.Attn(q=q, q_ld=hq * dim, q_hd=dim, q_heads=hq, scale=0.125, o=o, o_ld=hq * dim)
+            taps = d.put(w)
+
+            def step():
+                lib.rt_conv_silu_dev(R, c.byref(s), x, ch, ch, taps, 4, cs, cs, y, ch)
+                lib.rt_delta_rule_dev(R, c.byref(s), c.byref(delta))
+                lib.rt_rope_kv_dev(R, c.byref(s), c.byref(kv), c.byref(rope))
+                lib.rt_attn_kv_dev(R, c.byref(s), c.byref(kv), c.byref(attn))
+
+            graph = None
+            if recorded:
+                step()  # the workspaces; then the states as they were
+                for name, p, data in (("cs", cs, conv_in), ("ss", ss, state)):
+                    rt.to_dev(p, data)
+                lib.rt_graph_begin(R)
+                step()
+                graph = c.c_void_p(lib.rt_graph_end(R))
+            got = []
+            for i in range(steps):
+                rt.to_dev(x, xs[i])
+                rt.to_dev(src, qkv[i])
+                rt.to_dev(past, np.array(lens, np.int32) + i)
+                if graph:
+                    lib.rt_graph_launch(R, graph)
+                else:
+                    step()
+                got.append([d.get(k) for k in ("y", "do", "q", "o", "cs", "ss")])
+                if graph:  # eager work of the same operators between the replays
+                    run_attn(rt, q8rt, Paged(rng, kind, [900], 1, 128, 16), np.ones((1, 2, 128), np.float32), starts([1]), [899], 0.1)
+            if graph:
+                lib.rt_graph_free(R, graph)
+            return got
+
+    for i, (x, y) in enumerate(zip(run(False), run(True))):
+        for p, q in zip(x, y):
+            assert np.isfinite(p).all() and np.array_equal(p.view(np.uint32), q.view(np.uint32)), i
+
+
+def test_recorded_prompts(rt, q8rt):
+    """The chunks of a prompt and attention split over positions, recorded: three replays give the eager bits."""
+    rng = np.random.default_rng(22)
+    hk, hv, dk, dv, start = 1, 2, 128, 64, starts([300, 70])
+    x = delta_inputs(rng, 370, hk, hv, dk, dv, 2)
+    cache, q = Paged(rng, "bf16", [2000, 90], 2, 128, 16), rng.standard_normal((2, 8, 128)).astype(np.float32)
+    want = run_delta(rt, q8rt, x, start, True), run_attn(rt, q8rt, cache, q, starts([1, 1]), [1999, 89], 0.1)
+    real, records = rt.lib, []
+
+    class Recorded:
+        """The library with its calls recorded first, then replayed three times, an eager wait between."""
+
+        def __getattr__(self, name):
+            fn = getattr(real, name)
+            if name not in ("rt_delta_rule_dev", "rt_attn_kv_dev"):
+                return fn
+
+            def call(*args):
+                real.rt_graph_begin(rt.R)
+                fn(*args)
+                g = c.c_void_p(real.rt_graph_end(rt.R))
+                for _ in range(3):
+                    real.rt_graph_launch(rt.R, g)
+                    real.rt_dev_sync(rt.R)
+                records.append(name)
+                real.rt_graph_free(rt.R, g)
+
+            return call
+
+    rt.lib = Recorded()
+    try:
+        got = run_delta(rt, q8rt, x, start, True), run_attn(rt, q8rt, cache, q, starts([1, 1]), [1999, 89], 0.1)
+    finally:
+        rt.lib = real
+    assert len(records) == 2
+    for a, b in zip((*want[0], want[1][:, :1024]), (*got[0], got[1][:, :1024])):
+        assert np.array_equal(a.view(np.uint32), b.view(np.uint32))
+
+
+def test_two_runtimes_side_by_side(q8rt, rt):
+    """A second runtime's calls (a stream and workspaces of its own) between this one's, none waited for: both right."""
+    rng = np.random.default_rng(23)
+    cache = Paged(rng, "f16", [3000], 1, 128, 16)
+    q = rng.standard_normal((1, 4, 128)).astype(np.float32)
+    want, tol = ref.attn(q, cache.seq_k, cache.seq_v, 0.1, starts([1]), [2999])
+    other = q8rt.Runtime()
+    try:
+        calls = []
+        for r in (rt, other, rt, other):
+            d = Call(r, q8rt)
+            s, kv = d.seqs(starts([1]), [2999]), cache.struct(d)
+            a = q8rt.Attn(q=d.put(q), q_ld=512, q_hd=128, q_heads=4, scale=0.1, o=d.out("o", (1, 512), np.float32), o_ld=512)
+            calls.append((r, d, s, kv, a))
+        for r, d, s, kv, a in calls:
+            r.lib.rt_attn_kv_dev(r.R, c.byref(s), c.byref(kv), c.byref(a))
+        for r, d, *_ in calls:
+            assert (np.abs(d.get("o").reshape(1, 4, 128) - want) <= tol).all()
+            d.__exit__()
+    finally:
+        other.close()
+
+
+def test_first_call_of_a_size_while_recording_is_refused(q8rt):
+    """A recording may not grow the workspace: the call says so and ends the process (a child here, which never replays)."""
+    import os
+    import subprocess
+    import sys
+
+    code = """
+import ctypes as c, sys
+sys.path.insert(0, "tests")
+import numpy as np
+from conftest import load_package
+m = load_package()
+import mix_ref as ref
+rt = m.Runtime()
+cache = ref.Paged(np.random.default_rng(1), "f16", [500], 1, 64, 16)
+with ref.Call(rt, m) as d:
+    s, kv = d.seqs(ref.starts([1]), [499]), cache.struct(d)
+    a = m.Attn(q=d.put(np.ones((1, 2, 64), np.float32)), q_ld=128, q_hd=64, q_heads=2, scale=0.1, o=d.out("o", (1, 128), np.float32), o_ld=128)
+    rt.lib.rt_graph_begin(rt.R)
+    print("child: recording", flush=True)
+    rt.lib.rt_attn_kv_dev(rt.R, c.byref(s), c.byref(kv), c.byref(a))
+    print("child: returned", flush=True)
+"""
+    p = subprocess.run([sys.executable, "-c", code], env=dict(os.environ, Q8_ABORT_EXIT="43"), capture_output=True, text=True, timeout=120,
+                       cwd=os.path.dirname(os.path.dirname(os.path.abspath(__file__))))
+    assert p.returncode == 43 and "child: recording" in p.stdout and "child: returned" not in p.stdout, (p.returncode, p.stdout, p.stderr)
+    assert "must grow while a graph is being recorded" in p.stderr
