@@ -115,8 +115,8 @@ __global__ __launch_bounds__(NORM ? 64 * STEP_WAVES : 64) void delta_step_k(rt_s
             }
             float rq = 1.0f, rk = 1.0f;
             if (a.eps >= 0.0f) {
-                rq = 1.0f / sqrtf(lanes_sum<RG>(qq) + a.eps);
-                rk = 1.0f / sqrtf(lanes_sum<RG>(kk) + a.eps);
+                rq = rsqrtf(lanes_sum<RG>(qq) + a.eps);
+                rk = rsqrtf(lanes_sum<RG>(kk) + a.eps);
             }
             qk = lanes_sum<RG>(qk);
             sk = float4{lanes_sum<RG>(sk.x), lanes_sum<RG>(sk.y), lanes_sum<RG>(sk.z), lanes_sum<RG>(sk.w)};
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(NORM ? 64 * STEP_WAVES : 64) void delta_step_k(rt_s
                     sum += squares[j & 1][n];
                 const float mine = (g & 2) ? (g & 1 ? o.w : o.z) : (g & 1 ? o.y : o.x);
                 if (g < 4 && live)
-                    to[g] = w * (mine * (1.0f / sqrtf(a.nw_eps + sum / (float)a.v_dim))) * (z * q8_sigmoid(z));
+                    to[g] = w * (mine * rsqrtf(a.nw_eps + sum / (float)a.v_dim)) * (z * q8_sigmoid(z));
             } else if (g == 0 && live) {
                 *(float4 *)to = o;
             }
@@ -764,9 +764,10 @@ static bool launch_delta(hipStream_t s, const rt_seqs &b, const rt_delta &a, flo
     /* 16 columns a wave for several tokens, or as long as that gives no more waves than the GPU has places for two of
      * each SIMD */
     const bool few = b.longest > 1 || b.n * a.v_heads * waves(16) <= 2048;
-    /* the norm with it where that leaves no compute unit without a head: on fewer, a head's waves share one, and a launch
-     * more costs less (one sequence of 32 heads, 8 tokens: 21 us with it, 14 apart) */
-    const bool normed = a.z && !chunked && waves(32) <= STEP_WAVES && b.n * a.v_heads >= 256;
+    /* the norm in the same launch: for single tokens always (one sequence of 32 heads: 7.9 us, 7.7 to 9.9 as two launches),
+     * for several where there is a head for every compute unit: with fewer, a head's waves share one, and a launch more costs
+     * less (the same sequence, 8 tokens: 21 us and 14) */
+    const bool normed = a.z && !chunked && waves(32) <= STEP_WAVES && (b.longest == 1 || b.n * a.v_heads >= 256);
     if (normed && few && waves(16) <= STEP_WAVES)
         delta_step_k<DK, 16, true><<<dim3(1, (unsigned)a.v_heads, (unsigned)b.n), 64 * waves(16), 0, s>>>(b, a, limit);
     else if (normed)
