@@ -9,25 +9,27 @@ typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 
 constexpr int WAVES = 4;
 
-/* p / page for p < 2^31: (p * mul) >> shift with shift = 31 + ceil(log2 page), mul = ceil(2^shift / page): exact, as
- * the excess mul * page - 2^shift is below page <= 2^(shift - 31) */
-struct paging {
+/* x / d for x < 2^31: (x * mul) >> shift with shift = 31 + ceil(log2 d), mul = ceil(2^shift / d): exact, as the
+ * excess mul * d - 2^shift is below d <= 2^(shift - 31) */
+struct divisor {
     uint32_t mul;
     int shift;
+    __device__ __forceinline__ uint32_t of(uint32_t x) const { return (uint32_t)(((uint64_t)x * mul) >> shift); }
 };
 
 /* What a launch shares: row tiles are 16 query rows (token, head of the group) of one key-value head and
  * sequence; a sequence's positions, in tiles of 16, are cut into chunks of one size for the whole batch. */
 struct plan {
-    paging pg;
-    int group;   /* query heads a key-value head */
-    int cap;     /* positions that the table reaches */
-    int tile;    /* 16s of positions that a wave takes at once (a power of two): chunks are whole numbers of them */
-    int least;   /* 16s a chunk at least: one tile of each wave */
-    int target;  /* chunks (a key-value head) to spread all tiles over; 0: one a row tile */
-    int slots;   /* partial results a key-value head */
+    divisor page, group; /* by the positions of a page, by the query heads of a key-value head */
+    int heads;    /* query heads of a key-value head */
+    int cap;      /* positions that the table reaches */
+    int tile;     /* 16s of positions that a wave takes at once (a power of two): chunks are whole numbers of them */
+    int least;    /* 16s a chunk at least: one tile of each wave */
+    int target;   /* chunks (a key-value head) to spread all tiles over; 0: one a row tile */
+    int slots;    /* partial results a key-value head */
+    float share;  /* 1 / target, and a little: rounded sums must not make a chunk too small */
     float qscale; /* scale * log2 e: scores are in powers of two */
-    float *part; /* [heads][slots][16][dim], then [heads][slots][16][2]: maximum and sum */
+    float *part;  /* [heads][slots][16][dim], then [heads][slots][16][2]: maximum and sum */
 };
 
 struct seq_plan {
@@ -36,7 +38,7 @@ struct seq_plan {
     int rows, chunks; /* row tiles, and chunks of each */
 };
 
-__device__ __forceinline__ seq_plan plan_of(const rt_seqs &b, const plan &p, int s, int chunk)
+__device__ __forceinline__ seq_plan plan_of(const rt_seqs &b, const plan &p, int group, int s)
 {
     seq_plan q;
     long first, last;
@@ -46,66 +48,91 @@ __device__ __forceinline__ seq_plan plan_of(const rt_seqs &b, const plan &p, int
     q.past = b.past[s];
     const long len = (long)q.past + q.n;
     q.tiles = len <= 0 ? 0 : (int)((len < p.cap ? len : p.cap) + 15) / 16;
-    q.rows = (int)(((uint32_t)q.n * (uint32_t)p.group + 15) / 16);
-    q.chunks = chunk > 0 && q.tiles > chunk ? (int)((uint32_t)(q.tiles + chunk - 1) / (uint32_t)chunk) : 1;
+    q.rows = (int)(((uint32_t)q.n * (uint32_t)group + 15) / 16);
+    q.chunks = 1;
     return q;
 }
 
 __device__ __forceinline__ int first_lane(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-/* tiles a chunk: every sequence's tiles over the target, the same for each of them, so that workgroups
- * read the same amounts whatever the lengths (a share of each sequence's own length left the short ones'
- * workgroups waiting for the longest) */
-__device__ __forceinline__ int chunk_of(const rt_seqs &b, const plan &p)
+/* tiles a chunk, from all sequences' (row tiles x position tiles): the target's share, the same for each sequence, so
+ * that workgroups read the same amounts whatever the lengths (a share of each one's own length left the short ones'
+ * waiting for the longest). Rounded up, by floats: any size will do that every workgroup finds alike and that leaves no
+ * more chunks than slots. 0: a row tile is one chunk. */
+__device__ __forceinline__ int chunk_from(const plan &p, float all)
 {
-    if (p.target <= 0)
-        return 0;
-    double all = 0.0; /* whole numbers */
-    if (b.n == 1) {
-        const seq_plan q = plan_of(b, p, 0, 0);
-        all = (double)q.rows * q.tiles;
-    } else {
-        for (int s = threadIdx.x & 63; s < (int)b.n; s += 64) {
-            const seq_plan q = plan_of(b, p, s, 0);
-            all += (double)q.rows * q.tiles;
-        }
-        for (int o = 32; o >= 1; o >>= 1)
-            all += __shfl_xor(all, o, 64);
-    }
-    const double c = all / p.target + 1.0; /* as far as 2^27 tiles: one a row tile there */
-    return c < p.least ? p.least : c < 1e8 ? (first_lane((int)c) + p.tile - 1) & ~(p.tile - 1) : 0;
+    const float c = all * p.share + 1.0f;
+    const int n = c < 1e8f ? ((int)c + p.tile - 1) & ~(p.tile - 1) : 0;
+    return n == 0 || n > p.least ? n : p.least;
+}
+/* ceil(tiles / chunk), which is at most a few thousand */
+__device__ __forceinline__ int chunks_of(int tiles, int chunk)
+{
+    if (chunk == 0 || tiles <= chunk)
+        return 1;
+    int n = (int)((float)tiles * __builtin_amdgcn_rcpf((float)chunk));
+    n -= (long)n * chunk >= tiles ? 1 : 0;
+    n += (long)n * chunk < tiles ? 1 : 0;
+    n += (long)n * chunk < tiles ? 1 : 0;
+    return n;
 }
 
-/* The sequence whose row tiles' chunks hold number i of all, -1 behind the last; before = the chunks of
- * those before it */
-__device__ __forceinline__ int sequence_of_chunk(const rt_seqs &b, const plan &p, int chunk, int i, int &before)
+/* the sums of a value over the lanes up to each: by 1, 2, 4 and 8 within each 16, then the 16s' last to the next */
+#define UPTO(v, ctrl, rows) (v) += __builtin_amdgcn_update_dpp(0, (v), ctrl, rows, 0xf, false)
+__device__ __forceinline__ int wave_upto(int v)
+{
+    UPTO(v, 0x111, 0xf);
+    UPTO(v, 0x112, 0xf);
+    UPTO(v, 0x114, 0xf);
+    UPTO(v, 0x118, 0xf);
+    UPTO(v, 0x142, 0xa); /* row_bcast:15 into rows 1 and 3 */
+    UPTO(v, 0x143, 0xc); /* row_bcast:31 into rows 2 and 3 */
+    return v;
+}
+#undef UPTO
+
+/* The sequence that holds chunk `number` of all row tiles' (or, with number < 0, row `token`), its plan, and the
+ * chunks of the sequences before it; false: there is none. A lane a sequence, 64 at a time. */
+__device__ __forceinline__ bool locate(const rt_seqs &b, const plan &p, int group, int number, long token, int &s, seq_plan &q, int &before, int &chunk)
 {
     before = 0;
     if (b.n == 1) {
-        const seq_plan q = plan_of(b, p, 0, chunk);
-        return i < q.rows * q.chunks ? 0 : -1;
+        s = 0;
+        q = plan_of(b, p, group, 0);
+        chunk = p.target > 0 ? chunk_from(p, (float)q.rows * (float)q.tiles) : 0;
+        q.chunks = chunks_of(q.tiles, chunk);
+        return number >= 0 ? number < q.rows * q.chunks : token >= q.first && token < q.first + q.n;
     }
-    const int lane = threadIdx.x & 63;
-    for (int s0 = 0; s0 < (int)b.n; s0 += 64) {
-        int c = 0;
-        if (s0 + lane < (int)b.n) {
-            const seq_plan q = plan_of(b, p, s0 + lane, chunk);
-            c = q.rows * q.chunks;
-        }
-        int upto = c;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int u = __shfl_up(upto, o, 64);
-            upto += lane >= o ? u : 0;
-        }
-        const unsigned long long m = __ballot(i < before + upto);
+    const int lane = threadIdx.x & 63, n = (int)b.n;
+    const seq_plan none = {0, 0, 0, 0, 0, 1};
+    seq_plan at = lane < n ? plan_of(b, p, group, lane) : none;
+    chunk = 0;
+    if (p.target > 0) {
+        float all = (float)at.rows * (float)at.tiles;
+        for (int s0 = 64; s0 < n; s0 += 64)
+            if (s0 + lane < n) {
+                const seq_plan o = plan_of(b, p, group, s0 + lane);
+                all += (float)o.rows * (float)o.tiles;
+            }
+        chunk = first_lane(chunk_from(p, q8_wave_sum_dpp(all)));
+    }
+    for (int s0 = 0; s0 < n; s0 += 64) {
+        if (s0 > 0)
+            at = s0 + lane < n ? plan_of(b, p, group, s0 + lane) : none;
+        at.chunks = chunks_of(at.tiles, chunk);
+        const int mine = at.rows * at.chunks, upto = wave_upto(mine);
+        const unsigned long long m = __ballot(number >= 0 ? number < before + upto : token >= at.first && token < at.first + at.n);
         if (m) {
-            const int at = __ffsll((long long)m) - 1;
-            before += __builtin_amdgcn_readlane(upto - c, at);
-            return s0 + at;
+            const int l = __ffsll((long long)m) - 1;
+            const auto from = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            s = s0 + l;
+            before += from(upto - mine);
+            q = seq_plan{from(at.first), from(at.n), from(at.past), from(at.tiles), from(at.rows), from(at.chunks)};
+            return true;
         }
         before += __builtin_amdgcn_readlane(upto, 63);
     }
-    return -1;
+    return false;
 }
 
 template <int WORDS>
@@ -184,28 +211,32 @@ struct share {
     int t0, t1;      /* the chunk's position tiles, 16 each */
 };
 
-__device__ __forceinline__ bool share_of(const rt_seqs &b, const rt_kv &kv, const plan &p, int chunk, int number, share &u)
+__device__ __forceinline__ bool share_of(const rt_seqs &b, const rt_kv &kv, const plan &p, int group, int number, share &u)
 {
-    int before;
-    const int s = first_lane(sequence_of_chunk(b, p, chunk, number, before));
-    if (s < 0)
+    int before, s, chunk;
+    if (!locate(b, p, group, number, 0, s, u.q, before, chunk))
         return false;
-    u.q = plan_of(b, p, s, chunk);
     const seq_plan &q = u.q;
     number -= before;
-    u.z = first_lane((int)((uint32_t)number / (uint32_t)q.chunks));
+    int z = number;
+    if (q.chunks > 1) {
+        z = (int)((float)number * __builtin_amdgcn_rcpf((float)q.chunks)); /* below 2^14: one off at most */
+        z -= z * q.chunks > number ? 1 : 0;
+        z += (z + 1) * q.chunks <= number ? 1 : 0;
+    }
+    u.z = first_lane(z);
     const int part = number - u.z * q.chunks, row = u.z * 16 + (int)(threadIdx.x & 15);
     u.table = kv.table + s * kv.table_ld;
-    u.j = (int)((uint32_t)row / (uint32_t)p.group);
-    u.h = (int)blockIdx.y * p.group + (row - u.j * p.group);
+    u.j = (int)p.group.of(row);
+    u.h = (int)blockIdx.y * group + (row - u.j * group);
     u.live = u.j < q.n;
     const auto sees = [&](int j) { /* the last position that token j sees, within the table */
         const long pos = (long)q.past + j;
         return pos < 0 ? -1 : pos < p.cap ? (int)pos : p.cap - 1;
     };
     u.lim = u.live ? sees(u.j) : -1;
-    u.j0 = first_lane((int)((uint32_t)(u.z * 16) / (uint32_t)p.group));
-    u.j1 = first_lane((int)((uint32_t)(u.z * 16 + 15) / (uint32_t)p.group));
+    u.j0 = first_lane((int)p.group.of(u.z * 16));
+    u.j1 = first_lane((int)p.group.of(u.z * 16 + 15));
     u.j1 = u.j1 < q.n ? u.j1 : q.n - 1;
     u.last = sees(u.j1);
     u.least = sees(u.j0);
@@ -220,12 +251,12 @@ __device__ __forceinline__ bool share_of(const rt_seqs &b, const rt_kv &kv, cons
  * (-1: it has none) */
 __device__ __forceinline__ int entry_of(const rt_kv &kv, const plan &p, const int32_t *table, int pos)
 {
-    const uint32_t pg = (uint32_t)(((uint64_t)(uint32_t)pos * p.pg.mul) >> p.pg.shift);
+    const uint32_t pg = p.page.of(pos);
     return (long)pg < kv.table_ld ? table[pg] : -1;
 }
 __device__ __forceinline__ int row_of(const rt_kv &kv, const plan &p, int pos, int entry)
 {
-    const uint32_t pg = (uint32_t)(((uint64_t)(uint32_t)pos * p.pg.mul) >> p.pg.shift);
+    const uint32_t pg = p.page.of(pos);
     return entry >= 0 && entry < kv.pages ? entry * (int)(kv.heads * kv.page) + (pos - (int)(pg * (uint32_t)kv.page)) : -1;
 }
 __device__ __forceinline__ const char *address(const void *cache, int row, uint32_t head_rows, int bytes)
@@ -272,7 +303,7 @@ __device__ __forceinline__ void finish(char *lds, const rt_kv &kv, const rt_attn
     for (int w = 1; w < WAVES; w++)
         top = fmaxf(top, sm[w][c]);
     const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-    const int left = u.q.n * p.group - u.z * 16, rows = left < 16 ? left : 16;
+    const int group = p.heads, left = u.q.n * group - u.z * 16, rows = left < 16 ? left : 16;
     if (c < rows)
 #pragma unroll
         for (int i = 0; i < D / 16 / VEC; i++)
@@ -293,7 +324,7 @@ __device__ __forceinline__ void finish(char *lds, const rt_kv &kv, const rt_attn
             v = float4{v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w};
             sum += sl[w][r] * (sm[w][r] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(sm[w][r] - t));
         }
-        const int jr = (int)((uint32_t)(u.z * 16 + r) / (uint32_t)p.group), hr = kh * p.group + (u.z * 16 + r - jr * p.group);
+        const int jr = (int)p.group.of(u.z * 16 + r), hr = kh * group + (u.z * 16 + r - jr * group);
         const long pos = (long)u.q.past + jr;
         if (pos >= p.cap)
             sum = NAN; /* a position that the table does not reach */
@@ -319,12 +350,12 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
     constexpr int NK = D / 16, VE = D / 16, VEC = pieces(VE, 4), NV = VE / VEC;
     __shared__ __align__(16) char lds[joint_bytes<D>()];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-    const int chunk = chunk_of(b, p);
+    const int group = p.heads;
     const uint32_t head_rows = (uint32_t)(blockIdx.y * kv.page);
     /* with starts that overlap there may be more chunks than slots: those are left out */
     for (int number = (int)blockIdx.x; p.target == 0 || number < p.slots; number += (int)gridDim.x) {
         share u;
-        if (!share_of(b, kv, p, chunk, number, u))
+        if (!share_of(b, kv, p, group, number, u))
             return;
         v4f acc[VE];
 #pragma unroll
@@ -339,21 +370,19 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
                 load_words<4>(kw[i], at + i * 64);
         };
         uint32_t kw[NK][4], vw[4][NV][VEC];
-        int tile = (int)u.t0 + wave, row_now = -1, entry = -1;
-        const int stop = (int)u.t1;
-        if (tile < stop) {
-            row_now = row_of(kv, p, here(tile), entry_of(kv, p, u.table, here(tile)));
-            entry = entry_of(kv, p, u.table, here(tile + WAVES));
-            load_k(kw, row_now);
-        }
-        float qv[NK][4];
+        int tile = u.t0 + wave;
+        const int stop = u.t1, now = entry_of(kv, p, u.table, here(tile));
+        int entry = entry_of(kv, p, u.table, here(tile + WAVES));
+        float4 qv[NK]; /* under way with the table's entries; the keys need those */
+        const float *query = a.q + (u.live ? (long)(u.q.first + u.j) * a.q_ld + u.h * a.q_hd : 0) + g * 4;
 #pragma unroll
-        for (int i = 0; i < NK; i++) {
-            float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-            if (u.live)
-                v = *(const float4 *)(a.q + (long)(u.q.first + u.j) * a.q_ld + u.h * a.q_hd + (i * 4 + g) * 4);
-            qv[i][0] = v.x * p.qscale, qv[i][1] = v.y * p.qscale, qv[i][2] = v.z * p.qscale, qv[i][3] = v.w * p.qscale;
-        }
+        for (int i = 0; i < NK; i++)
+            qv[i] = *(const float4 *)(query + i * 16);
+        int row_now = row_of(kv, p, here(tile), now);
+        load_k(kw, row_now);
+#pragma unroll
+        for (int i = 0; i < NK; i++)
+            qv[i] = u.live ? float4{qv[i].x * p.qscale, qv[i].y * p.qscale, qv[i].z * p.qscale, qv[i].w * p.qscale} : float4{0.0f, 0.0f, 0.0f, 0.0f};
         for (; tile < stop; tile += WAVES) {
             int rows[4];
 #pragma unroll
@@ -369,7 +398,7 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
             for (int i = 0; i < NK; i++)
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    s[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kw[i][e]), qv[i][e], s[e & 1], 0, 0, 0);
+                    s[e & 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, kw[i][e]), (&qv[i].x)[e], s[e & 1], 0, 0, 0);
             if (tile + WAVES < stop) {
                 row_now = row_of(kv, p, here(tile + WAVES), entry);
                 entry = entry_of(kv, p, u.table, here(tile + 2 * WAVES));
@@ -511,14 +540,16 @@ __global__ __launch_bounds__(64 * WAVES, alone(D) ? 1 : 2) void attn_half_k(rt_s
 {
     typedef half_of<TYPE> H;
     constexpr int LIMBS = H::LIMBS, NK = D / 32, VE = D / 16, VEC = pieces(VE, 8), NV = VE / VEC, VW = VEC / 2, SUB = sixteens(D), POS = 16 * SUB;
-    __shared__ __align__(16) char lds[joint_bytes<D>() > NK * LIMBS * 1024 ? joint_bytes<D>() : NK * LIMBS * 1024];
+    static_assert(WAVES == 4);
+    constexpr int QUERIES = NK * LIMBS * 1024 + WAVES * 16 * 4;
+    __shared__ __align__(16) char lds[joint_bytes<D>() > QUERIES ? joint_bytes<D>() : QUERIES];
     uint4(*sq)[LIMBS][64] = (uint4(*)[LIMBS][64])lds; /* until the waves join */
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
-    const int chunk = chunk_of(b, p);
+    const int group = p.heads;
     const uint32_t head_rows = (uint32_t)(blockIdx.y * kv.page);
     for (int number = (int)blockIdx.x; p.target == 0 || number < p.slots; number += (int)gridDim.x) {
         share u;
-        if (!share_of(b, kv, p, chunk, number, u))
+        if (!share_of(b, kv, p, group, number, u))
             return;
         const int stop = (u.t1 + SUB - 1) / SUB; /* tiles: a chunk is a whole number of them, but for the last */
         int tile = u.t0 / SUB + wave, row[SUB], entry[SUB];
@@ -544,43 +575,51 @@ __global__ __launch_bounds__(64 * WAVES, alone(D) ? 1 : 2) void attn_half_k(rt_s
                 row[n] = row_of(kv, p, here(t * POS + 16 * n + c), entry[n]);
             load_entries(t + WAVES);
         };
-        if (tile < stop) {
-            load_entries(tile);
-            rows_next(tile);
-            load_k();
-        }
-        /* the queries' limbs, the same for every wave: wave w makes those of columns 32 i, i = w, w + WAVES, ... */
+        /* the table's entries, the queries, and with the entries the keys; wave w has the queries' columns 32 i, i = w,
+         * w + WAVES, ..., and makes their limbs, for all waves */
+        load_entries(tile);
+        constexpr int NQ = (NK + WAVES - 1) / WAVES;
         const float *query = a.q + (u.live ? (long)(u.q.first + u.j) * a.q_ld + u.h * a.q_hd : 0) + g * 8;
+        float4 qv[NQ][2];
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            const int i = wave + n * WAVES < NK ? wave + n * WAVES : 0;
+            qv[n][0] = *(const float4 *)(query + i * 32), qv[n][1] = *(const float4 *)(query + i * 32 + 4);
+        }
+        rows_next(tile);
+        load_k();
         float back = 1.0f;
         int up = 0;
         if (TYPE == RT_F16) {
+            float(*smost)[16] = (float(*)[16])(lds + NK * LIMBS * 1024); /* behind the limbs */
             float most = 0.0f;
-            for (int i = 0; i < NK; i++)
 #pragma unroll
-                for (int e = 0; e < 8; e += 4) {
-                    const float4 v = *(const float4 *)(query + i * 32 + e);
-                    most = fmaxf(fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y))), fmaxf(fabsf(v.z), fabsf(v.w)));
-                }
+            for (int n = 0; n < NQ; n++)
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    most = fmaxf(most, fabsf((&qv[n][0].x)[e]));
             most = group_max(most * fabsf(p.qscale));
+            if (g == 0)
+                smost[wave][c] = most;
+            __syncthreads();
+            most = fmaxf(fmaxf(smost[0][c], smost[1][c]), fmaxf(smost[2][c], smost[3][c]));
             up = most > 0.0f && most < INFINITY ? 14 - __builtin_amdgcn_frexp_expf(most) : 0;
             up = up > 120 ? 120 : up < -120 ? -120 : up;
             back = ldexpf(1.0f, -up);
         }
-        for (int i = wave; i < NK; i += WAVES) {
-            float qv[8];
+#pragma unroll
+        for (int n = 0; n < NQ; n++) {
+            const int i = wave + n * WAVES;
+            float x[8];
             uint4 w[LIMBS];
 #pragma unroll
-            for (int e = 0; e < 8; e += 4) {
-                const float4 v = *(const float4 *)(query + i * 32 + e);
-                qv[e] = v.x, qv[e + 1] = v.y, qv[e + 2] = v.z, qv[e + 3] = v.w;
-            }
-#pragma unroll
             for (int e = 0; e < 8; e++)
-                qv[e] = u.live ? ldexpf(qv[e] * p.qscale, up) : 0.0f;
-            limbs_of<TYPE>(qv, w);
+                x[e] = u.live ? ldexpf((&qv[n][0].x)[e] * p.qscale, up) : 0.0f;
+            limbs_of<TYPE>(x, w);
+            if (i < NK)
 #pragma unroll
-            for (int n = 0; n < LIMBS; n++)
-                sq[i][n][lane] = w[n];
+                for (int l = 0; l < LIMBS; l++)
+                    sq[i][l][lane] = w[l];
         }
         __syncthreads();
         v4f acc[VE];
@@ -751,24 +790,12 @@ __global__ __launch_bounds__(256) void attn_join_k(rt_seqs b, rt_kv kv, rt_attn 
     const int at = threadIdx.x & 15, turn = threadIdx.x >> 4;
     const long D = kv.dim, d = 64 * (long)blockIdx.z + 4 * at, dd = d < D ? d : 0;
     const float4 gate = gate_of(a, blockIdx.x, blockIdx.y, dd);
-    const long i = blockIdx.x, h = blockIdx.y, s = b.n == 1 ? (b.start[0] <= i && i < b.start[1] ? 0 : -1) : q8_sequence_of(b, i);
-    if (s < 0)
+    const long i = blockIdx.x, h = blockIdx.y;
+    int s, before, chunk;
+    seq_plan q;
+    if (!locate(b, p, p.heads, -1, i, s, q, before, chunk) || q.chunks == 1)
         return;
-    const int chunk = chunk_of(b, p);
-    const seq_plan q = plan_of(b, p, (int)s, chunk);
-    if (q.chunks == 1)
-        return;
-    int before = 0;
-    const int lane = threadIdx.x & 63;
-    if (s > 0) {
-        for (int k = lane; k < (int)s; k += 64) {
-            const seq_plan o = plan_of(b, p, k, chunk);
-            before += o.rows * o.chunks;
-        }
-        for (int o = 32; o >= 1; o >>= 1)
-            before += __shfl_xor(before, o, 64);
-    }
-    const int kh = (int)h / p.group, row = (int)(i - q.first) * p.group + (int)h % p.group, z = row / 16, r = row % 16;
+    const int kh = (int)p.group.of((uint32_t)h), row = (int)(i - q.first) * p.heads + (int)h - kh * p.heads, z = row / 16, r = row % 16;
     if ((long)before + (long)(z + 1) * q.chunks > p.slots)
         return;
     const long slot = (long)kh * p.slots + before + z * q.chunks;
@@ -869,12 +896,15 @@ void q8_launch_attn(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const
     p.target = (int)target;
     p.tile = tile_of(kv);
     p.least = WAVES * p.tile;
-    int up = 0;
-    while ((1L << up) < kv.page)
-        up++;
-    p.pg.shift = 31 + up;
-    p.pg.mul = (uint32_t)((((__uint128_t)1 << p.pg.shift) + kv.page - 1) / kv.page);
-    p.group = (int)(a.q_heads / kv.heads);
+    const auto by = [](long d) {
+        int up = 0;
+        while ((1L << up) < d)
+            up++;
+        return divisor{(uint32_t)((((__uint128_t)1 << (31 + up)) + d - 1) / d), 31 + up};
+    };
+    p.heads = (int)(a.q_heads / kv.heads);
+    p.page = by(kv.page), p.group = by(p.heads);
+    p.share = target ? 1.00001f / (float)target : 0.0f;
     const long reach = (1L << 31) - 4096;
     p.cap = (int)(kv.table_ld > reach / kv.page ? reach : kv.table_ld * kv.page);
     p.slots = (int)(target + (target ? tiles : 0));
