@@ -12,7 +12,12 @@
  *
  * Alignment: every float or cache address is 16-byte aligned and every stride a multiple of 4 floats,
  * except where said. Activations, norms, states and gates are F32. An array that a call writes must
- * not overlap one that it reads, but for a state (s_out may be s_in). */
+ * not overlap one that it reads (from its first element to its last, whatever lies between its rows), but for
+ * a state (s_out may be s_in) and a rotation in place.
+ *
+ * Workspaces (the delta rule's for runs of tokens, the attention's) grow to what a call needs, not while a
+ * graph is recorded: run a call with the same n, t and longest (and cache and heads) once before. All of a
+ * runtime's calls share them, in the order of its stream. */
 #ifndef Q8_MIX_H
 #define Q8_MIX_H
 

@@ -38,8 +38,8 @@ __device__ __forceinline__ float lanes_sum(float v)
  *   S' = alpha S + k d^T,  d = beta (v - alpha S^T k),  S'^T q = alpha S^T q + (q.k) d
  *
  * and so are |q|^2, |k|^2 and q.k, whose scales are applied to the results. The gates of 64 tokens are computed at
- * once, a lane a token. The next token's rows are loaded while this one's are used, and the first one's before the
- * state, as loads come back in order. With the output's norm the head's waves are one workgroup (NORM), whose sums of
+ * once, a lane a token. The next token's rows are loaded while this one's are used, and the state before anything is
+ * known of the tokens. With the output's norm the head's waves are one workgroup (NORM), whose sums of
  * squares meet in LDS, and each lane gates one column; else each wave is a workgroup.
  * Bound by HBM (the state, read and written once) on many sequences, by latency on one. 32 columns a wave read whole
  * 128-byte lines (64 sequences of 32 heads of 128 x 128: 52 us, 5.3 TB/s; with 16 columns 76) and their stores
@@ -57,6 +57,11 @@ __global__ __launch_bounds__(NORM ? 64 * STEP_WAVES : 64) void delta_step_k(rt_s
     const long s = blockIdx.z, h = blockIdx.y, own = COLS * ((long)blockIdx.x * waves + wave) + 4 * (lane / RG), col = own < a.v_dim ? own : 0;
     const bool live = own < a.v_dim;
     const long kh = a.tiled ? h % a.k_heads : h / (a.v_heads / a.k_heads);
+    const long base = ((s * a.v_heads + h) * DK + g * KR) * a.v_dim + col;
+    float4 st[KR];
+#pragma unroll
+    for (int r = 0; r < KR; r++)
+        st[r] = *(const float4 *)(a.s_in + base + r * a.v_dim);
     long first, last;
     q8_rows_of(b, s, first, last);
     if (last - first > most)
@@ -83,11 +88,6 @@ __global__ __launch_bounds__(NORM ? 64 * STEP_WAVES : 64) void delta_step_k(rt_s
         load(first);
     }
     const float w = NORM ? a.nw[col + (g & 3)] : 0.0f;
-    const long base = ((s * a.v_heads + h) * DK + g * KR) * a.v_dim + col;
-    float4 st[KR];
-#pragma unroll
-    for (int r = 0; r < KR; r++)
-        st[r] = *(const float4 *)(a.s_in + base + r * a.v_dim);
     for (long i0 = first; i0 < last; i0 += 64) {
         if (i0 > first) {
             const long i = i0 + lane < last ? i0 + lane : i0;
@@ -736,8 +736,9 @@ __global__ __launch_bounds__(256) void gated_norm_k(rt_seqs b, rt_delta a, int l
 
 } /* namespace */
 
-/* Sequences of more tokens than this go in chunks */
-constexpr int SHORT = 16;
+/* Sequences of more tokens than this go in chunks (heads of 128 x 128, 32 of them; us token by token and in chunks: one sequence
+ * of 24 tokens 25 / 31, of 32 30 / 31, of 48 42 / 32; 4 of 32 38 / 52, of 48 52 / 53; 16 of 48 138 / 141) */
+constexpr int SHORT = 32;
 /* The chunks' parts of all heads that a launch makes and takes, in bytes: longer calls alternate */
 constexpr long PREP_MAX = 256L << 20;
 

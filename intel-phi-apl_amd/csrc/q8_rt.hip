@@ -1714,10 +1714,13 @@ void check_words(const char *fn, const void *p, unsigned align, const char *what
         failf(fn, "%s must be a %u-byte aligned device address", what, align);
 }
 
+/* strides in floats: (t - 1) of them, in bytes, stay far from 2^63 */
+constexpr long RT_STRIDE_MAX = 1L << 36;
+
 /* a stride of token rows `width` wide */
 void check_ld(const char *fn, long ld, long width, const char *what)
 {
-    if (ld < width || ld % 4 || ld > 1L << 40)
+    if (ld < width || ld % 4 || ld > RT_STRIDE_MAX)
         failf(fn, "%s must be a multiple of 4 of at least %ld", what, width);
 }
 
@@ -1761,7 +1764,7 @@ span kv_span(const struct rt_kv *kv, const void *p)
 void check_heads(const char *fn, const void *p, long t, long ld, long hd, long heads, long dim, bool in, const char *what)
 {
     check_dev_ptr(fn, p, what);
-    if (ld < 0 || hd < 0 || ld % 4 || hd % 4 || ld > 1L << 40 || hd > 1L << 40)
+    if (ld < 0 || hd < 0 || ld % 4 || hd % 4 || ld > RT_STRIDE_MAX || hd > RT_STRIDE_MAX)
         failf(fn, "%s: strides are multiples of 4, 0 or more", what);
     if (!in && !((t == 1 || ld >= (heads - 1) * hd + dim) && (heads == 1 || hd >= dim)) && !((heads == 1 || hd >= (t - 1) * ld + dim) && (t == 1 || ld >= dim)))
         failf(fn, "%s: its heads must not overlap", what);
@@ -1836,7 +1839,7 @@ void rt_delta_rule_dev(struct rt *R, const struct rt_seqs *s, const struct rt_de
     check_words(fn, a->b, 4, "b");
     check_words(fn, a->decay, 4, "decay");
     check_words(fn, a->dt, 4, "dt");
-    if (a->a_ld < a->v_heads || a->b_ld < a->v_heads || a->a_ld > 1L << 40 || a->b_ld > 1L << 40)
+    if (a->a_ld < a->v_heads || a->b_ld < a->v_heads || a->a_ld > RT_STRIDE_MAX || a->b_ld > RT_STRIDE_MAX)
         fail(fn, "a_ld and b_ld must be at least v_heads");
     if (a->z) {
         check_dev_ptr(fn, a->z, "z");

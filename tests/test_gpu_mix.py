@@ -433,6 +433,18 @@ def test_attn_empty_rows_and_pages_that_are_not_there(rt, q8rt):
     assert np.isnan(got[:3]).all() and np.isfinite(got[3:7]).all() and (got[7:] == 0).all()
 
 
+@pytest.mark.parametrize("kind,small", [("f16", 2.0 ** -18), ("bf16", 2.0 ** -100), ("f32", 2.0 ** -100)])
+def test_attn_small_values(rt, q8rt, kind, small):
+    """Keys and values far below 1 (in F16 among its subnormals, which count in full), queries as far above."""
+    rng = np.random.default_rng(16)
+    n, hq, dim = 300, 4, 64
+    cache = Paged(rng, kind, [n], 1, dim, 16, k=[small * rng.standard_normal((n, 1, dim))], v=[small * rng.standard_normal((n, 1, dim))])
+    q = (rng.standard_normal((1, hq, dim)) / small).astype(np.float32)
+    want, tol = ref.attn(q, cache.seq_k, cache.seq_v, 0.125, starts([1]), [n - 1])
+    got = run_attn(rt, q8rt, cache, q, starts([1]), [n - 1], 0.125)[:, :hq * dim].reshape(1, hq, dim)
+    assert (np.abs(got - want) <= tol).all()
+
+
 # ---- starts that make no sense, several calls, graphs
 
 
