@@ -564,15 +564,34 @@ __device__ __forceinline__ void chunk_loop(const rt_delta &a, const chunk_unit &
     };
     if constexpr (KEYS)
         __builtin_amdgcn_s_setprio(1); /* the chain from state to state is theirs */
+    /* The queries' last product, of a chunk's P with its D, and the rows of O, are done a chunk later, while the keys have
+     * their longest part: D stays in LDS until then. As the chunk's last part every wave waited for it. */
+    v4f under_way = {0.0f, 0.0f, 0.0f, 0.0f};
+    bool open = false;
+    const auto finish = [&](long n) {
+        if (open) {
+#pragma unroll
+            for (int j = 0; j < TILES; j++)
+                if (j <= tile)
+                    under_way = mfma4(mv[j], m.sv[j][lane], under_way);
+            const int here = (int)(count - n * CHUNK < CHUNK ? count - n * CHUNK : CHUNK) - 16 * tile - 4 * g;
+            float *o = a.o + (u.first + n * CHUNK + 16 * tile + 4 * g) * a.o_ld + u.h * a.v_dim + u.col;
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                if (r < here)
+                    o[r * a.o_ld] = under_way[r];
+        }
+    };
     load_rows(u.c0);
-    load_matrix(u.c0);
+    if constexpr (KEYS)
+        load_matrix(u.c0);
     gamma = factors[u.c0 * part + 3 * CHUNK];
     __syncthreads();
     for (long n = u.c0; n < u.c1; n++) {
         const long next = n + 1 < u.c1 ? n + 1 : n;
         v4f z = {0.0f, 0.0f, 0.0f, 0.0f};
-        const int here = (int)(count - n * CHUNK < CHUNK ? count - n * CHUNK : CHUNK) - 16 * tile - 4 * g; /* rows from 4 g on that there are */
         if constexpr (KEYS) {
+            const int here = (int)(count - n * CHUNK < CHUNK ? count - n * CHUNK : CHUNK) - 16 * tile - 4 * g; /* rows from 4 g on that there are */
             v4f y[2] = {z, z};
 #pragma unroll
             for (int t = 0; t < NT; t++) {
@@ -593,6 +612,8 @@ __device__ __forceinline__ void chunk_loop(const rt_delta &a, const chunk_unit &
 #pragma unroll
             for (int t = 0; t < NT / 2; t++)
                 z = mfma4(xv[t], m.ss[t][lane], z);
+            finish(n - 1);
+            load_matrix(n);
         }
         __syncthreads();
         const bool whole = __builtin_amdgcn_readfirstlane(m.odd) == 0;
@@ -613,8 +634,9 @@ __device__ __forceinline__ void chunk_loop(const rt_delta &a, const chunk_unit &
 #pragma unroll
                 for (int t = NT / 2; t < NT; t++)
                     z = mfma4(xv[t], m.ss[t][lane], z);
-                z = v4f{scale.x * z[0], scale.y * z[1], scale.z * z[2], scale.w * z[3]};
+                under_way = v4f{scale.x * z[0], scale.y * z[1], scale.z * z[2], scale.w * z[3]};
             }
+            open = whole;
             load_rows(next);
         }
         __syncthreads();
@@ -631,24 +653,12 @@ __device__ __forceinline__ void chunk_loop(const rt_delta &a, const chunk_unit &
                     m.ss[t][lane] = as4(s[0] + s[1]);
                 }
             }
-            if constexpr (!KEYS)
-#pragma unroll
-                for (int j = 0; j < TILES; j++)
-                    if (j <= tile)
-                        z = mfma4(mv[j], m.sv[j][lane], z);
         }
         gamma = factors[next * part + 3 * CHUNK];
-        if constexpr (!KEYS) {
-            load_matrix(next);
-            float *o = a.o + (u.first + n * CHUNK + 16 * tile + 4 * g) * a.o_ld + u.h * a.v_dim + u.col;
-            if (whole)
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    if (r < here)
-                        o[r * a.o_ld] = z[r];
-        }
         __syncthreads();
     }
+    if constexpr (!KEYS)
+        finish(u.c1 - 1);
 }
 
 template <int DK>
