@@ -418,17 +418,23 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
                 x[r] = __builtin_amdgcn_exp2f(x[r] - ref);
                 l += x[r];
             }
-            const bool one = u.j0 == u.j1;
-            if (whole || one) {
-                /* values that the row tile's one token does not see are 0: 0 times an infinite or NaN one would be NaN */
-                if (!whole)
+            /* a weight of 0 times an infinite or NaN value would be NaN: values that no row of the tile sees are 0, and
+             * those that some do not see are looked at */
+            bool apart = false;
+            if (!whole) {
+                float odd = 0.0f; /* NaN: one is infinite or NaN */
 #pragma unroll
-                    for (int r = 0; r < 4; r++)
+                for (int r = 0; r < 4; r++)
 #pragma unroll
-                        for (int i = 0; i < NV; i++)
+                    for (int i = 0; i < NV; i++)
 #pragma unroll
-                            for (int e = 0; e < VEC; e++)
-                                vw[r][i][e] = tile * 16 + 4 * g + r > u.last ? 0 : vw[r][i][e];
+                        for (int e = 0; e < VEC; e++) {
+                            vw[r][i][e] = tile * 16 + 4 * g + r > u.last ? 0 : vw[r][i][e];
+                            odd = fmaf(__builtin_bit_cast(float, vw[r][i][e]), 0.0f, odd);
+                        }
+                apart = u.j0 < u.j1 && __ballot(odd != 0.0f);
+            }
+            if (!apart) {
 #pragma unroll
                 for (int r = 0; r < 4; r++)
 #pragma unroll
@@ -437,8 +443,7 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
                         for (int e = 0; e < VEC; e++)
                             acc[i * VEC + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vw[r][i][e]), x[r], acc[i * VEC + e], 0, 0, 0);
             } else {
-                /* positions that some of the rows do not see: 0 times an infinite or NaN value would be NaN,
-                 * so each token's rows are computed apart, without the values behind it */
+                /* each token's rows are computed apart, without the values behind it */
                 for (int jj = u.j0; jj <= u.j1; jj++) {
                     const long upto = (long)u.q.past + jj < u.last ? (long)u.q.past + jj : u.last;
 #pragma unroll
@@ -711,12 +716,11 @@ __global__ __launch_bounds__(64 * WAVES, alone(D) ? 1 : 2) void attn_half_k(rt_s
                 return uint4{__builtin_amdgcn_perm(v[1][e / 2], v[0][e / 2], pick), __builtin_amdgcn_perm(v[3][e / 2], v[2][e / 2], pick),
                              __builtin_amdgcn_perm(v[5][e / 2], v[4][e / 2], pick), __builtin_amdgcn_perm(v[7][e / 2], v[6][e / 2], pick)};
             };
-            /* values that the row tile's one token does not see are 0: 0 times an infinite or NaN one would be NaN */
-            const bool one = u.j0 == u.j1;
+            /* values that no row of the tile sees are 0: 0 times an infinite or NaN one would be NaN */
             uint32_t size = 0;
 #pragma unroll
             for (int r = 0; r < 4 * SUB; r++) {
-                const bool hide = !whole && one && place(r) > u.last;
+                const bool hide = !whole && place(r) > u.last;
 #pragma unroll
                 for (int i = 0; i < NV; i++)
 #pragma unroll
@@ -726,7 +730,7 @@ __global__ __launch_bounds__(64 * WAVES, alone(D) ? 1 : 2) void attn_half_k(rt_s
                     }
             }
             const bool finite = (size & 0xffffu) < H::INF && size >> 16 < H::INF;
-            if ((whole || one) && !__ballot(!finite)) {
+            if (!__ballot(!finite)) {
 #pragma unroll
                 for (int i = 0; i < NV; i++)
 #pragma unroll
@@ -742,9 +746,8 @@ __global__ __launch_bounds__(64 * WAVES, alone(D) ? 1 : 2) void attn_half_k(rt_s
                             __builtin_amdgcn_sched_barrier(0);
                     }
             } else {
-                /* several tokens that see different positions of the tile, or values that are not finite: each token's
-                 * rows computed apart, without the values behind it. The values are loaded again, so that the
-                 * fast path keeps its registers */
+                /* values that are not finite: each token's rows computed apart, without the values behind it, which are
+                 * loaded again, so that the fast path keeps its registers */
                 for (int jj = u.j0; jj <= u.j1; jj++) {
                     const long upto = (long)u.q.past + jj < u.last ? (long)u.q.past + jj : u.last;
 #pragma unroll
