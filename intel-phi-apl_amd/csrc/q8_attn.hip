@@ -224,8 +224,10 @@ __device__ __forceinline__ bool share_of(const rt_seqs &b, const rt_kv &kv, cons
         z -= z * q.chunks > number ? 1 : 0;
         z += (z + 1) * q.chunks <= number ? 1 : 0;
     }
-    u.z = first_lane(z);
-    const int part = number - u.z * q.chunks, row = u.z * 16 + (int)(threadIdx.x & 15);
+    z = first_lane(z);
+    const int part = number - z * q.chunks;
+    u.z = q.rows - 1 - z; /* those that see most first (8192 tokens of 16 heads of 256 3114 us, 3403 last) */
+    const int row = u.z * 16 + (int)(threadIdx.x & 15);
     u.table = kv.table + s * kv.table_ld;
     u.j = (int)p.group.of(row);
     u.h = (int)blockIdx.y * group + (row - u.j * group);
@@ -798,7 +800,7 @@ __global__ __launch_bounds__(256) void attn_join_k(rt_seqs b, rt_kv kv, rt_attn 
     seq_plan q;
     if (!locate(b, p, p.heads, -1, i, s, q, before, chunk) || q.chunks == 1)
         return;
-    const int kh = (int)p.group.of((uint32_t)h), row = (int)(i - q.first) * p.heads + (int)h - kh * p.heads, z = row / 16, r = row % 16;
+    const int kh = (int)p.group.of((uint32_t)h), row = (int)(i - q.first) * p.heads + (int)h - kh * p.heads, z = q.rows - 1 - row / 16, r = row % 16;
     if ((long)before + (long)(z + 1) * q.chunks > p.slots)
         return;
     const long slot = (long)kh * p.slots + before + z * q.chunks;
