@@ -120,8 +120,8 @@ void rt_rope_kv_dev(struct rt *R, const struct rt_seqs *s, const struct rt_kv *k
 
 /* o = softmax(scale q K^T) V over the cache: the token at position p sees positions 0 .. p of its sequence
  * (its own and earlier new ones included: append them first), query head h the key-value head
- * h / (q_heads / heads). Times 1 / (1 + exp(-gate)), where given. Made for one to a few new tokens on a
- * cache of any length, whose positions are split over the GPU and joined; a prompt's tokens are right too.
+ * h / (q_heads / heads). Times 1 / (1 + exp(-gate)), where given. For a few new tokens on a cache of any
+ * length the positions are split over the GPU and joined; a prompt's tokens go 16 rows (token, head) at a time.
  * A token that sees nothing (a position before 0) gives zeros; one that would have to see a position behind
  * the table's last page, or in a page that the cache does not have, gives NaN. */
 struct rt_attn {

@@ -44,16 +44,6 @@ __device__ __forceinline__ long q8_sequence_of(const rt_seqs &b, long i)
     return (long)b.start[s] <= i && i < (long)b.start[s + 1] ? s : -1;
 }
 
-/* the sum over each row of 16 lanes, in every lane of it: pairs i^1, i^2, then the mirrors */
-__device__ __forceinline__ float q8_row_sum(float v)
-{
-    v += Q8_DPP(v, 0xb1);
-    v += Q8_DPP(v, 0x4e);
-    v += Q8_DPP(v, 0x141);
-    v += Q8_DPP(v, 0x140);
-    return v;
-}
-
 /* 1 / (1 + exp(-x)) without an overflow on either side */
 __device__ __forceinline__ float q8_sigmoid(float x)
 {

@@ -11,7 +11,7 @@ namespace {
  * start once more, from L2) and a workgroup's loads are whole lines. Every load is unconditional: rows that there are not
  * are ones that there are, and their results are not stored. A sequence's first workgroup, the only one to read its
  * state, writes the new one at its end, so that the state may be updated in place. Bound by HBM on prompts (3400 tokens
- * of 8192 channels 57 us, 4.6 TB/s), by latency on single tokens, for which RUN is 1. */
+ * of 8192 channels 52 us, 5.0 TB/s), by latency on single tokens, for which RUN is 1. */
 template <int TAPS, int RUN>
 __global__ __launch_bounds__(256) void conv_k(rt_seqs b, const float *__restrict__ x, long x_ld, long ch, const float *__restrict__ w, const float *s_in,
                                               float *s_out, float *__restrict__ y, long y_ld)

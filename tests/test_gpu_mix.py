@@ -374,6 +374,21 @@ def test_attn(rt, q8rt, kind, hq, hk, dim, page, lens, news, first):
         assert (np.abs(got[live, :hq * dim].reshape(-1, hq, dim) - want[live]) <= tol[live]).all()
 
 
+PROMPTS = [
+    # prompts that fill the GPU by themselves, alone and with a sequence that is longer or shorter: cut, or not
+    (16, 8, 64, 16, [600], [600], 0),
+    (16, 8, 64, 16, [3001, 600], [1, 600], 3),
+    (8, 8, 256, 64, [900, 520, 5], [20, 520, 5], 0),
+    (16, 4, 128, 24, [270, 2100], [270, 33], 1),
+]
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hq,hk,dim,page,lens,news,first", PROMPTS)
+def test_attn_prompts(rt, q8rt, kind, hq, hk, dim, page, lens, news, first):
+    test_attn(rt, q8rt, kind, hq, hk, dim, page, lens, news, first)
+
+
 @pytest.mark.parametrize("kind", ["f32", "f16", "bf16"])
 def test_attn_large_scores(rt, q8rt, kind):
     """Scores of hundreds (their exponentials overflow without the maximum), negative scales, one key far above the rest."""
