@@ -183,7 +183,12 @@ constexpr int CHUNK = 64, TILES = CHUNK / 16, PAIRS = TILES * (TILES + 1) / 2;
 /* a chunk's part of a head: tiles (i, j), j <= i, of T and of P, 256 floats each in a first operand's order, and
  * gamma rk, scale gamma rq and D_C rk of its tokens, gamma_C, and whether anything of it is not finite (a wave each) */
 constexpr int PREP = 2 * PAIRS * 256 + 4 * CHUNK;
-constexpr int PREP_BYTES = 4 * PREP;
+/* a chunk's part in floats: its value heads', then each key head's rows of K and of Q as first operands lie, 256 floats
+ * a tile of 16 rows and 16 columns. There consecutive lanes load consecutive 16 bytes; from the rows themselves each lane's
+ * are in another row, and the vector cache takes a cycle for every lane. */
+__host__ __device__ __forceinline__ long part_of(const rt_delta &a) { return a.v_heads * PREP + a.k_heads * 2 * CHUNK * a.k_dim; }
+template <int DK>
+__device__ __forceinline__ long rows_at(const rt_delta &a, long kh, int q, int tile) { return a.v_heads * PREP + ((kh * 2 + q) * TILES + tile) * 16 * DK; }
 
 __device__ __forceinline__ v4f mfma4(float4 x, float4 y, v4f z)
 {
@@ -263,11 +268,14 @@ __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int m
         qv[t] = *(const float4 *)(qp + 16 * t);
     }
     load_gates(0);
+    float *part = out + blockIdx.x * part_of(a);
 #pragma unroll
     for (int t = 0; t < NT; t++) {
         kv[t] = kr < n ? kv[t] : float4{0.0f, 0.0f, 0.0f, 0.0f};
         qv[t] = qr < n ? qv[t] : float4{0.0f, 0.0f, 0.0f, 0.0f};
         *(float4 *)&sk[kr][16 * t + 4 * g] = kv[t];
+        *(float4 *)(part + rows_at<DK>(a, kh, 0, wave) + t * 256 + lane * 4) = kv[t];
+        *(float4 *)(part + rows_at<DK>(a, kh, 1, 3 - wave) + t * 256 + lane * 4) = qv[t];
         kk += dot4(kv[t], kv[t]);
         qq += dot4(qv[t], qv[t]);
     }
@@ -295,7 +303,7 @@ __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int m
 
     for (int hn = 0; hn < heads; hn++) {
         const long h = head(hn);
-        float *mine = out + ((long)blockIdx.x * a.v_heads + h) * PREP, *factor = mine + 2 * PAIRS * 256;
+        float *mine = part + h * PREP, *factor = mine + 2 * PAIRS * 256;
         /* lane i of every wave: token i's gates */
         const float alpha = lane < n ? decay_of(ga, dt, rate) : 1.0f;
         if (wave == 0)
@@ -510,19 +518,17 @@ __device__ __forceinline__ void chunk_loop(const rt_delta &a, const chunk_unit &
     constexpr int NT = DK / 16;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
     const int tile = KEYS ? wave : 7 - wave;
-    const long ld = KEYS ? a.k_ld : a.q_ld, part = a.v_heads * (long)PREP;
-    const float *rows = (KEYS ? a.k : a.q) + u.first * ld + u.kh * DK + 4 * g, *values = a.v + u.first * a.v_ld + u.h * a.v_dim + u.col;
+    const long part = part_of(a);
+    const float *rows = prep + u.slot * part + rows_at<DK>(a, u.kh, KEYS ? 0 : 1, tile) + lane * 4, *values = a.v + u.first * a.v_ld + u.h * a.v_dim + u.col;
     const float *matrix = prep + u.slot * part + u.h * PREP + ((KEYS ? 0 : PAIRS) + tile * (tile + 1) / 2) * 256 + lane * 4;
     const float *factors = prep + u.slot * part + u.h * PREP + 2 * PAIRS * 256;
     const long count = u.last - u.first;
     float4 xv[NT], mv[TILES], scale, left;
     float v[4], gamma, odd;
     const auto load_rows = [&](long n) {
-        const long i = n * CHUNK + 16 * tile + c;
-        const float *p = rows + (i < count ? i : n * CHUNK) * ld;
 #pragma unroll
         for (int t = 0; t < NT; t++)
-            xv[t] = *(const float4 *)(p + 16 * t);
+            xv[t] = *(const float4 *)(rows + n * part + t * 256);
         scale = *(const float4 *)(factors + n * part + (KEYS ? 0 : CHUNK) + 16 * tile + 4 * g);
         if constexpr (KEYS) {
             odd = factors[n * part + 3 * CHUNK + 4 + wave];
@@ -545,20 +551,14 @@ __device__ __forceinline__ void chunk_loop(const rt_delta &a, const chunk_unit &
      * find their lines there come back within a line of the chunk; from HBM they did not. */
     float ahead = 0.0f;
     const auto fetch = [&](long n) {
-        constexpr int ROW = DK / 32, SHARED = 2 * CHUNK * ROW + PREP_BYTES / 128;
-        const long i0 = n * CHUNK, rest = count - i0;
-        int l = u.slice + u.slices * ((wave - 4) * 64 + lane);
-        const float *p = nullptr;
-        if (wave == 7) {
-            p = values + (i0 + (lane < rest ? lane : 0)) * a.v_ld - c;
-        } else if (l < 2 * CHUNK * ROW) {
-            const bool q = l >= CHUNK * ROW;
-            l -= q ? CHUNK * ROW : 0;
-            const long i = i0 + (l / ROW < rest ? l / ROW : 0);
-            p = (q ? a.q + (u.first + i) * a.q_ld : a.k + (u.first + i) * a.k_ld) + u.kh * DK + l % ROW * 32;
-        } else if (l < SHARED) {
-            p = prep + (u.slot + n) * part + u.h * PREP + (l - 2 * CHUNK * ROW) * 32;
-        }
+        constexpr int ROWS = 2 * CHUNK * DK / 32, SHARED = ROWS + PREP / 32;
+        const long rest = count - n * CHUNK;
+        const int l = u.slice + u.slices * ((wave - 4) * 64 + lane);
+        const float *chunk = prep + (u.slot + n) * part, *p = nullptr;
+        if (wave == 7)
+            p = values + (n * CHUNK + (lane < rest ? lane : 0)) * a.v_ld - c;
+        else if (l < SHARED)
+            p = chunk + (l < ROWS ? rows_at<DK>(a, u.kh, 0, 0) + l * 32 : u.h * PREP + (l - ROWS) * 32);
         if (p)
             ahead = *p;
     };
@@ -755,14 +755,14 @@ constexpr long PREP_MAX = 256L << 20;
 static long slots_of(const rt_seqs &b) { return b.t / CHUNK + b.n; }
 static long slots_a_launch(const rt_delta &a)
 {
-    const long n = PREP_MAX / (PREP_BYTES * a.v_heads);
+    const long n = PREP_MAX / (4 * part_of(a));
     return n < 1 ? 1 : n;
 }
 
 long q8_delta_prep_floats(const rt_seqs &b, const rt_delta &a)
 {
     const long all = slots_of(b), most = slots_a_launch(a);
-    return b.longest > SHORT ? (all < most ? all : most) * a.v_heads * PREP : 0;
+    return b.longest > SHORT ? (all < most ? all : most) * part_of(a) : 0;
 }
 
 /* true where the output's norm and gate were done with it */
