@@ -440,15 +440,18 @@ __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int m
  * rows 16 v .., 16 (v + 8) ... The state stays in LDS from chunk to chunk. A chunk, with a barrier behind each
  * line (the second half's work stands in brackets):
  *
- *   R = V - gamma K S0                             [Q S0, half of it]
- *   d = T R, D_C d                                 [the other half]
- *   S = gamma_C S0 + K^T (D_C d)                   [the same, and O = gamma Q S0 + P d]
+ *   R = V - gamma K S0                             [Q S0, half of it; O = Z + P d of the chunk before]
+ *   d = T R, D_C d                                 [the other half: Z = gamma Q S0]
+ *   S = gamma_C S0 + K^T (D_C d)                   [the same]
  *
  * What a wave needs of the next chunk is loaded as soon as this one's has been used. The workgroups of a head are
- * on one XCD, whose L2 then has K, Q, T and P for all of them.
+ * on one XCD, whose L2 then has K, Q, T and P for all of them. A chunk takes 2.9 us (8192 tokens of 32 heads, a workgroup a
+ * compute unit), 1.5 of them the matrix instructions' own; the rest is what the three barriers leave waiting, which a
+ * second workgroup on the compute unit, where the call has as many, fills in part.
  *
  * A chunk with anything that is not finite goes token by token: in the products 0 times a later token's NaN
- * would reach earlier ones. */
+ * would reach earlier ones. So do the chunks behind it: a way back into the loop would hold its registers meanwhile, and
+ * there would be no second workgroup (16 heads of 1003, 963 and 692 tokens 72 us, 84 that way). */
 constexpr int CHUNK_THREADS = 512;
 
 template <int DK>
@@ -504,16 +507,13 @@ __device__ __forceinline__ void odd_chunk(const rt_delta &a, const chunk_unit &u
         }
         __syncthreads();
     }
-    if (tid == 0)
-        m.odd = 0;
-    __syncthreads();
 }
 
 /* The chunks, as one half of the waves sees them. Every load is unconditional (rows behind the sequence's end are
  * the chunk's first one again, whose products go nowhere), and the halves have loops of their own: under a branch the
  * compiler no longer knows how many loads are in flight, and waits for those of the next chunk with this one's. */
 template <int DK, bool KEYS>
-__device__ __forceinline__ void chunk_loop(const rt_delta &a, const chunk_unit &u, chunk_lds<DK> &m, const float *prep)
+__device__ __forceinline__ long chunk_loop(const rt_delta &a, const chunk_unit &u, chunk_lds<DK> &m, const float *prep)
 {
     constexpr int NT = DK / 16;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
@@ -567,20 +567,17 @@ __device__ __forceinline__ void chunk_loop(const rt_delta &a, const chunk_unit &
     /* The queries' last product, of a chunk's P with its D, and the rows of O, are done a chunk later, while the keys have
      * their longest part: D stays in LDS until then. As the chunk's last part every wave waited for it. */
     v4f under_way = {0.0f, 0.0f, 0.0f, 0.0f};
-    bool open = false;
     const auto finish = [&](long n) {
-        if (open) {
 #pragma unroll
-            for (int j = 0; j < TILES; j++)
-                if (j <= tile)
-                    under_way = mfma4(mv[j], m.sv[j][lane], under_way);
-            const int here = (int)(count - n * CHUNK < CHUNK ? count - n * CHUNK : CHUNK) - 16 * tile - 4 * g;
-            float *o = a.o + (u.first + n * CHUNK + 16 * tile + 4 * g) * a.o_ld + u.h * a.v_dim + u.col;
+        for (int j = 0; j < TILES; j++)
+            if (j <= tile)
+                under_way = mfma4(mv[j], m.sv[j][lane], under_way);
+        const int here = (int)(count - n * CHUNK < CHUNK ? count - n * CHUNK : CHUNK) - 16 * tile - 4 * g;
+        float *o = a.o + (u.first + n * CHUNK + 16 * tile + 4 * g) * a.o_ld + u.h * a.v_dim + u.col;
 #pragma unroll
-            for (int r = 0; r < 4; r++)
-                if (r < here)
-                    o[r * a.o_ld] = under_way[r];
-        }
+        for (int r = 0; r < 4; r++)
+            if (r < here)
+                o[r * a.o_ld] = under_way[r];
     };
     load_rows(u.c0);
     if constexpr (KEYS)
@@ -612,46 +609,39 @@ __device__ __forceinline__ void chunk_loop(const rt_delta &a, const chunk_unit &
 #pragma unroll
             for (int t = 0; t < NT / 2; t++)
                 z = mfma4(xv[t], m.ss[t][lane], z);
-            finish(n - 1);
+            if (n > u.c0)
+                finish(n - 1);
             load_matrix(n);
         }
         __syncthreads();
-        const bool whole = __builtin_amdgcn_readfirstlane(m.odd) == 0;
-        if (!whole)
-            odd_chunk(a, u, m, n);
+        if (__builtin_amdgcn_readfirstlane(m.odd))
+            return n;
         if constexpr (KEYS) {
-            if (whole) {
 #pragma unroll
-                for (int j = 0; j < TILES; j++)
-                    if (j <= tile)
-                        z = mfma4(mv[j], m.sr[j][lane], z);
-                m.sv[tile][lane] = as4(z);
-                m.sw[tile][lane] = as4(z) * left;
-            }
+            for (int j = 0; j < TILES; j++)
+                if (j <= tile)
+                    z = mfma4(mv[j], m.sr[j][lane], z);
+            m.sv[tile][lane] = as4(z);
+            m.sw[tile][lane] = as4(z) * left;
             load_matrix(next);
         } else {
-            if (whole) {
 #pragma unroll
-                for (int t = NT / 2; t < NT; t++)
-                    z = mfma4(xv[t], m.ss[t][lane], z);
-                under_way = v4f{scale.x * z[0], scale.y * z[1], scale.z * z[2], scale.w * z[3]};
-            }
-            open = whole;
+            for (int t = NT / 2; t < NT; t++)
+                z = mfma4(xv[t], m.ss[t][lane], z);
+            under_way = v4f{scale.x * z[0], scale.y * z[1], scale.z * z[2], scale.w * z[3]};
             load_rows(next);
         }
         __syncthreads();
-        if (whole) {
 #pragma unroll
-            for (int t0 = 0; t0 < NT; t0 += 8) {
-                const int t = t0 + wave;
-                if (t < NT) {
-                    const float4 o = m.ss[t][lane];
-                    v4f s[2] = {v4f{gamma * o.x, gamma * o.y, gamma * o.z, gamma * o.w}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
+        for (int t0 = 0; t0 < NT; t0 += 8) {
+            const int t = t0 + wave;
+            if (t < NT) {
+                const float4 o = m.ss[t][lane];
+                v4f s[2] = {v4f{gamma * o.x, gamma * o.y, gamma * o.z, gamma * o.w}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-                    for (int j = 0; j < TILES; j++)
-                        s[j & 1] = mfma4(*(const float4 *)&m.sk[16 * t + c][16 * j + 4 * g], m.sw[j][lane], s[j & 1]);
-                    m.ss[t][lane] = as4(s[0] + s[1]);
-                }
+                for (int j = 0; j < TILES; j++)
+                    s[j & 1] = mfma4(*(const float4 *)&m.sk[16 * t + c][16 * j + 4 * g], m.sw[j][lane], s[j & 1]);
+                m.ss[t][lane] = as4(s[0] + s[1]);
             }
         }
         gamma = factors[next * part + 3 * CHUNK];
@@ -659,6 +649,7 @@ __device__ __forceinline__ void chunk_loop(const rt_delta &a, const chunk_unit &
     }
     if constexpr (!KEYS)
         finish(u.c1 - 1);
+    return u.c1;
 }
 
 template <int DK>
@@ -690,10 +681,8 @@ __global__ __launch_bounds__(CHUNK_THREADS) void delta_chunk_k(rt_seqs b, rt_del
     }
     if (tid == 0)
         m.odd = 0;
-    if (wave < 4)
-        chunk_loop<DK, true>(a, u, m, prep);
-    else
-        chunk_loop<DK, false>(a, u, m, prep);
+    for (long n = wave < 4 ? chunk_loop<DK, true>(a, u, m, prep) : chunk_loop<DK, false>(a, u, m, prep); n < u.c1; n++)
+        odd_chunk(a, u, m, n);
     for (int t = wave; t < DK / 16; t += 8) {
         float *p = a.s_out + state + (16 * t + 4 * g) * a.v_dim;
         const float4 z = m.ss[t][lane];
