@@ -736,7 +736,7 @@ __global__ __launch_bounds__(256) void gated_norm_k(rt_seqs b, rt_delta a, int l
 } /* namespace */
 
 /* Sequences of more tokens than this go in chunks (heads of 128 x 128, 32 of them; us token by token and in chunks: one sequence
- * of 24 tokens 25 / 31, of 32 30 / 31, of 48 42 / 32; 4 of 32 38 / 52, of 48 52 / 53; 16 of 48 138 / 141) */
+ * of 24 tokens 25 / 31, of 32 30 / 31, of 48 41 / 31; 4 of 32 36 / 46, of 48 50 / 47; 16 of 32 95 / 101, of 48 136 / 106) */
 constexpr int SHORT = 32;
 /* The chunks' parts of all heads that a launch makes and takes, in bytes: longer calls alternate */
 constexpr long PREP_MAX = 256L << 20;
