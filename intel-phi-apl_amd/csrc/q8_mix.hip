@@ -10,7 +10,7 @@ namespace {
  * before them in registers, all loaded before any arithmetic, so each x is read from HBM once (the rows at a run's
  * start once more, from L2) and a workgroup's loads are whole lines. Every load is unconditional: rows that there are not
  * are ones that there are, and their results are not stored. A sequence's first workgroup, the only one to read its
- * state, writes the new one at its end, so that the state may be updated in place. Bound by HBM on prompts (3400 tokens
+ * state, writes the new one at its end, so that the state may be updated in place. Bound by HBM on prompts (3996 tokens
  * of 8192 channels 52 us, 5.0 TB/s), by latency on single tokens, for which RUN is 1. */
 template <int TAPS, int RUN>
 __global__ __launch_bounds__(256) void conv_k(rt_seqs b, const float *__restrict__ x, long x_ld, long ch, const float *__restrict__ w, const float *s_in,
@@ -246,7 +246,7 @@ void q8_launch_rope(q8_stream_t s, const rt_seqs &b, const rt_kv &kv, const rt_r
     while (lanes * 4 < kv.dim)
         lanes *= 2;
     const long heads = a.q_heads + 2 * kv.heads, per = ROPE_THREADS / lanes, groups = (heads + per - 1) / per;
-    /* two tokens a workgroup where that still gives every compute unit eight of them (3351 tokens, 24 heads of 256: 57 us, 4.0
+    /* two tokens a workgroup where that still gives every compute unit eight of them (5027 tokens, 24 heads of 256: 57 us, 4.0
      * TB/s; four 66, eight 82) */
     if (b.t * groups >= 4096)
         launch_rope<2>((hipStream_t)s, dim3((unsigned)((b.t + 1) / 2), (unsigned)groups), b, kv, a, lanes);
