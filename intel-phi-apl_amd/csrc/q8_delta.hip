@@ -445,7 +445,7 @@ __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int m
  *   S = gamma_C S0 + K^T (D_C d)                   [the same]
  *
  * What a wave needs of the next chunk is loaded as soon as this one's has been used. The workgroups of a head are
- * on one XCD, whose L2 then has K, Q, T and P for all of them. A chunk takes 2.9 us (8192 tokens of 32 heads, a workgroup a
+ * on one XCD, whose L2 then has K, Q, T and P for all of them. A chunk takes 2.7 us (8192 tokens of 32 heads, a workgroup a
  * compute unit), 1.5 of them the matrix instructions' own; the rest is what the three barriers leave waiting, which a
  * second workgroup on the compute unit, where the call has as many, fills in part.
  *
@@ -584,7 +584,9 @@ __device__ __forceinline__ long chunk_loop(const rt_delta &a, const chunk_unit &
         load_matrix(u.c0);
     gamma = factors[u.c0 * part + 3 * CHUNK];
     __syncthreads();
-    for (long n = u.c0; n < u.c1; n++) {
+    bool whole = true; /* left at the loop's end only: a way out from its middle would let the compiler count fewer loads in flight */
+    long n = u.c0;
+    for (; n < u.c1 && whole; n++) {
         const long next = n + 1 < u.c1 ? n + 1 : n;
         v4f z = {0.0f, 0.0f, 0.0f, 0.0f};
         if constexpr (KEYS) {
@@ -614,8 +616,7 @@ __device__ __forceinline__ long chunk_loop(const rt_delta &a, const chunk_unit &
             load_matrix(n);
         }
         __syncthreads();
-        if (__builtin_amdgcn_readfirstlane(m.odd))
-            return n;
+        whole = __builtin_amdgcn_readfirstlane(m.odd) == 0;
         if constexpr (KEYS) {
 #pragma unroll
             for (int j = 0; j < TILES; j++)
@@ -641,19 +642,25 @@ __device__ __forceinline__ long chunk_loop(const rt_delta &a, const chunk_unit &
 #pragma unroll
                 for (int j = 0; j < TILES; j++)
                     s[j & 1] = mfma4(*(const float4 *)&m.sk[16 * t + c][16 * j + 4 * g], m.sw[j][lane], s[j & 1]);
-                m.ss[t][lane] = as4(s[0] + s[1]);
+                if (whole)
+                    m.ss[t][lane] = as4(s[0] + s[1]);
             }
         }
         gamma = factors[next * part + 3 * CHUNK];
         __syncthreads();
     }
+    if (!whole)
+        return n - 1;
     if constexpr (!KEYS)
-        finish(u.c1 - 1);
-    return u.c1;
+        finish(n - 1);
+    return n;
 }
 
-template <int DK>
-__global__ __launch_bounds__(CHUNK_THREADS) void delta_chunk_k(rt_seqs b, rt_delta a, int most, long from, long count, const float *prep)
+/* WAVES: of a SIMD, 4 for two workgroups a compute unit, for which k_dim 128 has a few registers too many (smaller ones have
+ * room as they are, larger ones none in LDS): 8 times 512 tokens of 32 heads, 8 workgroups a compute unit, 175 us, 195 with one
+ * at a time; 8192 tokens, one workgroup, 373 and 342 */
+template <int DK, int WAVES>
+__global__ __launch_bounds__(CHUNK_THREADS, WAVES) void delta_chunk_k(rt_seqs b, rt_delta a, int most, long from, long count, const float *prep)
 {
     __shared__ __align__(16) chunk_lds<DK> m;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
@@ -782,7 +789,11 @@ static bool launch_delta(hipStream_t s, const rt_seqs &b, const rt_delta &a, flo
     for (long from = 0; from < all; from += most) {
         const long count = all - from < most ? all - from : most;
         delta_prep_k<DK><<<dim3((unsigned)count, (unsigned)a.k_heads), 256, 0, s>>>(b, a, SHORT, from, prep);
-        delta_chunk_k<DK><<<dim3((unsigned)(units * (a.v_dim / 16))), CHUNK_THREADS, 0, s>>>(b, a, SHORT, from, count, prep);
+        const unsigned groups = (unsigned)(units * (a.v_dim / 16));
+        if (DK == 128 && groups > 256)
+            delta_chunk_k<DK, DK == 128 ? 4 : 2><<<groups, CHUNK_THREADS, 0, s>>>(b, a, SHORT, from, count, prep);
+        else
+            delta_chunk_k<DK, 2><<<groups, CHUNK_THREADS, 0, s>>>(b, a, SHORT, from, count, prep);
     }
     return false;
 }
