@@ -219,6 +219,26 @@ def test_delta_nan_stays_in_its_head(rt, q8rt, n):
     assert np.isfinite(got).all() and np.isfinite(state).all()
 
 
+@pytest.mark.parametrize("lens,hk,hv,dv", [([260], 2, 4, 32), ([260, 33, 64, 65, 200], 8, 8, 128)])  # one workgroup a compute unit, or more
+@pytest.mark.parametrize("bad", [None, 0, 70, 150, 259])
+def test_delta_chunks_around_a_nan(rt, q8rt, lens, hk, hv, dv, bad):
+    """The chunks before, with and after a value that is NaN: all that it does not reach is as without it."""
+    say("delta nan", lens, hk, hv, dv, bad)
+    rng = np.random.default_rng(len(lens))
+    start = starts(lens)
+    t = int(start[-1])
+    x = delta_inputs(rng, t, hk, hv, 128, dv, len(lens))
+    want, wstate, size = ref.delta(*x[:7], EPS, 128 ** -0.5, x[7], start, False)
+    if bad is not None:
+        x[2][bad, 1, 5] = np.nan
+    got, state = run_delta(rt, q8rt, x, start, False)
+    if bad is not None:
+        o = got[:, :hv * dv].reshape(t, hv, dv)
+        assert np.isnan(o[bad:lens[0], 1, 5]).all() and np.isnan(state[0, 1, :, 5]).all()
+        o[bad:lens[0], 1, 5], state[0, 1, :, 5] = want[bad:lens[0], 1, 5], wstate[0, 1, :, 5]
+    check_delta(got, state, want, wstate, size, start, 128, hv * dv)
+
+
 # ---- heads: norm, rotation, append
 
 
