@@ -175,6 +175,13 @@ def test_delta(rt, q8rt, hk, hv, dk, dv, tiled, lens, first, longest, gated, in_
     check_delta(got, state, want, wstate, size, start, dk, hv * dv)
 
 
+@pytest.mark.parametrize("hk,hv,dk,dv,lens,in_place", [(256, 256, 32, 16, [1100, 20, 900, 40], True), (32, 256, 128, 16, [2500, 33], False)])
+def test_delta_alternating(rt, q8rt, hk, hv, dk, dv, lens, in_place):
+    """So many heads that the chunks' parts do not fit the workspace at once: runs of chunks are made and taken in turn,
+    and a sequence's state goes from one to the next."""
+    test_delta(rt, q8rt, hk, hv, dk, dv, False, lens, 0, None, in_place, in_place)
+
+
 @pytest.mark.parametrize("n", [1, 5, 64, 150])
 @pytest.mark.parametrize("what", ["forget", "keep", "write", "one_key", "zero", "alternate", "plain"])
 def test_delta_extremes(rt, q8rt, what, n):
