@@ -228,9 +228,9 @@ __device__ __forceinline__ long sequence_of_slot(const rt_seqs &b, long i)
 }
 
 /* A workgroup a chunk and key head; wave w has key rows 16 w .. of K K^T and query rows 16 (3 - w) .. of Q K^T, five
- * tiles of 16 x 16 each, which the key head's value heads share. Bound by the matrix products and, for each value
- * head, the latency of the inverse: 16 x 16 on the diagonal by substitution, a column a lane, then by diagonals
- * T_ij = -T_ii sum_k A_ik T_kj. */
+ * tiles of 16 x 16 each, which the key head's value heads share. The inverse of each value head is 16 x 16 on the
+ * diagonal by substitution, a column a lane, then by diagonals T_ij = -T_ii sum_k A_ik T_kj. Bound by HBM (8192 tokens of 16
+ * and 32 heads of 128: 418 MB in 108 us, 3.9 TB/s; its matrix instructions take 20 us). */
 template <int DK>
 __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int most, long from, float *out)
 {
@@ -509,8 +509,9 @@ __device__ __forceinline__ void odd_chunk(const rt_delta &a, const chunk_unit &u
     }
 }
 
-/* The chunks, as one half of the waves sees them. Every load is unconditional (rows behind the sequence's end are
- * the chunk's first one again, whose products go nowhere), and the halves have loops of their own: under a branch the
+/* The chunks, as one half of the waves sees them: up to the last, or to one that is not finite, whose number it returns.
+ * Every load of the next chunk is unconditional (rows of V behind the sequence's end are the chunk's first one again,
+ * whose products go nowhere; those of K and Q are 0), and the halves have loops of their own: under a branch the
  * compiler no longer knows how many loads are in flight, and waits for those of the next chunk with this one's. */
 template <int DK, bool KEYS>
 __device__ __forceinline__ long chunk_loop(const rt_delta &a, const chunk_unit &u, chunk_lds<DK> &m, const float *prep)
@@ -548,7 +549,8 @@ __device__ __forceinline__ long chunk_loop(const rt_delta &a, const chunk_unit &
     };
     /* Into the XCD's L2, two chunks ahead: the head's workgroups there take a share of the chunk's lines each (128
      * bytes: its keys, its queries, its part of prep), and the last wave the rows of V that are its own. Loads that
-     * find their lines there come back within a line of the chunk; from HBM they did not. */
+     * find their lines there come back within a line of the chunk; from HBM they did not (8192 tokens, one workgroup a compute
+     * unit: a quarter slower). */
     float ahead = 0.0f;
     const auto fetch = [&](long n) {
         constexpr int ROWS = 2 * CHUNK * DK / 32, SHARED = ROWS + PREP / 32;
