@@ -842,7 +842,7 @@ __global__ __launch_bounds__(256) void attn_join_k(rt_seqs b, rt_kv kv, rt_attn 
             v = float4{fmaf(x.x, f, v.x), fmaf(x.y, f, v.y), fmaf(x.z, f, v.z), fmaf(x.w, f, v.w)};
             sum = fmaf(sl[k], f, sum);
         }
-        store_row(a, D, i, h, d, v, sum, false, gate);
+        store_row(a, D, i, h, d, v, sum, (long)q.past + (i - q.first) < 0, gate);
     }
 }
 
