@@ -195,7 +195,7 @@ __device__ __forceinline__ void store_row(const rt_attn &a, long dim, long token
  * * VEC + e of query row c is acc[i * VEC + e][r].
  *
  * The softmax's maximum is a running one that is raised only when a score passes it by more than SLACK (a
- * power of two: the exponentials stay below 2^SLACK): then the sums and outputs are scaled, which a tile
+ * power of two: the exponentials stay below 2^SLACK; an F16 cache has less, for its weights' range): then the sums and outputs are scaled, which a tile
  * rarely needs after the first. Each lane sums its own positions; the four lanes of a row add up at the end. */
 constexpr float SLACK = 8.0f;
 
@@ -266,12 +266,12 @@ __device__ __forceinline__ const char *address(const void *cache, int row, uint3
     return (const char *)cache + (uint64_t)((uint32_t)(row < 0 ? 0 : row) + head_rows) * (uint32_t)bytes;
 }
 
-/* The running maximum raised where a lane's largest score passes it by SLACK, and the reference that
+/* The running maximum raised where a lane's largest score passes it by slack, and the reference that
  * the exponents are taken from */
 template <int VE>
-__device__ __forceinline__ float reference(float top, float &m, float &l, v4f (&acc)[VE])
+__device__ __forceinline__ float reference(float top, float slack, float &m, float &l, v4f (&acc)[VE])
 {
-    if (__ballot(top > m + SLACK)) {
+    if (__ballot(top > m + slack)) {
         const float raised = fmaxf(m, group_max(top)), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - raised);
         m = raised;
         l *= f;
@@ -414,7 +414,7 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
                 if (!whole && tile * 16 + 4 * g + r > u.lim)
                     x[r] = -INFINITY;
             }
-            const float ref = reference(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), m, l, acc);
+            const float ref = reference(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), SLACK, m, l, acc);
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 x[r] = __builtin_amdgcn_exp2f(x[r] - ref);
@@ -468,11 +468,19 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
 
 /* A 16-bit cache, 32 or 64 positions a tile, on v_mfma_f32_16x16x32: the cache's values are its
  * operands as they are, and the F32 queries and weights are cut into LIMBS 16-bit values each, every one the
- * rest of those before rounded to nearest: in F16 two of them are off by 2^-24 of the value, in BF16 three by 2^-27,
- * so the products are as exact as F32 ones, at 2/16 and 3/16 of their time. F16 has few exponents: a row of queries
- * is scaled by the power of two that brings its largest to 2^14 (and its scores back), and the weights are
- * taken 2^(14 - SLACK) times as large, which the sum that divides them is, too: what then falls below F16's smallest
- * steps is 2^-31 of the largest weight.
+ * rest of those before rounded to nearest: in F16 two of them are off by at most 2^-23 of the value, in BF16 three by 2^-26, at
+ * 2/16 and 3/16 of the time of F32 products.
+ *
+ * F16 has few exponents: its smallest step is 2^-24. A row of queries is scaled by the power of two that brings its
+ * largest to 2^14 (and its scores back), so an element is off by up to 2^-39 of the row's largest. The weights are taken
+ * 2^LIFT times as large (the sum that divides them is, too), up to 2^15: those from LEAST up are off by 2^-20 of themselves
+ * at most, the others by more, and below 2^-25 they would be lost. They are a row's output where its largest weights' values
+ * are near 0, as a sequence's first position's often are. So in a tile with a weight below LEAST each row's are scaled until
+ * the largest is at 2^14 to 2^15, the sums with them. Where that leaves one below LEAST, too (20 powers of two between two
+ * positions of a tile, as beside such a first position itself), what the limbs leave of it is taken again 2^38 times as large,
+ * and again, until it is below 2^-22 of the weight. The sums wait in LDS meanwhile. 8 sequences of 4000 to 20000 positions, 32
+ * heads of 128: 81 us, 93 where a first position of 18 nats above the rest makes every tile scale; a prompt of 2048 335
+ * and 459.
  * The queries' limbs stay in LDS for the four waves. The second product's first operand is V transposed: of a
  * lane's 8 rows, the same element of two at a time by v_perm_b32. */
 template <int TYPE>
@@ -480,7 +488,7 @@ struct half_of;
 template <>
 struct half_of<RT_F16> {
     static constexpr int LIMBS = 2;
-    static constexpr float LIFT = 14.0f - SLACK;
+    static constexpr float SLACK = 1.0f, LIFT = 15.0f - SLACK, LEAST = 0x1p-5f;
     static constexpr uint32_t INF = 0x7c00;
     static __device__ __forceinline__ uint16_t round(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
     static __device__ __forceinline__ float back(uint16_t x) { return (float)__builtin_bit_cast(_Float16, x); }
@@ -489,7 +497,7 @@ struct half_of<RT_F16> {
 template <>
 struct half_of<RT_BF16> {
     static constexpr int LIMBS = 3;
-    static constexpr float LIFT = 0.0f;
+    static constexpr float SLACK = ::SLACK, LIFT = 0.0f, LEAST = 0.0f;
     static constexpr uint32_t INF = 0x7f80;
     static __device__ __forceinline__ uint16_t round(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
     static __device__ __forceinline__ float back(uint16_t x) { return __builtin_bit_cast(float, (uint32_t)x << 16); }
@@ -519,8 +527,9 @@ __device__ __forceinline__ void limbs_of(const float *x, uint4 *out)
     }
 }
 
-/* An infinite key or value is one in its product with the first limb; the others would make NaN of it (they
- * may be 0, or of the other sign), so where there may be one they get it as 0, and NaN, too */
+/* An infinite key is one in its product with the first limb; the others would make NaN of it (they
+ * may be 0, or of the other sign), so where there may be one they get it as 0, and NaN, too. A value's weights are all
+ * taken with this, and what it leaves out with 1 (where the weight is not 0): their first limb may be 0, too */
 template <int TYPE>
 __device__ __forceinline__ uint4 finite_only(uint4 x)
 {
@@ -528,6 +537,8 @@ __device__ __forceinline__ uint4 finite_only(uint4 x)
     const auto one = [](uint32_t w) { return ((w & TOP) == TOP ? 0u : w & 0xffffu) | ((w >> 16 & TOP) == TOP ? 0u : w & 0xffff0000u); };
     return uint4{one(x.x), one(x.y), one(x.z), one(x.w)};
 }
+
+__device__ __forceinline__ uint4 without(uint4 x, uint4 y) { return uint4{x.x ^ y.x, x.y ^ y.y, x.z ^ y.z, x.w ^ y.w}; }
 
 typedef unsigned short u2 __attribute__((ext_vector_type(2)));
 /* the larger magnitudes of two pairs of 16-bit values, as their bits: an infinity or NaN stays the largest */
@@ -548,10 +559,13 @@ __global__ __launch_bounds__(64 * WAVES, alone(D) ? 1 : 2) void attn_half_k(rt_s
     typedef half_of<TYPE> H;
     constexpr int LIMBS = H::LIMBS, NK = D / 32, VE = D / 16, VEC = pieces(VE, 8), NV = VE / VEC, VW = VEC / 2, SUB = sixteens(D), POS = 16 * SUB;
     static_assert(WAVES == 4);
-    constexpr int QUERIES = NK * LIMBS * 1024 + WAVES * 16 * 4;
+    constexpr int KEPT = NK * LIMBS * 1024 + WAVES * 16 * 4, QUERIES = KEPT + (TYPE == RT_F16 ? WAVES * 64 * 4 * (VE * 4 + 4 * SUB) : 0);
     __shared__ __align__(16) char lds[joint_bytes<D>() > QUERIES ? joint_bytes<D>() : QUERIES];
     uint4(*sq)[LIMBS][64] = (uint4(*)[LIMBS][64])lds; /* until the waves join */
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    /* (F16) the lane's output and weights, while a tile's are on another scale */
+    v4f *kept_acc = (v4f *)(lds + KEPT) + wave * 64 * VE + lane;
+    float *kept = (float *)(lds + KEPT + WAVES * 64 * 16 * VE) + wave * 64 * 4 * SUB + lane;
     const int group = p.heads;
     const uint32_t head_rows = (uint32_t)(blockIdx.y * kv.page);
     for (int number = (int)blockIdx.x; p.target == 0 || number < p.slots; number += (int)gridDim.x) {
@@ -703,11 +717,52 @@ __global__ __launch_bounds__(64 * WAVES, alone(D) ? 1 : 2) void attn_half_k(rt_s
                     x[r] = -INFINITY;
                 top = fmaxf(top, x[r]);
             }
-            const float ref = reference(top, m, l, acc) - H::LIFT;
+            const float ref = reference(top, H::SLACK, m, l, acc) - H::LIFT;
+            const auto limb = [](uint4 w, int e) { return H::back((uint16_t)((&w.x)[e / 2] >> (e & 1 ? 16 : 0))); };
+            uint32_t least = ~0u; /* the smallest weight's bits but 0's, less 1 */
 #pragma unroll
             for (int r = 0; r < 4 * SUB; r++) {
                 x[r] = __builtin_amdgcn_exp2f(x[r] - ref);
                 l += x[r];
+                const uint32_t bits = __builtin_bit_cast(uint32_t, x[r]) - 1;
+                least = least < bits ? least : bits;
+            }
+            constexpr uint32_t LEAST = __builtin_bit_cast(uint32_t, H::LEAST) - 1;
+            const bool small = TYPE == RT_F16 && __ballot(least < LEAST);
+            bool apart = false; /* the output is in LDS, and the tile's own in acc */
+            float down = 1.0f;
+            if (TYPE == RT_F16 && small) {
+                float most = x[0];
+#pragma unroll
+                for (int r = 1; r < 4 * SUB; r++)
+                    most = fmaxf(most, x[r]);
+                most = group_max(most);
+                int lift = most > 0.0f ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+                lift = lift < 140 ? lift : 140;
+                down = ldexpf(1.0f, -lift);
+                least = ~0u;
+#pragma unroll
+                for (int r = 0; r < 4 * SUB; r++) {
+                    x[r] = ldexpf(x[r], lift);
+                    const uint32_t bits = __builtin_bit_cast(uint32_t, x[r]) - 1;
+                    least = least < bits ? least : bits;
+                }
+                apart = __ballot(least < LEAST || lift > 40);
+                if (apart) {
+#pragma unroll
+                    for (int r = 0; r < 4 * SUB; r++)
+                        kept[64 * r] = x[r];
+#pragma unroll
+                    for (int i = 0; i < VE; i++) {
+                        kept_acc[64 * i] = acc[i];
+                        acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                    }
+                } else {
+                    const float up = ldexpf(1.0f, lift); /* outputs are below 2^(15 + 16 + 31): no overflow */
+#pragma unroll
+                    for (int i = 0; i < VE; i++)
+                        acc[i] *= up;
+                }
             }
             uint4 w[SUB / 2][LIMBS];
 #pragma unroll
@@ -731,8 +786,8 @@ __global__ __launch_bounds__(64 * WAVES, alone(D) ? 1 : 2) void attn_half_k(rt_s
                         size = larger(size, vw[i][r][e]);
                     }
             }
-            const bool finite = (size & 0xffffu) < H::INF && size >> 16 < H::INF;
-            if (!__ballot(!finite)) {
+            const bool odd_values = __ballot((size & 0xffffu) >= H::INF || size >> 16 >= H::INF);
+            if (!odd_values) {
 #pragma unroll
                 for (int i = 0; i < NV; i++)
 #pragma unroll
@@ -747,38 +802,98 @@ __global__ __launch_bounds__(64 * WAVES, alone(D) ? 1 : 2) void attn_half_k(rt_s
                         if (e & 1)
                             __builtin_amdgcn_sched_barrier(0);
                     }
-            } else {
-                /* values that are not finite: each token's rows computed apart, without the values behind it, which are
-                 * loaded again, so that the fast path keeps its registers */
-                for (int jj = u.j0; jj <= u.j1; jj++) {
-                    const long upto = (long)u.q.past + jj < u.last ? (long)u.q.past + jj : u.last;
+            }
+            if (!odd_values && !apart) {
+                if (TYPE == RT_F16 && small)
 #pragma unroll
-                    for (int k = 0; k < SUB / 2; k++)
+                    for (int i = 0; i < VE; i++)
+                        acc[i] *= down;
+                continue;
+            }
+            for (int pass = 0;; pass++) {
+                if (odd_values || pass > 0) {
+                    /* with values that are not finite each token's rows are computed apart, without the values behind it.
+                     * The values are loaded again, so that the fast path keeps its registers */
+                    uint4 seen[SUB / 2]; /* F16: 1 where there is a weight */
+                    if constexpr (TYPE == RT_F16)
 #pragma unroll
-                        for (int i = 0; i < NV; i++) {
-                            uint32_t again[8][VW];
+                        for (int k = 0; k < SUB / 2; k++) {
+                            uint32_t one[8];
 #pragma unroll
-                            for (int r = 0; r < 8; r++) {
-                                load_words<VW>(again[r], address(kv.v, rows[8 * k + r], head_rows, D * 2) + (i * 16 + c) * VEC * 2);
-                                const bool hide = place(8 * k + r) > upto;
-#pragma unroll
-                                for (int e = 0; e < VW; e++)
-                                    again[r][e] = hide ? 0 : again[r][e];
+                            for (int e = 0; e < 8; e++) {
+                                const float at = apart ? kept[64 * (8 * k + e)] : limb(w[k][0], e);
+                                one[e] = H::round(at > 0.0f ? 1.0f : at);
                             }
-#pragma unroll
-                            for (int e = 0; e < VEC; e++) {
-                                const uint4 v = turned(again, e);
-                                v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                                for (int n = 0; n < LIMBS; n++)
-                                    o = H::mfma(n ? finite_only<TYPE>(v) : v, w[k][n], o);
-                                if (u.j == jj)
-                                    acc[i * VEC + e] += o;
-                                __builtin_amdgcn_sched_barrier(0);
-                            }
-                            asm volatile("" ::: "memory"); /* the loads stay in the loop, and out of registers */
+                            seen[k] = uint4{one[0] | one[1] << 16, one[2] | one[3] << 16, one[4] | one[5] << 16, one[6] | one[7] << 16};
                         }
+                    for (int jj = odd_values ? u.j0 : u.j1; jj <= u.j1; jj++) {
+                        const long upto = (long)u.q.past + jj < u.last ? (long)u.q.past + jj : u.last;
+#pragma unroll
+                        for (int k = 0; k < SUB / 2; k++)
+#pragma unroll
+                            for (int i = 0; i < NV; i++) {
+                                uint32_t again[8][VW];
+#pragma unroll
+                                for (int r = 0; r < 8; r++) {
+                                    load_words<VW>(again[r], address(kv.v, rows[8 * k + r], head_rows, D * 2) + (i * 16 + c) * VEC * 2);
+                                    const bool hide = place(8 * k + r) > upto;
+#pragma unroll
+                                    for (int e = 0; e < VW; e++)
+                                        again[r][e] = hide ? 0 : again[r][e];
+                                }
+#pragma unroll
+                                for (int e = 0; e < VEC; e++) {
+                                    const uint4 v = turned(again, e), part = finite_only<TYPE>(v);
+                                    v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                                    for (int n = 0; n < LIMBS; n++)
+                                        o = H::mfma(TYPE == RT_F16 || n ? part : v, w[k][n], o);
+                                    if (TYPE == RT_F16 && pass == 0)
+                                        o = H::mfma(without(v, part), seen[k], o);
+                                    if (!odd_values || u.j == jj)
+                                        acc[i * VEC + e] += o;
+                                    __builtin_amdgcn_sched_barrier(0);
+                                }
+                                asm volatile("" ::: "memory"); /* the loads stay in the loop, and out of registers */
+                            }
+                    }
                 }
+                if (TYPE != RT_F16)
+                    break;
+                if (!apart) {
+#pragma unroll
+                    for (int i = 0; i < VE; i++)
+                        acc[i] *= down;
+                    break;
+                }
+                bool more = false; /* the limbs leave something of a weight that counts */
+#pragma unroll
+                for (int k = 0; k < SUB / 2; k++) {
+                    float next[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float had = kept[64 * (8 * k + e)];
+                        float left = had;
+#pragma unroll
+                        for (int n = 0; n < LIMBS; n++)
+                            left -= limb(w[k][n], e);
+                        const bool counts = fabsf(left) > 0x1p-22f * fabsf(had);
+                        more |= counts;
+                        next[e] = counts ? left * 0x1p38f : 0.0f;
+                        kept[64 * (8 * k + e)] = next[e];
+                    }
+                    limbs_of<TYPE>(next, w[k]);
+                }
+                const bool done = pass == 5 || !__ballot(more);
+#pragma unroll
+                for (int i = 0; i < VE; i++) {
+                    const v4f sum = kept_acc[64 * i] + acc[i] * down;
+                    kept_acc[64 * i] = sum;
+                    acc[i] = done ? sum : v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                }
+                if (done)
+                    break;
+                down *= 0x1p-38f;
             }
         }
         finish<D, VEC>(lds, kv, a, p, u, number, m, l, acc);
