@@ -3,11 +3,27 @@
 
 namespace {
 
-/* The two gates of a token's head. softplus as max(x, 0) + log1p(exp(-|x|)): no overflow. */
-__device__ __forceinline__ float decay_of(float a, float dt, float rate)
+/* The decay of a token's head. softplus as max(x, 0) + log1p(exp(-|x|)): no overflow. A decay near 1 rounded to F32 is off by
+ * up to 2^-25, which is far more of 1 - decay: under a gate that stays as it is that error has one sign, and the
+ * state, which remembers 1 / (1 - decay) tokens, would be off by it so many times. So it goes with what it is apart from
+ * 1, which keeps its own 24 bits (8192 tokens at 1 - decay = 3e-4: the state is off by 2e-6, without it by 1.7e-4). */
+struct decay {
+    float all, rest; /* rest: all - 1 where all is near 1, else all again */
+    __device__ __forceinline__ bool near() const { return rest != all; }
+};
+__device__ __forceinline__ decay decay_of(float a, float dt, float rate)
 {
-    const float x = a + dt;
-    return expf(rate * (fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x)))));
+    const float x = a + dt, e = rate * (fmaxf(x, 0.0f) + log1pf(expf(-fabsf(x))));
+    if (fabsf(e) < 0.6875f) {
+        /* e^x - 1 by its series: the next term is below 1e-8 of it */
+        float y = fmaf(e, 1.0f / 362880, 1.0f / 40320);
+        y = fmaf(e, fmaf(e, fmaf(e, y, 1.0f / 5040), 1.0f / 720), 1.0f / 120);
+        y = fmaf(e, fmaf(e, fmaf(e, y, 1.0f / 24), 1.0f / 6), 0.5f);
+        y = fmaf(e * e, y, e);
+        return decay{1.0f + y, y};
+    }
+    const float all = expf(e);
+    return decay{all, all};
 }
 
 __device__ __forceinline__ float dot4(float4 x, float4 y) { return fmaf(x.w, y.w, fmaf(x.z, y.z, fmaf(x.y, y.y, x.x * y.x))); }
@@ -93,7 +109,8 @@ __global__ __launch_bounds__(NORM ? 64 * STEP_WAVES : 64) void delta_step_k(rt_s
             const long i = i0 + lane < last ? i0 + lane : i0;
             ga = a.a[i * a.a_ld + h], gb = a.b[i * a.b_ld + h];
         }
-        const int alphas = __builtin_bit_cast(int, decay_of(ga, dt, rate)), betas = __builtin_bit_cast(int, q8_sigmoid(gb));
+        const decay gate = decay_of(ga, dt, rate);
+        const int alphas = __builtin_bit_cast(int, gate.all), rests = __builtin_bit_cast(int, gate.rest), betas = __builtin_bit_cast(int, q8_sigmoid(gb));
         const int count = (int)(last - i0 < 64 ? last - i0 : 64);
         for (int j = 0; j < count; j++) {
             const long i = i0 + j;
@@ -102,6 +119,7 @@ __global__ __launch_bounds__(NORM ? 64 * STEP_WAVES : 64) void delta_step_k(rt_s
                 q[r] = qn[r], k[r] = kn[r];
             v = vn, z = zn;
             load(i + 1 < last ? i + 1 : i);
+            float rest = __builtin_bit_cast(float, __builtin_amdgcn_readlane(rests, j));
             const float alpha = __builtin_bit_cast(float, __builtin_amdgcn_readlane(alphas, j)), beta = __builtin_bit_cast(float, __builtin_amdgcn_readlane(betas, j));
             float qq = 0.0f, kk = 0.0f, qk = 0.0f;
             float4 sq = {0.0f, 0.0f, 0.0f, 0.0f}, sk = sq;
@@ -133,10 +151,17 @@ __global__ __launch_bounds__(NORM ? 64 * STEP_WAVES : 64) void delta_step_k(rt_s
                 if (lane == 0)
                     squares[j & 1][wave] = sum;
             }
+            if (!decay{alpha, rest}.near()) {
+#pragma unroll
+                for (int r = 0; r < KR; r++)
+                    st[r] *= alpha;
+                rest = 0.0f;
+            }
 #pragma unroll
             for (int r = 0; r < KR; r++) {
                 const float kr = rk * k[r];
-                st[r] = float4{fmaf(kr, d.x, alpha * st[r].x), fmaf(kr, d.y, alpha * st[r].y), fmaf(kr, d.z, alpha * st[r].z), fmaf(kr, d.w, alpha * st[r].w)};
+                st[r] = float4{fmaf(kr, d.x, fmaf(rest, st[r].x, st[r].x)), fmaf(kr, d.y, fmaf(rest, st[r].y, st[r].y)), fmaf(kr, d.z, fmaf(rest, st[r].z, st[r].z)),
+                               fmaf(kr, d.w, fmaf(rest, st[r].w, st[r].w))};
             }
             float *to = a.o + i * a.o_ld + h * a.v_dim + col;
             if (NORM) {
@@ -181,7 +206,8 @@ __global__ __launch_bounds__(NORM ? 64 * STEP_WAVES : 64) void delta_step_k(rt_s
  * as they lie, 16 bytes a lane, and a first operand's lane takes row c, columns 4 g .. 4 g + 3 of 16 with one load. */
 constexpr int CHUNK = 64, TILES = CHUNK / 16, PAIRS = TILES * (TILES + 1) / 2;
 /* a chunk's part of a head: tiles (i, j), j <= i, of T and of P, 256 floats each in a first operand's order, and
- * gamma rk, scale gamma rq and D_C rk of its tokens, gamma_C, and whether anything of it is not finite (a wave each) */
+ * gamma rk, scale gamma rq and D_C rk of its tokens, gamma_C as 1 or 0 and
+ * the rest, and whether anything of it is not finite (a wave each) */
 constexpr int PREP = 2 * PAIRS * 256 + 4 * CHUNK;
 /* a chunk's part in floats: its value heads', then each key head's rows of K and of Q as first operands lie, 256 floats
  * a tile of 16 rows and 16 columns. There consecutive lanes load consecutive 16 bytes; from the rows themselves each lane's
@@ -225,6 +251,17 @@ __device__ __forceinline__ long sequence_of_slot(const rt_seqs &b, long i)
             break;
     }
     return c - 1;
+}
+
+/* A product of decays as an unevaluated sum of two floats. gamma_C, which a state is multiplied by chunk after chunk, is
+ * computed in these, and taken like a token's decay; the others reach a state once a token */
+struct pair {
+    float hi, lo;
+};
+__device__ __forceinline__ pair operator*(pair x, pair y)
+{
+    const float p = x.hi * y.hi;
+    return pair{p, fmaf(x.hi, y.hi, -p) + fmaf(x.hi, y.lo, x.lo * y.hi)};
 }
 
 /* A workgroup a chunk and key head; wave w has key rows 16 w .. of K K^T and query rows 16 (3 - w) .. of Q K^T, five
@@ -305,10 +342,31 @@ __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int m
         const long h = head(hn);
         float *mine = part + h * PREP, *factor = mine + 2 * PAIRS * 256;
         /* lane i of every wave: token i's gates */
-        const float alpha = lane < n ? decay_of(ga, dt, rate) : 1.0f;
+        const decay gate = lane < n ? decay_of(ga, dt, rate) : decay{1.0f, 0.0f};
+        const float alpha = gate.all;
         if (wave == 0)
             sbeta[lane] = lane < n ? q8_sigmoid(gb) : 0.0f;
         load_gates(hn + 1 < heads ? hn + 1 : hn);
+        if (wave == 0) {
+            /* gamma_C, with its rest: over each 16 lanes from the back, then the four first ones' */
+#define LANE(v, old, ctrl) __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(old, __builtin_bit_cast(int, v), ctrl, 0xf, 0xf, false))
+#define BEHIND(ctrl) all = all * pair{LANE(all.hi, 0x3f800000, ctrl), LANE(all.lo, 0, ctrl)}
+            pair all = gate.near() ? pair{alpha, gate.rest - (alpha - 1.0f)} : pair{alpha, 0.0f};
+            BEHIND(0x101);
+            BEHIND(0x102);
+            BEHIND(0x104);
+            BEHIND(0x108);
+#undef BEHIND
+#undef LANE
+            const auto of_lane = [&](int i) {
+                return pair{__builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, all.hi), i)),
+                            __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, all.lo), i))};
+            };
+            const pair whole = (of_lane(0) * of_lane(16)) * (of_lane(32) * of_lane(48));
+            const bool near = whole.hi > 0.5f && whole.hi < 2.0f;
+            if (lane == 0)
+                *(float2 *)(factor + 3 * CHUNK) = float2{near ? 1.0f : 0.0f, near ? (whole.hi - 1.0f) + whole.lo : whole.hi + whole.lo};
+        }
         {
             /* the decays between tokens, lane j with column j: up to the end of its own 16 rows by a scan from the
              * back, then by whole 16s, then down the wave's rows */
@@ -340,8 +398,6 @@ __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int m
             factor[CHUNK + lane] = gamma * srq[lane];
         else if (wave == 2)
             factor[2 * CHUNK + lane] = sd[CHUNK - 1][lane] * srk[lane];
-        else if (lane == CHUNK - 1)
-            factor[3 * CHUNK] = gamma;
         /* A, and P, which takes the decays' place */
         const float4 bk = *(const float4 *)&sbeta[16 * wave + 4 * g] * *(const float4 *)&srk[16 * wave + 4 * g], qf = *(const float4 *)&srq[16 * (3 - wave) + 4 * g];
         const float *bf = &bk.x, *qs = &qf.x;
@@ -496,14 +552,16 @@ __device__ __forceinline__ void odd_chunk(const rt_delta &a, const chunk_unit &u
             for (int w = 0; w < 8; w++)
                 sum[k] += m.red[k][w][c];
         }
-        const float alpha = decay_of(a.a[i * a.a_ld + u.h], a.dt[u.h], a.decay[u.h]), beta = q8_sigmoid(a.b[i * a.b_ld + u.h]);
+        const decay gate = decay_of(a.a[i * a.a_ld + u.h], a.dt[u.h], a.decay[u.h]);
+        const float alpha = gate.all, rest = gate.rest, keep = gate.near() ? 1.0f : 0.0f, beta = q8_sigmoid(a.b[i * a.b_ld + u.h]);
         const float rk = a.eps >= 0.0f ? 1.0f / sqrtf(sum[2] + a.eps) : 1.0f, rq = a.scale * (a.eps >= 0.0f ? 1.0f / sqrtf(sum[3] + a.eps) : 1.0f);
         const float d = beta * (a.v[i * a.v_ld + u.h * a.v_dim + u.col] - alpha * rk * sum[0]);
         if (tid < 16)
             a.o[i * a.o_ld + u.h * a.v_dim + u.col] = fmaf(rq * alpha, sum[1], rq * (rk * sum[4]) * d);
         for (int t = wave; t < DK / 16; t += 8) {
             const float4 kj = *(const float4 *)(kp + 16 * t), o = m.ss[t][lane];
-            m.ss[t][lane] = float4{fmaf(rk * kj.x, d, alpha * o.x), fmaf(rk * kj.y, d, alpha * o.y), fmaf(rk * kj.z, d, alpha * o.z), fmaf(rk * kj.w, d, alpha * o.w)};
+            m.ss[t][lane] = float4{fmaf(rk * kj.x, d, fmaf(rest, o.x, keep * o.x)), fmaf(rk * kj.y, d, fmaf(rest, o.y, keep * o.y)),
+                                   fmaf(rk * kj.z, d, fmaf(rest, o.z, keep * o.z)), fmaf(rk * kj.w, d, fmaf(rest, o.w, keep * o.w))};
         }
         __syncthreads();
     }
@@ -525,7 +583,8 @@ __device__ __forceinline__ long chunk_loop(const rt_delta &a, const chunk_unit &
     const float *factors = prep + u.slot * part + u.h * PREP + 2 * PAIRS * 256;
     const long count = u.last - u.first;
     float4 xv[NT], mv[TILES], scale, left;
-    float v[4], gamma, odd;
+    float v[4], odd;
+    float2 gamma;
     const auto load_rows = [&](long n) {
 #pragma unroll
         for (int t = 0; t < NT; t++)
@@ -584,7 +643,7 @@ __device__ __forceinline__ long chunk_loop(const rt_delta &a, const chunk_unit &
     load_rows(u.c0);
     if constexpr (KEYS)
         load_matrix(u.c0);
-    gamma = factors[u.c0 * part + 3 * CHUNK];
+    gamma = *(const float2 *)(factors + u.c0 * part + 3 * CHUNK);
     __syncthreads();
     bool whole = true; /* left at the loop's end only: a way out from its middle would let the compiler count fewer loads in flight */
     long n = u.c0;
@@ -640,7 +699,7 @@ __device__ __forceinline__ long chunk_loop(const rt_delta &a, const chunk_unit &
             const int t = t0 + wave;
             if (t < NT) {
                 const float4 o = m.ss[t][lane];
-                v4f s[2] = {v4f{gamma * o.x, gamma * o.y, gamma * o.z, gamma * o.w}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
+                v4f s[2] = {v4f{gamma.x * o.x, gamma.x * o.y, gamma.x * o.z, gamma.x * o.w}, v4f{gamma.y * o.x, gamma.y * o.y, gamma.y * o.z, gamma.y * o.w}};
 #pragma unroll
                 for (int j = 0; j < TILES; j++)
                     s[j & 1] = mfma4(*(const float4 *)&m.sk[16 * t + c][16 * j + 4 * g], m.sw[j][lane], s[j & 1]);
@@ -648,7 +707,7 @@ __device__ __forceinline__ long chunk_loop(const rt_delta &a, const chunk_unit &
                     m.ss[t][lane] = as4(s[0] + s[1]);
             }
         }
-        gamma = factors[next * part + 3 * CHUNK];
+        gamma = *(const float2 *)(factors + next * part + 3 * CHUNK);
         __syncthreads();
     }
     if (!whole)

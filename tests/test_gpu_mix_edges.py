@@ -1,11 +1,11 @@
 """The operators of include/q8_mix.h at the edges of their ranges, against their definitions in 64 bits: rows that see
-nothing in sequences that are cut, weights far below a row's largest."""
+nothing in sequences that are cut, weights far below a row's largest, decays near 1."""
 import numpy as np
 import pytest
 
 import mix_ref as ref
 from mix_ref import Paged, starts
-from test_gpu_mix import run_attn, say
+from test_gpu_mix import EPS, check_delta, delta_bound, delta_inputs, run_attn, run_delta, say
 
 pytestmark = pytest.mark.gpu
 
@@ -86,3 +86,23 @@ def test_attn_infinite_values_of_small_weights(rt, q8rt, kind, nats, hq, hk, dim
     fine = np.isfinite(want)
     assert (np.abs(got - want)[fine] <= tol[fine]).all()
     assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+
+
+# ---- decays near 1
+
+
+@pytest.mark.parametrize("count,longest", [(8192, None), (4000, 1), (100, None)])  # in chunks, token by token, a short prompt
+@pytest.mark.parametrize("a,b", [(-5.5, -5.0), (-6.9, -5.0), (-8.0, -7.0), (-10.0, -3.0), (0.5, -5.0)])
+def test_delta_constant_slow_gates(rt, q8rt, count, longest, a, b):
+    """The same gate at every token, its decay near 1: what the decay is off by is off the same way at every token, and adds up
+    over the 1 / (1 - decay) tokens that a state remembers, so it has to be far below a half step of F32."""
+    say("delta slow gate", count, longest, a, b)
+    rng = np.random.default_rng(count)
+    hv, dk, dv, start = 3, 128, 32, starts([count])
+    q, k, v, ga, gb, decay, dt, s_in = delta_inputs(rng, count, 1, hv, dk, dv, 1)
+    ga[:], gb[:], decay[:], dt[:] = a, b, np.float32([-1.0, -0.7, -1.9]), 0.0
+    x = (q, k, v, ga, gb, decay, dt, s_in)
+    got, state = run_delta(rt, q8rt, x, start, False, longest=longest)
+    want, wstate, size = ref.delta(*x[:7], EPS, dk ** -0.5, s_in, start, False)
+    say("state", [float(np.sqrt(((state[0, h] - wstate[0, h]) ** 2).mean() / (wstate[0, h] ** 2).mean())) for h in range(hv)], "bound", delta_bound(dk, count))
+    check_delta(got, state, want, wstate, size, start, dk, hv * dv)
