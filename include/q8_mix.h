@@ -15,9 +15,9 @@
  * not overlap one that it reads (from its first element to its last, whatever lies between its rows), but for
  * a state (s_out may be s_in) and a rotation in place.
  *
- * Workspaces (the delta rule's for runs of tokens, the attention's) grow to what a call needs, not while a
- * graph is recorded: run a call with the same n, t and longest (and cache and heads) once before. All of a
- * runtime's calls share them, in the order of its stream. */
+ * The workspace (the delta rule's for runs of tokens, the attention's) grows to what a call needs, or to twice what it
+ * was, not while a graph is recorded: run a call with the same n, t and longest (and cache and heads) once before. All
+ * of a runtime's calls share it, in the order of its stream; one that was replaced is freed by rt_fini. */
 #ifndef Q8_MIX_H
 #define Q8_MIX_H
 

@@ -316,15 +316,22 @@ float *reserve_rpart(ctx *c, size_t need)
     return c->rpart;
 }
 
-/* the workspace of the operators between the products, at least n floats */
+/* the workspace of the operators between the products, at least n floats. One that is too small stays until rt_fini (a
+ * recorded graph may use it), so the next is twice its size, where the GPU has that much: prompts that get longer call by call
+ * then leave less behind them than what they use (4096 tokens of 32 heads in steps of 64: 0.4 GB in all, 3.6 by exact sizes) */
 float *reserve_mix(ctx *c, size_t n)
 {
     if (n > c->mix_cap) {
         no_capture(c, "the workspace of the operators between the products");
         if (c->mix)
             c->retired.push_back(c->mix);
-        HIPCHECK(hipMalloc((void **)&c->mix, n * sizeof(float)));
-        c->mix_cap = n;
+        size_t size = n > 2 * c->mix_cap ? n : 2 * c->mix_cap;
+        if (hipMalloc((void **)&c->mix, size * sizeof(float)) != hipSuccess) {
+            (void)hipGetLastError();
+            size = n;
+            HIPCHECK(hipMalloc((void **)&c->mix, size * sizeof(float)));
+        }
+        c->mix_cap = size;
     }
     return c->mix;
 }

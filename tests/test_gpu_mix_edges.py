@@ -1,10 +1,13 @@
 """The operators of include/q8_mix.h at the edges of their ranges, against their definitions in 64 bits: rows that see
-nothing in sequences that are cut, weights far below a row's largest, decays near 1."""
+nothing in sequences that are cut, weights far below a row's largest, decays near 1; and what
+the workspace holds."""
+import ctypes as c
+
 import numpy as np
 import pytest
 
 import mix_ref as ref
-from mix_ref import Paged, starts
+from mix_ref import Call, Paged, starts
 from test_gpu_mix import EPS, check_delta, delta_bound, delta_inputs, run_attn, run_delta, say
 
 pytestmark = pytest.mark.gpu
@@ -106,3 +109,36 @@ def test_delta_constant_slow_gates(rt, q8rt, count, longest, a, b):
     want, wstate, size = ref.delta(*x[:7], EPS, dk ** -0.5, s_in, start, False)
     say("state", [float(np.sqrt(((state[0, h] - wstate[0, h]) ** 2).mean() / (wstate[0, h] ** 2).mean())) for h in range(hv)], "bound", delta_bound(dk, count))
     check_delta(got, state, want, wstate, size, start, dk, hv * dv)
+
+
+# ---- workspaces
+
+
+def test_growing_prompts_keep_little_memory(q8rt):
+    """Prompts that get longer call by call: what the runtime holds stays within a few times the largest call's need, whatever
+    it replaced on the way."""
+    r = q8rt.Runtime()
+    hk, hv, dk, dv, most = 16, 32, 128, 128, 4096
+    part = 4 * (hv * (2 * 10 * 256 + 256) + hk * 2 * 64 * dk)  # bytes a chunk of 64 tokens
+    try:
+        with Call(r, q8rt) as d:
+            x, ab = d.put(np.zeros((most, 2 * hk * dk + hv * dv), np.float32)), d.put(np.zeros((most, 2 * hv), np.float32))
+            state, o, head = d.put(np.zeros((hv, dk, dv), np.float32)), d.put(np.zeros((most, hv * dv), np.float32)), d.put(np.zeros(hv, np.float32))
+            ld = 2 * hk * dk + hv * dv
+            arg = q8rt.Delta(k_heads=hk, v_heads=hv, k_dim=dk, v_dim=dv, q=x, q_ld=ld, k=x + 4 * hk * dk, k_ld=ld, v=x + 8 * hk * dk, v_ld=ld, a=ab, a_ld=2 * hv,
+                             b=ab + 4 * hv, b_ld=2 * hv, decay=head, dt=head, eps=EPS, scale=1.0, s_in=state, s_out=state, o=o, o_ld=hv * dv)
+            free, total = c.c_size_t(), c.c_size_t()
+
+            def call(t):
+                s = d.seqs(starts([t]))
+                r.lib.rt_delta_rule_dev(r.R, c.byref(s), c.byref(arg))
+                r.lib.rt_dev_sync(r.R)
+                assert r.lib.hipMemGetInfo(c.byref(free), c.byref(total)) == 0
+                return free.value
+
+            first = call(64)
+            held = first - min(call(t) for t in range(128, most + 1, 64))
+            say("held", held / 2 ** 20, "MB, a call's need", part * (most // 64 + 1) / 2 ** 20)
+            assert held <= 4 * part * (most // 64 + 1)
+    finally:
+        r.close()
