@@ -60,7 +60,8 @@ void rt_conv_silu_dev(struct rt *R, const struct rt_seqs *s, const float *x, lon
  * Every sequence goes from s_in[s] to s_out[s], [n][v_heads][k_dim][v_dim] (one without tokens: a copy).
  * One token, or the few of a speculative check, run token by token; longer runs in chunks of tokens on
  * the matrix cores, in F32.
- * k_dim 32, 64, 96, 128, 192 or 256; v_dim a multiple of 16, 16 to 512; v_heads a multiple of k_heads. */
+ * k_dim 32, 64, 96, 128, 192 or 256; v_dim a multiple of 16, 16 to 512; v_heads a multiple of k_heads;
+ * n * v_heads * v_dim / 16 below 2^24. */
 struct rt_delta {
     long k_heads, v_heads, k_dim, v_dim;
     long tiled;

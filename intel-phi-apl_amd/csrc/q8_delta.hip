@@ -509,6 +509,8 @@ __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int m
  * would reach earlier ones. So do the chunks behind it: a way back into the loop would hold its registers meanwhile, and
  * there would be no second workgroup (16 heads of 1003, 963 and 692 tokens 72 us, 84 that way). */
 constexpr int CHUNK_THREADS = 512;
+/* a launch has fewer than 2^32 threads along x: this many workgroups (whole eighths, for the XCDs), the others along y */
+constexpr unsigned CHUNK_GRID = 1u << 22;
 
 template <int DK>
 struct chunk_lds {
@@ -725,7 +727,7 @@ __global__ __launch_bounds__(CHUNK_THREADS, WAVES) void delta_chunk_k(rt_seqs b,
 {
     __shared__ __align__(16) chunk_lds<DK> m;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), c = lane & 15, g = lane >> 4;
-    const int slices = (int)(a.v_dim / 16), x = (int)(blockIdx.x % 8), y = (int)(blockIdx.x / 8), slice = y % slices;
+    const int index = (int)(blockIdx.x + blockIdx.y * CHUNK_GRID), slices = (int)(a.v_dim / 16), x = index % 8, y = index / 8, slice = y % slices;
     const long unit = (long)(y / slices) * 8 + x, s = unit / a.v_heads;
     if (s >= b.n)
         return;
@@ -850,11 +852,12 @@ static bool launch_delta(hipStream_t s, const rt_seqs &b, const rt_delta &a, flo
     for (long from = 0; from < all; from += most) {
         const long count = all - from < most ? all - from : most;
         delta_prep_k<DK><<<dim3((unsigned)count, (unsigned)a.k_heads), 256, 0, s>>>(b, a, SHORT, from, prep);
-        const unsigned groups = (unsigned)(units * (a.v_dim / 16));
+        const long groups = units * (a.v_dim / 16);
+        const dim3 grid((unsigned)(groups < CHUNK_GRID ? groups : CHUNK_GRID), (unsigned)((groups + CHUNK_GRID - 1) / CHUNK_GRID));
         if (DK == 128 && groups > 256)
-            delta_chunk_k<DK, DK == 128 ? 4 : 2><<<groups, CHUNK_THREADS, 0, s>>>(b, a, SHORT, from, count, prep);
+            delta_chunk_k<DK, DK == 128 ? 4 : 2><<<grid, CHUNK_THREADS, 0, s>>>(b, a, SHORT, from, count, prep);
         else
-            delta_chunk_k<DK, 2><<<groups, CHUNK_THREADS, 0, s>>>(b, a, SHORT, from, count, prep);
+            delta_chunk_k<DK, 2><<<grid, CHUNK_THREADS, 0, s>>>(b, a, SHORT, from, count, prep);
     }
     return false;
 }

@@ -1,6 +1,6 @@
 """The operators of include/q8_mix.h at the edges of their ranges, against their definitions in 64 bits: rows that see
-nothing in sequences that are cut, weights far below a row's largest, decays near 1; and what
-the workspace holds."""
+nothing in sequences that are cut, weights far below a row's largest, decays near 1, the
+most sequences; and what the workspace holds."""
 import ctypes as c
 
 import numpy as np
@@ -142,3 +142,37 @@ def test_growing_prompts_keep_little_memory(q8rt):
             assert held <= 4 * part * (most // 64 + 1)
     finally:
         r.close()
+
+
+# ---- the most sequences and heads
+
+
+def test_delta_more_workgroups_than_a_launch_has_along_x(rt, q8rt):
+    """65535 sequences of 5 heads of 32 x 416, 17 GB of state in place: the first and last sequence's tokens in chunks, the
+    others, which have none, as they were."""
+    n, hk, hv, dk, dv, count = 65535, 1, 5, 32, 416, 70
+    rng = np.random.default_rng(1)
+    x = delta_inputs(rng, 2 * count, hk, hv, dk, dv, 4)
+    q, k, v, a, b, decay, dt, s_in = x
+    place = [0, n - 1, 1, n // 2]  # of s_in's four states
+    start = np.full(n + 1, count, np.int32)
+    start[0], start[n] = 0, 2 * count
+    size = hv * dk * dv * 4
+    with Call(rt, q8rt) as d:
+        state = rt.alloc(n * size)
+        d.bufs.append(state)
+        for i, s in zip(place, s_in):
+            rt.to_dev(state + i * size, s)
+        seqs = q8rt.Seqs(n=n, t=2 * count, longest=count, start=d.put(start))
+        arg = q8rt.Delta(k_heads=hk, v_heads=hv, k_dim=dk, v_dim=dv, q=d.put(q), q_ld=hk * dk, k=d.put(k), k_ld=hk * dk, v=d.put(v), v_ld=hv * dv, a=d.put(a), a_ld=hv,
+                         b=d.put(b), b_ld=hv, decay=d.put(decay), dt=d.put(dt), eps=EPS, scale=dk ** -0.5, s_in=state, s_out=state,
+                         o=d.out("o", (2 * count, hv * dv), np.float32), o_ld=hv * dv)
+        say("delta, sequences", n)
+        rt.lib.rt_delta_rule_dev(rt.R, c.byref(seqs), c.byref(arg))
+        got, after = d.get("o"), np.empty_like(s_in)
+        for i, s in zip(place, after):
+            rt.from_dev(s, state + i * size)
+    few = starts([count, count])
+    want, wstate, width = ref.delta(*x[:7], EPS, dk ** -0.5, s_in[:2], few, False)
+    check_delta(got, after[:2], want, wstate, width, few, dk, hv * dv)
+    assert np.array_equal(after[2:], s_in[2:])
