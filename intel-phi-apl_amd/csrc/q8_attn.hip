@@ -146,8 +146,9 @@ __device__ __forceinline__ void load_words(uint32_t *w, const char *p)
         *w = *(const uint32_t *)p;
 }
 
-/* The same for values, which are read once, in whole lines an instruction: not kept in the caches (32 sequences of 100 to
- * 16384 positions 220 us, 234 without). A key row's line is read by two instructions, and has to be. */
+/* The same for values, which a row tile reads once, in whole lines an instruction: not kept in the caches (32 sequences of
+ * 100 to 16384 positions 220 us, 234 without; a prompt's row tiles read them again each). A key row's line is read by two
+ * instructions, and has to be. */
 template <int WORDS>
 __device__ __forceinline__ void stream_words(uint32_t *w, const char *p)
 {
@@ -479,7 +480,7 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
  * the largest is at 2^14 to 2^15, the sums with them. Where that leaves one below LEAST, too (20 powers of two between two
  * positions of a tile, as beside such a first position itself), what the limbs leave of it is taken again 2^38 times as large,
  * and again, until it is below 2^-22 of the weight. The sums wait in LDS meanwhile. 8 sequences of 4000 to 20000 positions, 32
- * heads of 128: 81 us, 93 where a first position of 18 nats above the rest makes every tile scale; a prompt of 2048 335
+ * heads of 128: 81 us, 93 where a first position of 18 nats above the rest makes every tile scale; a prompt of 2048 351
  * and 459.
  * The queries' limbs stay in LDS for the four waves. The second product's first operand is V transposed: of a
  * lane's 8 rows, the same element of two at a time by v_perm_b32. */

@@ -206,8 +206,8 @@ __global__ __launch_bounds__(NORM ? 64 * STEP_WAVES : 64) void delta_step_k(rt_s
  * as they lie, 16 bytes a lane, and a first operand's lane takes row c, columns 4 g .. 4 g + 3 of 16 with one load. */
 constexpr int CHUNK = 64, TILES = CHUNK / 16, PAIRS = TILES * (TILES + 1) / 2;
 /* a chunk's part of a head: tiles (i, j), j <= i, of T and of P, 256 floats each in a first operand's order, and
- * gamma rk, scale gamma rq and D_C rk of its tokens, gamma_C as 1 or 0 and
- * the rest, and whether anything of it is not finite (a wave each) */
+ * gamma rk, scale gamma rq and D_C rk of its tokens, gamma_C as 1 or 0 and the rest, and whether anything of it is not
+ * finite (a wave each) */
 constexpr int PREP = 2 * PAIRS * 256 + 4 * CHUNK;
 /* a chunk's part in floats: its value heads', then each key head's rows of K and of Q as first operands lie, 256 floats
  * a tile of 16 rows and 16 columns. There consecutive lanes load consecutive 16 bytes; from the rows themselves each lane's
@@ -267,7 +267,7 @@ __device__ __forceinline__ pair operator*(pair x, pair y)
 /* A workgroup a chunk and key head; wave w has key rows 16 w .. of K K^T and query rows 16 (3 - w) .. of Q K^T, five
  * tiles of 16 x 16 each, which the key head's value heads share. The inverse of each value head is 16 x 16 on the
  * diagonal by substitution, a column a lane, then by diagonals T_ij = -T_ii sum_k A_ik T_kj. Bound by HBM (8192 tokens of 16
- * and 32 heads of 128: 418 MB in 108 us, 3.9 TB/s; its matrix instructions take 20 us). */
+ * and 32 heads of 128: 136 MB read and 222 written in 109 us, 3.3 TB/s; its matrix instructions take 20 us). */
 template <int DK>
 __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int most, long from, float *out)
 {
@@ -507,7 +507,8 @@ __global__ __launch_bounds__(256) void delta_prep_k(rt_seqs b, rt_delta a, int m
  *
  * A chunk with anything that is not finite goes token by token: in the products 0 times a later token's NaN
  * would reach earlier ones. So do the chunks behind it: a way back into the loop would hold its registers meanwhile, and
- * there would be no second workgroup (16 heads of 1003, 963 and 692 tokens 72 us, 84 that way). */
+ * there would be no second workgroup (16 heads of 1003, 963 and 692 tokens 72 us, 84 that way). A token there takes
+ * 2.5 us (8192 tokens of which the first holds a NaN 20 ms). */
 constexpr int CHUNK_THREADS = 512;
 /* a launch has fewer than 2^32 threads along x: this many workgroups (whole eighths, for the XCDs), the others along y */
 constexpr unsigned CHUNK_GRID = 1u << 22;
@@ -720,8 +721,8 @@ __device__ __forceinline__ long chunk_loop(const rt_delta &a, const chunk_unit &
 }
 
 /* WAVES: of a SIMD, 4 for two workgroups a compute unit, for which k_dim 128 has a few registers too many (smaller ones have
- * room as they are, larger ones none in LDS): 8 times 512 tokens of 32 heads, 8 workgroups a compute unit, 175 us, 195 with one
- * at a time; 8192 tokens, one workgroup, 373 and 342 */
+ * room as they are, larger ones none in LDS): 8 times 512 tokens of 32 heads, 8 workgroups a compute unit, 177 us, 200 with one
+ * at a time; 8192 tokens, one workgroup, 380 and 354 */
 template <int DK, int WAVES>
 __global__ __launch_bounds__(CHUNK_THREADS, WAVES) void delta_chunk_k(rt_seqs b, rt_delta a, int most, long from, long count, const float *prep)
 {
@@ -805,8 +806,8 @@ __global__ __launch_bounds__(256) void gated_norm_k(rt_seqs b, rt_delta a, int l
 
 } /* namespace */
 
-/* Sequences of more tokens than this go in chunks (heads of 128 x 128, 32 of them; us token by token and in chunks: one sequence
- * of 24 tokens 25 / 31, of 32 30 / 31, of 48 41 / 31; 4 of 32 36 / 46, of 48 50 / 47; 16 of 32 95 / 101, of 48 136 / 106) */
+/* Sequences of more tokens than this go in chunks (heads of 128 x 128, 32 of them, no norm; us token by token and in chunks: one
+ * sequence of 24 tokens 21 / 27, of 32 26 / 27, of 48 38 / 27; 4 of 32 32 / 41, of 48 45 / 42; 16 of 32 79 / 94, of 48 114 / 95) */
 constexpr int SHORT = 32;
 /* The chunks' parts of all heads that a launch makes and takes, in bytes: longer calls alternate */
 constexpr long PREP_MAX = 256L << 20;
