@@ -83,24 +83,33 @@ struct rt_delta {
 void rt_delta_rule_dev(struct rt *R, const struct rt_seqs *s, const struct rt_delta *a);
 
 /* A paged key-value cache: k and v [pages][heads][page][dim]. Position p of sequence s lies in page
- * table[s * table_ld + p / page], row p % page. */
+ * table[s * table_ld + p / page], row p % page.
+ *
+ * RT_Q8 holds a row (a position's head) as dim int8 values q and one F32 scale d, of which an element is q * d: k and v are the
+ * values [pages][heads][page][dim] with the scales [pages][heads][page] right behind them. Each row has a scale of its own, so that
+ * appending changes no row that is there: a cache is the same however its tokens came. */
 #define RT_F32 0
 #define RT_F16 1
 #define RT_BF16 2
+#define RT_Q8 8
 struct rt_kv {
     void *k, *v;
-    long type;        /* RT_F32, RT_F16 or RT_BF16 */
+    long type;        /* RT_F32, RT_F16, RT_BF16 or RT_Q8 */
     long dim;         /* a head's size: a multiple of 32, 32 to 256 */
     long heads;       /* key-value heads */
     long page, pages; /* positions a page (1 or more), pages in the cache: pages * heads * page < 2^31 */
     const int *table; /* device [n][table_ld]: entries that no position uses may be anything */
     long table_ld;    /* pages a sequence may have */
 };
+/* the bytes of such a cache's k, and of its v (the addresses are not looked at) */
+long rt_kv_bytes(const struct rt_kv *kv);
 
 /* Queries and keys to the cache and the attention: each head of q and k through its RMS norm (q_norm,
  * k_norm [dim]; NULL: none), then its first rot elements turned by the token's position p: pair i by
  * the angle p * freq[i], pair i being elements i and i + rot / 2, or 2 i and 2 i + 1 with pairs. q goes to
- * out in F32; k and v are rounded to the cache's type (to nearest, ties to even) into their position's row.
+ * out in F32; k and v are rounded to the cache's type (to nearest, ties to even) into their position's row. In 8 bits
+ * d = max|x| / 127 over the row and q = x / d rounded so; a row with an element that is not finite gets NaN for d, and so reads as
+ * NaN, and one whose d would be below 2^-126 gets zeros.
  * A position before 0, behind the table's last page, or in a page that the cache does not have is not
  * stored. freq is F64, and so is the angle: positions in the millions turn exactly.
  * out may be q (the same strides). */
@@ -119,6 +128,19 @@ struct rt_rope {
 };
 void rt_rope_kv_dev(struct rt *R, const struct rt_seqs *s, const struct rt_kv *kv, const struct rt_rope *a);
 
+/* Rows of the cache: K and V of the positions past[s], past[s] + 1, ... as rows start[s] .. of k and v (either may be NULL:
+ * not read), head h at k_hd * h, from any type of cache to F32, F16 or BF16 (8-bit values q * d rounded to F32, then to the rows'
+ * type). Strides in elements, multiples of 8 for 16-bit rows. A position before 0, behind the table's last page, or in a page that the
+ * cache does not have reads as NaN. */
+struct rt_kv_rows {
+    long type; /* RT_F32, RT_F16 or RT_BF16 */
+    void *k;
+    long k_ld, k_hd;
+    void *v;
+    long v_ld, v_hd;
+};
+void rt_kv_read_dev(struct rt *R, const struct rt_seqs *s, const struct rt_kv *kv, const struct rt_kv_rows *a);
+
 /* o = softmax(scale q K^T) V over the cache: the token at position p sees positions 0 .. p of its sequence
  * (its own and earlier new ones included: append them first), query head h the key-value head
  * h / (q_heads / heads). Times 1 / (1 + exp(-gate)), where given. For a few new tokens on a cache of any
@@ -135,6 +157,11 @@ struct rt_attn {
     long o_ld;
 };
 void rt_attn_kv_dev(struct rt *R, const struct rt_seqs *s, const struct rt_kv *kv, const struct rt_attn *a);
+
+/* The same through a sliding window: the token at position p sees the positions j <= p with j > p - window, and those with
+ * j < sinks, which stay visible. window 1 or more, sinks 0 or more; the time goes by what is seen. Pages of which no new token sees anything may be gone: the table's
+ * entries for them may be anything, and their positions' values too. */
+void rt_attn_window_dev(struct rt *R, const struct rt_seqs *s, const struct rt_kv *kv, const struct rt_attn *a, long window, long sinks);
 
 #ifdef __cplusplus
 }

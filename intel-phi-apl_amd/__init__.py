@@ -99,6 +99,9 @@ _SIGS = {
     "rt_delta_rule_dev": (None, [_vp, _vp, _vp]),
     "rt_rope_kv_dev": (None, [_vp, _vp, _vp, _vp]),
     "rt_attn_kv_dev": (None, [_vp, _vp, _vp, _vp]),
+    "rt_attn_window_dev": (None, [_vp, _vp, _vp, _vp, _long, _long]),
+    "rt_kv_read_dev": (None, [_vp, _vp, _vp, _vp]),
+    "rt_kv_bytes": (_long, [_vp]),
 }
 
 
@@ -117,8 +120,8 @@ class Delta(_c.Structure):
                 ("nw_eps", _c.c_float), ("o", _vp), ("o_ld", _long)]
 
 
-# the cache's types (RT_F32, RT_F16, RT_BF16)
-TYPES = {"f32": 0, "f16": 1, "bf16": 2}
+# the cache's types (RT_F32, RT_F16, RT_BF16, RT_Q8)
+TYPES = {"f32": 0, "f16": 1, "bf16": 2, "q8": 8}
 
 
 class Kv(_c.Structure):
@@ -126,6 +129,12 @@ class Kv(_c.Structure):
 
     _fields_ = [("k", _vp), ("v", _vp), ("type", _long), ("dim", _long), ("heads", _long), ("page", _long), ("pages", _long), ("table", _vp),
                 ("table_ld", _long)]
+
+
+class KvRows(_c.Structure):
+    """struct rt_kv_rows (include/q8_mix.h): rows read back from a cache."""
+
+    _fields_ = [("type", _long), ("k", _vp), ("k_ld", _long), ("k_hd", _long), ("v", _vp), ("v_ld", _long), ("v_hd", _long)]
 
 
 class Rope(_c.Structure):

@@ -1,0 +1,415 @@
+/* q8_attn.h: what the kernels of the attention over the paged cache share: the plan of a launch, a workgroup's share of it,
+ * the way from positions to rows, and the waves' joint result. */
+#ifndef Q8_ATTN_H
+#define Q8_ATTN_H
+
+#include "q8_mix.h"
+
+/* x / d for x < 2^31: (x * mul) >> shift with shift = 31 + ceil(log2 d), mul = ceil(2^shift / d): exact, as the
+ * excess mul * d - 2^shift is below d <= 2^(shift - 31) */
+struct q8_divisor {
+    uint32_t mul;
+    int shift;
+    __device__ __forceinline__ uint32_t of(uint32_t x) const { return (uint32_t)(((uint64_t)x * mul) >> shift); }
+};
+
+/* What a launch shares: row tiles are 16 query rows (token, head of the group) of one key-value head and
+ * sequence; the positions that one sees, in tiles of 16, are cut into chunks of one size for the whole batch. */
+struct q8_attn_plan {
+    q8_divisor page, group; /* by the positions of a page, by the query heads of a key-value head */
+    int heads;    /* query heads of a key-value head */
+    int cap;      /* positions that the table reaches */
+    int tile;     /* 16s of positions that a wave takes at once (a power of two): chunks are whole numbers of them */
+    int least;    /* 16s a chunk at least: one tile of each wave */
+    int target;   /* chunks (a key-value head) to spread all tiles over; 0: one a row tile */
+    int slots;    /* partial results a key-value head */
+    float share;  /* 1 / target, and a little: rounded sums must not make a chunk too small */
+    float qscale; /* scale * log2 e: scores are in powers of two */
+    int window;   /* positions that a token sees, itself and those before it; 0: all */
+    int sinks;    /* with a window, the first positions, which every later token sees, too */
+    float *part;  /* [heads][slots][16][dim], then [heads][slots][16][2]: maximum and sum */
+};
+
+/* the 8-bit cache's kernel on `blocks` x heads workgroups */
+void q8_launch_attn8(q8_stream_t stream, long blocks, const rt_seqs &b, const rt_kv &kv, const rt_attn &a, const q8_attn_plan &p);
+/* whether a compute unit holds one of its workgroups, not two */
+constexpr bool q8_attn8_alone(long dim) { return dim > 128; }
+
+namespace {
+
+typedef float v4f __attribute__((ext_vector_type(4)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+
+constexpr int WAVES = 4;
+
+typedef q8_attn_plan plan;
+
+struct seq_plan {
+    int first, n;     /* its rows of the token-major arrays */
+    int past, tiles;  /* position tiles of all that a row tile of it sees at most, within the table */
+    int rows, chunks; /* row tiles, and chunks of each */
+};
+
+/* With a window, the position tiles that a row tile sees at most: the sinks' tiles, and those from the first token's first
+ * position, rounded down to a wave's tile, to the last of up to 16 tokens. window and sinks are below 2^30 */
+__host__ __device__ __forceinline__ int window_tiles(const plan &p)
+{
+    return (p.sinks + 16 * p.tile - 1) / (16 * p.tile) * p.tile + (p.window + 15) / 16 + p.tile + 2;
+}
+
+__device__ __forceinline__ seq_plan plan_of(const rt_seqs &b, const plan &p, int group, int s)
+{
+    seq_plan q;
+    long first, last;
+    q8_rows_of(b, s, first, last);
+    q.first = (int)first;
+    q.n = (int)(last - first);
+    q.past = b.past[s];
+    const long len = (long)q.past + q.n;
+    q.tiles = len <= 0 ? 0 : (int)((len < p.cap ? len : p.cap) + 15) / 16;
+    if (p.window > 0) {
+        const int most = window_tiles(p);
+        q.tiles = q.tiles < most ? q.tiles : most;
+    }
+    q.rows = (int)(((uint32_t)q.n * (uint32_t)group + 15) / 16);
+    q.chunks = 1;
+    return q;
+}
+
+__device__ __forceinline__ int first_lane(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+/* tiles a chunk, from all sequences' (row tiles x position tiles): the target's share, the same for each sequence, so
+ * that workgroups read the same amounts whatever the lengths (a share of each one's own length left the short ones'
+ * waiting for the longest). Rounded up, by floats: any size will do that every workgroup finds alike and that leaves no
+ * more chunks than slots. 0: a row tile is one chunk. */
+__device__ __forceinline__ int chunk_from(const plan &p, float all)
+{
+    const float c = all * p.share + 1.0f;
+    const int n = c < 1e8f ? ((int)c + p.tile - 1) & ~(p.tile - 1) : 0;
+    return n == 0 || n > p.least ? n : p.least;
+}
+/* ceil(tiles / chunk), which is at most a few thousand */
+__device__ __forceinline__ int chunks_of(int tiles, int chunk)
+{
+    if (chunk == 0 || tiles <= chunk)
+        return 1;
+    int n = (int)((float)tiles * __builtin_amdgcn_rcpf((float)chunk));
+    n -= (long)n * chunk >= tiles ? 1 : 0;
+    n += (long)n * chunk < tiles ? 1 : 0;
+    n += (long)n * chunk < tiles ? 1 : 0;
+    return n;
+}
+
+/* the sums of a value over the lanes up to each: by 1, 2, 4 and 8 within each 16, then the 16s' last to the next */
+#define UPTO(v, ctrl, rows) (v) += __builtin_amdgcn_update_dpp(0, (v), ctrl, rows, 0xf, false)
+__device__ __forceinline__ int wave_upto(int v)
+{
+    UPTO(v, 0x111, 0xf);
+    UPTO(v, 0x112, 0xf);
+    UPTO(v, 0x114, 0xf);
+    UPTO(v, 0x118, 0xf);
+    UPTO(v, 0x142, 0xa); /* row_bcast:15 into rows 1 and 3 */
+    UPTO(v, 0x143, 0xc); /* row_bcast:31 into rows 2 and 3 */
+    return v;
+}
+#undef UPTO
+
+/* The sequence that holds chunk `number` of all row tiles' (or, with number < 0, row `token`), its plan, and the
+ * chunks of the sequences before it; false: there is none. A lane a sequence, 64 at a time. */
+__device__ __forceinline__ bool locate(const rt_seqs &b, const plan &p, int group, int number, long token, int &s, seq_plan &q, int &before, int &chunk)
+{
+    before = 0;
+    if (b.n == 1) {
+        s = 0;
+        q = plan_of(b, p, group, 0);
+        chunk = p.target > 0 ? chunk_from(p, (float)q.rows * (float)q.tiles) : 0;
+        q.chunks = chunks_of(q.tiles, chunk);
+        return number >= 0 ? number < q.rows * q.chunks : token >= q.first && token < q.first + q.n;
+    }
+    const int lane = threadIdx.x & 63, n = (int)b.n;
+    const seq_plan none = {0, 0, 0, 0, 0, 1};
+    seq_plan at = lane < n ? plan_of(b, p, group, lane) : none;
+    chunk = 0;
+    if (p.target > 0) {
+        float all = (float)at.rows * (float)at.tiles;
+        for (int s0 = 64; s0 < n; s0 += 64)
+            if (s0 + lane < n) {
+                const seq_plan o = plan_of(b, p, group, s0 + lane);
+                all += (float)o.rows * (float)o.tiles;
+            }
+        chunk = first_lane(chunk_from(p, q8_wave_sum_dpp(all)));
+    }
+    for (int s0 = 0; s0 < n; s0 += 64) {
+        if (s0 > 0)
+            at = s0 + lane < n ? plan_of(b, p, group, s0 + lane) : none;
+        at.chunks = chunks_of(at.tiles, chunk);
+        const int mine = at.rows * at.chunks, upto = wave_upto(mine);
+        const unsigned long long m = __ballot(number >= 0 ? number < before + upto : token >= at.first && token < at.first + at.n);
+        if (m) {
+            const int l = __ffsll((long long)m) - 1;
+            const auto from = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            s = s0 + l;
+            before += from(upto - mine);
+            q = seq_plan{from(at.first), from(at.n), from(at.past), from(at.tiles), from(at.rows), from(at.chunks)};
+            return true;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+}
+
+template <int WORDS>
+__device__ __forceinline__ void load_words(uint32_t *w, const char *p)
+{
+    if constexpr (WORDS == 4)
+        *(uint4 *)w = *(const uint4 *)p;
+    else if constexpr (WORDS == 2)
+        *(uint2 *)w = *(const uint2 *)p;
+    else
+        *w = *(const uint32_t *)p;
+}
+
+/* The same for values, which a row tile reads once, in whole lines an instruction: not kept in the caches (32 sequences of
+ * 100 to 16384 positions 220 us, 234 without; a prompt's row tiles read them again each). A key row's line is read by two
+ * instructions, and has to be. */
+template <int WORDS>
+__device__ __forceinline__ void stream_words(uint32_t *w, const char *p)
+{
+    typedef uint32_t words __attribute__((ext_vector_type(WORDS)));
+    const words x = __builtin_nontemporal_load((const words *)p);
+#pragma unroll
+    for (int i = 0; i < WORDS; i++)
+        w[i] = x[i];
+}
+
+/* the largest of a value's copies in lanes l, l ^ 16, l ^ 32, l ^ 48, and their sum */
+__device__ __forceinline__ float group_max(float v)
+{
+    v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return fmaxf(v, __shfl_xor(v, 32, 64));
+}
+__device__ __forceinline__ float group_sum(float v)
+{
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+
+/* o's final form: the gate, and what a row that sees nothing gives */
+__device__ __forceinline__ float4 gate_of(const rt_attn &a, long token, long head, long at)
+{
+    return a.gate ? *(const float4 *)(a.gate + token * a.gate_ld + head * a.gate_hd + at) : float4{0.0f, 0.0f, 0.0f, 0.0f};
+}
+__device__ __forceinline__ void store_row(const rt_attn &a, long dim, long token, long head, long at, float4 v, float l, bool empty, float4 g)
+{
+    v = empty ? float4{0.0f, 0.0f, 0.0f, 0.0f} : float4{v.x / l, v.y / l, v.z / l, v.w / l};
+    if (a.gate) {
+        v = float4{v.x * q8_sigmoid(g.x), v.y * q8_sigmoid(g.y), v.z * q8_sigmoid(g.z), v.w * q8_sigmoid(g.w)};
+    }
+    *(float4 *)(a.o + token * a.o_ld + head * dim + at) = v;
+}
+
+/* A workgroup takes a chunk of positions for a row tile (16 query rows); its waves take the chunk's position tiles
+ * in turn, and join at the end through LDS.
+ *
+ * A wave computes S^T = K Q^T, K's rows being the positions, so that lane 16 g + c has the scores of query
+ * row c at positions 4 g .. 4 g + 3 of 16. The next product, O^T += V^T P^T, takes them as its second operand as
+ * they lie, if its first has V's rows in the same order. So the cache's rows go from memory to the matrix cores in
+ * the registers that they were loaded into: lane 16 g + c loads K's row c, 16 bytes of each 64 from byte 16 g on,
+ * and V's rows 4 g .. 4 g + 3, VEC elements of each 16 * VEC from c * VEC on. The output's element (i * 16 + 4 g + r)
+ * * VEC + e of query row c is acc[i * VEC + e][r].
+ *
+ * The softmax's maximum is a running one that is raised only when a score passes it by more than SLACK (a
+ * power of two: the exponentials stay below 2^SLACK; an F16 cache has less, for its weights' range): then the sums and outputs are scaled, which a tile
+ * rarely needs after the first. Each lane sums its own positions; the four lanes of a row add up at the end. */
+constexpr float SLACK = 8.0f;
+
+/* A workgroup's share: chunk `part` of sequence s's row tile z, and what its lane has of it */
+struct share {
+    seq_plan q;
+    const int32_t *table;
+    int z, j0, j1;   /* the row tile, and its tokens */
+    int j, h;        /* the lane's query row: token and head */
+    bool live;       /* there is one */
+    int lim;         /* the last position that the lane's row sees, -1 none */
+    int last, least; /* the last that any row of the tile sees, and the last that all do */
+    int t0, t1;      /* the chunk's position tiles, 16 each */
+    /* with a window the tiles are counted without those that the row tile does not see: from tile `sunk` on, a tile is `skip`
+     * further on */
+    int sunk, skip;
+    int low;         /* the first position, but for the sinks, that the lane's row sees; lo0 and lo1: the first and last row's */
+    int lo0, lo1;
+};
+
+/* The first position of token j's window, or behind the table */
+__device__ __forceinline__ int window_from(const plan &p, const seq_plan &q, int j)
+{
+    const long pos = (long)q.past + j - (p.window - 1);
+    return pos < 0 ? 0 : pos < p.cap ? (int)pos : p.cap;
+}
+/* Whether a row whose window begins at low has position i before it, and not as a sink */
+template <bool WINDOW>
+__device__ __forceinline__ bool passed(const plan &p, int i, int low)
+{
+    return WINDOW && i < low && i >= p.sinks;
+}
+/* Whether all rows of u see the positions [i, i + n), so that no mask is needed */
+template <bool WINDOW>
+__device__ __forceinline__ bool all_seen(const plan &p, const share &u, int i, int n)
+{
+    return i + n - 1 <= u.least && (!WINDOW || i >= u.lo1 || i + n <= p.sinks);
+}
+/* The place of the row tile's tile t, in tiles of 16 * sub positions */
+template <bool WINDOW>
+__device__ __forceinline__ int place_of(const share &u, int t, int sub)
+{
+    return WINDOW && t * sub >= u.sunk ? t + u.skip / sub : t;
+}
+
+template <bool WINDOW>
+__device__ __forceinline__ bool share_of(const rt_seqs &b, const rt_kv &kv, const plan &p, int group, int number, share &u)
+{
+    int before, s, chunk;
+    if (!locate(b, p, group, number, 0, s, u.q, before, chunk))
+        return false;
+    const seq_plan &q = u.q;
+    number -= before;
+    int z = number;
+    if (q.chunks > 1) {
+        z = (int)((float)number * __builtin_amdgcn_rcpf((float)q.chunks)); /* below 2^14: one off at most */
+        z -= z * q.chunks > number ? 1 : 0;
+        z += (z + 1) * q.chunks <= number ? 1 : 0;
+    }
+    z = first_lane(z);
+    const int part = number - z * q.chunks;
+    u.z = q.rows - 1 - z; /* those that see most first (8192 tokens of 16 heads of 256 3114 us, 3403 last) */
+    const int row = u.z * 16 + (int)(threadIdx.x & 15);
+    u.table = kv.table + s * kv.table_ld;
+    u.j = (int)p.group.of(row);
+    u.h = (int)blockIdx.y * group + (row - u.j * group);
+    u.live = u.j < q.n;
+    const auto sees = [&](int j) { /* the last position that token j sees, within the table */
+        const long pos = (long)q.past + j;
+        return pos < 0 ? -1 : pos < p.cap ? (int)pos : p.cap - 1;
+    };
+    u.lim = u.live ? sees(u.j) : -1;
+    u.j0 = first_lane((int)p.group.of(u.z * 16));
+    u.j1 = first_lane((int)p.group.of(u.z * 16 + 15));
+    u.j1 = u.j1 < q.n ? u.j1 : q.n - 1;
+    u.last = sees(u.j1);
+    u.least = sees(u.j0);
+    u.t0 = part * chunk;
+    u.t1 = u.last < 0 ? 0 : u.last / 16 + 1;
+    if constexpr (WINDOW) {
+        u.low = u.live ? window_from(p, q, u.j) : 0;
+        u.lo0 = window_from(p, q, u.j0);
+        u.lo1 = window_from(p, q, u.j1);
+        const int first = u.lo0 / (16 * p.tile) * p.tile, some = (p.sinks + 16 * p.tile - 1) / (16 * p.tile) * p.tile;
+        u.sunk = some < first ? some : first;
+        u.skip = first - u.sunk;
+        u.t1 = u.t1 > first ? u.t1 - u.skip : u.t1 < u.sunk ? u.t1 : u.sunk;
+    }
+    if (q.chunks > 1 && u.t0 + chunk < u.t1)
+        u.t1 = u.t0 + chunk;
+    return true;
+}
+
+/* A position's page from the table, and its row in the cache's k and v counted from the head's first page
+ * (-1: it has none) */
+__device__ __forceinline__ int entry_of(const rt_kv &kv, const plan &p, const int32_t *table, int pos)
+{
+    const uint32_t pg = p.page.of(pos);
+    return (long)pg < kv.table_ld ? table[pg] : -1;
+}
+__device__ __forceinline__ int row_of(const rt_kv &kv, const plan &p, int pos, int entry)
+{
+    const uint32_t pg = p.page.of(pos);
+    return entry >= 0 && entry < kv.pages ? entry * (int)(kv.heads * kv.page) + (pos - (int)(pg * (uint32_t)kv.page)) : -1;
+}
+__device__ __forceinline__ const char *address(const void *cache, int row, uint32_t head_rows, int bytes)
+{
+    return (const char *)cache + (uint64_t)((uint32_t)(row < 0 ? 0 : row) + head_rows) * (uint32_t)bytes;
+}
+
+/* The running maximum raised where a lane's largest score passes it by slack, and the reference that
+ * the exponents are taken from */
+template <int VE>
+__device__ __forceinline__ float reference(float top, float slack, float &m, float &l, v4f (&acc)[VE])
+{
+    if (__ballot(top > m + slack)) {
+        const float raised = fmaxf(m, group_max(top)), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - raised);
+        m = raised;
+        l *= f;
+#pragma unroll
+        for (int i = 0; i < VE; i++)
+            acc[i] *= f;
+    }
+    return m == -INFINITY ? 0.0f : m;
+}
+
+/* The waves' results, scaled to the largest of their maxima and added in the waves' order: the output, or
+ * the chunk's part of it */
+template <int D>
+constexpr int joint_bytes() { return WAVES * 16 * (D + 4 + 2) * 4; }
+
+template <int D, int VEC, int VE = D / 16>
+__device__ __forceinline__ void finish(char *lds, const rt_kv &kv, const rt_attn &a, const plan &p, const share &u, int number, float m, float l, const v4f (&acc)[VE])
+{
+    constexpr int LD = D + 4; /* rows off each other's banks */
+    float(*so)[16][LD] = (float(*)[16][LD])lds;
+    float(*sm)[16] = (float(*)[16])(lds + WAVES * 16 * LD * 4), (*sl)[16] = sm + WAVES;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
+    const int kh = (int)blockIdx.y;
+    l = group_sum(l);
+    __syncthreads();
+    if (g == 0)
+        sm[wave][c] = m, sl[wave][c] = l;
+    __syncthreads();
+    float top = sm[0][c];
+#pragma unroll
+    for (int w = 1; w < WAVES; w++)
+        top = fmaxf(top, sm[w][c]);
+    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
+    const int group = p.heads, left = u.q.n * group - u.z * 16, rows = left < 16 ? left : 16;
+    if (c < rows)
+#pragma unroll
+        for (int i = 0; i < VE / VEC; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int e = 0; e < VEC; e += 2)
+                    if (VE * 16 == D || (i * 16 + 4 * g + r) * VEC < D)
+                        *(float2 *)&so[wave][c][(i * 16 + 4 * g + r) * VEC + e] = float2{acc[i * VEC + e][r] * f, acc[i * VEC + e + 1][r] * f};
+    __syncthreads();
+    for (int i = tid; i < rows * (D / 4); i += 64 * WAVES) {
+        const int r = i / (D / 4), d = 4 * (i % (D / 4));
+        float t = sm[0][r], sum = 0.0f;
+        for (int w = 1; w < WAVES; w++)
+            t = fmaxf(t, sm[w][r]);
+        float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int w = 0; w < WAVES; w++) {
+            const float4 x = *(const float4 *)&so[w][r][d];
+            v = float4{v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w};
+            sum += sl[w][r] * (sm[w][r] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(sm[w][r] - t));
+        }
+        const int jr = (int)p.group.of(u.z * 16 + r), hr = kh * group + (u.z * 16 + r - jr * group);
+        const long pos = (long)u.q.past + jr;
+        if (pos >= p.cap)
+            sum = NAN; /* a position that the table does not reach */
+        if (u.q.chunks == 1) {
+            store_row(a, D, u.q.first + jr, hr, d, v, sum, pos < 0, gate_of(a, u.q.first + jr, hr, d));
+        } else {
+            const long slot = (long)kh * p.slots + number;
+            *(float4 *)(p.part + (slot * 16 + r) * D + d) = v;
+            if (d == 0)
+                *(float2 *)(p.part + kv.heads * p.slots * 16 * D + (slot * 16 + r) * 2) = float2{t, sum};
+        }
+    }
+    __syncthreads();
+}
+
+/* The most elements (at most full) that a lane's VE elements of a V row divide into */
+constexpr int pieces(int ve, int full) { return ve % full == 0 ? full : ve % (full / 2) == 0 ? full / 2 : 2; }
+
+} /* namespace */
+
+#endif

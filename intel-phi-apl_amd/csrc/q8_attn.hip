@@ -1,353 +1,13 @@
-/* q8_attn.hip: attention of new tokens over the paged key-value cache (include/q8_mix.h). */
-#include "q8_mix.h"
+/* q8_attn.hip: attention of new tokens over the paged key-value cache of 32 or 16 bits, and the join of every type's parts
+ * (include/q8_mix.h). */
+#include "q8_attn.h"
 
 namespace {
 
-typedef float v4f __attribute__((ext_vector_type(4)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef __bf16 b8 __attribute__((ext_vector_type(8)));
-
-constexpr int WAVES = 4;
-
-/* x / d for x < 2^31: (x * mul) >> shift with shift = 31 + ceil(log2 d), mul = ceil(2^shift / d): exact, as the
- * excess mul * d - 2^shift is below d <= 2^(shift - 31) */
-struct divisor {
-    uint32_t mul;
-    int shift;
-    __device__ __forceinline__ uint32_t of(uint32_t x) const { return (uint32_t)(((uint64_t)x * mul) >> shift); }
-};
-
-/* What a launch shares: row tiles are 16 query rows (token, head of the group) of one key-value head and
- * sequence; a sequence's positions, in tiles of 16, are cut into chunks of one size for the whole batch. */
-struct plan {
-    divisor page, group; /* by the positions of a page, by the query heads of a key-value head */
-    int heads;    /* query heads of a key-value head */
-    int cap;      /* positions that the table reaches */
-    int tile;     /* 16s of positions that a wave takes at once (a power of two): chunks are whole numbers of them */
-    int least;    /* 16s a chunk at least: one tile of each wave */
-    int target;   /* chunks (a key-value head) to spread all tiles over; 0: one a row tile */
-    int slots;    /* partial results a key-value head */
-    float share;  /* 1 / target, and a little: rounded sums must not make a chunk too small */
-    float qscale; /* scale * log2 e: scores are in powers of two */
-    float *part;  /* [heads][slots][16][dim], then [heads][slots][16][2]: maximum and sum */
-};
-
-struct seq_plan {
-    int first, n;     /* its rows of the token-major arrays */
-    int past, tiles;  /* position tiles of all it sees, within the table */
-    int rows, chunks; /* row tiles, and chunks of each */
-};
-
-__device__ __forceinline__ seq_plan plan_of(const rt_seqs &b, const plan &p, int group, int s)
-{
-    seq_plan q;
-    long first, last;
-    q8_rows_of(b, s, first, last);
-    q.first = (int)first;
-    q.n = (int)(last - first);
-    q.past = b.past[s];
-    const long len = (long)q.past + q.n;
-    q.tiles = len <= 0 ? 0 : (int)((len < p.cap ? len : p.cap) + 15) / 16;
-    q.rows = (int)(((uint32_t)q.n * (uint32_t)group + 15) / 16);
-    q.chunks = 1;
-    return q;
-}
-
-__device__ __forceinline__ int first_lane(int v) { return __builtin_amdgcn_readfirstlane(v); }
-
-/* tiles a chunk, from all sequences' (row tiles x position tiles): the target's share, the same for each sequence, so
- * that workgroups read the same amounts whatever the lengths (a share of each one's own length left the short ones'
- * waiting for the longest). Rounded up, by floats: any size will do that every workgroup finds alike and that leaves no
- * more chunks than slots. 0: a row tile is one chunk. */
-__device__ __forceinline__ int chunk_from(const plan &p, float all)
-{
-    const float c = all * p.share + 1.0f;
-    const int n = c < 1e8f ? ((int)c + p.tile - 1) & ~(p.tile - 1) : 0;
-    return n == 0 || n > p.least ? n : p.least;
-}
-/* ceil(tiles / chunk), which is at most a few thousand */
-__device__ __forceinline__ int chunks_of(int tiles, int chunk)
-{
-    if (chunk == 0 || tiles <= chunk)
-        return 1;
-    int n = (int)((float)tiles * __builtin_amdgcn_rcpf((float)chunk));
-    n -= (long)n * chunk >= tiles ? 1 : 0;
-    n += (long)n * chunk < tiles ? 1 : 0;
-    n += (long)n * chunk < tiles ? 1 : 0;
-    return n;
-}
-
-/* the sums of a value over the lanes up to each: by 1, 2, 4 and 8 within each 16, then the 16s' last to the next */
-#define UPTO(v, ctrl, rows) (v) += __builtin_amdgcn_update_dpp(0, (v), ctrl, rows, 0xf, false)
-__device__ __forceinline__ int wave_upto(int v)
-{
-    UPTO(v, 0x111, 0xf);
-    UPTO(v, 0x112, 0xf);
-    UPTO(v, 0x114, 0xf);
-    UPTO(v, 0x118, 0xf);
-    UPTO(v, 0x142, 0xa); /* row_bcast:15 into rows 1 and 3 */
-    UPTO(v, 0x143, 0xc); /* row_bcast:31 into rows 2 and 3 */
-    return v;
-}
-#undef UPTO
-
-/* The sequence that holds chunk `number` of all row tiles' (or, with number < 0, row `token`), its plan, and the
- * chunks of the sequences before it; false: there is none. A lane a sequence, 64 at a time. */
-__device__ __forceinline__ bool locate(const rt_seqs &b, const plan &p, int group, int number, long token, int &s, seq_plan &q, int &before, int &chunk)
-{
-    before = 0;
-    if (b.n == 1) {
-        s = 0;
-        q = plan_of(b, p, group, 0);
-        chunk = p.target > 0 ? chunk_from(p, (float)q.rows * (float)q.tiles) : 0;
-        q.chunks = chunks_of(q.tiles, chunk);
-        return number >= 0 ? number < q.rows * q.chunks : token >= q.first && token < q.first + q.n;
-    }
-    const int lane = threadIdx.x & 63, n = (int)b.n;
-    const seq_plan none = {0, 0, 0, 0, 0, 1};
-    seq_plan at = lane < n ? plan_of(b, p, group, lane) : none;
-    chunk = 0;
-    if (p.target > 0) {
-        float all = (float)at.rows * (float)at.tiles;
-        for (int s0 = 64; s0 < n; s0 += 64)
-            if (s0 + lane < n) {
-                const seq_plan o = plan_of(b, p, group, s0 + lane);
-                all += (float)o.rows * (float)o.tiles;
-            }
-        chunk = first_lane(chunk_from(p, q8_wave_sum_dpp(all)));
-    }
-    for (int s0 = 0; s0 < n; s0 += 64) {
-        if (s0 > 0)
-            at = s0 + lane < n ? plan_of(b, p, group, s0 + lane) : none;
-        at.chunks = chunks_of(at.tiles, chunk);
-        const int mine = at.rows * at.chunks, upto = wave_upto(mine);
-        const unsigned long long m = __ballot(number >= 0 ? number < before + upto : token >= at.first && token < at.first + at.n);
-        if (m) {
-            const int l = __ffsll((long long)m) - 1;
-            const auto from = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-            s = s0 + l;
-            before += from(upto - mine);
-            q = seq_plan{from(at.first), from(at.n), from(at.past), from(at.tiles), from(at.rows), from(at.chunks)};
-            return true;
-        }
-        before += __builtin_amdgcn_readlane(upto, 63);
-    }
-    return false;
-}
-
-template <int WORDS>
-__device__ __forceinline__ void load_words(uint32_t *w, const char *p)
-{
-    if constexpr (WORDS == 4)
-        *(uint4 *)w = *(const uint4 *)p;
-    else if constexpr (WORDS == 2)
-        *(uint2 *)w = *(const uint2 *)p;
-    else
-        *w = *(const uint32_t *)p;
-}
-
-/* The same for values, which a row tile reads once, in whole lines an instruction: not kept in the caches (32 sequences of
- * 100 to 16384 positions 220 us, 234 without; a prompt's row tiles read them again each). A key row's line is read by two
- * instructions, and has to be. */
-template <int WORDS>
-__device__ __forceinline__ void stream_words(uint32_t *w, const char *p)
-{
-    typedef uint32_t words __attribute__((ext_vector_type(WORDS)));
-    const words x = __builtin_nontemporal_load((const words *)p);
-#pragma unroll
-    for (int i = 0; i < WORDS; i++)
-        w[i] = x[i];
-}
-
-/* the largest of a value's copies in lanes l, l ^ 16, l ^ 32, l ^ 48, and their sum */
-__device__ __forceinline__ float group_max(float v)
-{
-    v = fmaxf(v, __shfl_xor(v, 16, 64));
-    return fmaxf(v, __shfl_xor(v, 32, 64));
-}
-__device__ __forceinline__ float group_sum(float v)
-{
-    v += __shfl_xor(v, 16, 64);
-    return v + __shfl_xor(v, 32, 64);
-}
-
-/* o's final form: the gate, and what a row that sees nothing gives */
-__device__ __forceinline__ float4 gate_of(const rt_attn &a, long token, long head, long at)
-{
-    return a.gate ? *(const float4 *)(a.gate + token * a.gate_ld + head * a.gate_hd + at) : float4{0.0f, 0.0f, 0.0f, 0.0f};
-}
-__device__ __forceinline__ void store_row(const rt_attn &a, long dim, long token, long head, long at, float4 v, float l, bool empty, float4 g)
-{
-    v = empty ? float4{0.0f, 0.0f, 0.0f, 0.0f} : float4{v.x / l, v.y / l, v.z / l, v.w / l};
-    if (a.gate) {
-        v = float4{v.x * q8_sigmoid(g.x), v.y * q8_sigmoid(g.y), v.z * q8_sigmoid(g.z), v.w * q8_sigmoid(g.w)};
-    }
-    *(float4 *)(a.o + token * a.o_ld + head * dim + at) = v;
-}
-
-/* A workgroup takes a chunk of positions for a row tile (16 query rows); its waves take the chunk's position tiles
- * in turn, and join at the end through LDS.
- *
- * A wave computes S^T = K Q^T, K's rows being the positions, so that lane 16 g + c has the scores of query
- * row c at positions 4 g .. 4 g + 3 of 16. The next product, O^T += V^T P^T, takes them as its second operand as
- * they lie, if its first has V's rows in the same order. So the cache's rows go from memory to the matrix cores in
- * the registers that they were loaded into: lane 16 g + c loads K's row c, 16 bytes of each 64 from byte 16 g on,
- * and V's rows 4 g .. 4 g + 3, VEC elements of each 16 * VEC from c * VEC on. The output's element (i * 16 + 4 g + r)
- * * VEC + e of query row c is acc[i * VEC + e][r].
- *
- * The softmax's maximum is a running one that is raised only when a score passes it by more than SLACK (a
- * power of two: the exponentials stay below 2^SLACK; an F16 cache has less, for its weights' range): then the sums and outputs are scaled, which a tile
- * rarely needs after the first. Each lane sums its own positions; the four lanes of a row add up at the end. */
-constexpr float SLACK = 8.0f;
-
-/* A workgroup's share: chunk `part` of sequence s's row tile z, and what its lane has of it */
-struct share {
-    seq_plan q;
-    const int32_t *table;
-    int z, j0, j1;   /* the row tile, and its tokens */
-    int j, h;        /* the lane's query row: token and head */
-    bool live;       /* there is one */
-    int lim;         /* the last position that the lane's row sees, -1 none */
-    int last, least; /* the last that any row of the tile sees, and the last that all do */
-    int t0, t1;      /* the chunk's position tiles, 16 each */
-};
-
-__device__ __forceinline__ bool share_of(const rt_seqs &b, const rt_kv &kv, const plan &p, int group, int number, share &u)
-{
-    int before, s, chunk;
-    if (!locate(b, p, group, number, 0, s, u.q, before, chunk))
-        return false;
-    const seq_plan &q = u.q;
-    number -= before;
-    int z = number;
-    if (q.chunks > 1) {
-        z = (int)((float)number * __builtin_amdgcn_rcpf((float)q.chunks)); /* below 2^14: one off at most */
-        z -= z * q.chunks > number ? 1 : 0;
-        z += (z + 1) * q.chunks <= number ? 1 : 0;
-    }
-    z = first_lane(z);
-    const int part = number - z * q.chunks;
-    u.z = q.rows - 1 - z; /* those that see most first (8192 tokens of 16 heads of 256 3114 us, 3403 last) */
-    const int row = u.z * 16 + (int)(threadIdx.x & 15);
-    u.table = kv.table + s * kv.table_ld;
-    u.j = (int)p.group.of(row);
-    u.h = (int)blockIdx.y * group + (row - u.j * group);
-    u.live = u.j < q.n;
-    const auto sees = [&](int j) { /* the last position that token j sees, within the table */
-        const long pos = (long)q.past + j;
-        return pos < 0 ? -1 : pos < p.cap ? (int)pos : p.cap - 1;
-    };
-    u.lim = u.live ? sees(u.j) : -1;
-    u.j0 = first_lane((int)p.group.of(u.z * 16));
-    u.j1 = first_lane((int)p.group.of(u.z * 16 + 15));
-    u.j1 = u.j1 < q.n ? u.j1 : q.n - 1;
-    u.last = sees(u.j1);
-    u.least = sees(u.j0);
-    u.t0 = part * chunk;
-    u.t1 = u.last < 0 ? 0 : u.last / 16 + 1;
-    if (q.chunks > 1 && u.t0 + chunk < u.t1)
-        u.t1 = u.t0 + chunk;
-    return true;
-}
-
-/* A position's page from the table, and its row in the cache's k and v counted from the head's first page
- * (-1: it has none) */
-__device__ __forceinline__ int entry_of(const rt_kv &kv, const plan &p, const int32_t *table, int pos)
-{
-    const uint32_t pg = p.page.of(pos);
-    return (long)pg < kv.table_ld ? table[pg] : -1;
-}
-__device__ __forceinline__ int row_of(const rt_kv &kv, const plan &p, int pos, int entry)
-{
-    const uint32_t pg = p.page.of(pos);
-    return entry >= 0 && entry < kv.pages ? entry * (int)(kv.heads * kv.page) + (pos - (int)(pg * (uint32_t)kv.page)) : -1;
-}
-__device__ __forceinline__ const char *address(const void *cache, int row, uint32_t head_rows, int bytes)
-{
-    return (const char *)cache + (uint64_t)((uint32_t)(row < 0 ? 0 : row) + head_rows) * (uint32_t)bytes;
-}
-
-/* The running maximum raised where a lane's largest score passes it by slack, and the reference that
- * the exponents are taken from */
-template <int VE>
-__device__ __forceinline__ float reference(float top, float slack, float &m, float &l, v4f (&acc)[VE])
-{
-    if (__ballot(top > m + slack)) {
-        const float raised = fmaxf(m, group_max(top)), f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - raised);
-        m = raised;
-        l *= f;
-#pragma unroll
-        for (int i = 0; i < VE; i++)
-            acc[i] *= f;
-    }
-    return m == -INFINITY ? 0.0f : m;
-}
-
-/* The waves' results, scaled to the largest of their maxima and added in the waves' order: the output, or
- * the chunk's part of it */
-template <int D>
-constexpr int joint_bytes() { return WAVES * 16 * (D + 4 + 2) * 4; }
-
-template <int D, int VEC>
-__device__ __forceinline__ void finish(char *lds, const rt_kv &kv, const rt_attn &a, const plan &p, const share &u, int number, float m, float l, const v4f (&acc)[D / 16])
-{
-    constexpr int LD = D + 4; /* rows off each other's banks */
-    float(*so)[16][LD] = (float(*)[16][LD])lds;
-    float(*sm)[16] = (float(*)[16])(lds + WAVES * 16 * LD * 4), (*sl)[16] = sm + WAVES;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, g = lane >> 4;
-    const int kh = (int)blockIdx.y;
-    l = group_sum(l);
-    __syncthreads();
-    if (g == 0)
-        sm[wave][c] = m, sl[wave][c] = l;
-    __syncthreads();
-    float top = sm[0][c];
-#pragma unroll
-    for (int w = 1; w < WAVES; w++)
-        top = fmaxf(top, sm[w][c]);
-    const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - top);
-    const int group = p.heads, left = u.q.n * group - u.z * 16, rows = left < 16 ? left : 16;
-    if (c < rows)
-#pragma unroll
-        for (int i = 0; i < D / 16 / VEC; i++)
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-#pragma unroll
-                for (int e = 0; e < VEC; e += 2)
-                    *(float2 *)&so[wave][c][(i * 16 + 4 * g + r) * VEC + e] = float2{acc[i * VEC + e][r] * f, acc[i * VEC + e + 1][r] * f};
-    __syncthreads();
-    for (int i = tid; i < rows * (D / 4); i += 64 * WAVES) {
-        const int r = i / (D / 4), d = 4 * (i % (D / 4));
-        float t = sm[0][r], sum = 0.0f;
-        for (int w = 1; w < WAVES; w++)
-            t = fmaxf(t, sm[w][r]);
-        float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int w = 0; w < WAVES; w++) {
-            const float4 x = *(const float4 *)&so[w][r][d];
-            v = float4{v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w};
-            sum += sl[w][r] * (sm[w][r] == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(sm[w][r] - t));
-        }
-        const int jr = (int)p.group.of(u.z * 16 + r), hr = kh * group + (u.z * 16 + r - jr * group);
-        const long pos = (long)u.q.past + jr;
-        if (pos >= p.cap)
-            sum = NAN; /* a position that the table does not reach */
-        if (u.q.chunks == 1) {
-            store_row(a, D, u.q.first + jr, hr, d, v, sum, pos < 0, gate_of(a, u.q.first + jr, hr, d));
-        } else {
-            const long slot = (long)kh * p.slots + number;
-            *(float4 *)(p.part + (slot * 16 + r) * D + d) = v;
-            if (d == 0)
-                *(float2 *)(p.part + kv.heads * p.slots * 16 * D + (slot * 16 + r) * 2) = float2{t, sum};
-        }
-    }
-    __syncthreads();
-}
-
-/* The most elements (at most full) that a lane's VE elements of a V row divide into */
-constexpr int pieces(int ve, int full) { return ve % full == 0 ? full : ve % (full / 2) == 0 ? full / 2 : 2; }
 
 /* An F32 cache, 16 positions a tile, on v_mfma_f32_16x16x4_f32: position 4 g + r in the second product's step r. */
-template <int D>
+template <int D, bool WINDOW>
 __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seqs b, rt_kv kv, rt_attn a, plan p)
 {
     constexpr int NK = D / 16, VE = D / 16, VEC = pieces(VE, 4), NV = VE / VEC;
@@ -358,14 +18,17 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
     /* with starts that overlap there may be more chunks than slots: those are left out */
     for (int number = (int)blockIdx.x; p.target == 0 || number < p.slots; number += (int)gridDim.x) {
         share u;
-        if (!share_of(b, kv, p, group, number, u))
+        if (!share_of<WINDOW>(b, kv, p, group, number, u))
             return;
         v4f acc[VE];
 #pragma unroll
         for (int i = 0; i < VE; i++)
             acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         float m = -INFINITY, l = 0.0f;
-        const auto here = [&](int tile) { return tile * 16 + c < u.last ? tile * 16 + c : u.last; };
+        const auto here = [&](int tile) {
+            const int i = place_of<WINDOW>(u, tile, 1) * 16 + c;
+            return i < u.last ? i : u.last;
+        };
         const auto load_k = [&](uint32_t (*kw)[4], int row) {
             const char *at = address(kv.k, row, head_rows, D * 4) + g * 16;
 #pragma unroll
@@ -408,11 +71,12 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
                 load_k(kw, row_now);
             }
             float x[4];
-            const bool whole = tile * 16 + 15 <= u.least; /* every row sees every position of the tile */
+            const int base = place_of<WINDOW>(u, tile, 1) * 16;
+            const bool whole = all_seen<WINDOW>(p, u, base, 16); /* every row sees every position of the tile */
 #pragma unroll
             for (int r = 0; r < 4; r++) {
                 x[r] = rows[r] < 0 ? NAN : s[0][r] + s[1][r];
-                if (!whole && tile * 16 + 4 * g + r > u.lim)
+                if (!whole && (base + 4 * g + r > u.lim || passed<WINDOW>(p, base + 4 * g + r, u.low)))
                     x[r] = -INFINITY;
             }
             const float ref = reference(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), SLACK, m, l, acc);
@@ -432,7 +96,7 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
                     for (int i = 0; i < NV; i++)
 #pragma unroll
                         for (int e = 0; e < VEC; e++) {
-                            vw[r][i][e] = tile * 16 + 4 * g + r > u.last ? 0 : vw[r][i][e];
+                            vw[r][i][e] = base + 4 * g + r > u.last || passed<WINDOW>(p, base + 4 * g + r, u.lo0) ? 0 : vw[r][i][e];
                             odd = fmaf(__builtin_bit_cast(float, vw[r][i][e]), 0.0f, odd);
                         }
                 apart = u.j0 < u.j1 && __ballot(odd != 0.0f);
@@ -446,9 +110,10 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
                         for (int e = 0; e < VEC; e++)
                             acc[i * VEC + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, vw[r][i][e]), x[r], acc[i * VEC + e], 0, 0, 0);
             } else {
-                /* each token's rows are computed apart, without the values behind it */
+                /* each token's rows are computed apart, without the values that it does not see */
                 for (int jj = u.j0; jj <= u.j1; jj++) {
                     const long upto = (long)u.q.past + jj < u.last ? (long)u.q.past + jj : u.last;
+                    const int from = WINDOW ? window_from(p, u.q, jj) : 0;
 #pragma unroll
                     for (int i = 0; i < NV; i++)
 #pragma unroll
@@ -456,7 +121,8 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
                             v4f o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                             for (int r = 0; r < 4; r++)
-                                o = __builtin_amdgcn_mfma_f32_16x16x4f32(tile * 16 + 4 * g + r <= upto ? __builtin_bit_cast(float, vw[r][i][e]) : 0.0f, x[r], o, 0, 0, 0);
+                                o = __builtin_amdgcn_mfma_f32_16x16x4f32(base + 4 * g + r <= upto && !passed<WINDOW>(p, base + 4 * g + r, from) ? __builtin_bit_cast(float, vw[r][i][e]) : 0.0f,
+                                                                         x[r], o, 0, 0, 0);
                             if (u.j == jj)
                                 acc[i * VEC + e] += o;
                         }
@@ -554,7 +220,7 @@ __device__ __forceinline__ uint32_t larger(uint32_t x, uint32_t y)
 constexpr int sixteens(long d) { return d == 128 ? 4 : 2; }
 constexpr bool alone(long d) { return d >= 128; }
 
-template <int D, int TYPE>
+template <int D, int TYPE, bool WINDOW>
 __global__ __launch_bounds__(64 * WAVES, alone(D) ? 1 : 2) void attn_half_k(rt_seqs b, rt_kv kv, rt_attn a, plan p)
 {
     typedef half_of<TYPE> H;
@@ -571,7 +237,7 @@ __global__ __launch_bounds__(64 * WAVES, alone(D) ? 1 : 2) void attn_half_k(rt_s
     const uint32_t head_rows = (uint32_t)(blockIdx.y * kv.page);
     for (int number = (int)blockIdx.x; p.target == 0 || number < p.slots; number += (int)gridDim.x) {
         share u;
-        if (!share_of(b, kv, p, group, number, u))
+        if (!share_of<WINDOW>(b, kv, p, group, number, u))
             return;
         const int stop = (u.t1 + SUB - 1) / SUB; /* tiles: a chunk is a whole number of them, but for the last */
         int tile = u.t0 / SUB + wave, row[SUB], entry[SUB];
@@ -589,12 +255,12 @@ __global__ __launch_bounds__(64 * WAVES, alone(D) ? 1 : 2) void attn_half_k(rt_s
         const auto load_entries = [&](int t) {
 #pragma unroll
             for (int n = 0; n < SUB; n++)
-                entry[n] = entry_of(kv, p, u.table, here(t * POS + 16 * n + c));
+                entry[n] = entry_of(kv, p, u.table, here(place_of<WINDOW>(u, t, SUB) * POS + 16 * n + c));
         };
         const auto rows_next = [&](int t) {
 #pragma unroll
             for (int n = 0; n < SUB; n++)
-                row[n] = row_of(kv, p, here(t * POS + 16 * n + c), entry[n]);
+                row[n] = row_of(kv, p, here(place_of<WINDOW>(u, t, SUB) * POS + 16 * n + c), entry[n]);
             load_entries(t + WAVES);
         };
         /* the table's entries, the queries, and with the entries the keys; wave w has the queries' columns 32 i, i = w,
@@ -707,14 +373,15 @@ __global__ __launch_bounds__(64 * WAVES, alone(D) ? 1 : 2) void attn_half_k(rt_s
                 rows_next(tile + WAVES);
                 load_k();
             }
-            const auto place = [&](int r) { return tile * POS + r / 4 * 16 + 4 * g + r % 4; }; /* the lane's positions */
+            const int base = place_of<WINDOW>(u, tile, SUB) * POS;
+            const auto place = [&](int r) { return base + r / 4 * 16 + 4 * g + r % 4; }; /* the lane's positions */
             float x[4 * SUB];
-            const bool whole = tile * POS + POS - 1 <= u.least; /* every row sees every position of the tile */
+            const bool whole = all_seen<WINDOW>(p, u, base, POS); /* every row sees every position of the tile */
             float top = -INFINITY;
 #pragma unroll
             for (int r = 0; r < 4 * SUB; r++) {
                 x[r] = rows[r] < 0 ? NAN : back * s[r / 4][r % 4];
-                if (!whole && place(r) > u.lim)
+                if (!whole && (place(r) > u.lim || passed<WINDOW>(p, place(r), u.low)))
                     x[r] = -INFINITY;
                 top = fmaxf(top, x[r]);
             }
@@ -778,7 +445,7 @@ __global__ __launch_bounds__(64 * WAVES, alone(D) ? 1 : 2) void attn_half_k(rt_s
             uint32_t size = 0;
 #pragma unroll
             for (int r = 0; r < 4 * SUB; r++) {
-                const bool hide = !whole && place(r) > u.last;
+                const bool hide = !whole && (place(r) > u.last || passed<WINDOW>(p, place(r), u.lo0));
 #pragma unroll
                 for (int i = 0; i < NV; i++)
 #pragma unroll
@@ -813,7 +480,7 @@ __global__ __launch_bounds__(64 * WAVES, alone(D) ? 1 : 2) void attn_half_k(rt_s
             }
             for (int pass = 0;; pass++) {
                 if (odd_values || pass > 0) {
-                    /* with values that are not finite each token's rows are computed apart, without the values behind it.
+                    /* with values that are not finite each token's rows are computed apart, without the values that it does not see.
                      * The values are loaded again, so that the fast path keeps its registers */
                     uint4 seen[SUB / 2]; /* F16: 1 where there is a weight */
                     if constexpr (TYPE == RT_F16)
@@ -829,6 +496,7 @@ __global__ __launch_bounds__(64 * WAVES, alone(D) ? 1 : 2) void attn_half_k(rt_s
                         }
                     for (int jj = odd_values ? u.j0 : u.j1; jj <= u.j1; jj++) {
                         const long upto = (long)u.q.past + jj < u.last ? (long)u.q.past + jj : u.last;
+                        const int from = !WINDOW ? 0 : odd_values ? window_from(p, u.q, jj) : u.lo0;
 #pragma unroll
                         for (int k = 0; k < SUB / 2; k++)
 #pragma unroll
@@ -837,7 +505,7 @@ __global__ __launch_bounds__(64 * WAVES, alone(D) ? 1 : 2) void attn_half_k(rt_s
 #pragma unroll
                                 for (int r = 0; r < 8; r++) {
                                     load_words<VW>(again[r], address(kv.v, rows[8 * k + r], head_rows, D * 2) + (i * 16 + c) * VEC * 2);
-                                    const bool hide = place(8 * k + r) > upto;
+                                    const bool hide = place(8 * k + r) > upto || passed<WINDOW>(p, place(8 * k + r), from);
 #pragma unroll
                                     for (int e = 0; e < VW; e++)
                                         again[r][e] = hide ? 0 : again[r][e];
@@ -962,16 +630,16 @@ __global__ __launch_bounds__(256) void attn_join_k(rt_seqs b, rt_kv kv, rt_attn 
     }
 }
 
-template <int TYPE>
+template <int TYPE, bool WINDOW>
 void launch(hipStream_t s, dim3 grid, const rt_seqs &b, const rt_kv &kv, const rt_attn &a, const plan &p)
 {
     switch (kv.dim) {
 #define DIM(D)                                                                                                                                             \
     case D:                                                                                                                                                \
         if constexpr (TYPE == RT_F32)                                                                                                                      \
-            attn_f32_k<D><<<grid, 64 * WAVES, 0, s>>>(b, kv, a, p);                                                                                        \
+            attn_f32_k<D, WINDOW><<<grid, 64 * WAVES, 0, s>>>(b, kv, a, p);                                                                                \
         else                                                                                                                                               \
-            attn_half_k<D, TYPE><<<grid, 64 * WAVES, 0, s>>>(b, kv, a, p);                                                                                 \
+            attn_half_k<D, TYPE, WINDOW><<<grid, 64 * WAVES, 0, s>>>(b, kv, a, p);                                                                         \
         break;
         DIM(32)
         DIM(64)
@@ -993,14 +661,25 @@ void launch(hipStream_t s, dim3 grid, const rt_seqs &b, const rt_kv &kv, const r
  * alone are more than SLOTS */
 constexpr long SLOTS = 4096;
 
-int tile_of(const rt_kv &kv) { return kv.type == RT_F32 ? 1 : sixteens(kv.dim); }
+int tile_of(const rt_kv &kv) { return kv.type == RT_F32 ? 1 : kv.type == RT_Q8 ? 4 : sixteens(kv.dim); }
 
-void plan_chunks(const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long &tiles, long &target)
+/* The positions that the table reaches */
+long reach_of(const rt_kv &kv)
+{
+    const long most = (1L << 31) - 4096;
+    return kv.table_ld > most / kv.page ? most : kv.table_ld * kv.page;
+}
+
+/* A window that holds all positions is none */
+bool cuts(const rt_kv &kv, long window, long sinks) { return window > 0 && window < reach_of(kv) && sinks < reach_of(kv); }
+
+void plan_chunks(const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long window, long sinks, long &tiles, long &target)
 {
     tiles = b.t * (a.q_heads / kv.heads) / 16 + b.n;
-    const bool single = kv.type == RT_F32 ? kv.dim > 128 : alone(kv.dim);
+    const bool single = kv.type == RT_F32 ? kv.dim > 128 : kv.type == RT_Q8 ? q8_attn8_alone(kv.dim) : alone(kv.dim);
     const long once = ((single ? 256 : 512) + kv.heads - 1) / kv.heads;
-    if (tiles * kv.heads > SLOTS || kv.table_ld * kv.page <= 16 * WAVES * tile_of(kv))
+    const long most = reach_of(kv), seen = cuts(kv, window, sinks) && window + sinks + 16 < most ? window + sinks + 16 : most;
+    if (tiles * kv.heads > SLOTS || seen <= 16 * WAVES * tile_of(kv))
         target = 0;
     else if (b.t >= 16 * b.n && tiles >= once)
         target = once;
@@ -1010,18 +689,18 @@ void plan_chunks(const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long &tile
 
 } /* namespace */
 
-long q8_attn_part_floats(const rt_seqs &b, const rt_kv &kv, const rt_attn &a)
+long q8_attn_part_floats(const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long window, long sinks)
 {
     long tiles, target;
-    plan_chunks(b, kv, a, tiles, target);
+    plan_chunks(b, kv, a, window, sinks, tiles, target);
     return target ? kv.heads * (target + tiles) * 16 * (kv.dim + 2) : 0;
 }
 
-void q8_launch_attn(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const rt_attn &a, float *part)
+void q8_launch_attn(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long window, long sinks, float *part)
 {
     plan p;
     long tiles, target;
-    plan_chunks(b, kv, a, tiles, target);
+    plan_chunks(b, kv, a, window, sinks, tiles, target);
     p.target = (int)target;
     p.tile = tile_of(kv);
     p.least = WAVES * p.tile;
@@ -1029,25 +708,28 @@ void q8_launch_attn(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const
         int up = 0;
         while ((1L << up) < d)
             up++;
-        return divisor{(uint32_t)((((__uint128_t)1 << (31 + up)) + d - 1) / d), 31 + up};
+        return q8_divisor{(uint32_t)((((__uint128_t)1 << (31 + up)) + d - 1) / d), 31 + up};
     };
     p.heads = (int)(a.q_heads / kv.heads);
     p.page = by(kv.page), p.group = by(p.heads);
     p.share = target ? 1.00001f / (float)target : 0.0f;
-    const long reach = (1L << 31) - 4096;
-    p.cap = (int)(kv.table_ld > reach / kv.page ? reach : kv.table_ld * kv.page);
+    p.cap = (int)reach_of(kv);
+    p.window = cuts(kv, window, sinks) ? (int)window : 0;
+    p.sinks = p.window ? (int)sinks : 0;
     p.slots = (int)(target + (target ? tiles : 0));
     p.part = part;
     p.qscale = (float)((double)a.scale * 1.4426950408889634074);
     const hipStream_t s = (hipStream_t)stream;
     const long n = p.target ? p.slots : tiles < 1L << 20 ? tiles : 1L << 20;
     const dim3 grid((unsigned)n, (unsigned)kv.heads);
-    if (kv.type == RT_F32)
-        launch<RT_F32>(s, grid, b, kv, a, p);
+    if (kv.type == RT_Q8)
+        q8_launch_attn8(stream, n, b, kv, a, p);
+    else if (kv.type == RT_F32)
+        p.window ? launch<RT_F32, true>(s, grid, b, kv, a, p) : launch<RT_F32, false>(s, grid, b, kv, a, p);
     else if (kv.type == RT_F16)
-        launch<RT_F16>(s, grid, b, kv, a, p);
+        p.window ? launch<RT_F16, true>(s, grid, b, kv, a, p) : launch<RT_F16, false>(s, grid, b, kv, a, p);
     else
-        launch<RT_BF16>(s, grid, b, kv, a, p);
+        p.window ? launch<RT_BF16, true>(s, grid, b, kv, a, p) : launch<RT_BF16, false>(s, grid, b, kv, a, p);
     if (p.target)
         attn_join_k<<<dim3((unsigned)b.t, (unsigned)a.q_heads, (unsigned)((kv.dim + 63) / 64)), 256, 0, s>>>(b, kv, a, p);
 }

@@ -1,0 +1,331 @@
+/* q8_attn8.hip: attention of new tokens over the paged key-value cache of 8 bits, and reading a cache back (include/q8_mix.h). */
+#include "q8_attn.h"
+#include "q8_bf16.h"
+
+namespace {
+
+typedef int v4i __attribute__((ext_vector_type(4)));
+
+/* A row of the cache is d * q, q in -127 .. 127 and d the F32 scale of that position and head. So
+ *
+ *   score = scale d_k (query . q_k)          o = sum_j (p_j d_v) q_v / sum_j p_j
+ *
+ * Keys are the integer instruction's operand as they lie (v_mfma_i32_16x16x64_i8): a query row is rounded to 24 bits of its
+ * largest element, X = rint(query * FULL / most), and cut into three balanced bytes; the three integer sums are exact (below
+ * 2^23 each), and joined in F32. An element is off by 2^-24 of its row's largest.
+ *
+ * Values have to meet weights of any size: where a large weight's value is 0 in an element, the small ones are its output. So
+ * the weights p_j d_v are cut into three bf16 limbs that hold all 24 bits at their own exponents, and a value is made bf16
+ * (exact, 8 bits) on the way. Integers are always finite: a scale that is not finite makes its score or its row's
+ * weights NaN, and where it is masked the weight is 0 by choice, not by product.
+ *
+ * A wave takes 64 positions at a time, one a lane for the page table and the scales, which go through LDS to where the
+ * products have them. Otherwise as the 16-bit caches' kernel: scores S^T = K Q^T leave lane 16 g + c with positions
+ * 16 n + 4 g + r of query row c, which is how the second product's operand has them. */
+constexpr int SUB = 4, POS = 64;
+constexpr float FULL = 8355584.0f; /* 2^23 - 2^15: 127.99 * 2^16, and what the rounding of the quotient adds, in balanced bytes */
+
+/* 4 floats as FULL's integers, their three balanced bytes gathered by byte: w[n] is byte n of the four */
+__device__ __forceinline__ void bytes_of(float4 x, float up, uint32_t (&w)[3])
+{
+    uint32_t y[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        y[e] = (uint32_t)((int)__builtin_rintf((&x.x)[e] * up) + 0x808080);
+    const uint32_t a = __builtin_amdgcn_perm(y[1], y[0], 0x05010400u), b = __builtin_amdgcn_perm(y[3], y[2], 0x05010400u); /* bytes 0 0 1 1 */
+    w[0] = __builtin_amdgcn_perm(b, a, 0x05040100u) ^ 0x80808080u;
+    w[1] = __builtin_amdgcn_perm(b, a, 0x07060302u) ^ 0x80808080u;
+    w[2] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(y[3], y[2], 0x0c0c0602u), __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0602u), 0x05040100u) ^ 0x80808080u;
+}
+
+/* The lane's scores from the three sums: exact integers, two roundings */
+__device__ __forceinline__ float joined(int l0, int l1, int l2) { return fmaf((float)l2, 65536.0f, (float)((l1 << 8) + l0)); }
+
+/* Elements of a V row that a lane has: the largest of 4, 8 and 16 that 16 lanes cover the row with; with heads that are no
+ * power of two the last lanes have none */
+constexpr int each(int d) { return d <= 64 ? 4 : d <= 128 ? 8 : 16; }
+template <int D, bool WINDOW>
+__global__ __launch_bounds__(64 * WAVES, q8_attn8_alone(D) ? 1 : 2) void attn8_k(rt_seqs b, rt_kv kv, rt_attn a, plan p)
+{
+    constexpr int NK = (D + 63) / 64, VE = each(D), VW = VE / 4;
+    struct shared {
+        uint4 query[NK][3][64];
+        float most[WAVES][16];
+        int row[WAVES][64];
+        float dk[WAVES][64], dv[WAVES][64];
+    };
+    constexpr int NEED = sizeof(shared);
+    __shared__ __align__(16) char lds[joint_bytes<D>() > NEED ? joint_bytes<D>() : NEED];
+    shared &sh = *(shared *)lds;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 15, g = lane >> 4;
+    const int group = p.heads;
+    const uint32_t head_rows = (uint32_t)(blockIdx.y * kv.page);
+    const size_t all_rows = (size_t)(kv.pages * kv.heads * kv.page);
+    const float *const scale_k = (const float *)((const char *)kv.k + all_rows * D), *const scale_v = (const float *)((const char *)kv.v + all_rows * D);
+    for (int number = (int)blockIdx.x; p.target == 0 || number < p.slots; number += (int)gridDim.x) {
+        share u;
+        if (!share_of<WINDOW>(b, kv, p, group, number, u))
+            return;
+        const int stop = (u.t1 + SUB - 1) / SUB;
+        int tile = u.t0 / SUB + wave;
+        const auto here = [&](int t) { /* the lane's position of tile t, or the last that there is */
+            const int i = place_of<WINDOW>(u, t, SUB) * POS + lane;
+            return u.last < 0 ? 0 : i < u.last ? i : u.last;
+        };
+        uint4 kx[SUB][NK];
+        float dk, dv; /* of the lane's position of the tile whose keys kx has */
+        int entry;
+        /* rows of tile t from its entries, by way of LDS to the lanes that load them, and the next entries */
+        const auto load_keys = [&](int t) {
+            const int row = row_of(kv, p, here(t), entry);
+            sh.row[wave][lane] = row < 0 ? 0 : row;
+            const size_t at = (uint32_t)(row < 0 ? 0 : row) + head_rows;
+            dk = scale_k[at], dv = scale_v[at];
+            dk = row < 0 ? NAN : dk;
+            entry = entry_of(kv, p, u.table, here(t + WAVES));
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int n = 0; n < SUB; n++) {
+                const char *k = address(kv.k, sh.row[wave][16 * n + c], head_rows, D);
+#pragma unroll
+                for (int i = 0; i < NK; i++)
+                    kx[n][i] = *(const uint4 *)(k + (64 * i + 16 * g < D ? 64 * i + 16 * g : 0));
+            }
+        };
+        entry = entry_of(kv, p, u.table, here(tile));
+        /* wave w has the queries' columns 64 i, i = w, w + WAVES, ..., and makes their bytes for all waves */
+        static_assert(NK <= WAVES);
+        const float *query = a.q + (u.live ? (long)(u.q.first + u.j) * a.q_ld + u.h * a.q_hd : 0);
+        const bool mine = wave < NK && 64 * wave + 16 * g < D;
+        float4 qv[4];
+        uint32_t most = 0; /* of the magnitudes' bits: an infinity or NaN stays the largest */
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            qv[e] = *(const float4 *)(query + (mine ? 64 * wave + 16 * g : 0) + 4 * e);
+        load_keys(tile);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                float &x = (&qv[e].x)[k];
+                x = mine && u.live ? x * p.qscale : 0.0f;
+                const uint32_t bits = __builtin_bit_cast(uint32_t, fabsf(x));
+                most = most > bits ? most : bits;
+            }
+        {
+            const uint32_t o = __shfl_xor(most, 16, 64);
+            most = most > o ? most : o;
+            const uint32_t o2 = __shfl_xor(most, 32, 64);
+            most = most > o2 ? most : o2;
+        }
+        if (g == 0)
+            sh.most[wave][c] = __builtin_bit_cast(float, most);
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            const uint32_t o = __builtin_bit_cast(uint32_t, sh.most[w][c]);
+            most = most > o ? most : o;
+        }
+        const float top_query = fmaxf(__builtin_bit_cast(float, most), 1e-30f); /* below that: the products are below 1e-26 d_k */
+        const float up = FULL / top_query, back = most < 0x7f800000u ? top_query / FULL : NAN;
+        if (wave < NK) {
+            uint32_t w[4][3];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                bytes_of(qv[e], up, w[e]);
+#pragma unroll
+            for (int n = 0; n < 3; n++)
+                sh.query[wave][n][lane] = uint4{w[0][n], w[1][n], w[2][n], w[3][n]};
+        }
+        __syncthreads();
+        v4f acc[VE];
+#pragma unroll
+        for (int i = 0; i < VE; i++)
+            acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        float m = -INFINITY, l = 0.0f;
+        for (; tile < stop; tile += WAVES) {
+            sh.dk[wave][lane] = dk;
+            sh.dv[wave][lane] = dv;
+            __builtin_amdgcn_wave_barrier();
+            uint32_t vw[4 * SUB][VW]; /* rows 16 n + 4 g + r */
+#pragma unroll
+            for (int n = 0; n < SUB; n++) {
+                const int4 rows = *(const int4 *)&sh.row[wave][16 * n + 4 * g];
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    stream_words<VW>(vw[4 * n + r], address(kv.v, (&rows.x)[r], head_rows, D) + (c * VE < D ? c * VE : 0));
+            }
+            v4i s[SUB][3];
+#pragma unroll
+            for (int n = 0; n < SUB; n++)
+#pragma unroll
+                for (int e = 0; e < 3; e++)
+                    s[n][e] = v4i{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < NK; i++)
+#pragma unroll
+                for (int e = 0; e < 3; e++) {
+                    const v4i w = __builtin_bit_cast(v4i, sh.query[i][e][lane]);
+#pragma unroll
+                    for (int n = 0; n < SUB; n++)
+                        s[n][e] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(v4i, kx[n][i]), w, s[n][e], 0, 0, 0);
+                }
+            if (tile + WAVES < stop)
+                load_keys(tile + WAVES);
+            const int base = place_of<WINDOW>(u, tile, SUB) * POS;
+            const bool whole = all_seen<WINDOW>(p, u, base, POS); /* every row sees every position of the tile */
+            const auto hidden = [&](int r) {
+                const int i = base + r / 4 * 16 + 4 * g + r % 4;
+                return i > u.lim || passed<WINDOW>(p, i, u.low);
+            };
+            float x[4 * SUB], top = -INFINITY;
+#pragma unroll
+            for (int n = 0; n < SUB; n++) {
+                const float4 d = *(const float4 *)&sh.dk[wave][16 * n + 4 * g];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    float &y = x[4 * n + r];
+                    y = joined(s[n][0][r], s[n][1][r], s[n][2][r]) * (back * (&d.x)[r]);
+                    if (!whole && hidden(4 * n + r))
+                        y = -INFINITY;
+                    top = fmaxf(top, y);
+                }
+            }
+            /* the weights stay at most 1: times a scale they do not overflow */
+            const float ref = reference(top, SLACK, m, l, acc) + SLACK;
+            uint4 w[SUB / 2][3];
+#pragma unroll
+            for (int n = 0; n < SUB; n++) {
+                const float4 d = *(const float4 *)&sh.dv[wave][16 * n + 4 * g];
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    float &y = x[4 * n + r];
+                    const float weight = __builtin_amdgcn_exp2f(y - ref);
+                    l += weight;
+                    y = !whole && hidden(4 * n + r) ? 0.0f : weight * (&d.x)[r];
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < SUB / 2; k++)
+                xsplit8(float4{x[8 * k], x[8 * k + 1], x[8 * k + 2], x[8 * k + 3]}, float4{x[8 * k + 4], x[8 * k + 5], x[8 * k + 6], x[8 * k + 7]}, w[k][0], w[k][1],
+                        w[k][2]);
+#pragma unroll
+            for (int e = 0; e < VE; e++) {
+#pragma unroll
+                for (int k = 0; k < SUB / 2; k++) {
+                    uint32_t v[4];
+#pragma unroll
+                    for (int r = 0; r < 8; r += 2)
+                        v[r / 2] = pack_hi((float)(int8_t)(vw[8 * k + r][e / 4] >> (8 * (e % 4))), (float)(int8_t)(vw[8 * k + r + 1][e / 4] >> (8 * (e % 4))));
+#pragma unroll
+                    for (int n = 0; n < 3; n++)
+                        acc[e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, uint4{v[0], v[1], v[2], v[3]}), __builtin_bit_cast(b8, w[k][n]), acc[e], 0, 0, 0);
+                }
+                if (e & 1)
+                    __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        finish<D, VE, VE>(lds, kv, a, p, u, number, m, l, acc);
+    }
+}
+
+/* ---- reading a cache back
+ *
+ * A thread has 8 neighbouring elements of a row: as many loads of whole lines as a wave can hold, one rounding to F32
+ * (of 8 bits) and one to the rows' type. Bound by HBM on long ranges, by the table's latency on short ones. */
+template <int TYPE>
+__device__ __forceinline__ void load8(float (&x)[8], const void *cache, size_t row, long at, long dim, size_t all_rows)
+{
+    if constexpr (TYPE == RT_F32) {
+        const float4 lo = *(const float4 *)((const float *)cache + row * dim + at), hi = *(const float4 *)((const float *)cache + row * dim + at + 4);
+        *(float4 *)x = lo, *(float4 *)(x + 4) = hi;
+    } else if constexpr (TYPE == RT_Q8) {
+        const uint2 q = *(const uint2 *)((const char *)cache + row * dim + at);
+        const float d = ((const float *)((const char *)cache + all_rows * dim))[row];
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            x[e] = (float)(int8_t)((e < 4 ? q.x : q.y) >> (8 * (e % 4))) * d;
+    } else {
+        typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+        const uint4 w = *(const uint4 *)((const uint16_t *)cache + row * dim + at);
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            x[e] = TYPE == RT_F16 ? (float)__builtin_bit_cast(h8, w)[e] : (float)__builtin_bit_cast(b8, w)[e];
+    }
+}
+
+template <int TYPE>
+__global__ __launch_bounds__(256) void read_k(rt_seqs b, rt_kv kv, rt_kv_rows a)
+{
+    const long i = blockIdx.x;
+    const int d = (int)kv.dim, per = d / 8, n = 2 * (int)kv.heads * per;
+    const long s = q8_sequence_of(b, i);
+    if (s < 0)
+        return;
+    const long pos = (long)b.past[s] + (i - b.start[s]), slot = pos < 0 ? -1 : pos / kv.page;
+    const long entry = slot >= 0 && slot < kv.table_ld ? kv.table[s * kv.table_ld + slot] : -1;
+    const bool there = entry >= 0 && entry < kv.pages;
+    const size_t all_rows = (size_t)(kv.pages * kv.heads * kv.page);
+    for (int k = (int)(blockIdx.y * 256 + threadIdx.x); k < n; k += 256 * (int)gridDim.y) {
+        const int which = k >= n / 2, h = (k - which * (n / 2)) / per, at = 8 * ((k - which * (n / 2)) % per);
+        void *out = which ? a.v : a.k;
+        if (!out)
+            continue;
+        float x[8];
+        if (there) {
+            load8<TYPE>(x, which ? kv.v : kv.k, (size_t)((entry * kv.heads + h) * kv.page + (pos - slot * kv.page)), at, d, all_rows);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                x[e] = NAN;
+        }
+        const long to = i * (which ? a.v_ld : a.k_ld) + h * (which ? a.v_hd : a.k_hd) + at;
+        if (a.type == RT_F32) {
+            *(float4 *)((float *)out + to) = *(float4 *)x, *(float4 *)((float *)out + to + 4) = *(float4 *)(x + 4);
+        } else if (a.type == RT_F16) {
+            typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+            *(h8 *)((_Float16 *)out + to) = h8{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3], (_Float16)x[4], (_Float16)x[5], (_Float16)x[6], (_Float16)x[7]};
+        } else {
+            *(b8 *)((__bf16 *)out + to) = b8{(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3], (__bf16)x[4], (__bf16)x[5], (__bf16)x[6], (__bf16)x[7]};
+        }
+    }
+}
+
+} /* namespace */
+
+void q8_launch_attn8(q8_stream_t stream, long blocks, const rt_seqs &b, const rt_kv &kv, const rt_attn &a, const q8_attn_plan &p)
+{
+    const dim3 grid((unsigned)blocks, (unsigned)kv.heads);
+    switch (kv.dim) {
+#define DIM(D)                                                                                                                                             \
+    case D:                                                                                                                                                \
+        if (p.window)                                                                                                                                      \
+            attn8_k<D, true><<<grid, 64 * WAVES, 0, (hipStream_t)stream>>>(b, kv, a, p);                                                                   \
+        else                                                                                                                                               \
+            attn8_k<D, false><<<grid, 64 * WAVES, 0, (hipStream_t)stream>>>(b, kv, a, p);                                                                  \
+        break;
+        DIM(32)
+        DIM(64)
+        DIM(96)
+        DIM(128)
+        DIM(160)
+        DIM(192)
+        DIM(224)
+        DIM(256)
+#undef DIM
+    }
+}
+
+void q8_launch_kv_read(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const rt_kv_rows &a)
+{
+    const dim3 grid((unsigned)b.t);
+    const hipStream_t s = (hipStream_t)stream;
+    if (kv.type == RT_F32)
+        read_k<RT_F32><<<grid, 256, 0, s>>>(b, kv, a);
+    else if (kv.type == RT_F16)
+        read_k<RT_F16><<<grid, 256, 0, s>>>(b, kv, a);
+    else if (kv.type == RT_BF16)
+        read_k<RT_BF16><<<grid, 256, 0, s>>>(b, kv, a);
+    else
+        read_k<RT_Q8><<<grid, 256, 0, s>>>(b, kv, a);
+}

@@ -12,8 +12,10 @@ void q8_launch_rope(q8_stream_t s, const rt_seqs &b, const rt_kv &kv, const rt_r
 long q8_delta_prep_floats(const rt_seqs &b, const rt_delta &a);
 void q8_launch_delta(q8_stream_t s, const rt_seqs &b, const rt_delta &a, float *prep);
 /* part: q8_attn_part_floats floats of workspace (none: may be NULL) */
-long q8_attn_part_floats(const rt_seqs &b, const rt_kv &kv, const rt_attn &a);
-void q8_launch_attn(q8_stream_t s, const rt_seqs &b, const rt_kv &kv, const rt_attn &a, float *part);
+long q8_attn_part_floats(const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long window, long sinks);
+/* window 0: every position up to a token's own */
+void q8_launch_attn(q8_stream_t s, const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long window, long sinks, float *part);
+void q8_launch_kv_read(q8_stream_t s, const rt_seqs &b, const rt_kv &kv, const rt_kv_rows &a);
 
 #if defined(__HIPCC__)
 

@@ -91,10 +91,32 @@ __device__ __forceinline__ void store4(void *cache, long at, float4 v)
     } else if constexpr (TYPE == RT_F16) {
         typedef _Float16 h4 __attribute__((ext_vector_type(4)));
         *(h4 *)((_Float16 *)cache + at) = h4{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
-    } else {
+    } else if constexpr (TYPE == RT_BF16) {
         typedef __bf16 b4 __attribute__((ext_vector_type(4)));
         *(b4 *)((__bf16 *)cache + at) = b4{(__bf16)v.x, (__bf16)v.y, (__bf16)v.z, (__bf16)v.w};
     }
+}
+
+/* A row of 8 bits: d = max|x| / 127 over the lanes that hold it, x as rint(x / d), which is within 127 (max / d is off by
+ * less than a step of 127). A row with an element that is not finite gets NaN for d, so that it reads as NaN, and one whose d has no
+ * full precision (below 2^-126) zeros. The scales lie behind all rows. */
+__device__ __forceinline__ void store_q8(const rt_kv &kv, void *cache, long row, int at, int lanes, bool live, float4 x)
+{
+    const auto bits = [](float v) { return __builtin_bit_cast(uint32_t, fabsf(v)); };
+    const uint32_t a = bits(x.x) > bits(x.y) ? bits(x.x) : bits(x.y), b = bits(x.z) > bits(x.w) ? bits(x.z) : bits(x.w);
+    uint32_t most = live ? a > b ? a : b : 0;
+    for (int o = lanes >> 1; o >= 1; o >>= 1) {
+        const uint32_t other = __shfl_xor(most, o, 64);
+        most = most > other ? most : other;
+    }
+    if (!live || row < 0)
+        return;
+    const float d = most < 0x7f800000u ? __builtin_bit_cast(float, most) / 127.0f : NAN;
+    const bool plain = d >= 0x1p-126f;
+    const auto byte = [&](float v) { return plain ? (uint32_t)(int)rintf(v / d) & 0xffu : 0u; };
+    *(uint32_t *)((char *)cache + row * kv.dim + at) = byte(x.x) | byte(x.y) << 8 | byte(x.z) << 16 | byte(x.w) << 24;
+    if (at == 0)
+        ((float *)((char *)cache + kv.pages * kv.heads * kv.page * kv.dim))[row] = d < 0x1p-126f ? 0.0f : d;
 }
 
 /* Query, key and value heads of a token alike: LANES lanes (a power of two, 8 to 64) hold a head, 4 elements a lane, of
@@ -152,7 +174,7 @@ __global__ __launch_bounds__(ROPE_THREADS) void rope_k(rt_seqs b, rt_kv kv, rt_r
         *(float4 *)&row[k][4 * tid] = v[k];
     }
     __syncthreads();
-    if (!live)
+    if (TYPE != RT_Q8 && !live)
         return;
     const int mine = 4 * (tid & ~(lanes - 1));
 #pragma unroll
@@ -179,17 +201,18 @@ __global__ __launch_bounds__(ROPE_THREADS) void rope_k(rt_seqs b, rt_kv kv, rt_r
                 }
             }
         }
-        if (kind == 0) {
+        if (kind == 0 && live) {
             *(float4 *)(a.out + (i0 + k) * a.out_ld + hh * a.out_hd + at) = x;
             continue;
         }
         const uint32_t pos = (uint32_t)p[k], slot = pos / (uint32_t)kv.page; /* p is below 2^32 */
-        if (p[k] < 0 || slot >= kv.table_ld)
-            continue;
-        const long page = kv.table[s[k] * kv.table_ld + slot];
-        if (page < 0 || page >= kv.pages)
-            continue;
-        store4<TYPE>(kind == 1 ? kv.k : kv.v, ((page * nk + hh) * kv.page + (pos - slot * (uint32_t)kv.page)) * kv.dim + at, x);
+        const long page = p[k] >= 0 && slot < kv.table_ld ? kv.table[s[k] * kv.table_ld + slot] : -1;
+        const bool there = page >= 0 && page < kv.pages;
+        const long to = (page * nk + hh) * kv.page + (pos - slot * (uint32_t)kv.page);
+        if constexpr (TYPE == RT_Q8)
+            store_q8(kv, kind == 1 ? kv.k : kv.v, there ? to : -1, at, lanes, live && kind > 0, x);
+        else if (there)
+            store4<TYPE>(kind == 1 ? kv.k : kv.v, to * kv.dim + at, x);
     }
 }
 
@@ -200,8 +223,10 @@ void launch_rope(hipStream_t s, dim3 grid, const rt_seqs &b, const rt_kv &kv, co
         rope_k<RT_F32, RUN><<<grid, ROPE_THREADS, 0, s>>>(b, kv, a, lanes);
     else if (kv.type == RT_F16)
         rope_k<RT_F16, RUN><<<grid, ROPE_THREADS, 0, s>>>(b, kv, a, lanes);
-    else
+    else if (kv.type == RT_BF16)
         rope_k<RT_BF16, RUN><<<grid, ROPE_THREADS, 0, s>>>(b, kv, a, lanes);
+    else
+        rope_k<RT_Q8, RUN><<<grid, ROPE_THREADS, 0, s>>>(b, kv, a, lanes);
 }
 
 template <int TAPS>

@@ -1742,12 +1742,12 @@ void check_seqs(const char *fn, const struct rt_seqs *s, bool past)
         check_words(fn, s->past, 4, "past");
 }
 
-void check_kv(const char *fn, const struct rt_kv *kv)
+void check_kv_shape(const char *fn, const struct rt_kv *kv)
 {
     if (!kv)
         fail(fn, "needs its cache (struct rt_kv)");
-    if (kv->type != RT_F32 && kv->type != RT_F16 && kv->type != RT_BF16)
-        fail(fn, "the cache's type must be RT_F32, RT_F16 or RT_BF16");
+    if (kv->type != RT_F32 && kv->type != RT_F16 && kv->type != RT_BF16 && kv->type != RT_Q8)
+        fail(fn, "the cache's type must be RT_F32, RT_F16, RT_BF16 or RT_Q8");
     if (kv->dim < 32 || kv->dim > 256 || kv->dim % 32)
         fail(fn, "a head's size must be a multiple of 32, 32 to 256");
     if (kv->heads < 1 || kv->heads > RT_HEADS_MAX)
@@ -1756,17 +1756,25 @@ void check_kv(const char *fn, const struct rt_kv *kv)
         fail(fn, "needs pages of 1 to 2^30 positions, 1 to 2^31 - 1 of them, and as many a sequence");
     if ((double)kv->pages * (double)kv->page * (double)kv->heads >= 2147483648.0)
         fail(fn, "needs fewer than 2^31 rows (pages x heads x page) in the cache");
+}
+
+void check_kv(const char *fn, const struct rt_kv *kv)
+{
+    check_kv_shape(fn, kv);
     check_dev_ptr(fn, kv->k, "the cache's k");
     check_dev_ptr(fn, kv->v, "the cache's v");
     check_words(fn, kv->table, 4, "the page table");
 }
 
-span kv_span(const struct rt_kv *kv, const void *p)
+/* of k or of v: with 8 bits the rows' scales behind all rows */
+size_t kv_bytes(const struct rt_kv *kv)
 {
-    return {(const char *)p, (size_t)(kv->pages * kv->page * kv->heads * kv->dim) * (kv->type == RT_F32 ? 4 : 2)};
+    const size_t rows = (size_t)(kv->pages * kv->page * kv->heads);
+    return rows * (kv->type == RT_Q8 ? (size_t)kv->dim + 4 : (size_t)kv->dim * (kv->type == RT_F32 ? 4 : 2));
 }
+span kv_span(const struct rt_kv *kv, const void *p) { return {(const char *)p, kv_bytes(kv)}; }
 
-/* heads that lie hd floats apart in rows ld apart: any order of the two, for an output each element
+/* heads that lie hd elements apart in rows ld apart: any order of the two, for an output each element
  * once. x is read where `in` */
 void check_heads(const char *fn, const void *p, long t, long ld, long hd, long heads, long dim, bool in, const char *what)
 {
@@ -1776,9 +1784,9 @@ void check_heads(const char *fn, const void *p, long t, long ld, long hd, long h
     if (!in && !((t == 1 || ld >= (heads - 1) * hd + dim) && (heads == 1 || hd >= dim)) && !((heads == 1 || hd >= (t - 1) * ld + dim) && (t == 1 || ld >= dim)))
         failf(fn, "%s: its heads must not overlap", what);
 }
-span heads_span(const void *p, long t, long ld, long hd, long heads, long dim)
+span heads_span(const void *p, long t, long ld, long hd, long heads, long dim, size_t size = sizeof(float))
 {
-    return {(const char *)p, p ? sizeof(float) * (size_t)((t - 1) * ld + (heads - 1) * hd + dim) : 0};
+    return {(const char *)p, p ? size * (size_t)((t - 1) * ld + (heads - 1) * hd + dim) : 0};
 }
 span words_span(const void *p, size_t bytes) { return {(const char *)p, p ? bytes : 0}; }
 
@@ -1789,6 +1797,34 @@ void check_state(const char *fn, const float *in, const float *out, size_t float
     check_dev_ptr(fn, out, "s_out");
     if (in != out && meet({(const char *)in, 4 * floats}, {(const char *)out, 4 * floats}))
         fail(fn, "s_out must be s_in or apart from it");
+}
+
+/* window 0: every position up to a token's own */
+void attn(struct rt *R, const char *fn, const struct rt_seqs *s, const struct rt_kv *kv, const struct rt_attn *a, long window, long sinks)
+{
+    ctx *c = get(R, fn);
+    check_seqs(fn, s, true);
+    check_kv(fn, kv);
+    if (!a)
+        fail(fn, "needs its arguments (struct rt_attn)");
+    if (a->q_heads < 1 || a->q_heads > RT_HEADS_MAX || a->q_heads % kv->heads)
+        failf(fn, "needs 1 to %ld query heads, a multiple of the key-value heads", RT_HEADS_MAX);
+    const long t = s->t, d = kv->dim;
+    if (t * (a->q_heads / kv->heads) >= 1L << 31)
+        fail(fn, "needs fewer than 2^31 query rows (tokens x query heads a key-value head)");
+    check_heads(fn, a->q, t, a->q_ld, a->q_hd, a->q_heads, d, true, "q");
+    if (a->gate)
+        check_heads(fn, a->gate, t, a->gate_ld, a->gate_hd, a->q_heads, d, true, "gate");
+    check_dev_ptr(fn, a->o, "o");
+    check_ld(fn, a->o_ld, a->q_heads * d, "o_ld");
+    check_apart(fn, "o", rows_span(a->o, t, a->o_ld, a->q_heads * d),
+                {heads_span(a->q, t, a->q_ld, a->q_hd, a->q_heads, d), heads_span(a->gate, t, a->gate_ld, a->gate_hd, a->q_heads, d), kv_span(kv, kv->k),
+                 kv_span(kv, kv->v), words_span(s->start, 4 * (size_t)(s->n + 1)), words_span(s->past, 4 * (size_t)s->n),
+                 words_span(kv->table, 4 * (size_t)(s->n * kv->table_ld))});
+    const on_gpu g(c);
+    q8_launch_attn((q8_stream_t)c->stream, *s, *kv, *a, window, sinks,
+                   reserve_mix(c, (size_t)q8_attn_part_floats(*s, *kv, *a, window, sinks)));
+    launched("the attention");
 }
 
 } /* namespace */
@@ -1906,31 +1942,54 @@ void rt_rope_kv_dev(struct rt *R, const struct rt_seqs *s, const struct rt_kv *k
     launched("the rotation");
 }
 
-void rt_attn_kv_dev(struct rt *R, const struct rt_seqs *s, const struct rt_kv *kv, const struct rt_attn *a)
+long rt_kv_bytes(const struct rt_kv *kv)
 {
-    const char *fn = "rt_attn_kv_dev";
+    check_kv_shape("rt_kv_bytes", kv);
+    return (long)kv_bytes(kv);
+}
+
+void rt_kv_read_dev(struct rt *R, const struct rt_seqs *s, const struct rt_kv *kv, const struct rt_kv_rows *a)
+{
+    const char *fn = "rt_kv_read_dev";
     ctx *c = get(R, fn);
     check_seqs(fn, s, true);
     check_kv(fn, kv);
     if (!a)
-        fail(fn, "needs its arguments (struct rt_attn)");
-    if (a->q_heads < 1 || a->q_heads > RT_HEADS_MAX || a->q_heads % kv->heads)
-        failf(fn, "needs 1 to %ld query heads, a multiple of the key-value heads", RT_HEADS_MAX);
+        fail(fn, "needs its arguments (struct rt_kv_rows)");
+    if (a->type != RT_F32 && a->type != RT_F16 && a->type != RT_BF16)
+        fail(fn, "the rows' type must be RT_F32, RT_F16 or RT_BF16");
+    if (!a->k && !a->v)
+        fail(fn, "needs k or v for the rows");
     const long t = s->t, d = kv->dim;
-    if (t * (a->q_heads / kv->heads) >= 1L << 31)
-        fail(fn, "needs fewer than 2^31 query rows (tokens x query heads a key-value head)");
-    check_heads(fn, a->q, t, a->q_ld, a->q_hd, a->q_heads, d, true, "q");
-    if (a->gate)
-        check_heads(fn, a->gate, t, a->gate_ld, a->gate_hd, a->q_heads, d, true, "gate");
-    check_dev_ptr(fn, a->o, "o");
-    check_ld(fn, a->o_ld, a->q_heads * d, "o_ld");
-    check_apart(fn, "o", rows_span(a->o, t, a->o_ld, a->q_heads * d),
-                {heads_span(a->q, t, a->q_ld, a->q_hd, a->q_heads, d), heads_span(a->gate, t, a->gate_ld, a->gate_hd, a->q_heads, d), kv_span(kv, kv->k),
-                 kv_span(kv, kv->v), words_span(s->start, 4 * (size_t)(s->n + 1)), words_span(s->past, 4 * (size_t)s->n),
-                 words_span(kv->table, 4 * (size_t)(s->n * kv->table_ld))});
+    const size_t size = a->type == RT_F32 ? 4 : 2;
+    if (a->k)
+        check_heads(fn, a->k, t, a->k_ld, a->k_hd, kv->heads, d, false, "k");
+    if (a->v)
+        check_heads(fn, a->v, t, a->v_ld, a->v_hd, kv->heads, d, false, "v");
+    if ((a->k && (a->k_ld % 8 || a->k_hd % 8) && size == 2) || (a->v && (a->v_ld % 8 || a->v_hd % 8) && size == 2))
+        fail(fn, "16-bit rows: strides are multiples of 8");
+    const span k = heads_span(a->k, t, a->k_ld, a->k_hd, kv->heads, d, size), v = heads_span(a->v, t, a->v_ld, a->v_hd, kv->heads, d, size);
+    const span in[] = {kv_span(kv, kv->k), kv_span(kv, kv->v), words_span(s->start, 4 * (size_t)(s->n + 1)), words_span(s->past, 4 * (size_t)s->n),
+                       words_span(kv->table, 4 * (size_t)(s->n * kv->table_ld))};
+    check_apart(fn, "k", k, {v, in[0], in[1], in[2], in[3], in[4]});
+    check_apart(fn, "v", v, {in[0], in[1], in[2], in[3], in[4]});
     const on_gpu g(c);
-    q8_launch_attn((q8_stream_t)c->stream, *s, *kv, *a, reserve_mix(c, (size_t)q8_attn_part_floats(*s, *kv, *a)));
-    launched("the attention");
+    q8_launch_kv_read((q8_stream_t)c->stream, *s, *kv, *a);
+    launched("reading the cache");
+}
+
+void rt_attn_kv_dev(struct rt *R, const struct rt_seqs *s, const struct rt_kv *kv, const struct rt_attn *a)
+{
+    attn(R, "rt_attn_kv_dev", s, kv, a, 0, 0);
+}
+
+void rt_attn_window_dev(struct rt *R, const struct rt_seqs *s, const struct rt_kv *kv, const struct rt_attn *a, long window, long sinks)
+{
+    const char *fn = "rt_attn_window_dev";
+    get(R, fn);
+    if (window < 1 || sinks < 0)
+        fail(fn, "needs a window of 1 or more positions and 0 or more sinks");
+    attn(R, fn, s, kv, a, window, sinks);
 }
 
 } /* extern "C" */
