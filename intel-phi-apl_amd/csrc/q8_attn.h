@@ -13,21 +13,22 @@ struct q8_divisor {
     __device__ __forceinline__ uint32_t of(uint32_t x) const { return (uint32_t)(((uint64_t)x * mul) >> shift); }
 };
 
-/* What a launch shares: row tiles are 16 query rows (token, head of the group) of one key-value head and
+/* What a launch shares: row tiles are 16 or 64 query rows (token, head of the group) of one key-value head and
  * sequence; the positions that one sees, in tiles of 16, are cut into chunks of one size for the whole batch. */
 struct q8_attn_plan {
     q8_divisor page, group; /* by the positions of a page, by the query heads of a key-value head */
     int heads;    /* query heads of a key-value head */
+    int shift;    /* a row tile has 1 << shift rows */
     int cap;      /* positions that the table reaches */
     int tile;     /* 16s of positions that a wave takes at once (a power of two): chunks are whole numbers of them */
     int least;    /* 16s a chunk at least: one tile of each wave */
     int target;   /* chunks (a key-value head) to spread all tiles over; 0: one a row tile */
-    int slots;    /* partial results a key-value head */
+    int slots;    /* partial results a key-value head, a row tile's each */
     float share;  /* 1 / target, and a little: rounded sums must not make a chunk too small */
     float qscale; /* scale * log2 e: scores are in powers of two */
     int window;   /* positions that a token sees, itself and those before it; 0: all */
     int sinks;    /* with a window, the first positions, which every later token sees, too */
-    float *part;  /* [heads][slots][16][dim], then [heads][slots][16][2]: maximum and sum */
+    float *part;  /* [heads][slots][rows][dim], then [heads][slots][rows][2]: maximum and sum */
 };
 
 /* the 8-bit cache's kernel on `blocks` x heads workgroups */
@@ -51,10 +52,10 @@ struct seq_plan {
 };
 
 /* With a window, the position tiles that a row tile sees at most: the sinks' tiles, and those from the first token's first
- * position, rounded down to a wave's tile, to the last of up to 16 tokens. window and sinks are below 2^30 */
+ * position, rounded down to a wave's tile, to the last of as many tokens as it may have rows */
 __host__ __device__ __forceinline__ int window_tiles(const plan &p)
 {
-    return (p.sinks + 16 * p.tile - 1) / (16 * p.tile) * p.tile + (p.window + 15) / 16 + p.tile + 2;
+    return (p.sinks + 16 * p.tile - 1) / (16 * p.tile) * p.tile + (p.window + 15) / 16 + (1 << p.shift) / 16 + p.tile + 1;
 }
 
 __device__ __forceinline__ seq_plan plan_of(const rt_seqs &b, const plan &p, int group, int s)
@@ -71,7 +72,7 @@ __device__ __forceinline__ seq_plan plan_of(const rt_seqs &b, const plan &p, int
         const int most = window_tiles(p);
         q.tiles = q.tiles < most ? q.tiles : most;
     }
-    q.rows = (int)(((uint32_t)q.n * (uint32_t)group + 15) / 16);
+    q.rows = (int)(((uint32_t)q.n * (uint32_t)group + (1u << p.shift) - 1) >> p.shift);
     q.chunks = 1;
     return q;
 }
@@ -227,16 +228,18 @@ constexpr float SLACK = 8.0f;
 struct share {
     seq_plan q;
     const int32_t *table;
-    int z, j0, j1;   /* the row tile, and its tokens */
+    int z, row;      /* the row tile, and the wave's first row: all waves have the same 16, or each its own 16 of 64 */
+    int j0, j1;      /* the tokens of the wave's rows */
     int j, h;        /* the lane's query row: token and head */
     bool live;       /* there is one */
     int lim;         /* the last position that the lane's row sees, -1 none */
-    int last, least; /* the last that any row of the tile sees, and the last that all do */
+    int end;         /* the last that any row of the tile sees */
+    int last, least; /* the last that any of the wave's rows sees, and the last that all do */
     int t0, t1;      /* the chunk's position tiles, 16 each */
     /* with a window the tiles are counted without those that the row tile does not see: from tile `sunk` on, a tile is `skip`
      * further on */
     int sunk, skip;
-    int low;         /* the first position, but for the sinks, that the lane's row sees; lo0 and lo1: the first and last row's */
+    int low;         /* the first position, but for the sinks, that the lane's row sees; lo0 and lo1: the wave's first and last row's */
     int lo0, lo1;
 };
 
@@ -252,7 +255,7 @@ __device__ __forceinline__ bool passed(const plan &p, int i, int low)
 {
     return WINDOW && i < low && i >= p.sinks;
 }
-/* Whether all rows of u see the positions [i, i + n), so that no mask is needed */
+/* Whether all of the wave's rows see the positions [i, i + n), so that no mask is needed */
 template <bool WINDOW>
 __device__ __forceinline__ bool all_seen(const plan &p, const share &u, int i, int n)
 {
@@ -265,7 +268,7 @@ __device__ __forceinline__ int place_of(const share &u, int t, int sub)
     return WINDOW && t * sub >= u.sunk ? t + u.skip / sub : t;
 }
 
-template <bool WINDOW>
+template <bool WINDOW, int ROWS = 16>
 __device__ __forceinline__ bool share_of(const rt_seqs &b, const rt_kv &kv, const plan &p, int group, int number, share &u)
 {
     int before, s, chunk;
@@ -282,7 +285,9 @@ __device__ __forceinline__ bool share_of(const rt_seqs &b, const rt_kv &kv, cons
     z = first_lane(z);
     const int part = number - z * q.chunks;
     u.z = q.rows - 1 - z; /* those that see most first (8192 tokens of 16 heads of 256 3114 us, 3403 last) */
-    const int row = u.z * 16 + (int)(threadIdx.x & 15);
+    constexpr int WAVE = 16; /* rows of a wave */
+    u.row = u.z * ROWS + (ROWS == 16 ? 0 : first_lane((int)threadIdx.x / 64 * WAVE));
+    const int row = u.row + (int)(threadIdx.x & (WAVE - 1));
     u.table = kv.table + s * kv.table_ld;
     u.j = (int)p.group.of(row);
     u.h = (int)blockIdx.y * group + (row - u.j * group);
@@ -292,18 +297,23 @@ __device__ __forceinline__ bool share_of(const rt_seqs &b, const rt_kv &kv, cons
         return pos < 0 ? -1 : pos < p.cap ? (int)pos : p.cap - 1;
     };
     u.lim = u.live ? sees(u.j) : -1;
-    u.j0 = first_lane((int)p.group.of(u.z * 16));
-    u.j1 = first_lane((int)p.group.of(u.z * 16 + 15));
-    u.j1 = u.j1 < q.n ? u.j1 : q.n - 1;
+    const auto token = [&](int i) {
+        const int j = first_lane((int)p.group.of(i));
+        return j < q.n ? j : q.n - 1;
+    };
+    u.j0 = token(u.row);
+    u.j1 = token(u.row + WAVE - 1);
     u.last = sees(u.j1);
     u.least = sees(u.j0);
+    u.end = ROWS == 16 ? u.last : sees(token(u.z * ROWS + ROWS - 1));
     u.t0 = part * chunk;
-    u.t1 = u.last < 0 ? 0 : u.last / 16 + 1;
+    u.t1 = u.end < 0 ? 0 : u.end / 16 + 1;
     if constexpr (WINDOW) {
         u.low = u.live ? window_from(p, q, u.j) : 0;
         u.lo0 = window_from(p, q, u.j0);
         u.lo1 = window_from(p, q, u.j1);
-        const int first = u.lo0 / (16 * p.tile) * p.tile, some = (p.sinks + 16 * p.tile - 1) / (16 * p.tile) * p.tile;
+        const int low = ROWS == 16 ? u.lo0 : window_from(p, q, token(u.z * ROWS));
+        const int first = low / (16 * p.tile) * p.tile, some = (p.sinks + 16 * p.tile - 1) / (16 * p.tile) * p.tile;
         u.sunk = some < first ? some : first;
         u.skip = first - u.sunk;
         u.t1 = u.t1 > first ? u.t1 - u.skip : u.t1 < u.sunk ? u.t1 : u.sunk;

@@ -584,11 +584,12 @@ __global__ __launch_bounds__(256) void attn_join_k(rt_seqs b, rt_kv kv, rt_attn 
     seq_plan q;
     if (!locate(b, p, p.heads, -1, i, s, q, before, chunk) || q.chunks == 1)
         return;
-    const int kh = (int)p.group.of((uint32_t)h), row = (int)(i - q.first) * p.heads + (int)h - kh * p.heads, z = q.rows - 1 - row / 16, r = row % 16;
+    const int kh = (int)p.group.of((uint32_t)h), row = (int)(i - q.first) * p.heads + (int)h - kh * p.heads, rows = 1 << p.shift,
+              z = q.rows - 1 - (row >> p.shift), r = row & (rows - 1);
     if ((long)before + (long)(z + 1) * q.chunks > p.slots)
         return;
     const long slot = (long)kh * p.slots + before + z * q.chunks;
-    const float *ml = p.part + kv.heads * p.slots * 16 * D + (slot * 16 + r) * 2, *part = p.part + (slot * 16 + r) * D + dd;
+    const float *ml = p.part + kv.heads * p.slots * rows * D + (slot * rows + r) * 2, *part = p.part + (slot * rows + r) * D + dd;
     float4 v = {0.0f, 0.0f, 0.0f, 0.0f};
     float m = -INFINITY, l = 0.0f;
     for (int k0 = turn; k0 < q.chunks; k0 += 64) {
@@ -597,8 +598,8 @@ __global__ __launch_bounds__(256) void attn_join_k(rt_seqs b, rt_kv kv, rt_attn 
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             const int at_chunk = k0 + 16 * k < q.chunks ? k0 + 16 * k : k0;
-            x[k] = *(const float2 *)(ml + (long)at_chunk * 32);
-            w[k] = *(const float4 *)(part + (long)at_chunk * 16 * D);
+            x[k] = *(const float2 *)(ml + (long)at_chunk * (2 * rows));
+            w[k] = *(const float4 *)(part + (long)at_chunk * rows * D);
         }
 #pragma unroll
         for (int k = 0; k < 4; k++)
@@ -627,6 +628,53 @@ __global__ __launch_bounds__(256) void attn_join_k(rt_seqs b, rt_kv kv, rt_attn 
             sum = fmaf(sl[k], f, sum);
         }
         store_row(a, D, i, h, d, v, sum, (long)q.past + (i - q.first) < 0, gate);
+    }
+}
+
+/* The same for prompts: a workgroup a chunk, as the chunks were computed, each with its part of the row tile's rows, so that a launch
+ * of many row tiles of which few or none were cut is few workgroups (8192 tokens of 16 heads of 256, none cut: 486 us with a
+ * workgroup for each token, head and 64 elements). 4 elements of a row a thread, 4 chunks' loads at once. */
+__global__ __launch_bounds__(256) void attn_join_rows_k(rt_seqs b, rt_kv kv, rt_attn a, plan p)
+{
+    int s, before, chunk, number = (int)blockIdx.x;
+    seq_plan q;
+    if (!locate(b, p, p.heads, number, 0, s, q, before, chunk) || q.chunks == 1)
+        return;
+    const int at = number - before, z = at / q.chunks, part = at - z * q.chunks, rows = 1 << p.shift, first = (q.rows - 1 - z) << p.shift;
+    if ((long)before + (long)(z + 1) * q.chunks > p.slots)
+        return;
+    const int D = (int)kv.dim, per = 256 / (D / 4), mine = (int)threadIdx.x / (D / 4), d = 4 * ((int)threadIdx.x - mine * (D / 4));
+    const int live = q.n * p.heads - first < rows ? q.n * p.heads - first : rows, r1 = (int)((long)live * (part + 1) / q.chunks);
+    const long slot = (long)blockIdx.y * p.slots + before + z * q.chunks;
+    if (mine >= per)
+        return;
+    for (int r = (int)((long)live * part / q.chunks) + mine; r < r1; r += per) {
+        const float *ml = p.part + kv.heads * p.slots * rows * D + (slot * rows + r) * 2, *v = p.part + (slot * rows + r) * D + d;
+        const int j = (int)p.group.of(first + r), h = (int)blockIdx.y * p.heads + (first + r - j * p.heads);
+        const float4 gate = gate_of(a, q.first + j, h, d);
+        float4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+        float m = -INFINITY, l = 0.0f;
+        for (int k0 = 0; k0 < q.chunks; k0 += 4) {
+            float2 x[4];
+            float4 w[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const long i = k0 + k < q.chunks ? k0 + k : k0;
+                x[k] = *(const float2 *)(ml + i * (2 * rows));
+                w[k] = *(const float4 *)(v + i * rows * D);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (k0 + k < q.chunks) {
+                    /* a chunk whose maximum is -infinity holds zeros, or NaN: taken as it is */
+                    const float top = fmaxf(m, x[k].x), f = m == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - top),
+                                e = x[k].x == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(x[k].x - top);
+                    sum = float4{fmaf(w[k].x, e, sum.x * f), fmaf(w[k].y, e, sum.y * f), fmaf(w[k].z, e, sum.z * f), fmaf(w[k].w, e, sum.w * f)};
+                    l = fmaf(x[k].y, e, l * f);
+                    m = top;
+                }
+        }
+        store_row(a, D, q.first + j, h, d, sum, l, (long)q.past + j < 0, gate);
     }
 }
 
@@ -673,10 +721,17 @@ long reach_of(const rt_kv &kv)
 /* A window that holds all positions is none */
 bool cuts(const rt_kv &kv, long window, long sinks) { return window > 0 && window < reach_of(kv) && sinks < reach_of(kv); }
 
+/* Row tiles of 64 (as a shift) from that many rows a sequence on, where a kernel has them */
+int shift_of(const rt_seqs &b, const rt_kv &kv, const rt_attn &a)
+{
+    return kv.type == RT_Q8 && b.longest * (a.q_heads / kv.heads) >= 64 && b.t * (a.q_heads / kv.heads) >= 32 * b.n ? 6 : 4;
+}
+
 void plan_chunks(const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long window, long sinks, long &tiles, long &target)
 {
-    tiles = b.t * (a.q_heads / kv.heads) / 16 + b.n;
-    const bool single = kv.type == RT_F32 ? kv.dim > 128 : kv.type == RT_Q8 ? q8_attn8_alone(kv.dim) : alone(kv.dim);
+    const int shift = shift_of(b, kv, a);
+    tiles = (b.t * (a.q_heads / kv.heads) >> shift) + b.n;
+    const bool single = kv.type == RT_F32 ? kv.dim > 128 : kv.type == RT_Q8 ? shift == 4 && q8_attn8_alone(kv.dim) : alone(kv.dim);
     const long once = ((single ? 256 : 512) + kv.heads - 1) / kv.heads;
     const long most = reach_of(kv), seen = cuts(kv, window, sinks) && window + sinks + 16 < most ? window + sinks + 16 : most;
     if (tiles * kv.heads > SLOTS || seen <= 16 * WAVES * tile_of(kv))
@@ -693,7 +748,7 @@ long q8_attn_part_floats(const rt_seqs &b, const rt_kv &kv, const rt_attn &a, lo
 {
     long tiles, target;
     plan_chunks(b, kv, a, window, sinks, tiles, target);
-    return target ? kv.heads * (target + tiles) * 16 * (kv.dim + 2) : 0;
+    return target ? kv.heads * (target + tiles) * (kv.dim + 2) << shift_of(b, kv, a) : 0;
 }
 
 void q8_launch_attn(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long window, long sinks, float *part)
@@ -702,6 +757,7 @@ void q8_launch_attn(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const
     long tiles, target;
     plan_chunks(b, kv, a, window, sinks, tiles, target);
     p.target = (int)target;
+    p.shift = shift_of(b, kv, a);
     p.tile = tile_of(kv);
     p.least = WAVES * p.tile;
     const auto by = [](long d) {
@@ -720,7 +776,7 @@ void q8_launch_attn(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const
     p.part = part;
     p.qscale = (float)((double)a.scale * 1.4426950408889634074);
     const hipStream_t s = (hipStream_t)stream;
-    const long n = p.target ? p.slots : tiles < 1L << 20 ? tiles : 1L << 20;
+    const long n = p.target ? p.slots : p.shift == 6 || tiles < 1L << 20 ? tiles : 1L << 20;
     const dim3 grid((unsigned)n, (unsigned)kv.heads);
     if (kv.type == RT_Q8)
         q8_launch_attn8(stream, n, b, kv, a, p);
@@ -730,6 +786,8 @@ void q8_launch_attn(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const
         p.window ? launch<RT_F16, true>(s, grid, b, kv, a, p) : launch<RT_F16, false>(s, grid, b, kv, a, p);
     else
         p.window ? launch<RT_BF16, true>(s, grid, b, kv, a, p) : launch<RT_BF16, false>(s, grid, b, kv, a, p);
-    if (p.target)
+    if (p.target && (kv.type == RT_Q8 || p.window) && b.t * p.heads >= 16 * b.n)
+        attn_join_rows_k<<<grid, 256, 0, s>>>(b, kv, a, p);
+    else if (p.target)
         attn_join_k<<<dim3((unsigned)b.t, (unsigned)a.q_heads, (unsigned)((kv.dim + 63) / 64)), 256, 0, s>>>(b, kv, a, p);
 }

@@ -229,6 +229,263 @@ __global__ __launch_bounds__(64 * WAVES, q8_attn8_alone(D) ? 1 : 2) void attn8_k
     }
 }
 
+/* ---- prompts
+ *
+ * 64 query rows a workgroup, 16 a wave, which share a tile of 64 positions in LDS: the keys as they lie, the values as bf16 and
+ * transposed, in the order in which the second product's operand has the positions. So a key or value is loaded, and a value
+ * converted, once for 64 rows and not for 16. The next tile's loads are under way in registers while the products of this one
+ * run, and two workgroups share a compute unit, so that one's softmax and staging go under the other's matrix instructions.
+ *
+ * LDS: the keys' rows are 16 bytes apart, which keeps 8 neighbouring rows off each other's banks; a value's row (one element, 64
+ * positions) is 8 pieces of 16 bytes, of which piece n lies at (n + spread) & 7, so that neither 8 elements' pieces read together nor 8 lanes'
+ * written together meet. */
+constexpr int ROWS = 64;
+
+__device__ __forceinline__ int spread(int d) { return (d >> 2) + 2 * (d & 3); }
+
+/* 8 finite F32 values as three bf16 limbs, 8 bits each: exact */
+__device__ __forceinline__ void limbs8(const float *x, v4i (&w)[3])
+{
+    float mid[8], lo[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        mid[e] = x[e] - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x[e]) & 0xffff0000u);
+        lo[e] = mid[e] - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, mid[e]) & 0xffff0000u);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        w[0][e] = (int)pack_hi(x[2 * e], x[2 * e + 1]);
+        w[1][e] = (int)pack_hi(mid[2 * e], mid[2 * e + 1]);
+        w[2][e] = (int)pack_hi(lo[2 * e], lo[2 * e + 1]);
+    }
+}
+
+template <int D, bool WINDOW>
+__global__ __launch_bounds__(64 * WAVES, 2) void attn8_rows_k(rt_seqs b, rt_kv kv, rt_attn a, plan p, int flip)
+{
+    constexpr int NK = (D + 63) / 64, VE = D / 16, PIECES = D / 16, NP = (POS * PIECES + 255) / 256, EACH = each(D) / 4;
+    struct shared {
+        uint8_t k[POS][D + 16];
+        v4i v[D][8];
+        float scale[2][POS]; /* of the keys, of the values */
+    };
+    __shared__ __align__(16) shared sh;
+    const int tid = threadIdx.x, lane = tid & 63, wave = first_lane(tid >> 6), c = lane & 15, g = lane >> 4;
+    const int group = p.heads;
+    const uint32_t head_rows = (uint32_t)(blockIdx.y * kv.page);
+    const size_t all_rows = (size_t)(kv.pages * kv.heads * kv.page);
+    const float *const scales = (const float *)((const char *)(wave == 0 ? kv.k : kv.v) + all_rows * D);
+    const int number = (flip >> (blockIdx.y & 31)) & 1 ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x;
+    share u;
+    if (!share_of<WINDOW, ROWS>(b, kv, p, group, number, u))
+        return;
+    const int stop = (u.t1 + SUB - 1) / SUB;
+    int tile = u.t0 / SUB;
+    const auto here = [&](int t) __attribute__((always_inline)) { /* the lane's position of tile t, or the last that there is */
+        const int i = place_of<WINDOW>(u, t, SUB) * POS + lane;
+        return u.end < 0 ? 0 : i < u.end ? i : u.end;
+    };
+    int entry = entry_of(kv, p, u.table, here(tile));
+    v4i kx[NP];
+    uint32_t vx[16];
+    float scale = 0.0f;
+    bool none = false; /* the lane's position has no row */
+    const auto load = [&](int t) __attribute__((always_inline)) {
+        const int row = row_of(kv, p, here(t), entry), at = row < 0 ? 0 : row;
+        entry = entry_of(kv, p, u.table, here(t + 1));
+        none = row < 0;
+        scale = scales[(size_t)(uint32_t)at + head_rows];
+#pragma unroll
+        for (int i = 0; i < NP; i++) {
+            const int piece = tid + 256 * i, n = piece / PIECES < POS ? piece / PIECES : 0;
+            kx[i] = *(const v4i *)(address(kv.k, __shfl(at, n, 64), head_rows, D) + piece % PIECES * 16);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            /* positions 16 n + 4 g + r: g the wave's number, i = 4 n + r */
+            const char *v = address(kv.v, __builtin_amdgcn_readlane(at, i / 4 * 16 + 4 * wave + i % 4), head_rows, D) + (lane * EACH < D ? lane * EACH : 0);
+            vx[i] = EACH == 4 ? *(const uint32_t *)v : EACH == 2 ? *(const uint16_t *)v : *(const uint8_t *)v;
+        }
+    };
+    const auto store = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < NP; i++) {
+            const int piece = tid + 256 * i;
+            if (POS * PIECES % 256 == 0 || piece < POS * PIECES)
+                *(v4i *)&sh.k[piece / PIECES][piece % PIECES * 16] = kx[i];
+        }
+        if (D % (64 * EACH) == 0 || lane * EACH < D)
+#pragma unroll
+            for (int e = 0; e < EACH; e++)
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    v4i w;
+#pragma unroll
+                    for (int r = 0; r < 8; r += 2)
+                        w[r / 2] = (int)pack_hi((float)(int8_t)(vx[8 * k + r] >> (8 * e)), (float)(int8_t)(vx[8 * k + r + 1] >> (8 * e)));
+                    const int d = lane * EACH + e;
+                    sh.v[d][(4 * k + wave + spread(d)) & 7] = w;
+                }
+        if (wave < 2)
+            sh.scale[wave][lane] = none && wave == 0 ? NAN : scale;
+    };
+    if (tile < stop)
+        load(tile);
+    /* the wave's queries as balanced bytes: elements 64 i + 16 g .. of row c */
+    v4i query[NK][3];
+    float back;
+    {
+        const float *q = a.q + (u.live ? (long)(u.q.first + u.j) * a.q_ld + u.h * a.q_hd : 0);
+        v4f x[NK][4];
+        uint32_t most = 0;
+#pragma unroll
+        for (int i = 0; i < NK; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                x[i][e] = *(const v4f *)(q + (64 * i + 16 * g < D ? 64 * i + 16 * g : 0) + 4 * e);
+#pragma unroll
+        for (int i = 0; i < NK; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    x[i][e][k] = 64 * i + 16 * g < D && u.live ? x[i][e][k] * p.qscale : 0.0f;
+                    const uint32_t bits = __builtin_bit_cast(uint32_t, fabsf(x[i][e][k]));
+                    most = most > bits ? most : bits;
+                }
+        const uint32_t o = __shfl_xor(most, 16, 64);
+        most = most > o ? most : o;
+        const uint32_t o2 = __shfl_xor(most, 32, 64);
+        most = most > o2 ? most : o2;
+        const float top = fmaxf(__builtin_bit_cast(float, most), 1e-30f), up = FULL / top;
+        back = most < 0x7f800000u ? top / FULL : NAN;
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+            uint32_t w[4][3];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                bytes_of(float4{x[i][e][0], x[i][e][1], x[i][e][2], x[i][e][3]}, up, w[e]);
+#pragma unroll
+            for (int n = 0; n < 3; n++)
+                query[i][n] = v4i{(int)w[0][n], (int)w[1][n], (int)w[2][n], (int)w[3][n]};
+        }
+    }
+    v4f acc[VE];
+#pragma unroll
+    for (int i = 0; i < VE; i++)
+        acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+    float m = -INFINITY, l = 0.0f;
+    const bool some = u.row < u.q.n * group; /* the wave has rows */
+    for (; tile < stop; tile++) {
+        __syncthreads(); /* the tile before has been read */
+        store();
+        __syncthreads();
+        if (tile + 1 < stop)
+            load(tile + 1);
+        const int base = place_of<WINDOW>(u, tile, SUB) * POS;
+        /* none of the wave's rows sees any of it */
+        if (!some || base > u.last || (WINDOW && base + POS <= u.lo0 && base >= p.sinks))
+            continue;
+        const bool whole = all_seen<WINDOW>(p, u, base, POS); /* every row sees every position of the tile */
+        const auto hidden = [&](int r) __attribute__((always_inline)) {
+            const int i = base + r / 4 * 16 + 4 * g + r % 4;
+            return i > u.lim || passed<WINDOW>(p, i, u.low);
+        };
+        float x[4 * SUB], top = -INFINITY;
+        const auto key = [&](int n, int i) __attribute__((always_inline)) { return *(const v4i *)&sh.k[16 * n + c][64 * i + 16 * g < D ? 64 * i + 16 * g : 0]; };
+        v4i kk[2][NK]; /* the operands of the next 16 positions are read under this one's products */
+#pragma unroll
+        for (int i = 0; i < NK; i++)
+            kk[0][i] = key(0, i);
+#pragma unroll
+        for (int n = 0; n < SUB; n++) {
+            if (n + 1 < SUB)
+#pragma unroll
+                for (int i = 0; i < NK; i++)
+                    kk[(n + 1) & 1][i] = key(n + 1, i);
+            const v4f d = *(const v4f *)&sh.scale[0][16 * n + 4 * g];
+            v4i s[3] = {v4i{0, 0, 0, 0}, v4i{0, 0, 0, 0}, v4i{0, 0, 0, 0}};
+#pragma unroll
+            for (int i = 0; i < NK; i++)
+#pragma unroll
+                for (int e = 0; e < 3; e++)
+                    s[e] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[n & 1][i], query[i][e], s[e], 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+                x[4 * n + r] = joined(s[0][r], s[1][r], s[2][r]) * (back * d[r]);
+        }
+        if (!whole)
+#pragma unroll
+            for (int r = 0; r < 4 * SUB; r++)
+                x[r] = hidden(r) ? -INFINITY : x[r];
+#pragma unroll
+        for (int r = 0; r < 4 * SUB; r++)
+            top = fmaxf(top, x[r]);
+        const float ref = reference(top, SLACK, m, l, acc) + SLACK;
+#pragma unroll
+        for (int n = 0; n < SUB; n++) {
+            const v4f d = *(const v4f *)&sh.scale[1][16 * n + 4 * g];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float weight = __builtin_amdgcn_exp2f(x[4 * n + r] - ref);
+                l += weight;
+                x[4 * n + r] = weight * d[r];
+            }
+        }
+        if (!whole)
+#pragma unroll
+            for (int r = 0; r < 4 * SUB; r++)
+                x[r] = hidden(r) ? 0.0f : x[r]; /* whatever the scale is */
+        const auto value = [&](int k, int e) __attribute__((always_inline)) { return sh.v[16 * e + c][(4 * k + g + 4 * e + spread(c)) & 7]; };
+#pragma unroll
+        for (int k = 0; k < SUB / 2; k++) {
+            v4i w[3], v[2][2];
+            v[0][0] = value(k, 0), v[0][1] = value(k, VE > 1 ? 1 : 0);
+            limbs8(x + 8 * k, w);
+#pragma unroll
+            for (int e = 0; e < VE; e += 2) {
+                if (e + 2 < VE)
+                    v[(e / 2 + 1) & 1][0] = value(k, e + 2), v[(e / 2 + 1) & 1][1] = value(k, e + 3);
+#pragma unroll
+                for (int n = 0; n < 3; n++)
+#pragma unroll
+                    for (int f = 0; f < 2; f++)
+                        acc[e + f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, v[e / 2 & 1][f]), __builtin_bit_cast(b8, w[n]), acc[e + f], 0, 0, 0);
+            }
+        }
+    }
+    l = group_sum(l);
+    if (!u.live)
+        return;
+    const long pos = (long)u.q.past + u.j, slot = ((long)blockIdx.y * p.slots + number) * ROWS + (u.row - u.z * ROWS + c);
+    const float sum = pos >= p.cap ? NAN : l; /* a position that the table does not reach */
+    if (u.q.chunks > 1) {
+#pragma unroll
+        for (int e = 0; e < VE; e++)
+            *(v4f *)(p.part + slot * D + 16 * e + 4 * g) = acc[e];
+        if (g == 0)
+            *(float2 *)(p.part + kv.heads * p.slots * ROWS * D + slot * 2) = float2{m, sum};
+        return;
+    }
+    const float r = 1.0f / sum;
+    const long token = u.q.first + u.j;
+    float *o = a.o + token * a.o_ld + (long)u.h * D + 4 * g;
+    const float *gate = a.gate ? a.gate + token * a.gate_ld + u.h * a.gate_hd + 4 * g : nullptr;
+    v4f gx[VE]; /* all gates under way at once, not one after the other */
+    if (gate)
+#pragma unroll
+        for (int e = 0; e < VE; e++)
+            gx[e] = *(const v4f *)(gate + 16 * e);
+#pragma unroll
+    for (int e = 0; e < VE; e++) {
+        v4f v;
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+            v[n] = pos < 0 ? 0.0f : acc[e][n] * r * (gate ? q8_sigmoid(gx[e][n]) : 1.0f);
+        *(v4f *)(o + 16 * e) = v;
+    }
+}
+
 /* ---- reading a cache back
  *
  * A thread has 8 neighbouring elements of a row: as many loads of whole lines as a wave can hold, one rounding to F32
@@ -296,10 +553,19 @@ __global__ __launch_bounds__(256) void read_k(rt_seqs b, rt_kv kv, rt_kv_rows a)
 void q8_launch_attn8(q8_stream_t stream, long blocks, const rt_seqs &b, const rt_kv &kv, const rt_attn &a, const q8_attn_plan &p)
 {
     const dim3 grid((unsigned)blocks, (unsigned)kv.heads);
+    /* Two workgroups run on each compute unit: where all run at once, the second ones take the row tiles from the shortest, the first
+     * from the longest, so that the units have equal shares. A bit a head */
+    int flip = 0;
+    if (blocks * kv.heads <= 1024)
+        for (long y = 0; y < kv.heads && y < 32; y++)
+            flip |= ((y * blocks + blocks / 2) / 256 & 1) << y;
     switch (kv.dim) {
 #define DIM(D)                                                                                                                                             \
     case D:                                                                                                                                                \
-        if (p.window)                                                                                                                                      \
+        if (p.shift == 6)                                                                                                                                  \
+            p.window ? attn8_rows_k<D, true><<<grid, 64 * WAVES, 0, (hipStream_t)stream>>>(b, kv, a, p, flip)                                              \
+                     : attn8_rows_k<D, false><<<grid, 64 * WAVES, 0, (hipStream_t)stream>>>(b, kv, a, p, flip);                                            \
+        else if (p.window)                                                                                                                                 \
             attn8_k<D, true><<<grid, 64 * WAVES, 0, (hipStream_t)stream>>>(b, kv, a, p);                                                                   \
         else                                                                                                                                               \
             attn8_k<D, false><<<grid, 64 * WAVES, 0, (hipStream_t)stream>>>(b, kv, a, p);                                                                  \
