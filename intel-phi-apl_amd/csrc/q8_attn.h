@@ -269,7 +269,7 @@ __device__ __forceinline__ int place_of(const share &u, int t, int sub)
 }
 
 template <bool WINDOW, int ROWS = 16>
-__device__ __forceinline__ bool share_of(const rt_seqs &b, const rt_kv &kv, const plan &p, int group, int number, share &u)
+__device__ __forceinline__ bool share_of(const rt_seqs &b, const rt_kv &kv, const plan &p, int group, int number, int kv_head, share &u)
 {
     int before, s, chunk;
     if (!locate(b, p, group, number, 0, s, u.q, before, chunk))
@@ -290,7 +290,7 @@ __device__ __forceinline__ bool share_of(const rt_seqs &b, const rt_kv &kv, cons
     const int row = u.row + (int)(threadIdx.x & (WAVE - 1));
     u.table = kv.table + s * kv.table_ld;
     u.j = (int)p.group.of(row);
-    u.h = (int)blockIdx.y * group + (row - u.j * group);
+    u.h = kv_head * group + (row - u.j * group);
     u.live = u.j < q.n;
     const auto sees = [&](int j) { /* the last position that token j sees, within the table */
         const long pos = (long)q.past + j;

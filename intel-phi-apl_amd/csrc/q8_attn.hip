@@ -18,7 +18,7 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
     /* with starts that overlap there may be more chunks than slots: those are left out */
     for (int number = (int)blockIdx.x; p.target == 0 || number < p.slots; number += (int)gridDim.x) {
         share u;
-        if (!share_of<WINDOW>(b, kv, p, group, number, u))
+        if (!share_of<WINDOW>(b, kv, p, group, number, (int)blockIdx.y, u))
             return;
         v4f acc[VE];
 #pragma unroll
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(64 * WAVES, alone(D) ? 1 : 2) void attn_half_k(rt_s
     const uint32_t head_rows = (uint32_t)(blockIdx.y * kv.page);
     for (int number = (int)blockIdx.x; p.target == 0 || number < p.slots; number += (int)gridDim.x) {
         share u;
-        if (!share_of<WINDOW>(b, kv, p, group, number, u))
+        if (!share_of<WINDOW>(b, kv, p, group, number, (int)blockIdx.y, u))
             return;
         const int stop = (u.t1 + SUB - 1) / SUB; /* tiles: a chunk is a whole number of them, but for the last */
         int tile = u.t0 / SUB + wave, row[SUB], entry[SUB];
@@ -786,7 +786,7 @@ void q8_launch_attn(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const
         p.window ? launch<RT_F16, true>(s, grid, b, kv, a, p) : launch<RT_F16, false>(s, grid, b, kv, a, p);
     else
         p.window ? launch<RT_BF16, true>(s, grid, b, kv, a, p) : launch<RT_BF16, false>(s, grid, b, kv, a, p);
-    if (p.target && (kv.type == RT_Q8 || p.window) && b.t * p.heads >= 16 * b.n)
+    if (p.target && (kv.type == RT_Q8 || p.window) && b.t * p.heads >= 32 * b.n)
         attn_join_rows_k<<<grid, 256, 0, s>>>(b, kv, a, p);
     else if (p.target)
         attn_join_k<<<dim3((unsigned)b.t, (unsigned)a.q_heads, (unsigned)((kv.dim + 63) / 64)), 256, 0, s>>>(b, kv, a, p);

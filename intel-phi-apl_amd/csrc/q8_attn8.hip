@@ -64,7 +64,7 @@ __global__ __launch_bounds__(64 * WAVES, q8_attn8_alone(D) ? 1 : 2) void attn8_k
     const float *const scale_k = (const float *)((const char *)kv.k + all_rows * D), *const scale_v = (const float *)((const char *)kv.v + all_rows * D);
     for (int number = (int)blockIdx.x; p.target == 0 || number < p.slots; number += (int)gridDim.x) {
         share u;
-        if (!share_of<WINDOW>(b, kv, p, group, number, u))
+        if (!share_of<WINDOW>(b, kv, p, group, number, (int)blockIdx.y, u))
             return;
         const int stop = (u.t1 + SUB - 1) / SUB;
         int tile = u.t0 / SUB + wave;
@@ -243,6 +243,53 @@ constexpr int ROWS = 64;
 
 __device__ __forceinline__ int spread(int d) { return (d >> 2) + 2 * (d & 3); }
 
+/* Which row tile (and chunk) of which key-value head a workgroup takes. Workgroups go to the 8 XCDs in turn, each with an L2 of its
+ * own, so a head's go to as few XCDs as there are for it, and an XCD's go through a head's row tiles in order: what they read together is
+ * a part of one head's cache. Two run on a compute unit: where all run at once, the second half of an XCD's goes from the
+ * shortest row tiles on, the first from the longest, so that the units have equal shares. */
+struct order {
+    int blocks, heads; /* row tiles or chunks a head; heads */
+    int each, count;   /* XCDs a head (0: several heads an XCD); workgroups an XCD */
+};
+order order_of(long blocks, long heads)
+{
+    order q = {(int)blocks, (int)heads, 0, 0};
+    if (heads < 8 && 8 % heads == 0)
+        q.each = (int)(8 / heads);
+    q.count = (int)(q.each ? (blocks + q.each - 1) / q.each : (heads * blocks + 7) / 8);
+    return q;
+}
+__device__ __forceinline__ bool place_in(const order &q, int block, int &number, int &head)
+{
+    const int xcd = block & 7;
+    int at = block >> 3;
+    constexpr int HALF = 32; /* compute units of an XCD */
+    if (q.count > HALF && q.count <= 2 * HALF + 2 && at >= HALF)
+        at = q.count - 1 - (at - HALF);
+    if (q.each) {
+        head = xcd / q.each;
+        number = at * q.each + xcd % q.each;
+    } else {
+        const int i = at * 8 + xcd; /* with a multiple of 8 heads each XCD has heads of its own */
+        if (q.heads % 8 == 0) {
+            head = at / q.blocks * 8 + xcd;
+            number = at % q.blocks;
+        } else {
+            head = i / q.blocks;
+            number = i % q.blocks;
+        }
+    }
+    return head < q.heads && number < q.blocks;
+}
+
+/* 1 / (1 + exp(-x)): the exponent in two parts, a reciprocal off by a step */
+__device__ __forceinline__ float gate_weight(float x)
+{
+    const float y = -fabsf(x), t = y * 1.44269504f, r = fmaf(y, 1.92596300e-8f, fmaf(y, 1.44269504f, -t)), e = __builtin_amdgcn_exp2f(t);
+    const float f = fmaf(e * r, 0.693147181f, e);
+    return (x >= 0.0f ? 1.0f : f) * __builtin_amdgcn_rcpf(1.0f + f);
+}
+
 /* 8 finite F32 values as three bf16 limbs, 8 bits each: exact */
 __device__ __forceinline__ void limbs8(const float *x, v4i (&w)[3])
 {
@@ -261,7 +308,7 @@ __device__ __forceinline__ void limbs8(const float *x, v4i (&w)[3])
 }
 
 template <int D, bool WINDOW>
-__global__ __launch_bounds__(64 * WAVES, 2) void attn8_rows_k(rt_seqs b, rt_kv kv, rt_attn a, plan p, int flip)
+__global__ __launch_bounds__(64 * WAVES, 2) void attn8_rows_k(rt_seqs b, rt_kv kv, rt_attn a, plan p, order places)
 {
     constexpr int NK = (D + 63) / 64, VE = D / 16, PIECES = D / 16, NP = (POS * PIECES + 255) / 256, EACH = each(D) / 4;
     struct shared {
@@ -272,12 +319,14 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn8_rows_k(rt_seqs b, rt_kv k
     __shared__ __align__(16) shared sh;
     const int tid = threadIdx.x, lane = tid & 63, wave = first_lane(tid >> 6), c = lane & 15, g = lane >> 4;
     const int group = p.heads;
-    const uint32_t head_rows = (uint32_t)(blockIdx.y * kv.page);
+    int number, head;
+    if (!place_in(places, (int)blockIdx.x, number, head))
+        return;
+    const uint32_t head_rows = (uint32_t)head * (uint32_t)kv.page;
     const size_t all_rows = (size_t)(kv.pages * kv.heads * kv.page);
     const float *const scales = (const float *)((const char *)(wave == 0 ? kv.k : kv.v) + all_rows * D);
-    const int number = (flip >> (blockIdx.y & 31)) & 1 ? (int)(gridDim.x - 1 - blockIdx.x) : (int)blockIdx.x;
     share u;
-    if (!share_of<WINDOW, ROWS>(b, kv, p, group, number, u))
+    if (!share_of<WINDOW, ROWS>(b, kv, p, group, number, head, u))
         return;
     const int stop = (u.t1 + SUB - 1) / SUB;
     int tile = u.t0 / SUB;
@@ -285,27 +334,33 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn8_rows_k(rt_seqs b, rt_kv k
         const int i = place_of<WINDOW>(u, t, SUB) * POS + lane;
         return u.end < 0 ? 0 : i < u.end ? i : u.end;
     };
-    int entry = entry_of(kv, p, u.table, here(tile));
+    int entry = u.table[p.page.of(here(tile))]; /* (the table reaches them all) */
     v4i kx[NP];
     uint32_t vx[16];
     float scale = 0.0f;
     bool none = false; /* the lane's position has no row */
     const auto load = [&](int t) __attribute__((always_inline)) {
-        const int row = row_of(kv, p, here(t), entry), at = row < 0 ? 0 : row;
-        entry = entry_of(kv, p, u.table, here(t + 1));
-        none = row < 0;
-        scale = scales[(size_t)(uint32_t)at + head_rows];
+        const uint32_t pos = (uint32_t)here(t), page_rows = (uint32_t)(kv.heads * kv.page);
+        none = (uint32_t)entry >= (uint32_t)kv.pages;
+        const uint32_t place = (none ? 0 : (uint32_t)entry * page_rows + (pos - p.page.of(pos) * (uint32_t)kv.page)) + head_rows; /* below 2^31 */
+        entry = u.table[p.page.of(here(t + 1))];
+        uint32_t rows[NP];
 #pragma unroll
         for (int i = 0; i < NP; i++) {
             const int piece = tid + 256 * i, n = piece / PIECES < POS ? piece / PIECES : 0;
-            kx[i] = *(const v4i *)(address(kv.k, __shfl(at, n, 64), head_rows, D) + piece % PIECES * 16);
+            rows[i] = (uint32_t)__shfl((int)place, n, 64);
         }
+        scale = scales[place];
 #pragma unroll
         for (int i = 0; i < 16; i++) {
             /* positions 16 n + 4 g + r: g the wave's number, i = 4 n + r */
-            const char *v = address(kv.v, __builtin_amdgcn_readlane(at, i / 4 * 16 + 4 * wave + i % 4), head_rows, D) + (lane * EACH < D ? lane * EACH : 0);
-            vx[i] = EACH == 4 ? *(const uint32_t *)v : EACH == 2 ? *(const uint16_t *)v : *(const uint8_t *)v;
+            const char *v = (const char *)kv.v + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)place, i / 4 * 16 + 4 * wave + i % 4) * D;
+            const uint32_t off = lane * EACH < D ? lane * EACH : 0;
+            vx[i] = EACH == 4 ? *(const uint32_t *)(v + off) : EACH == 2 ? *(const uint16_t *)(v + off) : *(const uint8_t *)(v + off);
         }
+#pragma unroll
+        for (int i = 0; i < NP; i++)
+            kx[i] = *(const v4i *)((const char *)kv.k + (uint64_t)rows[i] * D + (tid + 256 * i) % PIECES * 16);
     };
     const auto store = [&]() __attribute__((always_inline)) {
 #pragma unroll
@@ -412,7 +467,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn8_rows_k(rt_seqs b, rt_kv k
                     s[e] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[n & 1][i], query[i][e], s[e], 0, 0, 0);
 #pragma unroll
             for (int r = 0; r < 4; r++)
-                x[4 * n + r] = joined(s[0][r], s[1][r], s[2][r]) * (back * d[r]);
+                x[4 * n + r] = joined(s[0][r], s[1][r], s[2][r]) * d[r]; /* over back */
         }
         if (!whole)
 #pragma unroll
@@ -421,13 +476,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn8_rows_k(rt_seqs b, rt_kv k
 #pragma unroll
         for (int r = 0; r < 4 * SUB; r++)
             top = fmaxf(top, x[r]);
-        const float ref = reference(top, SLACK, m, l, acc) + SLACK;
+        const float ref = reference(top * back, SLACK, m, l, acc) + SLACK;
 #pragma unroll
         for (int n = 0; n < SUB; n++) {
             const v4f d = *(const v4f *)&sh.scale[1][16 * n + 4 * g];
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const float weight = __builtin_amdgcn_exp2f(x[4 * n + r] - ref);
+                const float weight = __builtin_amdgcn_exp2f(fmaf(x[4 * n + r], back, -ref));
                 l += weight;
                 x[4 * n + r] = weight * d[r];
             }
@@ -457,7 +512,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn8_rows_k(rt_seqs b, rt_kv k
     l = group_sum(l);
     if (!u.live)
         return;
-    const long pos = (long)u.q.past + u.j, slot = ((long)blockIdx.y * p.slots + number) * ROWS + (u.row - u.z * ROWS + c);
+    const long pos = (long)u.q.past + u.j, slot = ((long)head * p.slots + number) * ROWS + (u.row - u.z * ROWS + c);
     const float sum = pos >= p.cap ? NAN : l; /* a position that the table does not reach */
     if (u.q.chunks > 1) {
 #pragma unroll
@@ -481,7 +536,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn8_rows_k(rt_seqs b, rt_kv k
         v4f v;
 #pragma unroll
         for (int n = 0; n < 4; n++)
-            v[n] = pos < 0 ? 0.0f : acc[e][n] * r * (gate ? q8_sigmoid(gx[e][n]) : 1.0f);
+            v[n] = pos < 0 ? 0.0f : acc[e][n] * r * (gate ? gate_weight(gx[e][n]) : 1.0f);
         *(v4f *)(o + 16 * e) = v;
     }
 }
@@ -553,18 +608,14 @@ __global__ __launch_bounds__(256) void read_k(rt_seqs b, rt_kv kv, rt_kv_rows a)
 void q8_launch_attn8(q8_stream_t stream, long blocks, const rt_seqs &b, const rt_kv &kv, const rt_attn &a, const q8_attn_plan &p)
 {
     const dim3 grid((unsigned)blocks, (unsigned)kv.heads);
-    /* Two workgroups run on each compute unit: where all run at once, the second ones take the row tiles from the shortest, the first
-     * from the longest, so that the units have equal shares. A bit a head */
-    int flip = 0;
-    if (blocks * kv.heads <= 1024)
-        for (long y = 0; y < kv.heads && y < 32; y++)
-            flip |= ((y * blocks + blocks / 2) / 256 & 1) << y;
+    const order places = order_of(blocks, kv.heads);
+    const unsigned all = 8u * (unsigned)places.count;
     switch (kv.dim) {
 #define DIM(D)                                                                                                                                             \
     case D:                                                                                                                                                \
         if (p.shift == 6)                                                                                                                                  \
-            p.window ? attn8_rows_k<D, true><<<grid, 64 * WAVES, 0, (hipStream_t)stream>>>(b, kv, a, p, flip)                                              \
-                     : attn8_rows_k<D, false><<<grid, 64 * WAVES, 0, (hipStream_t)stream>>>(b, kv, a, p, flip);                                            \
+            p.window ? attn8_rows_k<D, true><<<all, 64 * WAVES, 0, (hipStream_t)stream>>>(b, kv, a, p, places)                                             \
+                     : attn8_rows_k<D, false><<<all, 64 * WAVES, 0, (hipStream_t)stream>>>(b, kv, a, p, places);                                           \
         else if (p.window)                                                                                                                                 \
             attn8_k<D, true><<<grid, 64 * WAVES, 0, (hipStream_t)stream>>>(b, kv, a, p);                                                                   \
         else                                                                                                                                               \
