@@ -25,6 +25,8 @@ struct q8_attn_plan {
     int target;   /* chunks (a key-value head) to spread all tiles over; 0: one a row tile */
     int slots;    /* partial results a key-value head, a row tile's each */
     float share;  /* 1 / target, and a little: rounded sums must not make a chunk too small */
+    int once;     /* the workgroups (a key-value head) that run at once, where the chunks' size is chosen by rounds of them; or 0 */
+    int *size;    /* then the size that was chosen, for the join */
     float qscale; /* scale * log2 e: scores are in powers of two */
     int window;   /* positions that a token sees, itself and those before it; 0: all */
     int sinks;    /* with a window, the first positions, which every later token sees, too */
@@ -101,6 +103,31 @@ __device__ __forceinline__ int chunks_of(int tiles, int chunk)
     return n;
 }
 
+/* The size of chunks of which the rounds of workgroups take least: of some sizes that make one or two rounds, the one with the
+ * smallest rounds x (size + FIXED), FIXED being what a workgroup takes besides, in tiles. A batch's last, partial round
+ * costs a whole one: 32 sequences of 1028 positions, 4 heads: chunks of a third of a sequence took two rounds, halves one. `chunks`: how
+ * many chunks there are of a size. */
+constexpr float FIXED = 10.0f;
+template <class F>
+__device__ __forceinline__ int chunk_of_rounds(const plan &p, float all, F chunks)
+{
+    constexpr float size[] = {2.0f, 1.5f, 1.25f, 1.125f, 1.0f, 0.75f, 0.625f, 0.55f};
+    const float even = all * __builtin_amdgcn_rcpf((float)p.once) * 1.00001f + 1.0f, turn = __builtin_amdgcn_rcpf((float)p.once);
+    float least = INFINITY;
+    int best = p.least;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        int c = ((int)(even * size[i]) + p.tile) / p.tile * p.tile;
+        c = c > p.least ? c : p.least;
+        const int count = chunks(c);
+        const float cost = ceilf((float)count * turn - 0.001f) * ((float)c + FIXED);
+        const bool better = i == 0 || (count <= p.slots && cost < least);
+        best = better ? c : best;
+        least = better ? cost : least;
+    }
+    return best;
+}
+
 /* the sums of a value over the lanes up to each: by 1, 2, 4 and 8 within each 16, then the 16s' last to the next */
 #define UPTO(v, ctrl, rows) (v) += __builtin_amdgcn_update_dpp(0, (v), ctrl, rows, 0xf, false)
 __device__ __forceinline__ int wave_upto(int v)
@@ -116,7 +143,8 @@ __device__ __forceinline__ int wave_upto(int v)
 #undef UPTO
 
 /* The sequence that holds chunk `number` of all row tiles' (or, with number < 0, row `token`), its plan, and the
- * chunks of the sequences before it; false: there is none. A lane a sequence, 64 at a time. */
+ * chunks of the sequences before it; false: there is none. A lane a sequence, 64 at a time. JOIN: after the launch of the chunks. */
+template <bool JOIN = false>
 __device__ __forceinline__ bool locate(const rt_seqs &b, const plan &p, int group, int number, long token, int &s, seq_plan &q, int &before, int &chunk)
 {
     before = 0;
@@ -131,14 +159,20 @@ __device__ __forceinline__ bool locate(const rt_seqs &b, const plan &p, int grou
     const seq_plan none = {0, 0, 0, 0, 0, 1};
     seq_plan at = lane < n ? plan_of(b, p, group, lane) : none;
     chunk = 0;
-    if (p.target > 0) {
+    if (JOIN && p.once) {
+        chunk = *p.size;
+    } else if (p.target > 0) {
         float all = (float)at.rows * (float)at.tiles;
         for (int s0 = 64; s0 < n; s0 += 64)
             if (s0 + lane < n) {
                 const seq_plan o = plan_of(b, p, group, s0 + lane);
                 all += (float)o.rows * (float)o.tiles;
             }
-        chunk = first_lane(chunk_from(p, q8_wave_sum_dpp(all)));
+        all = q8_wave_sum_dpp(all);
+        chunk = first_lane(p.once && n <= 64 && all < 1e8f ? chunk_of_rounds(p, all, [&](int c) { return (int)q8_wave_sum_dpp((float)(at.rows * chunks_of(at.tiles, c))); })
+                                                           : chunk_from(p, all));
+        if (!JOIN && p.once && number == 0 && threadIdx.x == 0)
+            *p.size = chunk; /* each head's first workgroup the same */
     }
     for (int s0 = 0; s0 < n; s0 += 64) {
         if (s0 > 0)

@@ -582,7 +582,7 @@ __global__ __launch_bounds__(256) void attn_join_k(rt_seqs b, rt_kv kv, rt_attn 
     const long i = blockIdx.x, h = blockIdx.y;
     int s, before, chunk;
     seq_plan q;
-    if (!locate(b, p, p.heads, -1, i, s, q, before, chunk) || q.chunks == 1)
+    if (!locate<true>(b, p, p.heads, -1, i, s, q, before, chunk) || q.chunks == 1)
         return;
     const int kh = (int)p.group.of((uint32_t)h), row = (int)(i - q.first) * p.heads + (int)h - kh * p.heads, rows = 1 << p.shift,
               z = q.rows - 1 - (row >> p.shift), r = row & (rows - 1);
@@ -638,7 +638,7 @@ __global__ __launch_bounds__(256) void attn_join_rows_k(rt_seqs b, rt_kv kv, rt_
 {
     int s, before, chunk, number = (int)blockIdx.x;
     seq_plan q;
-    if (!locate(b, p, p.heads, number, 0, s, q, before, chunk) || q.chunks == 1)
+    if (!locate<true>(b, p, p.heads, number, 0, s, q, before, chunk) || q.chunks == 1)
         return;
     const int at = number - before, z = at / q.chunks, part = at - z * q.chunks, rows = 1 << p.shift, first = (q.rows - 1 - z) << p.shift;
     if ((long)before + (long)(z + 1) * q.chunks > p.slots)
@@ -727,8 +727,10 @@ int shift_of(const rt_seqs &b, const rt_kv &kv, const rt_attn &a)
     return kv.type == RT_Q8 && b.longest * (a.q_heads / kv.heads) >= 64 && b.t * (a.q_heads / kv.heads) >= 32 * b.n ? 6 : 4;
 }
 
-void plan_chunks(const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long window, long sinks, long &tiles, long &target)
+/* The plan's target, and once (0: chunks of the target's size) */
+void plan_chunks(const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long window, long sinks, long &tiles, long &target, long &rounds)
 {
+    rounds = 0;
     const int shift = shift_of(b, kv, a);
     tiles = (b.t * (a.q_heads / kv.heads) >> shift) + b.n;
     const bool single = kv.type == RT_F32 ? kv.dim > 128 : kv.type == RT_Q8 ? shift == 4 && q8_attn8_alone(kv.dim) : alone(kv.dim);
@@ -738,24 +740,33 @@ void plan_chunks(const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long windo
         target = 0;
     else if (b.t >= 16 * b.n && tiles >= once)
         target = once;
-    else
+    else {
         target = (2 * tiles + once - 1) / once * once - tiles;
+        if (shift == 4 && b.n > 1 && (kv.type == RT_Q8 || cuts(kv, window, sinks))) {
+            /* (few row tiles fill one round evenly; every workgroup of a launch costs, also one without a chunk) */
+            if (tiles <= once) {
+                rounds = once;
+                target = (4 * tiles <= once ? 1 : 2) * once - tiles;
+            }
+        }
+    }
 }
 
 } /* namespace */
 
 long q8_attn_part_floats(const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long window, long sinks)
 {
-    long tiles, target;
-    plan_chunks(b, kv, a, window, sinks, tiles, target);
-    return target ? kv.heads * (target + tiles) * (kv.dim + 2) << shift_of(b, kv, a) : 0;
+    long tiles, target, rounds;
+    plan_chunks(b, kv, a, window, sinks, tiles, target, rounds);
+    return target ? (kv.heads * (target + tiles) * (kv.dim + 2) << shift_of(b, kv, a)) + 4 : 0;
 }
 
 void q8_launch_attn(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long window, long sinks, float *part)
 {
     plan p;
-    long tiles, target;
-    plan_chunks(b, kv, a, window, sinks, tiles, target);
+    long tiles, target, rounds;
+    plan_chunks(b, kv, a, window, sinks, tiles, target, rounds);
+    p.once = (int)rounds;
     p.target = (int)target;
     p.shift = shift_of(b, kv, a);
     p.tile = tile_of(kv);
@@ -774,6 +785,7 @@ void q8_launch_attn(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const
     p.sinks = p.window ? (int)sinks : 0;
     p.slots = (int)(target + (target ? tiles : 0));
     p.part = part;
+    p.size = (int *)(part + (kv.heads * p.slots * (kv.dim + 2) << p.shift)); /* behind the parts */
     p.qscale = (float)((double)a.scale * 1.4426950408889634074);
     const hipStream_t s = (hipStream_t)stream;
     const long n = p.target ? p.slots : p.shift == 6 || tiles < 1L << 20 ? tiles : 1L << 20;

@@ -67,7 +67,8 @@ __global__ __launch_bounds__(64 * WAVES, q8_attn8_alone(D) ? 1 : 2) void attn8_k
         if (!share_of<WINDOW>(b, kv, p, group, number, (int)blockIdx.y, u))
             return;
         const int stop = (u.t1 + SUB - 1) / SUB;
-        int tile = u.t0 / SUB + wave;
+        const int first = u.t0 / SUB + wave;
+        int tile = first;
         const auto here = [&](int t) { /* the lane's position of tile t, or the last that there is */
             const int i = place_of<WINDOW>(u, t, SUB) * POS + lane;
             return u.last < 0 ? 0 : i < u.last ? i : u.last;
@@ -75,14 +76,15 @@ __global__ __launch_bounds__(64 * WAVES, q8_attn8_alone(D) ? 1 : 2) void attn8_k
         uint4 kx[SUB][NK];
         float dk, dv; /* of the lane's position of the tile whose keys kx has */
         int entry;
+        bool none; /* the position has no row */
         /* rows of tile t from its entries, by way of LDS to the lanes that load them, and the next entries */
-        const auto load_keys = [&](int t) {
-            const int row = row_of(kv, p, here(t), entry);
-            sh.row[wave][lane] = row < 0 ? 0 : row;
-            const size_t at = (uint32_t)(row < 0 ? 0 : row) + head_rows;
-            dk = scale_k[at], dv = scale_v[at];
-            dk = row < 0 ? NAN : dk;
-            entry = entry_of(kv, p, u.table, here(t + WAVES));
+        const auto load_keys = [&](int t) __attribute__((always_inline)) {
+            const uint32_t pos = (uint32_t)here(t);
+            none = (uint32_t)entry >= (uint32_t)kv.pages;
+            const uint32_t row = none ? 0 : (uint32_t)entry * (uint32_t)(kv.heads * kv.page) + (pos - p.page.of(pos) * (uint32_t)kv.page);
+            sh.row[wave][lane] = (int)row;
+            dk = scale_k[row + head_rows], dv = scale_v[row + head_rows];
+            entry = u.table[p.page.of(here(t + WAVES))];
             __builtin_amdgcn_wave_barrier();
 #pragma unroll
             for (int n = 0; n < SUB; n++) {
@@ -92,7 +94,17 @@ __global__ __launch_bounds__(64 * WAVES, q8_attn8_alone(D) ? 1 : 2) void attn8_k
                     kx[n][i] = *(const uint4 *)(k + (64 * i + 16 * g < D ? 64 * i + 16 * g : 0));
             }
         };
-        entry = entry_of(kv, p, u.table, here(tile));
+        uint32_t vw[4 * SUB][VW]; /* rows 16 n + 4 g + r */
+        const auto load_values = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int n = 0; n < SUB; n++) {
+                const int4 rows = *(const int4 *)&sh.row[wave][16 * n + 4 * g];
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                    stream_words<VW>(vw[4 * n + r], address(kv.v, (&rows.x)[r], head_rows, D) + (c * VE < D ? c * VE : 0));
+            }
+        };
+        entry = u.table[p.page.of(here(tile))]; /* (the table reaches them all) */
         /* wave w has the queries' columns 64 i, i = w, w + WAVES, ..., and makes their bytes for all waves */
         static_assert(NK <= WAVES);
         const float *query = a.q + (u.live ? (long)(u.q.first + u.j) * a.q_ld + u.h * a.q_hd : 0);
@@ -103,6 +115,7 @@ __global__ __launch_bounds__(64 * WAVES, q8_attn8_alone(D) ? 1 : 2) void attn8_k
         for (int e = 0; e < 4; e++)
             qv[e] = *(const float4 *)(query + (mine ? 64 * wave + 16 * g : 0) + 4 * e);
         load_keys(tile);
+        load_values(); /* the first tile's with its keys */
 #pragma unroll
         for (int e = 0; e < 4; e++)
 #pragma unroll
@@ -144,17 +157,11 @@ __global__ __launch_bounds__(64 * WAVES, q8_attn8_alone(D) ? 1 : 2) void attn8_k
             acc[i] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         float m = -INFINITY, l = 0.0f;
         for (; tile < stop; tile += WAVES) {
-            sh.dk[wave][lane] = dk;
+            sh.dk[wave][lane] = none ? NAN : dk;
             sh.dv[wave][lane] = dv;
             __builtin_amdgcn_wave_barrier();
-            uint32_t vw[4 * SUB][VW]; /* rows 16 n + 4 g + r */
-#pragma unroll
-            for (int n = 0; n < SUB; n++) {
-                const int4 rows = *(const int4 *)&sh.row[wave][16 * n + 4 * g];
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                    stream_words<VW>(vw[4 * n + r], address(kv.v, (&rows.x)[r], head_rows, D) + (c * VE < D ? c * VE : 0));
-            }
+            if (tile != first)
+                load_values();
             v4i s[SUB][3];
 #pragma unroll
             for (int n = 0; n < SUB; n++)
@@ -543,64 +550,100 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn8_rows_k(rt_seqs b, rt_kv k
 
 /* ---- reading a cache back
  *
- * A thread has 8 neighbouring elements of a row: as many loads of whole lines as a wave can hold, one rounding to F32
- * (of 8 bits) and one to the rows' type. Bound by HBM on long ranges, by the table's latency on short ones. */
+ * A thread has 8 neighbouring elements of a row, of RUN tokens one behind the other, whose places and values are all under way at
+ * once; one rounding to F32 (of 8 bits) and one to the rows' type. Bound by HBM on long ranges, by latency (starts, positions, table,
+ * values) on short ones, for which RUN is 1. */
 template <int TYPE>
-__device__ __forceinline__ void load8(float (&x)[8], const void *cache, size_t row, long at, long dim, size_t all_rows)
+struct eight { /* 8 elements as they lie in the cache */
+    v4i w[TYPE == RT_F32 ? 2 : 1];
+    float d;
+};
+template <int TYPE>
+__device__ __forceinline__ eight<TYPE> load8(const void *cache, size_t row, long at, long dim, size_t all_rows)
 {
+    eight<TYPE> x;
     if constexpr (TYPE == RT_F32) {
-        const float4 lo = *(const float4 *)((const float *)cache + row * dim + at), hi = *(const float4 *)((const float *)cache + row * dim + at + 4);
-        *(float4 *)x = lo, *(float4 *)(x + 4) = hi;
+        x.w[0] = *(const v4i *)((const float *)cache + row * dim + at);
+        x.w[1] = *(const v4i *)((const float *)cache + row * dim + at + 4);
     } else if constexpr (TYPE == RT_Q8) {
-        const uint2 q = *(const uint2 *)((const char *)cache + row * dim + at);
-        const float d = ((const float *)((const char *)cache + all_rows * dim))[row];
-#pragma unroll
-        for (int e = 0; e < 8; e++)
-            x[e] = (float)(int8_t)((e < 4 ? q.x : q.y) >> (8 * (e % 4))) * d;
+        const int2 q = *(const int2 *)((const char *)cache + row * dim + at);
+        x.w[0][0] = q.x, x.w[0][1] = q.y;
+        x.d = ((const float *)((const char *)cache + all_rows * dim))[row];
     } else {
-        typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-        const uint4 w = *(const uint4 *)((const uint16_t *)cache + row * dim + at);
+        x.w[0] = *(const v4i *)((const uint16_t *)cache + row * dim + at);
+    }
+    return x;
+}
+template <int TYPE>
+__device__ __forceinline__ void values8(const eight<TYPE> &x, float (&v)[8])
+{
+    typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 #pragma unroll
-        for (int e = 0; e < 8; e++)
-            x[e] = TYPE == RT_F16 ? (float)__builtin_bit_cast(h8, w)[e] : (float)__builtin_bit_cast(b8, w)[e];
+    for (int e = 0; e < 8; e++) {
+        if constexpr (TYPE == RT_F32) {
+            const int word = x.w[e / 4][e % 4];
+            v[e] = __builtin_bit_cast(float, word);
+        } else if constexpr (TYPE == RT_Q8) {
+            const int word = x.w[0][e / 4];
+            v[e] = (float)(int8_t)(word >> (8 * (e % 4))) * x.d;
+        } else
+            v[e] = TYPE == RT_F16 ? (float)__builtin_bit_cast(h8, x.w[0])[e] : (float)__builtin_bit_cast(b8, x.w[0])[e];
     }
 }
 
-template <int TYPE>
+template <int TYPE, int RUN>
 __global__ __launch_bounds__(256) void read_k(rt_seqs b, rt_kv kv, rt_kv_rows a)
 {
-    const long i = blockIdx.x;
+    const long i0 = (long)blockIdx.x * RUN;
     const int d = (int)kv.dim, per = d / 8, n = 2 * (int)kv.heads * per;
-    const long s = q8_sequence_of(b, i);
-    if (s < 0)
-        return;
-    const long pos = (long)b.past[s] + (i - b.start[s]), slot = pos < 0 ? -1 : pos / kv.page;
-    const long entry = slot >= 0 && slot < kv.table_ld ? kv.table[s * kv.table_ld + slot] : -1;
-    const bool there = entry >= 0 && entry < kv.pages;
     const size_t all_rows = (size_t)(kv.pages * kv.heads * kv.page);
-    for (int k = (int)(blockIdx.y * 256 + threadIdx.x); k < n; k += 256 * (int)gridDim.y) {
+    long place[RUN]; /* of the token's first head in the cache; -1: it has none, -2: no sequence has the token */
+#pragma unroll
+    for (int k = 0; k < RUN; k++) {
+        const long s = i0 + k < b.t ? q8_sequence_of(b, i0 + k) : -1;
+        const long pos = s < 0 ? -1 : (long)b.past[s] + (i0 + k - b.start[s]), slot = (uint32_t)pos / (uint32_t)kv.page; /* below 2^32 */
+        const long entry = pos >= 0 && slot < kv.table_ld ? kv.table[s * kv.table_ld + slot] : -1;
+        place[k] = s < 0 ? -2 : entry >= 0 && entry < kv.pages ? entry * kv.heads * kv.page + (pos - slot * kv.page) : -1;
+    }
+    for (int k = (int)threadIdx.x; k < n; k += 256) {
         const int which = k >= n / 2, h = (k - which * (n / 2)) / per, at = 8 * ((k - which * (n / 2)) % per);
         void *out = which ? a.v : a.k;
         if (!out)
             continue;
-        float x[8];
-        if (there) {
-            load8<TYPE>(x, which ? kv.v : kv.k, (size_t)((entry * kv.heads + h) * kv.page + (pos - slot * kv.page)), at, d, all_rows);
-        } else {
+        eight<TYPE> x[RUN];
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                x[e] = NAN;
-        }
-        const long to = i * (which ? a.v_ld : a.k_ld) + h * (which ? a.v_hd : a.k_hd) + at;
-        if (a.type == RT_F32) {
-            *(float4 *)((float *)out + to) = *(float4 *)x, *(float4 *)((float *)out + to + 4) = *(float4 *)(x + 4);
-        } else if (a.type == RT_F16) {
-            typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-            *(h8 *)((_Float16 *)out + to) = h8{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3], (_Float16)x[4], (_Float16)x[5], (_Float16)x[6], (_Float16)x[7]};
-        } else {
-            *(b8 *)((__bf16 *)out + to) = b8{(__bf16)x[0], (__bf16)x[1], (__bf16)x[2], (__bf16)x[3], (__bf16)x[4], (__bf16)x[5], (__bf16)x[6], (__bf16)x[7]};
+        for (int r = 0; r < RUN; r++)
+            x[r] = load8<TYPE>(which ? kv.v : kv.k, (size_t)((place[r] < 0 ? 0 : place[r]) + h * kv.page), at, d, all_rows);
+#pragma unroll
+        for (int r = 0; r < RUN; r++) {
+            if (place[r] == -2)
+                continue;
+            float v[8];
+            values8<TYPE>(x[r], v);
+            if (place[r] < 0)
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    v[e] = NAN;
+            const long to = (i0 + r) * (which ? a.v_ld : a.k_ld) + h * (which ? a.v_hd : a.k_hd) + at;
+            if (a.type == RT_F32) {
+                *(v4f *)((float *)out + to) = v4f{v[0], v[1], v[2], v[3]}, *(v4f *)((float *)out + to + 4) = v4f{v[4], v[5], v[6], v[7]};
+            } else if (a.type == RT_F16) {
+                typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+                *(h8 *)((_Float16 *)out + to) = h8{(_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3], (_Float16)v[4], (_Float16)v[5], (_Float16)v[6], (_Float16)v[7]};
+            } else {
+                *(b8 *)((__bf16 *)out + to) = b8{(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3], (__bf16)v[4], (__bf16)v[5], (__bf16)v[6], (__bf16)v[7]};
+            }
         }
     }
+}
+
+template <int TYPE>
+void launch_read(hipStream_t s, const rt_seqs &b, const rt_kv &kv, const rt_kv_rows &a)
+{
+    if (b.t >= 4096)
+        read_k<TYPE, 4><<<(unsigned)((b.t + 3) / 4), 256, 0, s>>>(b, kv, a);
+    else
+        read_k<TYPE, 1><<<(unsigned)b.t, 256, 0, s>>>(b, kv, a);
 }
 
 } /* namespace */
@@ -635,14 +678,13 @@ void q8_launch_attn8(q8_stream_t stream, long blocks, const rt_seqs &b, const rt
 
 void q8_launch_kv_read(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const rt_kv_rows &a)
 {
-    const dim3 grid((unsigned)b.t);
     const hipStream_t s = (hipStream_t)stream;
     if (kv.type == RT_F32)
-        read_k<RT_F32><<<grid, 256, 0, s>>>(b, kv, a);
+        launch_read<RT_F32>(s, b, kv, a);
     else if (kv.type == RT_F16)
-        read_k<RT_F16><<<grid, 256, 0, s>>>(b, kv, a);
+        launch_read<RT_F16>(s, b, kv, a);
     else if (kv.type == RT_BF16)
-        read_k<RT_BF16><<<grid, 256, 0, s>>>(b, kv, a);
+        launch_read<RT_BF16>(s, b, kv, a);
     else
-        read_k<RT_Q8><<<grid, 256, 0, s>>>(b, kv, a);
+        launch_read<RT_Q8>(s, b, kv, a);
 }
