@@ -4,6 +4,7 @@
 #define Q8_ATTN_H
 
 #include "q8_mix.h"
+#include "q8_bf16.h"
 
 /* x / d for x < 2^31: (x * mul) >> shift with shift = 31 + ceil(log2 d), mul = ceil(2^shift / d): exact, as the
  * excess mul * d - 2^shift is below d <= 2^(shift - 31) */
@@ -35,13 +36,17 @@ struct q8_attn_plan {
 
 /* the 8-bit cache's kernel on `blocks` x heads workgroups */
 void q8_launch_attn8(q8_stream_t stream, long blocks, const rt_seqs &b, const rt_kv &kv, const rt_attn &a, const q8_attn_plan &p);
+/* the 16-bit caches' through a window, of many rows (p.shift 6) */
+void q8_launch_attn_rows(q8_stream_t stream, long blocks, const rt_seqs &b, const rt_kv &kv, const rt_attn &a, const q8_attn_plan &p);
 /* whether a compute unit holds one of its workgroups, not two */
 constexpr bool q8_attn8_alone(long dim) { return dim > 128; }
 
 namespace {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef int v4i __attribute__((ext_vector_type(4)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 
 constexpr int WAVES = 4;
 
@@ -453,6 +458,120 @@ __device__ __forceinline__ void finish(char *lds, const rt_kv &kv, const rt_attn
 
 /* The most elements (at most full) that a lane's VE elements of a V row divide into */
 constexpr int pieces(int ve, int full) { return ve % full == 0 ? full : ve % (full / 2) == 0 ? full / 2 : 2; }
+
+template <int TYPE>
+struct half_of;
+template <>
+struct half_of<RT_F16> {
+    static constexpr int LIMBS = 2;
+    static constexpr float SLACK = 1.0f, LIFT = 15.0f - SLACK, LEAST = 0x1p-5f;
+    static constexpr uint32_t INF = 0x7c00;
+    static __device__ __forceinline__ uint16_t round(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
+    static __device__ __forceinline__ float back(uint16_t x) { return (float)__builtin_bit_cast(_Float16, x); }
+    static __device__ __forceinline__ v4f mfma(uint4 x, uint4 y, v4f z) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, y), z, 0, 0, 0); }
+};
+template <>
+struct half_of<RT_BF16> {
+    static constexpr int LIMBS = 3;
+    static constexpr float SLACK = ::SLACK, LIFT = 0.0f, LEAST = 0.0f;
+    static constexpr uint32_t INF = 0x7f80;
+    static __device__ __forceinline__ uint16_t round(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
+    static __device__ __forceinline__ float back(uint16_t x) { return __builtin_bit_cast(float, (uint32_t)x << 16); }
+    static __device__ __forceinline__ v4f mfma(uint4 x, uint4 y, v4f z) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, x), __builtin_bit_cast(b8, y), z, 0, 0, 0); }
+};
+
+/* 8 F32 values as LIMBS operands */
+template <int TYPE>
+__device__ __forceinline__ void limbs_of(const float *x, uint4 *out)
+{
+    typedef half_of<TYPE> H;
+    float rest[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        rest[e] = x[e];
+#pragma unroll
+    for (int n = 0; n < H::LIMBS; n++) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+            const uint16_t lo = H::round(rest[e]), hi = H::round(rest[e + 1]);
+            w[e / 2] = lo | (uint32_t)hi << 16;
+            rest[e] -= H::back(lo);
+            rest[e + 1] -= H::back(hi);
+        }
+        out[n] = uint4{w[0], w[1], w[2], w[3]};
+    }
+}
+
+/* ---- what the kernels of prompts share: 64 query rows a workgroup on tiles of 64 positions in LDS */
+constexpr int ROWS = 64;
+
+/* A value's row in LDS (one element, 64 positions) is 8 pieces of 16 bytes, of which piece n lies at (n + spread) & 7 */
+__device__ __forceinline__ int spread(int d) { return (d >> 2) + 2 * (d & 3); }
+
+/* Which row tile (and chunk) of which key-value head a workgroup takes. Workgroups go to the 8 XCDs in turn, each with an L2 of its
+ * own, so a head's go to as few XCDs as there are for it, and an XCD's go through a head's row tiles in order: what they read together is
+ * a part of one head's cache. Two run on a compute unit: where all run at once, the second half of an XCD's goes from the
+ * shortest row tiles on, the first from the longest, so that the units have equal shares. */
+struct order {
+    int blocks, heads; /* row tiles or chunks a head; heads */
+    int each, count;   /* XCDs a head (0: several heads an XCD); workgroups an XCD */
+};
+order order_of(long blocks, long heads)
+{
+    order q = {(int)blocks, (int)heads, 0, 0};
+    if (heads < 8 && 8 % heads == 0)
+        q.each = (int)(8 / heads);
+    q.count = (int)(q.each ? (blocks + q.each - 1) / q.each : (heads * blocks + 7) / 8);
+    return q;
+}
+__device__ __forceinline__ bool place_in(const order &q, int block, int &number, int &head)
+{
+    const int xcd = block & 7;
+    int at = block >> 3;
+    constexpr int HALF = 32; /* compute units of an XCD */
+    if (q.count > HALF && q.count <= 2 * HALF + 2 && at >= HALF)
+        at = q.count - 1 - (at - HALF);
+    if (q.each) {
+        head = xcd / q.each;
+        number = at * q.each + xcd % q.each;
+    } else {
+        const int i = at * 8 + xcd; /* with a multiple of 8 heads each XCD has heads of its own */
+        if (q.heads % 8 == 0) {
+            head = at / q.blocks * 8 + xcd;
+            number = at % q.blocks;
+        } else {
+            head = i / q.blocks;
+            number = i % q.blocks;
+        }
+    }
+    return head < q.heads && number < q.blocks;
+}
+
+/* 1 / (1 + exp(-x)): the exponent in two parts, a reciprocal off by a step */
+__device__ __forceinline__ float gate_weight(float x)
+{
+    const float y = -fabsf(x), t = y * 1.44269504f, r = fmaf(y, 1.92596300e-8f, fmaf(y, 1.44269504f, -t)), e = __builtin_amdgcn_exp2f(t);
+    const float f = fmaf(e * r, 0.693147181f, e);
+    return (x >= 0.0f ? 1.0f : f) * __builtin_amdgcn_rcpf(1.0f + f);
+}
+
+/* 8 finite F32 values as three bf16 limbs, 8 bits each: exact */
+__device__ __forceinline__ void limbs8(const float *x, v4i (&w)[3])
+{
+    float mid[8], lo[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        mid[e] = x[e] - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x[e]) & 0xffff0000u);
+        lo[e] = mid[e] - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, mid[e]) & 0xffff0000u);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        w[0][e] = (int)pack_hi(x[2 * e], x[2 * e + 1]);
+        w[1][e] = (int)pack_hi(mid[2 * e], mid[2 * e + 1]);
+        w[2][e] = (int)pack_hi(lo[2 * e], lo[2 * e + 1]);
+    }
+}
 
 } /* namespace */
 

@@ -4,8 +4,6 @@
 
 namespace {
 
-typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-
 /* An F32 cache, 16 positions a tile, on v_mfma_f32_16x16x4_f32: position 4 g + r in the second product's step r. */
 template <int D, bool WINDOW>
 __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seqs b, rt_kv kv, rt_attn a, plan p)
@@ -150,50 +148,6 @@ __global__ __launch_bounds__(64 * WAVES, D > 128 ? 1 : 2) void attn_f32_k(rt_seq
  * and 459.
  * The queries' limbs stay in LDS for the four waves. The second product's first operand is V transposed: of a
  * lane's 8 rows, the same element of two at a time by v_perm_b32. */
-template <int TYPE>
-struct half_of;
-template <>
-struct half_of<RT_F16> {
-    static constexpr int LIMBS = 2;
-    static constexpr float SLACK = 1.0f, LIFT = 15.0f - SLACK, LEAST = 0x1p-5f;
-    static constexpr uint32_t INF = 0x7c00;
-    static __device__ __forceinline__ uint16_t round(float x) { return __builtin_bit_cast(uint16_t, (_Float16)x); }
-    static __device__ __forceinline__ float back(uint16_t x) { return (float)__builtin_bit_cast(_Float16, x); }
-    static __device__ __forceinline__ v4f mfma(uint4 x, uint4 y, v4f z) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, x), __builtin_bit_cast(h8, y), z, 0, 0, 0); }
-};
-template <>
-struct half_of<RT_BF16> {
-    static constexpr int LIMBS = 3;
-    static constexpr float SLACK = ::SLACK, LIFT = 0.0f, LEAST = 0.0f;
-    static constexpr uint32_t INF = 0x7f80;
-    static __device__ __forceinline__ uint16_t round(float x) { return __builtin_bit_cast(uint16_t, (__bf16)x); }
-    static __device__ __forceinline__ float back(uint16_t x) { return __builtin_bit_cast(float, (uint32_t)x << 16); }
-    static __device__ __forceinline__ v4f mfma(uint4 x, uint4 y, v4f z) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, x), __builtin_bit_cast(b8, y), z, 0, 0, 0); }
-};
-
-/* 8 F32 values as LIMBS operands */
-template <int TYPE>
-__device__ __forceinline__ void limbs_of(const float *x, uint4 *out)
-{
-    typedef half_of<TYPE> H;
-    float rest[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++)
-        rest[e] = x[e];
-#pragma unroll
-    for (int n = 0; n < H::LIMBS; n++) {
-        uint32_t w[4];
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-            const uint16_t lo = H::round(rest[e]), hi = H::round(rest[e + 1]);
-            w[e / 2] = lo | (uint32_t)hi << 16;
-            rest[e] -= H::back(lo);
-            rest[e + 1] -= H::back(hi);
-        }
-        out[n] = uint4{w[0], w[1], w[2], w[3]};
-    }
-}
-
 /* An infinite key is one in its product with the first limb; the others would make NaN of it (they
  * may be 0, or of the other sign), so where there may be one they get it as 0, and NaN, too. A value's weights are all
  * taken with this, and what it leaves out with 1 (where the weight is not 0): their first limb may be 0, too */
@@ -709,7 +663,7 @@ void launch(hipStream_t s, dim3 grid, const rt_seqs &b, const rt_kv &kv, const r
  * alone are more than SLOTS */
 constexpr long SLOTS = 4096;
 
-int tile_of(const rt_kv &kv) { return kv.type == RT_F32 ? 1 : kv.type == RT_Q8 ? 4 : sixteens(kv.dim); }
+int tile_of(const rt_kv &kv, int shift) { return kv.type == RT_F32 ? 1 : kv.type == RT_Q8 || shift == 6 ? 4 : sixteens(kv.dim); }
 
 /* The positions that the table reaches */
 long reach_of(const rt_kv &kv)
@@ -722,21 +676,21 @@ long reach_of(const rt_kv &kv)
 bool cuts(const rt_kv &kv, long window, long sinks) { return window > 0 && window < reach_of(kv) && sinks < reach_of(kv); }
 
 /* Row tiles of 64 (as a shift) from that many rows a sequence on, where a kernel has them */
-int shift_of(const rt_seqs &b, const rt_kv &kv, const rt_attn &a)
+int shift_of(const rt_seqs &b, const rt_kv &kv, const rt_attn &a, bool window)
 {
-    return kv.type == RT_Q8 && b.longest * (a.q_heads / kv.heads) >= 64 && b.t * (a.q_heads / kv.heads) >= 32 * b.n ? 6 : 4;
+    return (kv.type == RT_Q8 || (window && kv.type != RT_F32)) && b.longest * (a.q_heads / kv.heads) >= 64 && b.t * (a.q_heads / kv.heads) >= 32 * b.n ? 6 : 4;
 }
 
 /* The plan's target, and once (0: chunks of the target's size) */
 void plan_chunks(const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long window, long sinks, long &tiles, long &target, long &rounds)
 {
     rounds = 0;
-    const int shift = shift_of(b, kv, a);
+    const int shift = shift_of(b, kv, a, cuts(kv, window, sinks));
     tiles = (b.t * (a.q_heads / kv.heads) >> shift) + b.n;
-    const bool single = kv.type == RT_F32 ? kv.dim > 128 : kv.type == RT_Q8 ? shift == 4 && q8_attn8_alone(kv.dim) : alone(kv.dim);
+    const bool single = kv.type == RT_F32 ? kv.dim > 128 : kv.type == RT_Q8 ? shift == 4 && q8_attn8_alone(kv.dim) : shift == 6 ? kv.dim > 128 : alone(kv.dim);
     const long once = ((single ? 256 : 512) + kv.heads - 1) / kv.heads;
     const long most = reach_of(kv), seen = cuts(kv, window, sinks) && window + sinks + 16 < most ? window + sinks + 16 : most;
-    if (tiles * kv.heads > SLOTS || seen <= 16 * WAVES * tile_of(kv))
+    if (tiles * kv.heads > SLOTS || seen <= 16 * WAVES * tile_of(kv, shift))
         target = 0;
     else if (b.t >= 16 * b.n && tiles >= once)
         target = once;
@@ -758,7 +712,7 @@ long q8_attn_part_floats(const rt_seqs &b, const rt_kv &kv, const rt_attn &a, lo
 {
     long tiles, target, rounds;
     plan_chunks(b, kv, a, window, sinks, tiles, target, rounds);
-    return target ? (kv.heads * (target + tiles) * (kv.dim + 2) << shift_of(b, kv, a)) + 4 : 0;
+    return target ? (kv.heads * (target + tiles) * (kv.dim + 2) << shift_of(b, kv, a, cuts(kv, window, sinks))) + 4 : 0;
 }
 
 void q8_launch_attn(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long window, long sinks, float *part)
@@ -768,8 +722,8 @@ void q8_launch_attn(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const
     plan_chunks(b, kv, a, window, sinks, tiles, target, rounds);
     p.once = (int)rounds;
     p.target = (int)target;
-    p.shift = shift_of(b, kv, a);
-    p.tile = tile_of(kv);
+    p.shift = shift_of(b, kv, a, cuts(kv, window, sinks));
+    p.tile = tile_of(kv, p.shift);
     p.least = WAVES * p.tile;
     const auto by = [](long d) {
         int up = 0;
@@ -792,6 +746,8 @@ void q8_launch_attn(q8_stream_t stream, const rt_seqs &b, const rt_kv &kv, const
     const dim3 grid((unsigned)n, (unsigned)kv.heads);
     if (kv.type == RT_Q8)
         q8_launch_attn8(stream, n, b, kv, a, p);
+    else if (p.shift == 6)
+        q8_launch_attn_rows(stream, n, b, kv, a, p);
     else if (kv.type == RT_F32)
         p.window ? launch<RT_F32, true>(s, grid, b, kv, a, p) : launch<RT_F32, false>(s, grid, b, kv, a, p);
     else if (kv.type == RT_F16)

@@ -4,8 +4,6 @@
 
 namespace {
 
-typedef int v4i __attribute__((ext_vector_type(4)));
-
 /* A row of the cache is d * q, q in -127 .. 127 and d the F32 scale of that position and head. So
  *
  *   score = scale d_k (query . q_k)          o = sum_j (p_j d_v) q_v / sum_j p_j
@@ -67,8 +65,7 @@ __global__ __launch_bounds__(64 * WAVES, q8_attn8_alone(D) ? 1 : 2) void attn8_k
         if (!share_of<WINDOW>(b, kv, p, group, number, (int)blockIdx.y, u))
             return;
         const int stop = (u.t1 + SUB - 1) / SUB;
-        const int first = u.t0 / SUB + wave;
-        int tile = first;
+        int tile = u.t0 / SUB + wave;
         const auto here = [&](int t) { /* the lane's position of tile t, or the last that there is */
             const int i = place_of<WINDOW>(u, t, SUB) * POS + lane;
             return u.last < 0 ? 0 : i < u.last ? i : u.last;
@@ -115,7 +112,6 @@ __global__ __launch_bounds__(64 * WAVES, q8_attn8_alone(D) ? 1 : 2) void attn8_k
         for (int e = 0; e < 4; e++)
             qv[e] = *(const float4 *)(query + (mine ? 64 * wave + 16 * g : 0) + 4 * e);
         load_keys(tile);
-        load_values(); /* the first tile's with its keys */
 #pragma unroll
         for (int e = 0; e < 4; e++)
 #pragma unroll
@@ -160,8 +156,7 @@ __global__ __launch_bounds__(64 * WAVES, q8_attn8_alone(D) ? 1 : 2) void attn8_k
             sh.dk[wave][lane] = none ? NAN : dk;
             sh.dv[wave][lane] = dv;
             __builtin_amdgcn_wave_barrier();
-            if (tile != first)
-                load_values();
+            load_values();
             v4i s[SUB][3];
 #pragma unroll
             for (int n = 0; n < SUB; n++)
@@ -246,74 +241,6 @@ __global__ __launch_bounds__(64 * WAVES, q8_attn8_alone(D) ? 1 : 2) void attn8_k
  * LDS: the keys' rows are 16 bytes apart, which keeps 8 neighbouring rows off each other's banks; a value's row (one element, 64
  * positions) is 8 pieces of 16 bytes, of which piece n lies at (n + spread) & 7, so that neither 8 elements' pieces read together nor 8 lanes'
  * written together meet. */
-constexpr int ROWS = 64;
-
-__device__ __forceinline__ int spread(int d) { return (d >> 2) + 2 * (d & 3); }
-
-/* Which row tile (and chunk) of which key-value head a workgroup takes. Workgroups go to the 8 XCDs in turn, each with an L2 of its
- * own, so a head's go to as few XCDs as there are for it, and an XCD's go through a head's row tiles in order: what they read together is
- * a part of one head's cache. Two run on a compute unit: where all run at once, the second half of an XCD's goes from the
- * shortest row tiles on, the first from the longest, so that the units have equal shares. */
-struct order {
-    int blocks, heads; /* row tiles or chunks a head; heads */
-    int each, count;   /* XCDs a head (0: several heads an XCD); workgroups an XCD */
-};
-order order_of(long blocks, long heads)
-{
-    order q = {(int)blocks, (int)heads, 0, 0};
-    if (heads < 8 && 8 % heads == 0)
-        q.each = (int)(8 / heads);
-    q.count = (int)(q.each ? (blocks + q.each - 1) / q.each : (heads * blocks + 7) / 8);
-    return q;
-}
-__device__ __forceinline__ bool place_in(const order &q, int block, int &number, int &head)
-{
-    const int xcd = block & 7;
-    int at = block >> 3;
-    constexpr int HALF = 32; /* compute units of an XCD */
-    if (q.count > HALF && q.count <= 2 * HALF + 2 && at >= HALF)
-        at = q.count - 1 - (at - HALF);
-    if (q.each) {
-        head = xcd / q.each;
-        number = at * q.each + xcd % q.each;
-    } else {
-        const int i = at * 8 + xcd; /* with a multiple of 8 heads each XCD has heads of its own */
-        if (q.heads % 8 == 0) {
-            head = at / q.blocks * 8 + xcd;
-            number = at % q.blocks;
-        } else {
-            head = i / q.blocks;
-            number = i % q.blocks;
-        }
-    }
-    return head < q.heads && number < q.blocks;
-}
-
-/* 1 / (1 + exp(-x)): the exponent in two parts, a reciprocal off by a step */
-__device__ __forceinline__ float gate_weight(float x)
-{
-    const float y = -fabsf(x), t = y * 1.44269504f, r = fmaf(y, 1.92596300e-8f, fmaf(y, 1.44269504f, -t)), e = __builtin_amdgcn_exp2f(t);
-    const float f = fmaf(e * r, 0.693147181f, e);
-    return (x >= 0.0f ? 1.0f : f) * __builtin_amdgcn_rcpf(1.0f + f);
-}
-
-/* 8 finite F32 values as three bf16 limbs, 8 bits each: exact */
-__device__ __forceinline__ void limbs8(const float *x, v4i (&w)[3])
-{
-    float mid[8], lo[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        mid[e] = x[e] - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x[e]) & 0xffff0000u);
-        lo[e] = mid[e] - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, mid[e]) & 0xffff0000u);
-    }
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-        w[0][e] = (int)pack_hi(x[2 * e], x[2 * e + 1]);
-        w[1][e] = (int)pack_hi(mid[2 * e], mid[2 * e + 1]);
-        w[2][e] = (int)pack_hi(lo[2 * e], lo[2 * e + 1]);
-    }
-}
-
 template <int D, bool WINDOW>
 __global__ __launch_bounds__(64 * WAVES, 2) void attn8_rows_k(rt_seqs b, rt_kv kv, rt_attn a, plan p, order places)
 {
