@@ -219,21 +219,33 @@ __global__ __launch_bounds__(64 * WAVES, single<D> ? 1 : 2) void attn_rows_k(rt_
         const bool whole = all_seen<WINDOW>(p, u, base, POS); /* every row sees every position of the tile */
         float x[4 * SUB], top = -INFINITY;
         const auto key = [&](int n, int i) __attribute__((always_inline)) { return *(const uint4 *)&sh.k[16 * n + c][64 * i + 16 * g]; };
+        uint4 kk[2][NK]; /* the operands of the next 16 positions are read under this one's products */
+#pragma unroll
+        for (int i = 0; i < NK; i++)
+            kk[0][i] = key(0, i);
 #pragma unroll
         for (int n = 0; n < SUB; n++) {
-            uint4 kk[NK];
+            if (n + 1 < SUB)
 #pragma unroll
-            for (int i = 0; i < NK; i++)
-                kk[i] = key(n, i);
-            v4f s[2] = {v4f{0.0f, 0.0f, 0.0f, 0.0f}, v4f{0.0f, 0.0f, 0.0f, 0.0f}};
+                for (int i = 0; i < NK; i++)
+                    kk[(n + 1) & 1][i] = key(n + 1, i);
+            v4f s[LIMBS];
+#pragma unroll
+            for (int e = 0; e < LIMBS; e++)
+                s[e] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < NK; i++)
 #pragma unroll
                 for (int e = 0; e < LIMBS; e++)
-                    s[i & 1] = H::mfma(kk[i], __builtin_bit_cast(uint4, query[i][e]), s[i & 1]);
+                    s[e] = H::mfma(kk[n & 1][i], __builtin_bit_cast(uint4, query[i][e]), s[e]);
 #pragma unroll
-            for (int r = 0; r < 4; r++)
-                x[4 * n + r] = (s[0][r] + s[1][r]) * back;
+            for (int r = 0; r < 4; r++) {
+                float y = s[LIMBS - 1][r]; /* the smallest first */
+#pragma unroll
+                for (int e = LIMBS - 2; e >= 0; e--)
+                    y += s[e][r];
+                x[4 * n + r] = y * back;
+            }
         }
         if (lost)
 #pragma unroll
