@@ -675,10 +675,13 @@ long reach_of(const rt_kv &kv)
 /* A window that holds all positions is none */
 bool cuts(const rt_kv &kv, long window, long sinks) { return window > 0 && window < reach_of(kv) && sinks < reach_of(kv); }
 
-/* Row tiles of 64 (as a shift) from that many rows a sequence on, where a kernel has them */
+/* Row tiles of 64 (as a shift), where a kernel has them, from 64 rows of the longest sequence and 32 of each on (and as far as their
+ * workgroups are one launch) */
 int shift_of(const rt_seqs &b, const rt_kv &kv, const rt_attn &a, bool window)
 {
-    return (kv.type == RT_Q8 || (window && kv.type != RT_F32)) && b.longest * (a.q_heads / kv.heads) >= 64 && b.t * (a.q_heads / kv.heads) >= 32 * b.n ? 6 : 4;
+    const long group = a.q_heads / kv.heads;
+    const bool some = kv.type == RT_Q8 || (window && kv.type != RT_F32), many = b.longest * group >= 64 && b.t * group >= 32 * b.n;
+    return some && many && ((b.t * group >> 6) + b.n) * kv.heads < 1L << 23 ? 6 : 4;
 }
 
 /* The plan's target, and once (0: chunks of the target's size) */

@@ -445,6 +445,91 @@ def test_far_rows(rt, q8rt):
             assert (np.abs(d.get("o").reshape(n, hq, dim) - want) <= tol).all()
 
 
+MANY = [
+    # hq, hk, dim, page, positions a sequence, new tokens
+    (16, 4, 256, 16, [20000], [70]),  # a few row tiles on a long history: cut, and joined by rows
+    (8, 4, 128, 24, [9000, 40, 3000], [50, 40, 33]),
+    (6, 2, 96, 7, [5000], [43]),
+    (4, 1, 32, 64, [4000, 64], [64, 64]),
+    (16, 2, 224, 16, [1500, 900, 2], [40, 8, 2]),
+    (4, 2, 128, 16, list(range(1, 2000, 45)), [1] * 45),  # chunks by rounds, over one and two of them
+    (8, 8, 64, 16, [3000, 0, 17, 900, 2999, 64], [1, 0, 2, 1, 3, 1]),
+    (4, 1, 256, 16, [700] * 33, [1] * 33),
+    (2, 1, 128, 16, [37 * i % 1500 + 1 for i in range(150)], [1] * 150),  # more sequences than a wave has lanes
+    (8, 1, 64, 16, [60 + 5 * i for i in range(70)], [40 + i % 20 for i in range(70)]),
+    (16, 8, 64, 16, [1000], [1000]),  # several heads an XCD
+    (6, 3, 64, 16, [500, 700], [500, 90]),  # three heads, which 8 XCDs do not divide into
+]
+
+
+@pytest.mark.parametrize("kind,window,sinks", [("q8", None, 0), ("q8", 700, 5), ("bf16", 700, 5), ("f16", 1500, 33), ("f32", 300, 0), ("bf16", 5000, 0)])
+@pytest.mark.parametrize("hq,hk,dim,page,lens,news", MANY)
+def test_many_and_long(rt, q8rt, kind, window, sinks, hq, hk, dim, page, lens, news):
+    """Calls that are cut and joined in every way: row tiles of 64 on long histories, batches in one and two rounds of chunks,
+    more sequences than lanes, head counts that do and do not divide the XCDs."""
+    say("many and long", kind, window, sinks, hq, hk, dim, page, lens[:5], news[:5])
+    check_attn(rt, q8rt, kind, hq, hk, dim, page, lens, news, 0, window, sinks, (None,))
+
+
+@pytest.mark.parametrize("kind", ["q8", "bf16", "f16"])
+def test_the_same_bits_again(rt, q8rt, kind):
+    """A call's bits are the same every time, cut and joined or not."""
+    rng = np.random.default_rng(14)
+    hq, hk, dim = 8, 2, 128
+    for lens, news in (([9000], [60]), ([700, 3000, 90], [1, 1, 1]), ([1200], [1200])):
+        cache = paged(rng, kind, lens, hk, dim, 16)
+        q = rng.standard_normal((sum(news), hq, dim)).astype(F)
+        pasts = [a - b for a, b in zip(lens, news)]
+        first = run_attn(rt, q8rt, cache, q, starts(news), pasts, 0.1, 600, 4)
+        for _ in range(3):
+            assert np.array_equal(run_attn(rt, q8rt, cache, q, starts(news), pasts, 0.1, 600, 4).view(np.uint32), first.view(np.uint32))
+
+
+@pytest.mark.parametrize("kind", ["q8", "f32", "f16", "bf16"])
+@pytest.mark.parametrize("past,new", [(10 ** 9 + 7, 1), (10 ** 9 + 7, 5), (10 ** 9 + 7, 40), (2 ** 31 - 2 ** 21 - 100, 30)])
+def test_window_at_far_positions(rt, q8rt, kind, past, new):
+    """A thousand million positions behind the sequence's first, of which the pages of the window and the sinks are there."""
+    say("far", kind, past, new)
+    rng = np.random.default_rng(15)
+    hq, hk, dim, page, window, sinks = 4, 1, 32, 1 << 18, 100, 3
+    ld = (past + new) // page + 1
+    first = (past - window + 1) // page
+    table = np.full((1, ld), -1, np.int32)
+    table[0, first:], table[0, 0] = np.arange(ld - first) + 1, 0
+    pages = ld - first + 1
+    pos = np.r_[np.arange(sinks), np.arange(past - window + 1, past + new)]
+    rows = np.where(pos < sinks, pos, table[0, pos // page].astype(np.int64) * page + pos % page)
+    x = {n: rng.standard_normal((len(pos), dim)).astype(F) for n in "kv"}
+    held = {}
+    with Call(rt, q8rt) as d:
+        ptr = {}
+        for n in "kv":
+            if kind == "q8":
+                q, s = quantise(x[n])
+                held[n] = value(q, s)
+                mem = np.full(pages * page * (dim + 4), 0x7F, np.uint8)
+                mem[:pages * page * dim].reshape(-1, dim)[rows] = q.view(np.uint8)
+                mem[pages * page * dim:].view(F)[rows] = s
+            else:
+                raw = ref.to_cache(x[n], kind)
+                held[n] = ref.of_cache(raw, kind)
+                mem = ref.to_cache(np.full((pages * page, dim), np.nan), kind)
+                mem[rows] = raw
+            ptr[n] = d.put(mem)
+        q = rng.standard_normal((new, hq, dim)).astype(F)
+        s = d.seqs(starts([new]), [past])
+        kv = q8rt.Kv(k=ptr["k"], v=ptr["v"], type=q8rt.TYPES[kind], dim=dim, heads=hk, page=page, pages=pages, table=d.put(table), table_ld=ld)
+        a = q8rt.Attn(q=d.put(q), q_ld=hq * dim, q_hd=dim, q_heads=hq, scale=0.2, o=d.out("o", (new, hq * dim), F), o_ld=hq * dim)
+        rt.lib.rt_attn_window_dev(rt.R, c.byref(s), c.byref(kv), c.byref(a), window, sinks)
+        got = d.get("o").reshape(new, hq, dim)
+    for j in range(new):
+        at = (pos < sinks) | ((pos > past + j - window) & (pos <= past + j))
+        k, v = (np.concatenate([held[n][at][:, None], np.zeros((0, 1, dim))]) for n in "kv")
+        want, tol = ref8.attn(q[j:j + 1], [k], [v], 0.2, [0, 1], [int(at.sum()) - 1])
+        assert (np.abs(got[j] - want[0]) <= tol[0]).all(), j
+
+
+
 # ---- as a layer uses them
 
 
