@@ -219,34 +219,37 @@ __global__ __launch_bounds__(64 * WAVES, single<D> ? 1 : 2) void attn_rows_k(rt_
         const bool whole = all_seen<WINDOW>(p, u, base, POS); /* every row sees every position of the tile */
         float x[4 * SUB], top = -INFINITY;
         const auto key = [&](int n, int i) __attribute__((always_inline)) { return *(const uint4 *)&sh.k[16 * n + c][64 * i + 16 * g]; };
-        uint4 kk[2][NK]; /* the operands of the next 16 positions are read under this one's products */
-#pragma unroll
-        for (int i = 0; i < NK; i++)
-            kk[0][i] = key(0, i);
+        uint4 kk[2][SUB]; /* the next 32 elements' operands are read under these ones' products */
+        v4f s[SUB][LIMBS];
 #pragma unroll
         for (int n = 0; n < SUB; n++) {
-            if (n + 1 < SUB)
-#pragma unroll
-                for (int i = 0; i < NK; i++)
-                    kk[(n + 1) & 1][i] = key(n + 1, i);
-            v4f s[LIMBS];
+            kk[0][n] = key(n, 0);
 #pragma unroll
             for (int e = 0; e < LIMBS; e++)
-                s[e] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+                s[n][e] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        }
 #pragma unroll
-            for (int i = 0; i < NK; i++)
+        for (int i = 0; i < NK; i++) {
+            if (i + 1 < NK)
 #pragma unroll
-                for (int e = 0; e < LIMBS; e++)
-                    s[e] = H::mfma(kk[n & 1][i], __builtin_bit_cast(uint4, query[i][e]), s[e]);
+                for (int n = 0; n < SUB; n++)
+                    kk[(i + 1) & 1][n] = key(n, i + 1);
+#pragma unroll
+            for (int e = 0; e < LIMBS; e++)
+#pragma unroll
+                for (int n = 0; n < SUB; n++)
+                    s[n][e] = H::mfma(kk[i & 1][n], __builtin_bit_cast(uint4, query[i][e]), s[n][e]);
+        }
+#pragma unroll
+        for (int n = 0; n < SUB; n++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                float y = s[LIMBS - 1][r]; /* the smallest first */
+                float y = s[n][LIMBS - 1][r]; /* the smallest first */
 #pragma unroll
                 for (int e = LIMBS - 2; e >= 0; e--)
-                    y += s[e][r];
+                    y += s[n][e][r];
                 x[4 * n + r] = y * back;
             }
-        }
         if (lost)
 #pragma unroll
             for (int r = 0; r < 4 * SUB; r++)

@@ -627,3 +627,40 @@ def test_recorded_steps(rt, q8rt, kind):
             for x, y in zip(eager, (d.get(x) for x in ("o", "k", "ck", "cv"))):
                 assert np.array_equal(x.view(np.uint8), y.view(np.uint8))
         rt.lib.rt_graph_free(rt.R, c.c_void_p(graph))
+
+
+def test_two_runtimes(rt, q8rt):
+    """Calls of two runtimes on one cache, one behind the other without a wait between them, each with a workspace of its own:
+    each one's bits alone."""
+    rng = np.random.default_rng(16)
+    hq, hk, dim, lens = 8, 2, 128, [5000, 900]
+    cache = Paged8(rng, lens, hk, dim, 16)
+    other = q8rt.Runtime()
+    try:
+        with Call(rt, q8rt) as d:
+            kv = cache.struct(d)
+            calls = []
+            for r, news, window in ((rt, [1, 1], 800), (other, [70, 30], 300), (rt, [40, 200], 2000), (other, [2, 1], 4000)):
+                s = d.seqs(starts(news), [a - b for a, b in zip(lens, news)])
+                q = d.put(rng.standard_normal((sum(news), hq, dim)).astype(F))
+                name = f"o{len(calls)}"
+                a = q8rt.Attn(q=q, q_ld=hq * dim, q_hd=dim, q_heads=hq, scale=0.1, o=d.out(name, (sum(news), hq * dim), F), o_ld=hq * dim)
+                calls.append((r, s, a, window, name))
+
+            def run(r, s, a, window, name):
+                r.lib.rt_attn_window_dev(r.R, c.byref(s), c.byref(kv), c.byref(a), window, 4)
+
+            alone = []
+            for call in calls:
+                run(*call)
+                call[0].sync()
+                alone.append(d.get(call[4]))
+            for _ in range(5):
+                for call in calls:
+                    run(*call)
+                rt.sync()
+                other.sync()
+                for call, x in zip(calls, alone):
+                    assert np.array_equal(d.get(call[4]).view(np.uint32), x.view(np.uint32))
+    finally:
+        other.close()
