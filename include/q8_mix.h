@@ -16,7 +16,7 @@
  * a state (s_out may be s_in) and a rotation in place.
  *
  * The workspace (the delta rule's for runs of tokens, the attention's) grows to what a call needs, or to twice what it
- * was, not while a graph is recorded: run a call with the same n, t and longest (and cache and heads) once before. All
+ * was, not while a graph is recorded: run a call with the same n, t and longest (and cache, heads and window) once before. All
  * of a runtime's calls share it, in the order of its stream; one that was replaced is freed by rt_fini. */
 #ifndef Q8_MIX_H
 #define Q8_MIX_H
@@ -86,8 +86,9 @@ void rt_delta_rule_dev(struct rt *R, const struct rt_seqs *s, const struct rt_de
  * table[s * table_ld + p / page], row p % page.
  *
  * RT_Q8 holds a row (a position's head) as dim int8 values q and one F32 scale d, of which an element is q * d: k and v are the
- * values [pages][heads][page][dim] with the scales [pages][heads][page] right behind them. Each row has a scale of its own, so that
- * appending changes no row that is there: a cache is the same however its tokens came. */
+ * values [pages][heads][page][dim] with the scales [pages][heads][page] right behind them (4-byte aligned, whatever page is). A scale
+ * is 0 or more and finite; a row whose scale is NaN reads as NaN. Each row has a scale of its own, so that appending changes no row
+ * that is there: a cache is the same however its tokens came, one by one or as a prompt, drafts taken back or not. */
 #define RT_F32 0
 #define RT_F16 1
 #define RT_BF16 2
@@ -144,7 +145,8 @@ void rt_kv_read_dev(struct rt *R, const struct rt_seqs *s, const struct rt_kv *k
 /* o = softmax(scale q K^T) V over the cache: the token at position p sees positions 0 .. p of its sequence
  * (its own and earlier new ones included: append them first), query head h the key-value head
  * h / (q_heads / heads). Times 1 / (1 + exp(-gate)), where given. For a few new tokens on a cache of any
- * length the positions are split over the GPU and joined; a prompt's tokens go 16 rows (token, head) at a time.
+ * length the positions are split over the GPU and joined; a prompt's tokens go 16 rows (token, head) at a time, 64 over
+ * RT_Q8. There a query is held in 24 bits of its row's largest element; everything else is as exact as F32 sums.
  * A token that sees nothing (a position before 0) gives zeros; one that would have to see a position behind
  * the table's last page, or in a page that the cache does not have, gives NaN. */
 struct rt_attn {
@@ -159,8 +161,10 @@ struct rt_attn {
 void rt_attn_kv_dev(struct rt *R, const struct rt_seqs *s, const struct rt_kv *kv, const struct rt_attn *a);
 
 /* The same through a sliding window: the token at position p sees the positions j <= p with j > p - window, and those with
- * j < sinks, which stay visible. window 1 or more, sinks 0 or more; the time goes by what is seen. Pages of which no new token sees anything may be gone: the table's
- * entries for them may be anything, and their positions' values too. */
+ * j < sinks, which stay visible. window 1 or more, sinks 0 or more; the time goes by what is seen. Pages of which no new token sees
+ * anything may be gone: the table's entries for them may be anything, and so may what lies at positions that no new token sees.
+ * (Over F16 and BF16 caches a prompt's rows that see infinities or NaN are computed apart, one by one, and slowly: 50 times where
+ * all do.) */
 void rt_attn_window_dev(struct rt *R, const struct rt_seqs *s, const struct rt_kv *kv, const struct rt_attn *a, long window, long sinks);
 
 #ifdef __cplusplus

@@ -1,6 +1,5 @@
 /* q8_attn8.hip: attention of new tokens over the paged key-value cache of 8 bits, and reading a cache back (include/q8_mix.h). */
 #include "q8_attn.h"
-#include "q8_bf16.h"
 
 namespace {
 
@@ -19,7 +18,9 @@ namespace {
  *
  * A wave takes 64 positions at a time, one a lane for the page table and the scales, which go through LDS to where the
  * products have them. Otherwise as the 16-bit caches' kernel: scores S^T = K Q^T leave lane 16 g + c with positions
- * 16 n + 4 g + r of query row c, which is how the second product's operand has them. */
+ * 16 n + 4 g + r of query row c, which is how the second product's operand has them. Bound by HBM on long histories (32 sequences of
+ * 100 to 16384 positions, 4 heads of 256: 107 us, 5.3 TB/s; 4 tokens at 131072 positions 49, 5.5 TB/s), by the latency of its dependent loads
+ * on short ones. The first values under way with the first keys measured 4 us slower on the former: the keys come later. */
 constexpr int SUB = 4, POS = 64;
 constexpr float FULL = 8355584.0f; /* 2^23 - 2^15: 127.99 * 2^16, and what the rounding of the quotient adds, in balanced bytes */
 
@@ -42,6 +43,7 @@ __device__ __forceinline__ float joined(int l0, int l1, int l2) { return fmaf((f
 /* Elements of a V row that a lane has: the largest of 4, 8 and 16 that 16 lanes cover the row with; with heads that are no
  * power of two the last lanes have none */
 constexpr int each(int d) { return d <= 64 ? 4 : d <= 128 ? 8 : 16; }
+
 template <int D, bool WINDOW>
 __global__ __launch_bounds__(64 * WAVES, q8_attn8_alone(D) ? 1 : 2) void attn8_k(rt_seqs b, rt_kv kv, rt_attn a, plan p)
 {
@@ -135,7 +137,7 @@ __global__ __launch_bounds__(64 * WAVES, q8_attn8_alone(D) ? 1 : 2) void attn8_k
             const uint32_t o = __builtin_bit_cast(uint32_t, sh.most[w][c]);
             most = most > o ? most : o;
         }
-        const float top_query = fmaxf(__builtin_bit_cast(float, most), 1e-30f); /* below that: the products are below 1e-26 d_k */
+        const float top_query = fmaxf(__builtin_bit_cast(float, most), 1e-30f); /* smaller rows: in steps of 1e-37 */
         const float up = FULL / top_query, back = most < 0x7f800000u ? top_query / FULL : NAN;
         if (wave < NK) {
             uint32_t w[4][3];
@@ -237,6 +239,12 @@ __global__ __launch_bounds__(64 * WAVES, q8_attn8_alone(D) ? 1 : 2) void attn8_k
  * transposed, in the order in which the second product's operand has the positions. So a key or value is loaded, and a value
  * converted, once for 64 rows and not for 16. The next tile's loads are under way in registers while the products of this one
  * run, and two workgroups share a compute unit, so that one's softmax and staging go under the other's matrix instructions.
+ *
+ * Heads of 256, 16 on 4: a prompt of 2048 112 us (16 rows a workgroup, as single tokens go: 299, the join's 95 among them); 8192
+ * tokens through 1024 positions 355 (1075). A wave's tile is 144 matrix instructions, 2304 cycles, and some 550 others (queries and gates
+ * among them), 2200, of 5100 that it takes of its SIMD: between two matrix instructions two others go unnoticed, the third costs,
+ * so the issue of both bounds it. Tried and not faster: 32 rows a wave on the 32x32 instructions, one wave a SIMD (213 and 530); tiles of 32 positions in double buffers with one
+ * barrier and the next scores beside this softmax (115 and 379); 128 rows a workgroup (141 and 356).
  *
  * LDS: the keys' rows are 16 bytes apart, which keeps 8 neighbouring rows off each other's banks; a value's row (one element, 64
  * positions) is 8 pieces of 16 bytes, of which piece n lies at (n + spread) & 7, so that neither 8 elements' pieces read together nor 8 lanes'
@@ -478,8 +486,9 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn8_rows_k(rt_seqs b, rt_kv k
 /* ---- reading a cache back
  *
  * A thread has 8 neighbouring elements of a row, of RUN tokens one behind the other, whose places and values are all under way at
- * once; one rounding to F32 (of 8 bits) and one to the rows' type. Bound by HBM on long ranges, by latency (starts, positions, table,
- * values) on short ones, for which RUN is 1. */
+ * once; one rounding to F32 (of 8 bits) and one to the rows' type. Bound by HBM on long ranges (32767 positions of 4 heads of 256 to
+ * BF16 49 us, 4.1 TB/s; a token a workgroup 64, two 56, eight 54), by latency (starts, positions, table, values) on short ones, for
+ * which RUN is 1. */
 template <int TYPE>
 struct eight { /* 8 elements as they lie in the cache */
     v4i w[TYPE == RT_F32 ? 2 : 1];

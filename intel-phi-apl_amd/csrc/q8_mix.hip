@@ -99,7 +99,8 @@ __device__ __forceinline__ void store4(void *cache, long at, float4 v)
 
 /* A row of 8 bits: d = max|x| / 127 over the lanes that hold it, x as rint(x / d), which is within 127 (max / d is off by
  * less than a step of 127). A row with an element that is not finite gets NaN for d, so that it reads as NaN, and one whose d has no
- * full precision (below 2^-126) zeros. The scales lie behind all rows. */
+ * full precision (below 2^-126) zeros. The scales lie behind all rows. The quotients are F32's own, so that a row's bits are those of
+ * the definition (reciprocals: 2 us of 61 in a prompt of 3936 tokens, 24 heads of 256). */
 __device__ __forceinline__ void store_q8(const rt_kv &kv, void *cache, long row, int at, int lanes, bool live, float4 x)
 {
     const auto bits = [](float v) { return __builtin_bit_cast(uint32_t, fabsf(v)); };
