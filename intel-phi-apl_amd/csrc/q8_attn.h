@@ -38,6 +38,8 @@ struct q8_attn_plan {
 void q8_launch_attn8(q8_stream_t stream, long blocks, const rt_seqs &b, const rt_kv &kv, const rt_attn &a, const q8_attn_plan &p);
 /* the 16-bit caches' through a window, of many rows (p.shift 6) */
 void q8_launch_attn_rows(q8_stream_t stream, long blocks, const rt_seqs &b, const rt_kv &kv, const rt_attn &a, const q8_attn_plan &p);
+/* 16s of positions that it takes at once */
+constexpr int q8_attn_rows_tile(long dim) { return dim > 128 ? 2 : 4; }
 /* whether a compute unit holds one of its workgroups, not two */
 constexpr bool q8_attn8_alone(long dim) { return dim > 128; }
 
@@ -361,6 +363,9 @@ __device__ __forceinline__ bool share_of(const rt_seqs &b, const rt_kv &kv, cons
     }
     if (q.chunks > 1 && u.t0 + chunk < u.t1)
         u.t1 = u.t0 + chunk;
+    if constexpr (ROWS != 16) /* a wave's, not a lane's: in scalar registers */
+        for (int *v : {&u.last, &u.least, &u.end, &u.t0, &u.t1, &u.lo0, &u.lo1, &u.sunk, &u.skip})
+            *v = first_lane(*v);
     return true;
 }
 

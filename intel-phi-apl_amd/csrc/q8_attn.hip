@@ -663,7 +663,7 @@ void launch(hipStream_t s, dim3 grid, const rt_seqs &b, const rt_kv &kv, const r
  * alone are more than SLOTS */
 constexpr long SLOTS = 4096;
 
-int tile_of(const rt_kv &kv, int shift) { return kv.type == RT_F32 ? 1 : kv.type == RT_Q8 || shift == 6 ? 4 : sixteens(kv.dim); }
+int tile_of(const rt_kv &kv, int shift) { return kv.type == RT_F32 ? 1 : kv.type == RT_Q8 ? 4 : shift == 6 ? q8_attn_rows_tile(kv.dim) : sixteens(kv.dim); }
 
 /* The positions that the table reaches */
 long reach_of(const rt_kv &kv)
@@ -690,7 +690,7 @@ void plan_chunks(const rt_seqs &b, const rt_kv &kv, const rt_attn &a, long windo
     rounds = 0;
     const int shift = shift_of(b, kv, a, cuts(kv, window, sinks));
     tiles = (b.t * (a.q_heads / kv.heads) >> shift) + b.n;
-    const bool single = kv.type == RT_F32 ? kv.dim > 128 : kv.type == RT_Q8 ? shift == 4 && q8_attn8_alone(kv.dim) : shift == 6 ? kv.dim > 128 : alone(kv.dim);
+    const bool single = kv.type == RT_F32 ? kv.dim > 128 : kv.type == RT_Q8 ? shift == 4 && q8_attn8_alone(kv.dim) : shift == 4 && alone(kv.dim);
     const long once = ((single ? 256 : 512) + kv.heads - 1) / kv.heads;
     const long most = reach_of(kv), seen = cuts(kv, window, sinks) && window + sinks + 16 < most ? window + sinks + 16 : most;
     if (tiles * kv.heads > SLOTS || seen <= 16 * WAVES * tile_of(kv, shift))

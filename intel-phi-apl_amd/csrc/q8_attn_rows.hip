@@ -3,19 +3,22 @@
 
 namespace {
 
-/* As the 8-bit cache's prompts: 64 query rows a workgroup, 16 a wave, which share a tile of 64 positions in LDS, the keys as they
+/* As the 8-bit cache's prompts: 64 query rows a workgroup, 16 a wave, which share a tile of positions in LDS, the keys as they
  * lie and the values transposed, the next tile's loads under way in registers. The products are those of the 16-bit caches: the
  * queries as LIMBS 16-bit values each, in registers. The weights are three bf16 limbs here, which hold any F32 weight, so that none
  * is too small; a BF16 value is their operand as it is, an F16 one is the sum of two (its upper 8 bits, and the 3 that
- * are left, which the third limb need not meet: 2^-24 of the product). With heads of more than 128 a wave's registers are one wave
- * a SIMD (two, with what does not fit spilled, take 1.5 times as long), whose products, softmax and waits stand one behind the
- * other: prompts of 4001 tokens and less through 512 positions, 8 heads on 2 of 256, BF16, 204 us; 394 with 16 rows a workgroup.
+ * are left, which the third limb need not meet: 2^-24 of the product).
+ *
+ * A wave of 256 elements has 64 registers of output and 96 of queries. With tiles of 32 positions the rest of a tile fits beside
+ * them for two waves a SIMD, one of which multiplies while the other waits or is in its softmax: prompts of 4001 tokens and
+ * less through 512 positions, 8 heads on 2 of 256, BF16, 142 us, 204 with 64 positions and one wave; 394 with 16 rows a workgroup. With
+ * nothing spilled, that is: who waits for a reload waits for the next tile's loads, which were issued before it (45 registers: 193 us). Heads of up to 128 have room for 64 positions. The limbs' products go to one sum, as
+ * three would be 16 registers more; two LDS buffers with one barrier a tile measured the same, and so did layouts with a fifth of
+ * the bank conflicts (which are a third of LDS's time).
  *
  * Infinities and NaN in a key or a value make a product with a limb or a weight of 0 NaN where the definition has none. So a
  * wave whose sums are not all finite at the end computes its rows again, one by one and in F32, without what a row does not
  * see (50 times slower, where all do). Positions that none of the workgroup's rows sees are 0 in LDS, whatever lies there. */
-template <int D>
-constexpr bool single = D > 128;
 
 template <int D, int TYPE>
 __device__ __forceinline__ float element(const void *cache, uint64_t row, int d)
@@ -27,15 +30,16 @@ __device__ __forceinline__ float element(const void *cache, uint64_t row, int d)
 template <int D, int TYPE, bool WINDOW>
 __device__ __forceinline__ void slowly(const rt_kv &kv, const rt_attn &a, const plan &p, const share &u, uint32_t head_rows, int i, float &m, float &l, float (&o)[(D + 63) / 64])
 {
+    constexpr int SUB = q8_attn_rows_tile(D);
     const int lane = threadIdx.x & 63, j = __shfl(u.j, i, 64), head = __shfl(u.h, i, 64), lim = __shfl(u.lim, i, 64), low = WINDOW ? __shfl(u.low, i, 64) : 0;
     const float *q = a.q + (long)(u.q.first + j) * a.q_ld + head * a.q_hd;
     m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int n = 0; n < (D + 63) / 64; n++)
         o[n] = 0.0f;
-    for (int tile = u.t0 / 4; tile < (u.t1 + 3) / 4; tile++) {
-        const int pos = place_of<WINDOW>(u, tile, 4) * 64 + lane;
-        const bool seen = pos <= lim && !passed<WINDOW>(p, pos, low);
+    for (int tile = u.t0 / SUB; tile < (u.t1 + SUB - 1) / SUB; tile++) {
+        const int pos = place_of<WINDOW>(u, tile, SUB) * 16 * SUB + lane;
+        const bool seen = lane < 16 * SUB && pos <= lim && !passed<WINDOW>(p, pos, low);
         const int entry = seen ? u.table[p.page.of(pos)] : 0;
         const bool there = (uint32_t)entry < (uint32_t)kv.pages;
         const uint32_t row = (seen && there ? (uint32_t)entry * (uint32_t)(kv.heads * kv.page) + ((uint32_t)pos - p.page.of(pos) * (uint32_t)kv.page) : 0) + head_rows;
@@ -69,16 +73,22 @@ __device__ __forceinline__ void slowly(const rt_kv &kv, const rt_attn &a, const 
 }
 
 template <int D, int TYPE, bool WINDOW>
-__global__ __launch_bounds__(64 * WAVES, single<D> ? 1 : 2) void attn_rows_k(rt_seqs b, rt_kv kv, rt_attn a, plan p, order places)
+__global__ __launch_bounds__(64 * WAVES, 2) void attn_rows_k(rt_seqs b, rt_kv kv, rt_attn a, plan p, order places)
 {
     typedef half_of<TYPE> H;
-    constexpr int SUB = 4, POS = 64, LIMBS = H::LIMBS, NK = D / 32, VE = D / 16, PIECES = D / 8, NP = POS * PIECES / 256, EACH = D > 128 ? 4 : D > 64 ? 2 : 1;
+    constexpr int SUB = q8_attn_rows_tile(D), POS = 16 * SUB, LIMBS = H::LIMBS, NK = D / 32, VE = D / 16, PIECES = D / 8, NP = (POS * PIECES + 255) / 256, FOURTH = 17 * D / 16 + 1, EACH = D > 128 ? 4 : D > 64 ? 2 : 1;
     constexpr int PARTS = TYPE == RT_F16 ? 2 : 1; /* bf16 values that a value is the sum of */
     struct shared {
         uint8_t k[POS][2 * D + 16];
-        v4i v[PARTS][D][8];
+        v4i v[PARTS][SUB == 4 ? 8 * D : 4 * FOURTH];
     };
     __shared__ __align__(16) shared sh;
+    /* Positions 8 n .. 8 n + 7 of element d, so that neither 16 lanes' reads (of d, d + 1, ..) nor their writes (of d, d + 4, ..) meet in a
+     * bank. With 4 pieces an element: every fourth element's in a row, 16 bytes between each 4, which takes no register for
+     * the next elements' places. */
+    const auto value = [&](int part, int d, int n) __attribute__((always_inline)) -> v4i & {
+        return sh.v[part][SUB == 4 ? 8 * d + ((n + spread(d)) & 7) : (d & 3) * FOURTH + 4 * (d >> 2) + (d >> 4) + n];
+    };
     const int tid = threadIdx.x, lane = tid & 63, wave = first_lane(tid >> 6), c = lane & 15, g = lane >> 4;
     const int group = p.heads;
     int number, head;
@@ -97,7 +107,7 @@ __global__ __launch_bounds__(64 * WAVES, single<D> ? 1 : 2) void attn_rows_k(rt_
     };
     int entry = u.table[p.page.of(here(tile))]; /* (the table reaches them all) */
     v4i kx[NP];
-    uint32_t vx[16][EACH > 2 ? 2 : 1];
+    uint32_t vx[4 * SUB][EACH > 2 ? 2 : 1];
     bool none = false, gone = false; /* the lane's position of the tile has no row; no row of the workgroup sees it */
     const auto load = [&](int t) __attribute__((always_inline)) {
         const uint32_t pos = (uint32_t)here(t);
@@ -110,7 +120,7 @@ __global__ __launch_bounds__(64 * WAVES, single<D> ? 1 : 2) void attn_rows_k(rt_
         for (int i = 0; i < NP; i++)
             rows[i] = (uint32_t)__shfl((int)place, (tid + 256 * i) / PIECES, 64);
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
+        for (int i = 0; i < 4 * SUB; i++) {
             /* positions 16 n + 4 g + r: g the wave's number, i = 4 n + r */
             const char *v = (const char *)kv.v + (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)place, i / 4 * 16 + 4 * wave + i % 4) * (2 * D);
             const uint32_t off = lane * EACH < D ? lane * EACH * 2 : 0;
@@ -130,20 +140,20 @@ __global__ __launch_bounds__(64 * WAVES, single<D> ? 1 : 2) void attn_rows_k(rt_
         missing = __ballot(none && !gone);
         if (__ballot(gone))
 #pragma unroll
-            for (int i = 0; i < 16; i++)
+            for (int i = 0; i < 4 * SUB; i++)
                 if (__builtin_amdgcn_readlane(gone ? 1 : 0, i / 4 * 16 + 4 * wave + i % 4))
 #pragma unroll
                     for (int e = 0; e < (EACH > 2 ? 2 : 1); e++)
                         vx[i][e] = 0;
 #pragma unroll
         for (int i = 0; i < NP; i++)
-            *(v4i *)&sh.k[(tid + 256 * i) / PIECES][(tid + 256 * i) % PIECES * 16] = kx[i];
+            if (POS * PIECES % 256 == 0 || tid + 256 * i < POS * PIECES)
+                *(v4i *)&sh.k[(tid + 256 * i) / PIECES][(tid + 256 * i) % PIECES * 16] = kx[i];
         if (D % (64 * EACH) == 0 || lane * EACH < D)
 #pragma unroll
             for (int e = 0; e < EACH; e++)
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const int d = lane * EACH + e;
+                for (int k = 0; k < SUB / 2; k++) {
                     v4i w[PARTS];
 #pragma unroll
                     for (int r = 0; r < 8; r += 2) {
@@ -159,7 +169,7 @@ __global__ __launch_bounds__(64 * WAVES, single<D> ? 1 : 2) void attn_rows_k(rt_
                     }
 #pragma unroll
                     for (int n = 0; n < PARTS; n++)
-                        sh.v[n][d][(4 * k + wave + spread(d)) & 7] = w[n];
+                        value(n, lane * EACH + e, 4 * k + wave) = w[n];
                 }
     };
     if (tile < stop)
@@ -222,13 +232,11 @@ __global__ __launch_bounds__(64 * WAVES, single<D> ? 1 : 2) void attn_rows_k(rt_
         float x[4 * SUB], top = -INFINITY;
         const auto key = [&](int n, int i) __attribute__((always_inline)) { return *(const uint4 *)&sh.k[16 * n + c][64 * i + 16 * g]; };
         uint4 kk[2][SUB]; /* the next 32 elements' operands are read under these ones' products */
-        v4f s[SUB][LIMBS];
+        v4f s[SUB];
 #pragma unroll
         for (int n = 0; n < SUB; n++) {
             kk[0][n] = key(n, 0);
-#pragma unroll
-            for (int e = 0; e < LIMBS; e++)
-                s[n][e] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            s[n] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
         }
 #pragma unroll
         for (int i = 0; i < NK; i++) {
@@ -237,25 +245,20 @@ __global__ __launch_bounds__(64 * WAVES, single<D> ? 1 : 2) void attn_rows_k(rt_
                 for (int n = 0; n < SUB; n++)
                     kk[(i + 1) & 1][n] = key(n, i + 1);
 #pragma unroll
-            for (int e = 0; e < LIMBS; e++)
+            for (int e = LIMBS - 1; e >= 0; e--) /* the smallest first */
 #pragma unroll
                 for (int n = 0; n < SUB; n++)
-                    s[n][e] = H::mfma(kk[i & 1][n], __builtin_bit_cast(uint4, query[i][e]), s[n][e]);
+                    s[n] = H::mfma(kk[i & 1][n], __builtin_bit_cast(uint4, query[i][e]), s[n]);
         }
 #pragma unroll
         for (int n = 0; n < SUB; n++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                float y = s[n][LIMBS - 1][r]; /* the smallest first */
-#pragma unroll
-                for (int e = LIMBS - 2; e >= 0; e--)
-                    y += s[n][e][r];
-                x[4 * n + r] = y * back;
-            }
+            for (int r = 0; r < 4; r++)
+                x[4 * n + r] = s[n][r] * back;
         if (lost)
 #pragma unroll
             for (int r = 0; r < 4 * SUB; r++)
-                x[r] = lost >> (r / 4 * 16 + 4 * g + r % 4) & 1 ? NAN : x[r];
+                x[r] = (uint32_t)(lost >> (r / 8 * 32)) >> 4 * g & 1u << (r / 4 % 2 * 16 + r % 4) ? NAN : x[r];
         if (!whole)
 #pragma unroll
             for (int r = 0; r < 4 * SUB; r++) {
@@ -275,26 +278,21 @@ __global__ __launch_bounds__(64 * WAVES, single<D> ? 1 : 2) void attn_rows_k(rt_
         for (int k = 0; k < SUB / 2; k++) {
             v4i w[3];
             limbs8(x + 8 * k, w);
-            v4i v[2][PARTS][2];
-            const auto values = [&](int e) __attribute__((always_inline)) {
+#pragma unroll
+            for (int e = 0; e < VE; e += 2) {
+                v4i v[PARTS][2];
 #pragma unroll
                 for (int n = 0; n < PARTS; n++)
 #pragma unroll
                     for (int f = 0; f < 2; f++)
-                        v[e / 2 & 1][n][f] = sh.v[n][16 * (e + f) + c][(4 * k + g + 4 * (e + f) + spread(c)) & 7];
-            };
-            values(0);
-#pragma unroll
-            for (int e = 0; e < VE; e += 2) {
-                if (e + 2 < VE)
-                    values(e + 2);
+                        v[n][f] = value(n, 16 * (e + f) + c, 4 * k + g);
 #pragma unroll
                 for (int n = 0; n < PARTS; n++)
 #pragma unroll
                     for (int i = 0; i < 3 - n; i++)
 #pragma unroll
                         for (int f = 0; f < 2; f++)
-                            acc[e + f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, v[e / 2 & 1][n][f]), __builtin_bit_cast(b8, w[i]), acc[e + f], 0, 0, 0);
+                            acc[e + f] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, v[n][f]), __builtin_bit_cast(b8, w[i]), acc[e + f], 0, 0, 0);
             }
         }
     }
