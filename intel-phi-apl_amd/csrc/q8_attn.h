@@ -363,9 +363,13 @@ __device__ __forceinline__ bool share_of(const rt_seqs &b, const rt_kv &kv, cons
     }
     if (q.chunks > 1 && u.t0 + chunk < u.t1)
         u.t1 = u.t0 + chunk;
-    if constexpr (ROWS != 16) /* a wave's, not a lane's: in scalar registers */
-        for (int *v : {&u.last, &u.least, &u.end, &u.t0, &u.t1, &u.lo0, &u.lo1, &u.sunk, &u.skip})
+    if constexpr (ROWS != 16) { /* a wave's, not a lane's: in scalar registers */
+        for (int *v : {&u.last, &u.least, &u.end, &u.t0, &u.t1})
             *v = first_lane(*v);
+        if constexpr (WINDOW)
+            for (int *v : {&u.lo0, &u.lo1, &u.sunk, &u.skip})
+                *v = first_lane(*v);
+    }
     return true;
 }
 

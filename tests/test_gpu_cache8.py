@@ -256,6 +256,15 @@ def test_window_prompts(rt, q8rt, kind, window, sinks, hq, hk, dim, page, lens, 
     check_attn(rt, q8rt, kind, hq, hk, dim, page, lens, news, first, window, sinks, (None,))
 
 
+@pytest.mark.parametrize("kind", ["q8", "f16", "bf16"])
+@pytest.mark.parametrize("window,sinks", [(33, 1), (96, 31), (200, 40)])
+@pytest.mark.parametrize("dim", range(32, 257, 32))
+def test_window_prompts_of_every_head_size(rt, q8rt, kind, window, sinks, dim):
+    """The kernels of many rows at each size of a head: their threads' shares of a tile are odd at some."""
+    say("window", kind, window, sinks, dim)
+    check_attn(rt, q8rt, kind, 8, 2, dim, 9, [430, 150, 77], [390, 77, 77], 0, window, sinks, (None,))
+
+
 @pytest.mark.parametrize("kind", ["q8", "f32", "f16", "bf16"])
 def test_window_of_everything(rt, q8rt, kind):
     """A window or sinks as long as the table, or the longest there are, are no window: the bits of the call without."""
@@ -301,11 +310,11 @@ def test_window_pages_that_are_gone(rt, q8rt, kind, hq, hk, dim, page, lens, new
 
 @pytest.mark.parametrize("kind", ["q8", "f32", "f16", "bf16"])
 @pytest.mark.parametrize("lens,news,window,sinks", [([2100], [70], 40, 3), ([90], [90], 9, 0), ([40], [6], 5, 2)])
-def test_window_masked_places(rt, q8rt, kind, lens, news, window, sinks):
+def test_window_masked_places(rt, q8rt, kind, lens, news, window, sinks, dim=64):
     """NaN and infinities in a key and in values that some tokens of a tile see and others do not: in the rows that see
     them as the definition has it, in no other."""
     rng = np.random.default_rng(7)
-    hq, hk, dim, n, new = 4, 2, 64, lens[0], news[0]
+    hq, hk, n, new = 4, 2, lens[0], news[0]
     k, v = (rng.standard_normal((n, hk, dim)) for _ in range(2))
     if kind == "q8":
         k[n - 3, 0, 5], v[n - new + 2, 1, 3], v[sinks, 0, 1] = np.nan, np.inf, np.nan  # a row's scale: all of its elements
@@ -320,6 +329,16 @@ def test_window_masked_places(rt, q8rt, kind, lens, news, window, sinks):
     assert fine.any() and not fine.all()
     assert (np.abs(got - want)[fine] <= tol[fine]).all()
     assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
+
+
+@pytest.mark.parametrize("kind", ["q8", "f16", "bf16"])
+@pytest.mark.parametrize("dim", [160, 224, 256])
+def test_window_prompts_of_large_heads_over_what_is_not_there(rt, q8rt, kind, dim):
+    """The two tests above for the kernels of many rows on heads of more than 128, whose tiles are shorter."""
+    for page, lens, news, window, sinks in [(5, [600, 90], [120, 80], 70, 3), (64, [3000], [150], 200, 0), (24, [400], [60], 33, 40)]:
+        test_window_pages_that_are_gone(rt, q8rt, kind, 8, 2, dim, page, lens, news, window, sinks)
+    for lens, news, window, sinks in [([2100], [70], 40, 3), ([90], [90], 9, 0), ([700], [300], 65, 30)]:
+        test_window_masked_places(rt, q8rt, kind, lens, news, window, sinks, dim)
 
 
 @pytest.mark.parametrize("kind", ["q8", "f32", "f16", "bf16"])
