@@ -30,16 +30,17 @@ __device__ __forceinline__ float element(const void *cache, uint64_t row, int d)
 template <int D, int TYPE, bool WINDOW>
 __device__ __forceinline__ void slowly(const rt_kv &kv, const rt_attn &a, const plan &p, const share &u, uint32_t head_rows, int i, float &m, float &l, float (&o)[(D + 63) / 64])
 {
-    constexpr int SUB = q8_attn_rows_tile(D);
+    constexpr int SUB = q8_attn_rows_tile(D), POS = 16 * SUB;
     const int lane = threadIdx.x & 63, j = __shfl(u.j, i, 64), head = __shfl(u.h, i, 64), lim = __shfl(u.lim, i, 64), low = WINDOW ? __shfl(u.low, i, 64) : 0;
     const float *q = a.q + (long)(u.q.first + j) * a.q_ld + head * a.q_hd;
     m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int n = 0; n < (D + 63) / 64; n++)
         o[n] = 0.0f;
-    for (int tile = u.t0 / SUB; tile < (u.t1 + SUB - 1) / SUB; tile++) {
-        const int pos = place_of<WINDOW>(u, tile, SUB) * 16 * SUB + lane;
-        const bool seen = lane < 16 * SUB && pos <= lim && !passed<WINDOW>(p, pos, low);
+    const int stop = (u.t1 + SUB - 1) / SUB;
+    for (int first = u.t0 / SUB; first < stop; first += 64 / POS) {
+        const int tile = first + lane / POS, pos = place_of<WINDOW>(u, tile, SUB) * POS + lane % POS;
+        const bool seen = tile < stop && pos <= lim && !passed<WINDOW>(p, pos, low);
         const int entry = seen ? u.table[p.page.of(pos)] : 0;
         const bool there = (uint32_t)entry < (uint32_t)kv.pages;
         const uint32_t row = (seen && there ? (uint32_t)entry * (uint32_t)(kv.heads * kv.page) + ((uint32_t)pos - p.page.of(pos) * (uint32_t)kv.page) : 0) + head_rows;
