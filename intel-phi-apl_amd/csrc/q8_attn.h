@@ -560,10 +560,11 @@ __device__ __forceinline__ bool place_in(const order &q, int block, int &number,
     return head < q.heads && number < q.blocks;
 }
 
-/* 1 / (1 + exp(-x)): the exponent in two parts, a reciprocal off by a step */
+/* 1 / (1 + exp(-x)): the exponent in two parts, a reciprocal off by a step. An exponential below 2^-126 is 0, and so it is from |x| =
+ * 104 on, infinity among them, where neither part could be made of x itself; NaN stays NaN */
 __device__ __forceinline__ float gate_weight(float x)
 {
-    const float y = -fabsf(x), t = y * 1.44269504f, r = fmaf(y, 1.92596300e-8f, fmaf(y, 1.44269504f, -t)), e = __builtin_amdgcn_exp2f(t);
+    const float y = fabsf(x) > 104.0f ? -104.0f : -fabsf(x), t = y * 1.44269504f, r = fmaf(y, 1.92596300e-8f, fmaf(y, 1.44269504f, -t)), e = __builtin_amdgcn_exp2f(t);
     const float f = fmaf(e * r, 0.693147181f, e);
     return (x >= 0.0f ? 1.0f : f) * __builtin_amdgcn_rcpf(1.0f + f);
 }
