@@ -400,7 +400,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn8_rows_k(rt_seqs b, rt_kv k
 #pragma unroll
                 for (int i = 0; i < NK; i++)
                     kk[(n + 1) & 1][i] = key(n + 1, i);
-            const v4f d = *(const v4f *)&sh.scale[0][16 * n + 4 * g];
+            const v4f d = *(const v4f *)&sh.scale[0][16 * n + 4 * g] * back; /* first: the sums times a large scale may overflow */
             v4i s[3] = {v4i{0, 0, 0, 0}, v4i{0, 0, 0, 0}, v4i{0, 0, 0, 0}};
 #pragma unroll
             for (int i = 0; i < NK; i++)
@@ -409,7 +409,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn8_rows_k(rt_seqs b, rt_kv k
                     s[e] = __builtin_amdgcn_mfma_i32_16x16x64_i8(kk[n & 1][i], query[i][e], s[e], 0, 0, 0);
 #pragma unroll
             for (int r = 0; r < 4; r++)
-                x[4 * n + r] = joined(s[0][r], s[1][r], s[2][r]) * d[r]; /* over back */
+                x[4 * n + r] = joined(s[0][r], s[1][r], s[2][r]) * d[r];
         }
         if (!whole)
 #pragma unroll
@@ -418,13 +418,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn8_rows_k(rt_seqs b, rt_kv k
 #pragma unroll
         for (int r = 0; r < 4 * SUB; r++)
             top = fmaxf(top, x[r]);
-        const float ref = reference(top * back, SLACK, m, l, acc) + SLACK;
+        const float ref = reference(top, SLACK, m, l, acc) + SLACK;
 #pragma unroll
         for (int n = 0; n < SUB; n++) {
             const v4f d = *(const v4f *)&sh.scale[1][16 * n + 4 * g];
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                const float weight = __builtin_amdgcn_exp2f(fmaf(x[4 * n + r], back, -ref));
+                const float weight = __builtin_amdgcn_exp2f(x[4 * n + r] - ref);
                 l += weight;
                 x[4 * n + r] = weight * d[r];
             }

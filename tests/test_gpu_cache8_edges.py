@@ -41,3 +41,46 @@ def test_gates_far_from_0(rt, q8rt, kind, dim, lens, news, window, sinks):
     there = ~np.isnan(want)
     assert (np.abs(got - want)[there] <= tol[there]).all()
     assert (got[gate < -150] == 0).all()
+
+
+@pytest.mark.parametrize("what", ["far keys", "huge", "tiny", "inf", "nan", "values", "small values", "spike", "zero"])
+@pytest.mark.parametrize("new,window,sinks", [(5, None, 0), (90, None, 0), (90, 70, 3)])
+def test_range_of_queries_and_scales(rt, q8rt, what, new, window, sinks):
+    """Single rows and prompts alike: scores that are ordinary numbers though keys are near 2^103 and queries near 2^-97, or the other
+    way round; queries of zeros, not finite, with one element above all others; values' scales from 2^-100 to 2^100, or near 2^-105.
+
+    Far below 1 a weight's product with its value's scale d has few bits left. The weights are taken 2^-8 to 1 for the largest, so
+    that they add up to 2^-8 at least; one below 2^-126 is 0, and a product is held to 2^-133, the least step of the bf16 limbs. So a
+    position adds up to 127 (2^-126 d + 2^-133) / 2^-8, which is below 2^-118 (127 d + 1), whatever the kernel."""
+    say("range", what, new, window, sinks)
+    rng = np.random.default_rng(17)
+    hq, hk, dim, n = 4, 2, 64, 300
+    k, v = (rng.standard_normal((n, hk, dim)) for _ in range(2))
+    q = rng.standard_normal((new, hq, dim))
+    if what == "far keys":
+        q, k = q * 2.0 ** -97, k * 2.0 ** 103  # scores of some 60 either way
+    elif what == "huge":
+        q, k = q * 2.0 ** 100, k * 2.0 ** -100
+    elif what == "tiny":
+        q, k = q * 2.0 ** -60, k * 2.0 ** 60
+    elif what in ("inf", "nan"):
+        q[new // 2, 1, 3] = float(what)
+    elif what == "values":
+        v *= 2.0 ** rng.integers(-100, 100, (n, hk, 1))
+    elif what == "small values":
+        v *= 2.0 ** -100
+    elif what == "spike":
+        q[..., 7] = 300.0
+        k[..., 7] *= 0.01
+    else:
+        q[:] = 0
+    cache = paged(rng, "q8", [n], hk, dim, 16, k=[k], v=[v])
+    q = q.astype(F)
+    want, tol = ref8.attn(q, cache.seq_k, cache.seq_v, 0.125, starts([new]), [n - new], window or 0, sinks)
+    tol += 2.0 ** -118 * n * (1 + np.abs(cache.seq_v[0]).max())
+    got = run_attn(rt, q8rt, cache, q, starts([new]), [n - new], 0.125, window, sinks)[:, :hq * dim].reshape(new, hq, dim)
+    if what in ("inf", "nan"):
+        at = new // 2, 1
+        assert np.isnan(got[at]).all()
+        want[at], got[at], tol[at] = 0, 0, 0
+    assert (np.abs(got - want) <= tol).all()
