@@ -522,9 +522,9 @@ __device__ __forceinline__ int spread(int d) { return (d >> 2) + 2 * (d & 3); }
 
 /* Which row tile (and chunk) of which key-value head a workgroup takes. Workgroups go to the 8 XCDs in turn, each with an L2 of its
  * own, so a head's go to as few XCDs as there are for it, and an XCD's go through a head's row tiles in order: what they read together is
- * a part of one head's cache. Two run on a compute unit, an XCD's n-th and (n + 32)-th: where all run at once, the second half of an
- * XCD's goes from the shortest row tiles on, the first from the longest, so that the units have equal shares. (A prompt of 2048
- * tokens 114 us, 152 in the grid's order.) */
+ * a part of one head's cache. (A prompt of 2048 tokens 114 us, 152 in the grid's order. Left out: the second 32 of an XCD's, which share
+ * the compute units with the first, from the shortest row tiles on: 850 tokens 59 us, 60 as it is; 1400 through a window of 1024 96, 95 as
+ * it is.) */
 struct order {
     int blocks, heads; /* row tiles or chunks a head; heads */
     int each, count;   /* XCDs a head (0: several heads an XCD); workgroups an XCD */
@@ -540,10 +540,7 @@ order order_of(long blocks, long heads)
 __device__ __forceinline__ bool place_in(const order &q, int block, int &number, int &head)
 {
     const int xcd = block & 7;
-    int at = block >> 3;
-    constexpr int HALF = 32; /* compute units of an XCD */
-    if (q.count > HALF && q.count <= 2 * HALF + 2 && at >= HALF)
-        at = q.count - 1 - (at - HALF);
+    const int at = block >> 3;
     if (q.each) {
         head = xcd / q.each;
         number = at * q.each + xcd % q.each;
