@@ -27,11 +27,11 @@ __device__ __forceinline__ float element(const void *cache, uint64_t row, int d)
 }
 
 /* Row `i` of the wave's again: its maximum and sum, and element lane + 64 n of its output in o[n] */
-template <int D, int TYPE, bool WINDOW>
+template <int D, int TYPE>
 __device__ __forceinline__ void slowly(const rt_kv &kv, const rt_attn &a, const plan &p, const share &u, uint32_t head_rows, int i, float &m, float &l, float (&o)[(D + 63) / 64])
 {
     constexpr int SUB = q8_attn_rows_tile(D), POS = 16 * SUB;
-    const int lane = threadIdx.x & 63, j = __shfl(u.j, i, 64), head = __shfl(u.h, i, 64), lim = __shfl(u.lim, i, 64), low = WINDOW ? __shfl(u.low, i, 64) : 0;
+    const int lane = threadIdx.x & 63, j = __shfl(u.j, i, 64), head = __shfl(u.h, i, 64), lim = __shfl(u.lim, i, 64), low = __shfl(u.low, i, 64);
     const float *q = a.q + (long)(u.q.first + j) * a.q_ld + head * a.q_hd;
     m = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -39,8 +39,8 @@ __device__ __forceinline__ void slowly(const rt_kv &kv, const rt_attn &a, const 
         o[n] = 0.0f;
     const int stop = (u.t1 + SUB - 1) / SUB;
     for (int first = u.t0 / SUB; first < stop; first += 64 / POS) {
-        const int tile = first + lane / POS, pos = place_of<WINDOW>(u, tile, SUB) * POS + lane % POS;
-        const bool seen = tile < stop && pos <= lim && !passed<WINDOW>(p, pos, low);
+        const int tile = first + lane / POS, pos = place_of<true>(u, tile, SUB) * POS + lane % POS;
+        const bool seen = tile < stop && pos <= lim && !passed<true>(p, pos, low);
         const int entry = seen ? u.table[p.page.of(pos)] : 0;
         const bool there = (uint32_t)entry < (uint32_t)kv.pages;
         const uint32_t row = (seen && there ? (uint32_t)entry * (uint32_t)(kv.heads * kv.page) + ((uint32_t)pos - p.page.of(pos) * (uint32_t)kv.page) : 0) + head_rows;
@@ -73,7 +73,7 @@ __device__ __forceinline__ void slowly(const rt_kv &kv, const rt_attn &a, const 
     }
 }
 
-template <int D, int TYPE, bool WINDOW>
+template <int D, int TYPE>
 __global__ __launch_bounds__(64 * WAVES, 2) void attn_rows_k(rt_seqs b, rt_kv kv, rt_attn a, plan p, order places)
 {
     typedef half_of<TYPE> H;
@@ -97,13 +97,13 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn_rows_k(rt_seqs b, rt_kv kv
         return;
     const uint32_t head_rows = (uint32_t)head * (uint32_t)kv.page;
     share u;
-    if (!share_of<WINDOW, ROWS>(b, kv, p, group, number, head, u))
+    if (!share_of<true, ROWS>(b, kv, p, group, number, head, u))
         return;
     const int stop = (u.t1 + SUB - 1) / SUB;
     int tile = u.t0 / SUB;
-    const int least = WINDOW ? window_from(p, u.q, first_lane((int)p.group.of(u.z * ROWS))) : 0; /* the first that any row's window has */
+    const int least = window_from(p, u.q, first_lane((int)p.group.of(u.z * ROWS))); /* the first that any row's window has */
     const auto here = [&](int t) __attribute__((always_inline)) { /* the lane's position of tile t, or the last that there is */
-        const int i = place_of<WINDOW>(u, t, SUB) * POS + lane;
+        const int i = place_of<true>(u, t, SUB) * POS + lane;
         return u.end < 0 ? 0 : i < u.end ? i : u.end;
     };
     int entry = u.table[p.page.of(here(tile))]; /* (the table reaches them all) */
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn_rows_k(rt_seqs b, rt_kv kv
     const auto load = [&](int t) __attribute__((always_inline)) {
         const uint32_t pos = (uint32_t)here(t);
         none = (uint32_t)entry >= (uint32_t)kv.pages;
-        gone = passed<WINDOW>(p, (int)pos, least);
+        gone = passed<true>(p, (int)pos, least);
         const uint32_t place = (none ? 0 : (uint32_t)entry * (uint32_t)(kv.heads * kv.page) + (pos - p.page.of(pos) * (uint32_t)kv.page)) + head_rows; /* below 2^31 */
         entry = u.table[p.page.of(here(t + 1))];
         uint32_t rows[NP];
@@ -225,11 +225,11 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn_rows_k(rt_seqs b, rt_kv kv
         const unsigned long long lost = missing;
         if (tile + 1 < stop)
             load(tile + 1);
-        const int base = place_of<WINDOW>(u, tile, SUB) * POS;
+        const int base = place_of<true>(u, tile, SUB) * POS;
         /* none of the wave's rows sees any of it */
-        if (!some || base > u.last || (WINDOW && base + POS <= u.lo0 && base >= p.sinks))
+        if (!some || base > u.last || (base + POS <= u.lo0 && base >= p.sinks))
             continue;
-        const bool whole = all_seen<WINDOW>(p, u, base, POS); /* every row sees every position of the tile */
+        const bool whole = all_seen<true>(p, u, base, POS); /* every row sees every position of the tile */
         float x[4 * SUB], top = -INFINITY;
         const auto key = [&](int n, int i) __attribute__((always_inline)) { return *(const uint4 *)&sh.k[16 * n + c][64 * i + 16 * g]; };
         uint4 kk[2][SUB]; /* the next 32 elements' operands are read under these ones' products */
@@ -264,7 +264,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn_rows_k(rt_seqs b, rt_kv kv
 #pragma unroll
             for (int r = 0; r < 4 * SUB; r++) {
                 const int i = base + r / 4 * 16 + 4 * g + r % 4;
-                x[r] = i > u.lim || passed<WINDOW>(p, i, u.low) ? -INFINITY : x[r];
+                x[r] = i > u.lim || passed<true>(p, i, u.low) ? -INFINITY : x[r];
             }
 #pragma unroll
         for (int r = 0; r < 4 * SUB; r++)
@@ -308,7 +308,7 @@ __global__ __launch_bounds__(64 * WAVES, 2) void attn_rows_k(rt_seqs b, rt_kv kv
     if (__ballot(u.live && odd != 0.0f)) { /* something is infinite or NaN */
         for (int i = 0; i < 16 && u.row + i < u.q.n * group; i++) {
             float o[(D + 63) / 64];
-            slowly<D, TYPE, WINDOW>(kv, a, p, u, head_rows, i, m, l, o);
+            slowly<D, TYPE>(kv, a, p, u, head_rows, i, m, l, o);
             const int j = __shfl(u.j, i, 64), h = __shfl(u.h, i, 64);
             const long token = u.q.first + j, pos = (long)u.q.past + j;
             l = pos >= p.cap ? NAN : l;
@@ -367,8 +367,8 @@ void q8_launch_attn_rows(q8_stream_t stream, long blocks, const rt_seqs &b, cons
     switch (kv.dim) {
 #define DIM(D)                                                                                                                                             \
     case D:                                                                                                                                                \
-        kv.type == RT_F16 ? attn_rows_k<D, RT_F16, true><<<all, 64 * WAVES, 0, (hipStream_t)stream>>>(b, kv, a, p, places)                                 \
-                          : attn_rows_k<D, RT_BF16, true><<<all, 64 * WAVES, 0, (hipStream_t)stream>>>(b, kv, a, p, places);                               \
+        kv.type == RT_F16 ? attn_rows_k<D, RT_F16><<<all, 64 * WAVES, 0, (hipStream_t)stream>>>(b, kv, a, p, places)                                       \
+                          : attn_rows_k<D, RT_BF16><<<all, 64 * WAVES, 0, (hipStream_t)stream>>>(b, kv, a, p, places);                                     \
         break;
         DIM(32)
         DIM(64)
