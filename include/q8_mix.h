@@ -16,7 +16,7 @@
  * a state (s_out may be s_in) and a rotation in place.
  *
  * The workspace (the delta rule's for runs of tokens, the attention's) grows to what a call needs, or to twice what it
- * was, not while a graph is recorded: run a call with the same n, t and longest (and cache, heads and window) once before. All
+ * was, not while a graph is recorded: run a call with the same n, t and longest (and cache, heads, window and sinks) once before. All
  * of a runtime's calls share it, in the order of its stream; one that was replaced is freed by rt_fini. */
 #ifndef Q8_MIX_H
 #define Q8_MIX_H
@@ -39,7 +39,7 @@ struct rt_seqs {
                        * chooses kernels and grids. Sequences with more are computed all the same, slower */
     const int *start; /* device [n + 1] */
     const int *past;  /* device [n]: sequence s's tokens are at positions past[s], past[s] + 1, ...
-                       * (rt_rope_kv_dev, rt_attn_kv_dev; else unused) */
+                       * (rt_rope_kv_dev, rt_kv_read_dev, rt_attn_kv_dev, rt_attn_window_dev; else unused) */
 };
 
 /* y[i] = SiLU(sum_j w[c][j] u[i - taps + 1 + j]) per channel c and token i of a sequence, u the
@@ -131,7 +131,7 @@ void rt_rope_kv_dev(struct rt *R, const struct rt_seqs *s, const struct rt_kv *k
 
 /* Rows of the cache: K and V of the positions past[s], past[s] + 1, ... as rows start[s] .. of k and v (either may be NULL:
  * not read), head h at k_hd * h, from any type of cache to F32, F16 or BF16 (8-bit values q * d rounded to F32, then to the rows'
- * type). Strides in elements, multiples of 8 for 16-bit rows. A position before 0, behind the table's last page, or in a page that the
+ * type). Strides in elements, multiples of 8 for 16-bit rows; k's rows, from the first to the last, lie apart from v's. A position before 0, behind the table's last page, or in a page that the
  * cache does not have reads as NaN. */
 struct rt_kv_rows {
     long type; /* RT_F32, RT_F16 or RT_BF16 */
@@ -146,7 +146,9 @@ void rt_kv_read_dev(struct rt *R, const struct rt_seqs *s, const struct rt_kv *k
  * (its own and earlier new ones included: append them first), query head h the key-value head
  * h / (q_heads / heads). Times 1 / (1 + exp(-gate)), where given. For a few new tokens on a cache of any
  * length the positions are split over the GPU and joined; a prompt's tokens go 16 rows (token, head) at a time, 64 over
- * RT_Q8. There a query is held in 24 bits of its row's largest element; everything else is as exact as F32 sums.
+ * RT_Q8. There a query, times scale, is held in 24 bits of its row's largest element, and in steps of 1.2e-37 where that is below 1e-30; a
+ * position whose weight is far below its row's largest, or whose value is near F32's smallest, may be off by 2^-118 (1 + |value|);
+ * everything else is as exact as F32 sums.
  * A token that sees nothing (a position before 0) gives zeros; one that would have to see a position behind
  * the table's last page, or in a page that the cache does not have, gives NaN. */
 struct rt_attn {

@@ -22,7 +22,7 @@ namespace {
  * 100 to 16384 positions, 4 heads of 256: 107 us, 5.3 TB/s; 4 tokens at 131072 positions 49, 5.5 TB/s), by the latency of its dependent loads
  * on short ones. The first values under way with the first keys measured 4 us slower on the former: the keys come later. */
 constexpr int SUB = 4, POS = 64;
-constexpr float FULL = 8355584.0f; /* 2^23 - 2^15: 127.99 * 2^16, and what the rounding of the quotient adds, in balanced bytes */
+constexpr float FULL = 8355584.0f; /* 127 * 2^16 + 127 * 2^8: three balanced bytes hold 127 more, and the quotient's rounding adds 1 at most */
 
 /* 4 floats as FULL's integers, their three balanced bytes gathered by byte: w[n] is byte n of the four */
 __device__ __forceinline__ void bytes_of(float4 x, float up, uint32_t (&w)[3])
@@ -240,9 +240,9 @@ __global__ __launch_bounds__(64 * WAVES, q8_attn8_alone(D) ? 1 : 2) void attn8_k
  * converted, once for 64 rows and not for 16. The next tile's loads are under way in registers while the products of this one
  * run, and two workgroups share a compute unit, so that one's softmax and staging go under the other's matrix instructions.
  *
- * Heads of 256, 16 on 4: a prompt of 2048 112 us (16 rows a workgroup, as single tokens go: 299, the join's 95 among them); 8192
- * tokens through 1024 positions 355 (1075). A wave's tile is 144 matrix instructions, 2304 cycles, and some 550 others (queries and gates
- * among them), 2200, of 5100 that it takes of its SIMD: between two matrix instructions two others go unnoticed, the third costs,
+ * Heads of 256, 16 on 4: a prompt of 2048 115 us (16 rows a workgroup, as single tokens go: 299, the join's 95 among them); 8192
+ * tokens through 1024 positions 358 (1075). A wave's tile is 144 matrix instructions, 2304 cycles, and some 575 others (queries and gates
+ * among them), 2300, of 5100 that it takes of its SIMD: between two matrix instructions two others go unnoticed, the third costs,
  * so the issue of both bounds it. Tried and not faster: 32 rows a wave on the 32x32 instructions, one wave a SIMD (213 and 530); tiles of 32 positions in double buffers with one
  * barrier and the next scores beside this softmax (115 and 379); 128 rows a workgroup (141 and 356).
  *
